@@ -680,6 +680,77 @@ int smq_cpu_smaq_compress_f64(const double* x, int64_t n, const SmqSmaqParams* p
                               size_t workspace_bytes, int n_threads);
 int smq_cpu_smaq_decompress_f64(const void* packed, double* y, int64_t n, int n_threads);
 
+/* ---- operators of a training step ------------------------------------------------------------
+ * The normalisation, the loss and the update that stand next to the codecs in a training step, each
+ * keeping less than the operations it replaces (no normalised copy, no logits, one momentum). They
+ * have no counterpart among the reference's plugins. Device pointers; dtype SMQ_DTYPE_F32 / _F16 /
+ * _BF16; sums, statistics and gradients of parameters in fp32 or wider. Results do not depend on
+ * timing: no floating-point atomics. Workspaces need no initialisation. */
+
+/* Softmax cross entropy of a linear head over a vocabulary:
+ *   logits[m, v] = hidden[m] . weight[v] + bias[v], loss[m] = log sum_v exp logits[m, v] - logits[m, target[m]].
+ * hidden [tokens, dim] and weight [vocab, dim] have unit column stride and the given row pitches
+ * (elements); bias [vocab] fp32 or NULL. The logits are never stored: the forward keeps lse [tokens]
+ * and `head` (SMQ_CE_HEAD_BYTES of device memory, 8-byte aligned), the backward computes them again for
+ * `piece` vocabulary entries at a time (0: as many as 1 GiB of workspace allows). Rows whose target is
+ * ignore_index have loss and gradient 0, whatever they hold; any other target outside [0, vocab) makes
+ * its loss and gradient NaN. loss: one fp32 (mean over the rows taking part, NaN if there are none;
+ * sum) or [tokens] (none); grad_loss the same shape. Gradients are written whole, in the inputs' dtype
+ * (grad_bias fp32), rows packed; a NULL gradient is not computed. */
+#define SMQ_REDUCE_NONE 0
+#define SMQ_REDUCE_MEAN 1
+#define SMQ_REDUCE_SUM 2
+#define SMQ_CE_GRAD_HIDDEN 1
+#define SMQ_CE_GRAD_WEIGHT 2
+#define SMQ_CE_GRAD_BIAS 4
+#define SMQ_CE_HEAD_BYTES 64
+/* grad_flags 0: the forward's workspace; else the backward's for these gradients. 0 on bad arguments. */
+size_t smq_linear_ce_workspace_bytes(const void* hidden, int64_t hidden_ld, const void* weight,
+                                     int64_t weight_ld, int dtype, int64_t tokens, int64_t dim,
+                                     int64_t vocab, int64_t piece, int grad_flags);
+int smq_linear_ce_forward(const void* hidden, int64_t hidden_ld, const void* weight, int64_t weight_ld,
+                          int dtype, const int64_t* target, const float* bias, int64_t tokens,
+                          int64_t dim, int64_t vocab, int64_t ignore_index, int reduction, float* loss,
+                          float* lse, void* head, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int smq_linear_ce_backward(const void* hidden, int64_t hidden_ld, const void* weight,
+                           int64_t weight_ld, int dtype, const int64_t* target, const float* bias,
+                           int64_t tokens, int64_t dim, int64_t vocab, int64_t ignore_index,
+                           int reduction, const float* lse, const void* head, const float* grad_loss,
+                           void* grad_hidden, void* grad_weight, float* grad_bias, int64_t piece,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Group norm with an activation on channels-last tensors: x [n, positions, channels], contiguous,
+ *   y = act((x - mean) * rstd * weight + bias), mean and variance (biased) over a group's channels and
+ * the sample's positions. weight / bias [channels] fp32 or NULL (1 / 0). The forward writes mean and
+ * rstd [n, groups]; the backward needs x, dy and those two, and writes dx and (where not NULL) dweight
+ * and dbias [channels], fp32. */
+#define SMQ_ACT_NONE 0
+#define SMQ_ACT_RELU 1
+#define SMQ_ACT_SILU 2
+#define SMQ_ACT_GELU 3 /* z * Phi(z), by the error function */
+size_t smq_group_norm_workspace_bytes(int dtype, int64_t n, int64_t positions, int64_t channels,
+                                      int64_t groups, int backward);
+int smq_group_norm_act(const void* x, int dtype, void* y, int64_t n, int64_t positions, int64_t channels,
+                       int64_t groups, const float* weight, const float* bias, double eps, int activation,
+                       float* mean, float* rstd, void* workspace, size_t workspace_bytes, void* stream);
+int smq_group_norm_act_backward(const void* x, const void* dy, int dtype, void* dx, int64_t n,
+                                int64_t positions, int64_t channels, int64_t groups,
+                                const float* weight, const float* bias, int activation,
+                                const float* mean, const float* rstd, float* dweight, float* dbias,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* Orthogonalised update by Newton-Schulz products: for each of `batch` matrices
+ *   X = x / (|x|_F + eps); steps times: A = X X^T, B = b A + c A A, X = a X + B X   (rows <= cols; else x^T)
+ * into y [batch, rows, cols], packed, same dtype. x has unit column stride, row pitch ld and
+ * batch_stride between matrices (elements); it may not overlap y. coefficients = {a, b, c} must keep
+ * the singular values (at most 1 at the start) below 256 through all steps. */
+size_t smq_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);
+int smq_orthogonalize(const void* x, int64_t ld, int64_t batch_stride, int dtype, void* y,
+                      int64_t batch, int64_t rows, int64_t cols, int steps,
+                      const double* coefficients, double eps, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

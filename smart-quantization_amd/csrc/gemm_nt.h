@@ -1,0 +1,613 @@
+// gemm_nt.h — the matrix product the training-step operators share: C[m, n] = sum_k A[m, k] B[n, k]
+// with both operands contiguous along k, fp16 or bf16 MFMA, fp32 accumulation.
+//
+// Operand formats (16-bit elements, row pitch ld, rows 16-byte aligned, k padded with zeros):
+//   one plane   k padded to 64: a k tile is 64 consecutive elements of a row;
+//   two planes  an fp32 value x is held as hi = fp16(x), lo = fp16(x - hi) (23 significant bits, the
+//               caller scales by a power of two so that nothing overflows), k padded to 32, and each
+//               32 columns stored as [32 hi | 32 lo]: a k tile is again 64 consecutive elements.
+//               Three products hi*hi + hi*lo + lo*hi per k step; the dropped lo*lo is below 2^-24 of
+//               the largest product. An fp32-class product at a third of the fp16 rate, where the
+//               fp32 MFMA runs at a sixteenth.
+//
+// Kernel: a workgroup of WM x WN waves computes a BM x BN tile; a k tile of both operands (128 bytes
+// a row) goes from global memory straight into one of two LDS buffers (buffer_load ... lds, 16 bytes
+// a lane), while the other is read. Rows are 128 bytes apart, so the 16-byte chunk c of row r is kept
+// at chunk c ^ (r & 7): the 8 rows a quarter wave reads with one ds_read_b128 lie in 8 different bank
+// groups. The waves hold their fragments of the next 16 columns in registers while the MFMAs of the
+// current ones run, across the barrier between k tiles too. The four LDS buffers are separate
+// variables: the compiler then knows that a read of one does not wait for the loads into another.
+//
+// What bounds it: a wave's 128 x 64 part reads (128 + 64) * 16 * 2 bytes of LDS per 128 x 64 x 16
+// product, 75 % of the LDS rate at the full MFMA rate; 64 x 64 parts need 100 %.
+#pragma once
+
+#include "smq_common.h"
+
+namespace smq {
+void set_error(const char* fmt, ...);
+int check_launch(const char* what);
+
+namespace gemm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <typename H> struct Frag;
+template <> struct Frag<__bf16> {
+  typedef bf16x8 type;
+  static __device__ __forceinline__ f32x16 mma(type a, type b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Frag<_Float16> {
+  typedef f16x8 type;
+  static __device__ __forceinline__ f32x16 mma(type a, type b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+struct Operand {
+  const void* p;
+  int64_t ld;     // elements between rows
+  int64_t batch;  // elements between matrices of a batch
+  int rows;
+};
+
+// Output / source formats of a matrix an epilogue reads or writes.
+enum Fmt : int { kNone = 0, kF32 = 1, kF16 = 2, kBF16 = 3, kSplit = 4 };
+struct Mat {
+  void* p;
+  int64_t ld;
+  int64_t batch;
+  int fmt;
+  int pad;  // columns in [columns, pad) are written as zeros
+};
+
+__device__ __forceinline__ int64_t split_at(int64_t c) { return ((c >> 5) << 6) + (c & 31); }
+
+// Four consecutive columns c..c+3 (c a multiple of 4) of row r.
+__device__ __forceinline__ float4 load4(const Mat& s, int64_t b, int64_t r, int64_t c) {
+  typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+  typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+  const int64_t row = b * s.batch + r * s.ld;
+  if (s.fmt == kSplit) {
+    const _Float16* p = reinterpret_cast<const _Float16*>(s.p) + row + split_at(c);
+    const h4 hi = *reinterpret_cast<const h4*>(p), lo = *reinterpret_cast<const h4*>(p + 32);
+    return make_float4((float)hi.x + (float)lo.x, (float)hi.y + (float)lo.y,
+                       (float)hi.z + (float)lo.z, (float)hi.w + (float)lo.w);
+  }
+  if (s.fmt == kF16) {
+    const h4 v = *reinterpret_cast<const h4*>(reinterpret_cast<const _Float16*>(s.p) + row + c);
+    return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w);
+  }
+  if (s.fmt == kBF16) {
+    const b4 v = *reinterpret_cast<const b4*>(reinterpret_cast<const __bf16*>(s.p) + row + c);
+    return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w);
+  }
+  return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(s.p) + row + c);
+}
+
+__device__ __forceinline__ void store1(const Mat& d, int64_t row, int64_t c, float v) {
+  if (d.fmt == kSplit) {
+    _Float16* p = reinterpret_cast<_Float16*>(d.p) + row + split_at(c);
+    const _Float16 hi = (_Float16)v;
+    p[0] = hi;
+    p[32] = (_Float16)(v - (float)hi);
+  } else if (d.fmt == kF16) {
+    reinterpret_cast<_Float16*>(d.p)[row + c] = (_Float16)v;
+  } else if (d.fmt == kBF16) {
+    reinterpret_cast<__bf16*>(d.p)[row + c] = (__bf16)v;
+  } else {
+    reinterpret_cast<float*>(d.p)[row + c] = v;
+  }
+}
+
+// N consecutive columns (N = 4 or 8, c a multiple of N) of row r; columns from `cols` on are padding
+// (zeros up to d.pad, nothing behind it). Padded matrices (d.pad >= cols rounded up to N) and rows
+// with whole vectors take vector stores.
+template <int N>
+__device__ __forceinline__ void store_n(const Mat& d, int64_t b, int64_t r, int64_t c, int cols,
+                                        const float (&v)[N]) {
+  typedef _Float16 hN __attribute__((ext_vector_type(N)));
+  typedef __bf16 bN __attribute__((ext_vector_type(N)));
+  typedef float fN __attribute__((ext_vector_type(4)));
+  const int64_t row = b * d.batch + r * d.ld;
+  const int end = d.pad > cols ? d.pad : cols;
+  if (c >= end) return;
+  float w[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) w[i] = c + i < cols ? v[i] : 0.0f;
+  const int size = d.fmt == kF32 ? 4 : 2, need = N * size < 16 ? N * size : 16;
+  const bool whole = c + N <= end && (d.fmt == kSplit ||
+                     ((reinterpret_cast<uintptr_t>(d.p) + (row + c) * size) & (need - 1)) == 0);
+  if (!whole) {
+    for (int i = 0; i < N; i++)
+      if (c + i < end) store1(d, row, c + i, w[i]);
+    return;
+  }
+  if (d.fmt == kSplit) {
+    hN hi, lo;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      hi[i] = (_Float16)w[i];
+      lo[i] = (_Float16)(w[i] - (float)hi[i]);
+    }
+    _Float16* p = reinterpret_cast<_Float16*>(d.p) + row + split_at(c);
+    *reinterpret_cast<hN*>(p) = hi;
+    *reinterpret_cast<hN*>(p + 32) = lo;
+  } else if (d.fmt == kF16) {
+    hN h;
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = (_Float16)w[i];
+    *reinterpret_cast<hN*>(reinterpret_cast<_Float16*>(d.p) + row + c) = h;
+  } else if (d.fmt == kBF16) {
+    bN h;
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = (__bf16)w[i];
+    *reinterpret_cast<bN*>(reinterpret_cast<__bf16*>(d.p) + row + c) = h;
+  } else {
+    float* p = reinterpret_cast<float*>(d.p) + row + c;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      fN f = {w[i], w[i + 1], w[i + 2], w[i + 3]};
+      *reinterpret_cast<fN*>(p + i) = f;
+    }
+  }
+}
+
+// The tile a workgroup computes. Workgroup ids go round the 8 XCDs, each with its own L2: ids of one
+// XCD get consecutive tiles, in bands of kBand tile rows, so the tiles an XCD has in flight share
+// their rows of A and B. `tri`: only the tiles on and above the diagonal of a square tile grid (a
+// symmetric product; the epilogue writes the mirrored part).
+constexpr int kBand = 8;
+__device__ __forceinline__ void pick_tile(int tm, int tn, int tri, int& im, int& in) {
+  const int total = tri ? tm * (tm + 1) / 2 : tm * tn;
+  const int id = blockIdx.x, x = id & 7, q = total >> 3, rem = total & 7;
+  const int t = x * q + (x < rem ? x : rem) + (id >> 3);
+  if (tri) {
+    int r = (int)((2.0f * tm + 1.0f - sqrtf((2.0f * tm + 1.0f) * (2.0f * tm + 1.0f) - 8.0f * t)) * 0.5f);
+    while (r > 0 && r * tm - r * (r - 1) / 2 > t) r--;
+    while ((r + 1) * tm - (r + 1) * r / 2 <= t) r++;
+    im = r;
+    in = r + t - (r * tm - r * (r - 1) / 2);
+    return;
+  }
+  const int band = t / (kBand * tn), first = band * kBand;
+  const int high = tm - first < kBand ? tm - first : kBand;
+  const int u = t - band * kBand * tn;
+  im = first + u % high;
+  in = u / high;
+}
+
+template <typename H, int BM, int BN, int WM, int WN, bool SPLIT, typename Epi>
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Operand B, int kt,
+                                                                 int tm, int tn, int tri, Epi epi) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the buffer builtins' types do not exist in the host pass
+  typedef typename Frag<H>::type frag;
+  constexpr int kWaves = WM * WN;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int LA = BM / 8 / kWaves, LB = BN / 8 / kWaves;  // loads a wave issues per k tile
+  static_assert(TM * WM * 32 == BM && TN * WN * 32 == BN, "tile");
+  static_assert(LA * 8 * kWaves == BM && LB * 8 * kWaves == BN, "loads");
+  __shared__ __attribute__((aligned(1024))) H a0[BM * 64];
+  __shared__ __attribute__((aligned(1024))) H b0[BN * 64];
+  __shared__ __attribute__((aligned(1024))) H a1[BM * 64];
+  __shared__ __attribute__((aligned(1024))) H b1[BN * 64];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  int im, in;
+  pick_tile(tm, tn, tri, im, in);
+  const int row_a = im * BM, row_b = in * BN;
+  const int64_t batch = blockIdx.z;
+  // split k: this workgroup's share of the k tiles (gridDim.y = 1: all of them)
+  const int k0 = (int)((int64_t)kt * blockIdx.y / gridDim.y);
+  const int k1 = (int)((int64_t)kt * (blockIdx.y + 1) / gridDim.y);
+  const int nk = k1 - k0;
+
+  const int rows_a = A.rows - row_a < BM ? A.rows - row_a : BM;
+  const int rows_b = B.rows - row_b < BN ? B.rows - row_b : BN;
+  const char* pa = reinterpret_cast<const char*>(A.p) + 2 * (batch * A.batch + (int64_t)row_a * A.ld) + (int64_t)k0 * 128;
+  const char* pb = reinterpret_cast<const char*>(B.p) + 2 * (batch * B.batch + (int64_t)row_b * B.ld) + (int64_t)k0 * 128;
+  const int lda = (int)A.ld * 2, ldb = (int)B.ld * 2;
+  const __amdgpu_buffer_rsrc_t ra =
+      __builtin_amdgcn_make_buffer_rsrc((void*)pa, 0, (rows_a - 1) * lda + nk * 128, 0x00027000);
+  const __amdgpu_buffer_rsrc_t rb =
+      __builtin_amdgcn_make_buffer_rsrc((void*)pb, 0, (rows_b - 1) * ldb + nk * 128, 0x00027000);
+  int va[LA], vb[LB];
+  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+#pragma unroll
+  for (int i = 0; i < LA; i++) {
+    const int r = (i * kWaves + wave) * 8 + (lane >> 3);
+    va[i] = (r < rows_a ? r : rows_a - 1) * lda + chunk;
+  }
+#pragma unroll
+  for (int i = 0; i < LB; i++) {
+    const int r = (i * kWaves + wave) * 8 + (lane >> 3);
+    vb[i] = (r < rows_b ? r : rows_b - 1) * ldb + chunk;
+  }
+  auto fetch = [&](H* la, H* lb, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LA; i++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(la + (i * kWaves + wave) * 512), 16,
+                                               va[i], t * 128, 0, 0);
+#pragma unroll
+    for (int i = 0; i < LB; i++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(lb + (i * kWaves + wave) * 512), 16,
+                                               vb[i], t * 128, 0, 0);
+  };
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; i++)
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+
+  const int fr = lane & 31, fk = lane >> 5, fx = lane & 7;
+  auto read = [&](const H* la, const H* lb, int s, frag(&fa)[TM], frag(&fb)[TN])
+      __attribute__((always_inline)) {
+    const int at = ((s * 2 + fk) ^ fx) * 8;
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+      fa[i] = *reinterpret_cast<const frag*>(la + (wm * TM * 32 + i * 32 + fr) * 64 + at);
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+      fb[j] = *reinterpret_cast<const frag*>(lb + (wn * TN * 32 + j * 32 + fr) * 64 + at);
+  };
+  // operands swapped: a lane then holds runs of 4 consecutive n of one m
+  auto mma = [&](const frag(&fa)[TM], const frag(&fb)[TN]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = Frag<H>::mma(fb[j], fa[i], acc[i][j]);
+  };
+  frag fa0[TM], fb0[TN], fa1[TM], fb1[TN];
+  // One k tile in (la, lb), whose first fragments are in f0; (ma, mb) is the next tile's buffer.
+  auto tile = [&](H* la, H* lb, H* ma, H* mb, int t) __attribute__((always_inline)) {
+    if constexpr (!SPLIT) {
+      read(la, lb, 1, fa1, fb1);
+      mma(fa0, fb0);
+      read(la, lb, 2, fa0, fb0);
+      mma(fa1, fb1);
+      read(la, lb, 3, fa1, fb1);
+      mma(fa0, fb0);
+    } else {
+      // chunks 0-3 are hi, 4-7 are lo
+      read(la, lb, 2, fa1, fb1);
+      mma(fa0, fb0);
+      mma(fa0, fb1);
+      mma(fa1, fb0);
+      read(la, lb, 1, fa0, fb0);
+      read(la, lb, 3, fa1, fb1);
+      mma(fa0, fb0);
+    }
+    // every wave has its fragments of this tile, and the next tile has landed
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 2 < nk) fetch(la, lb, t + 2);
+    if constexpr (!SPLIT) {
+      read(ma, mb, 0, fa0, fb0);
+      mma(fa1, fb1);
+    } else {
+      mma(fa0, fb1);
+      mma(fa1, fb0);
+      read(ma, mb, 0, fa0, fb0);
+    }
+  };
+  if (nk > 0) {
+    fetch(a0, b0, 0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (nk > 1) fetch(a1, b1, 1);
+    read(a0, b0, 0, fa0, fb0);
+    int t = 0;
+    for (; t + 1 < nk; t += 2) {
+      tile(a0, b0, a1, b1, t);
+      tile(a1, b1, a0, b0, t + 1);
+    }
+    if (t < nk) tile(a0, b0, a1, b1, t);
+  }
+  __syncthreads();  // the LDS buffers are free for the epilogue
+
+  // 32 rows of the wave's part as fp32, in one of the four buffers
+  constexpr int kPitch = TN * 32 + 4;
+  constexpr int kNeed = 32 * kPitch * 4;
+  constexpr int kInA = BM * 128 / kNeed, kInB = BN * 128 / kNeed;
+  static_assert(2 * (kInA + kInB) >= kWaves, "staging");
+  float* stage;
+  {
+    int w = wave;
+    if (w < kInA) stage = reinterpret_cast<float*>(a0) + w * 32 * kPitch;
+    else if ((w -= kInA) < kInB) stage = reinterpret_cast<float*>(b0) + w * 32 * kPitch;
+    else if ((w -= kInB) < kInA) stage = reinterpret_cast<float*>(a1) + w * 32 * kPitch;
+    else stage = reinterpret_cast<float*>(b1) + (w - kInA) * 32 * kPitch;
+  }
+  epi.template finish<BM, BN, WM, WN, TM, TN>(acc, stage, row_a + wm * TM * 32,
+                                              row_b + wn * TN * 32, A.rows, B.rows, im, in, wm, wn,
+                                              lane, batch);
+#endif
+}
+
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Walks a wave's part of C through its LDS stage, 32 rows at a time: `f(m, n, v)` turns four
+// consecutive accumulators of row m into the values to be written, which go to `o` row by row and,
+// where `ot` is set, to `ot` transposed. `colsum(n, v)`, where given, gets the sum over the part's
+// rows of column n. Lanes past the edges call neither.
+template <int TM, int TN, typename F, typename S>
+__device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* stage, int m0, int n0,
+                                          int M, int N, int lane, int64_t batch, const Mat& o,
+                                          const Mat& ot, bool mirror, bool sums, F f, S colsum) {
+  constexpr int kCols = TN * 32, kPitch = kCols + 4;
+  constexpr int kPer = kCols / 4, kRows = 64 / kPer;  // row phase: lanes a row, rows a pass
+  float total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < TM; i++) {
+    const int mb = m0 + i * 32;
+    if (mb < M || (mirror && mb < ot.pad)) {  // rows from M on are the transposed matrix's padding
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          *reinterpret_cast<float4*>(stage + (lane & 31) * kPitch + j * 32 + 2 * r + 4 * (lane >> 5)) =
+              make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]);
+      wave_sync();
+#pragma unroll 4
+      for (int p = 0; p < 32; p += kRows) {
+        const int r = p + lane / kPer, c = (lane % kPer) * 4;
+        float* at = stage + r * kPitch + c;
+        float4 v = *reinterpret_cast<const float4*>(at);
+        if (mb + r < M) {
+          if (n0 + c < N) v = f(mb + r, n0 + c, v);
+          if (o.fmt != kNone) {
+            const float w[4] = {v.x, v.y, v.z, v.w};
+            store_n<4>(o, batch, mb + r, n0 + c, N, w);
+          }
+          if (mirror || sums) *reinterpret_cast<float4*>(at) = v;
+        }
+      }
+      if (mirror || sums) {
+        wave_sync();
+        if (lane < kCols) {
+          const int n = n0 + (lane % kCols);
+          if (n < N) {
+#pragma unroll
+            for (int r = 0; r < 32; r += 8) {
+              float w[8];
+#pragma unroll
+              for (int k = 0; k < 8; k++) {
+                w[k] = mb + r + k < M ? stage[(r + k) * kPitch + lane % kCols] : 0.0f;
+                total += w[k];
+              }
+              if (mirror) store_n<8>(ot, batch, n, mb + r, M, w);
+            }
+          }
+        }
+      }
+      wave_sync();
+    }
+  }
+  if (mirror && m0 < M && m0 + TM * 32 >= M && lane < kCols && n0 + lane < N) {
+    // padding behind the tile's own rows (a 32-row tile under a 64-column pad)
+    const float zero[8] = {};
+    for (int m = m0 + TM * 32; m < ot.pad; m += 8) store_n<8>(ot, batch, n0 + lane, m, M, zero);
+  }
+  if (sums && (lane < kCols) && n0 + lane < N) colsum(n0 + lane, total);
+}
+
+// C = alpha * acc + beta * src, to `o` and / or transposed to `ot` (a symmetric product writes the
+// same matrix twice; its diagonal tiles once). `scale`: a factor of alpha in device memory, or NULL.
+// A launch split over k (gridDim.y shares) writes share y to o + y * share.
+struct StoreEpi {
+  float alpha, beta;
+  const float* scale;
+  Mat src, o, ot;
+  int tri;
+  int64_t share;
+  template <int BM, int BN, int WM, int WN, int TM, int TN>
+  __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float* stage, int m0, int n0, int M,
+                                         int N, int im, int in, int, int, int lane,
+                                         int64_t batch) const {
+    const float al = scale ? alpha * *scale : alpha;
+    Mat s = src, d = o;
+    if (gridDim.y > 1) {
+      d.p = reinterpret_cast<float*>(d.p) + blockIdx.y * share;
+      if (s.fmt != kNone) s.p = reinterpret_cast<float*>(s.p) + blockIdx.y * share;
+    }
+    const float be = beta;
+    stage_out<TM, TN>(
+        acc, stage, m0, n0, M, N, lane, batch, d, ot, ot.fmt != kNone && !(tri && im == in), false,
+        [&](int m, int n, float4 v) {
+          v.x *= al, v.y *= al, v.z *= al, v.w *= al;
+          if (s.fmt != kNone) {
+            const float4 c = load4(s, batch, m, n);
+            v.x += be * c.x, v.y += be * c.y, v.z += be * c.z, v.w += be * c.w;
+          }
+          return v;
+        },
+        [](int, float) {});
+  }
+};
+
+// The second half of a product split over k: C = alpha * sum over the shares + beta * src, 64 x 64 a
+// workgroup (the same walk as the product's own epilogue, with the tile in LDS from the start).
+static __global__ __launch_bounds__(256) void split_sum_kernel(const float* part, int64_t ld,
+                                                               int64_t share, int shares,
+                                                               int64_t batch_stride, int M, int N,
+                                                               int mirror, StoreEpi e) {
+  __shared__ float tile[64][68];
+  const int im = blockIdx.y, in = blockIdx.x;
+  if (e.tri && in < im) return;
+  const int64_t batch = blockIdx.z;
+  const float al = e.scale ? e.alpha * *e.scale : e.alpha;
+  const int c = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
+  const bool turn = mirror && !(e.tri && im == in);
+#pragma unroll
+  for (int p = 0; p < 64; p += 16) {
+    const int m = im * 64 + p + r0, n = in * 64 + c;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (m < M) {
+      if (n < N) {
+        const float* q = part + batch * batch_stride + (int64_t)m * ld + n;
+        for (int k = 0; k < shares; k++) {
+          const float4 w = *reinterpret_cast<const float4*>(q + k * share);
+          v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+        v.x *= al, v.y *= al, v.z *= al, v.w *= al;
+        if (e.src.fmt != kNone) {
+          const float4 s = load4(e.src, batch, m, n);
+          v.x += e.beta * s.x, v.y += e.beta * s.y, v.z += e.beta * s.z, v.w += e.beta * s.w;
+        }
+      }
+      const float w[4] = {v.x, v.y, v.z, v.w};
+      if (e.o.fmt != kNone) store_n<4>(e.o, batch, m, n, N, w);
+    }
+    if (turn) *reinterpret_cast<float4*>(&tile[p + r0][c]) = v;
+  }
+  if (!turn) return;
+  __syncthreads();
+  const int n = in * 64 + (threadIdx.x & 63), m0 = im * 64 + (threadIdx.x >> 6) * 16;
+  if (n < N) {
+#pragma unroll
+    for (int h = 0; h < 16; h += 8) {
+      float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        w[k] = m0 + h + k < M ? tile[(threadIdx.x >> 6) * 16 + h + k][threadIdx.x & 63] : 0.0f;
+      store_n<8>(e.ot, batch, n, m0 + h, M, w);
+    }
+  }
+}
+
+// Tile shapes. 256 x 256 runs fastest per tile, but a grid below the CU count leaves CUs idle;
+// smaller tiles fill them. kSkinny: up to 32 rows of A, the product bounded by the read of B.
+enum Tile : int { kT256 = 0, kT128 = 1, kT64 = 2, kSkinny = 3 };
+struct TileShape {
+  int bm, bn, wn, cols;  // cols: columns one wave holds
+};
+static inline TileShape shape_of(int t) {
+  switch (t) {
+    case kT256: return {256, 256, 4, 64};
+    case kT128: return {128, 128, 2, 64};
+    case kT64: return {64, 64, 2, 32};
+    default: return {32, 128, 4, 32};
+  }
+}
+static inline int64_t tile_count(int64_t m, int64_t n, int t, int tri) {
+  const TileShape s = shape_of(t);
+  const int64_t a = (m + s.bm - 1) / s.bm, b = (n + s.bn - 1) / s.bn;
+  return tri ? a * (a + 1) / 2 : a * b;
+}
+static inline int choose_tile(int64_t m, int64_t n, int64_t batch, int tri) {
+  if (m <= 32 && !tri) return kSkinny;
+  if (batch * tile_count(m, n, kT256, tri) >= 192) return kT256;
+  if (batch * tile_count(m, n, kT128, tri) >= 128) return kT128;
+  return kT64;
+}
+template <typename H, int BM, int BN, int WM, int WN, bool SPLIT, typename Epi>
+static inline void launch_tile(const Operand& A, const Operand& B, int kt, int batch, int tri,
+                               int shares, const Epi& epi, hipStream_t st) {
+  const int tm = (A.rows + BM - 1) / BM, tn = (B.rows + BN - 1) / BN;
+  const int grid = tri ? tm * (tm + 1) / 2 : tm * tn;
+  hipLaunchKernelGGL((gemm_nt_kernel<H, BM, BN, WM, WN, SPLIT, Epi>), dim3(grid, shares, batch),
+                     dim3(WM * WN * 64), 0, st, A, B, kt, tm, tn, tri, epi);
+}
+template <typename H, bool SPLIT, typename Epi>
+static inline void launch(int tile, const Operand& A, const Operand& B, int kt, int batch, int tri,
+                          int shares, const Epi& epi, hipStream_t st) {
+  if (tile == kT256)
+    launch_tile<H, 256, 256, 2, 4, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+  else if (tile == kT128)
+    launch_tile<H, 128, 128, 2, 2, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+  else if (tile == kT64)
+    launch_tile<H, 64, 64, 2, 2, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+  else
+    launch_tile<H, 32, 128, 1, 4, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+}
+
+// Layout pass: src [rows, cols] of type T, row pitch ld, times 2^*exponent (NULL: 1) times *factor
+// (NULL: 1), to `d` row by row and / or to `dt` transposed (either may be absent), both zero padded.
+// Rows whose keep[row] equals `skip` are written as zeros (keep NULL: none). 64 x 64 a workgroup;
+// bound by its reads and writes of memory.
+template <typename T>
+static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_t ld,
+                                                            int64_t batch_stride, int rows, int cols,
+                                                            const int* exponent,
+                                                            const float* factor,
+                                                            const int64_t* keep, int64_t skip,
+                                                            Mat d, Mat dt) {
+  __shared__ float tile[64][65];
+  const int64_t batch = blockIdx.z;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  const int ex = exponent ? *exponent : 0;
+  const float fa = factor ? factor[batch] : 1.0f;
+  const T* p = src + batch * batch_stride;
+  const int q = threadIdx.x & 15, y = threadIdx.x >> 4;
+  const bool wide = (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && (ld & 3) == 0;
+#pragma unroll
+  for (int i = 0; i < 64; i += 16) {
+    const int r = r0 + y + i, c = c0 + q * 4;
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (r < rows && !(keep && keep[r] == skip)) {
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      if (wide && c + 4 <= cols) {
+        const t4 v = *reinterpret_cast<const t4*>(p + (int64_t)r * ld + c);
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = (float)v[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (c + k < cols) w[k] = (float)p[(int64_t)r * ld + c + k];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) w[k] = ldexpf(w[k] * fa, ex);
+    }
+    if (d.fmt != kNone && r < rows) store_n<4>(d, batch, r, c, cols, w);
+    if (dt.fmt != kNone) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) tile[y + i][q * 4 + k] = w[k];
+    }
+  }
+  if (dt.fmt == kNone) return;
+  __syncthreads();
+  // lanes: 8 runs of 8 rows, 8 columns a wave and pass
+  const int run = (threadIdx.x & 7) * 8, cc = threadIdx.x >> 3;
+#pragma unroll
+  for (int i = 0; i < 64; i += 32) {
+    const int c = c0 + cc + i;
+    if (c < cols) {
+      float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) w[k] = tile[run + k][cc + i];
+      store_n<8>(dt, batch, c, r0 + run, rows, w);
+    }
+  }
+}
+template <typename T>
+static inline void launch_layout(const T* src, int64_t ld, int64_t batch_stride, int rows, int cols,
+                                 int batch, const int* exponent, const float* factor,
+                                 const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt,
+                                 hipStream_t st) {
+  hipLaunchKernelGGL(layout_kernel<T>, dim3((cols + 63) / 64, (rows + 63) / 64, batch), dim3(256), 0,
+                     st, src, ld, batch_stride, rows, cols, exponent, factor, keep, skip, d, dt);
+}
+
+static inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+// Row pitch (elements) and padded columns of a k-contiguous operand of k columns.
+static inline int64_t operand_ld(int64_t k, bool split) {
+  return split ? 2 * round_up(k, 32) : round_up(k, 64);
+}
+static inline int operand_pad(int64_t k, bool split) { return (int)round_up(k, split ? 32 : 64); }
+static inline int operand_kt(int64_t k, bool split) {
+  return (int)(split ? round_up(k, 32) / 32 : round_up(k, 64) / 64);
+}
+
+}  // namespace gemm
+}  // namespace smq

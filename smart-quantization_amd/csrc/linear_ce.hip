@@ -1,0 +1,621 @@
+// linear_ce.hip — softmax cross entropy of a linear head, without keeping the logits, and its gradient.
+//
+//   l[m, v] = h[m] . w[v] + b[v],   lse[m] = log sum_v exp l[m, v],   loss[m] = lse[m] - l[m, t[m]]
+//   dl[m, v] = g[m] (exp(l[m, v] - lse[m]) - [v = t[m]]),   dh = dl w,   dw = dl^T h,   db = sum_m dl
+//
+// Forward: one matrix product whose epilogue keeps, per row and per block of columns, the maximum and
+// the sum of exponentials (and the target's logit); a second small launch joins them. The logits
+// exist in registers only. Backward: the vocabulary in pieces. Per piece the logits are computed
+// again, dl is written once as the 16-bit operand of the two gradient products, row by row and
+// transposed, and used up. Only lse is kept between the two passes.
+//
+// float32 inputs run as two fp16 planes (gemm_nt.h) scaled by a power of two per tensor; bf16 and fp16
+// inputs as they are. In the gradient products every 16-bit operand is fp16: dl rounded to 11 bits
+// (8 bits of bf16 were off by up to 2e-3 in the gradient of a target's row), and bf16 inputs, exact in
+// fp16 once scaled (what lies 2^-28 below the largest magnitude loses bits), in the transposed copies
+// that these products need anyway. dl is kept relative to the largest |g| and times 2^14, so that fp16
+// holds probabilities from 4e-9 up in full precision; the factors come off in the fp32 epilogues.
+#include "gemm_nt.h"
+
+namespace smq {
+namespace ce {  // named: a kernel template's arguments need linkage
+using namespace gemm;
+
+constexpr float kDlScale = 16384.0f;
+constexpr size_t kPieceBytes = size_t(1) << 30;  // default limit of a backward piece's buffers
+
+// Words the forward leaves for the backward (device): exponents of the two operands, the count of
+// rows that take part.
+struct Head {
+  int exp_h, exp_w;  // power-of-two exponents of the fp16 operands made of the inputs
+  int exp_out;       // -(exp_h + exp_w)
+  int pad;
+  double count;
+  float scale_dh, scale_dw, scale_db;  // backward: the factors of the gradients
+};
+
+// ---- largest magnitude of a tensor -> exponent ---------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void absmax_kernel(const T* x, int64_t ld, int64_t rows, int cols,
+                                                     float* part) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(V)));
+  float top = 0.0f;
+  const int64_t stride = (int64_t)gridDim.x * 4;
+  const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % V == 0;
+  const int whole = wide ? cols / V * V : 0;
+  for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += stride) {
+    const T* p = x + r * ld;
+    for (int k = (threadIdx.x & 63) * V; k < whole; k += 64 * V) {
+      const vec v = *reinterpret_cast<const vec*>(p + k);
+#pragma unroll
+      for (int i = 0; i < V; i++) top = fmaxf(top, fabsf((float)v[i]));
+    }
+    for (int k = whole + (threadIdx.x & 63); k < cols; k += 64) top = fmaxf(top, fabsf((float)p[k]));
+  }
+  top = wave_max_dpp(top);
+  __shared__ float w[4];
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+}
+
+// Exponent e with max * 2^e in [2^13, 2^14): room for the fp16 planes and for sums of their products.
+__device__ int plane_exponent(float top) {
+  if (!(top > 0.0f) || !(top < __builtin_inff())) return 0;
+  int e;
+  frexpf(top, &e);
+  const int k = 14 - e;
+  return k > 120 ? 120 : k;
+}
+__global__ __launch_bounds__(256) void exponent_kernel(const float* ph, int nh, const float* pw, int nw,
+                                                       Head* head) {
+  __shared__ float w[8];
+  float a = 0.0f, b = 0.0f;
+  for (int i = threadIdx.x; i < nh; i += 256) a = fmaxf(a, ph[i]);
+  for (int i = threadIdx.x; i < nw; i += 256) b = fmaxf(b, pw[i]);
+  a = wave_max_dpp(a), b = wave_max_dpp(b);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = a, w[4 + (threadIdx.x >> 6)] = b;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int eh = plane_exponent(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
+    const int ew = plane_exponent(fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
+    head->exp_h = eh, head->exp_w = ew, head->exp_out = -(eh + ew);
+  }
+}
+
+// exp(x) for x <= about 0, within 2 ulp: the product with log2(e) is carried in two parts (a single
+// one is off by up to |x| 2^-24, 1e-6 of the result at x = -11). NaN stays NaN.
+__device__ __forceinline__ float exp_near(float x) {
+  x = x < -200.0f ? -200.0f : x;
+  const float t = x * 1.44269504f;
+  const float e = fmaf(x, 1.44269504f, -t) + x * 1.92596303e-8f;
+  const float p = __builtin_amdgcn_exp2f(t);
+  return fmaf(p, e * 0.693147181f, p);
+}
+
+// ---- forward epilogue ---------------------------------------------------------------------------
+// Per row and per wave's block of columns: the maximum and the sum of exp(l - maximum); the target's
+// logit goes straight out (one lane of the grid owns it).
+struct SoftmaxEpi {
+  const int* exponent;
+  const float* bias;
+  const int64_t* target;
+  float2* part;  // [blocks][rows]
+  float* picked;
+  template <int BM, int BN, int WM, int WN, int TM, int TN>
+  __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float*, int m0, int n0, int M, int N,
+                                         int, int in, int, int wn, int lane, int64_t) const {
+    const int ex = exponent ? *exponent : 0;
+    const float ninf = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int n = n0 + j * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        const float b = bias && n < N ? bias[n] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+          const float l = ex ? ldexpf(acc[i][j][r], ex) : acc[i][j][r];
+          acc[i][j][r] = n < N ? l + b : ninf;
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const int m = m0 + i * 32 + (lane & 31);
+      float top = ninf;
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) top = fmaxf(top, acc[i][j][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float at = top == ninf ? 0.0f : top;
+      float sum = 0.0f;
+      const int64_t t = m < M ? target[m] : -1;
+      const int off = t >= n0 && t < n0 + TN * 32 ? (int)(t - n0) : -1;
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          sum += exp_near(acc[i][j][r] - at);
+          if (off == j * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) && t < N)
+            picked[m] = acc[i][j][r];
+        }
+      sum += __shfl_xor(sum, 32, 64);
+      if (lane < 32 && m < M) part[(int64_t)(in * WN + wn) * M + m] = make_float2(top, sum);
+    }
+  }
+};
+
+// ---- joining the blocks -------------------------------------------------------------------------
+// 64 rows a workgroup, 4 waves share the blocks; the joined statistics of a row by thread. A target
+// that is neither ignored nor in [0, vocab) gives NaN (nothing is read for it).
+__global__ __launch_bounds__(256) void join_kernel(const float2* part, int blocks, int rows,
+                                                   const int64_t* target, int64_t ignore,
+                                                   int64_t vocab, const float* picked, float* lse,
+                                                   float* row_loss) {
+  const int m = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  float top = -__builtin_inff(), sum = 0.0f;
+  if (m < rows)
+    for (int k = w; k < blocks; k += 4) {
+      const float2 p = part[(int64_t)k * rows + m];
+      const float t = fmaxf(top, p.x), at = t == -__builtin_inff() ? 0.0f : t;
+      sum = sum * expf(top - at) + p.y * expf(p.x - at);
+      top = t;
+    }
+  __shared__ float st[4][64], ss[4][64];
+  st[w][threadIdx.x & 63] = top, ss[w][threadIdx.x & 63] = sum;
+  __syncthreads();
+  if (w || m >= rows) return;
+  const int x = threadIdx.x;
+  const float t = fmaxf(fmaxf(st[0][x], st[1][x]), fmaxf(st[2][x], st[3][x]));
+  const float at = t == -__builtin_inff() ? 0.0f : t;
+  float s = 0.0f;
+  for (int k = 0; k < 4; k++) s += ss[k][x] * expf(st[k][x] - at);
+  const float l = at + logf(s);
+  lse[m] = l;
+  const int64_t y = target[m];
+  row_loss[m] = y == ignore ? 0.0f : y >= 0 && y < vocab ? l - picked[m] : __builtin_nanf("");
+}
+
+// One workgroup: the loss over rows (fp64 sums in a fixed order) and the count of rows taking part.
+__global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const int64_t* target,
+                                                    int64_t ignore, int rows, int reduction,
+                                                    int planes, float* loss, Head* head) {
+  double s = 0.0, c = 0.0;
+  for (int m = threadIdx.x; m < rows; m += 1024) {
+    s += (double)row_loss[m];
+    c += target[m] != ignore ? 1.0 : 0.0;
+    if (reduction == SMQ_REDUCE_NONE) loss[m] = row_loss[m];
+  }
+  s = wave_sum(s), c = wave_sum(c);
+  __shared__ double a[16], b[16];
+  if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = s, b[threadIdx.x >> 6] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = c = 0.0;
+    for (int k = 0; k < 16; k++) s += a[k], c += b[k];
+    head->count = c;
+    if (!planes) head->exp_h = head->exp_w = head->exp_out = 0;
+    if (reduction == SMQ_REDUCE_MEAN) *loss = (float)(s / c);
+    if (reduction == SMQ_REDUCE_SUM) *loss = (float)s;
+  }
+}
+
+// ---- backward -----------------------------------------------------------------------------------
+// One workgroup: the rows' factors relative to their largest magnitude, and what comes off again in
+// the epilogues. Ignored rows get 0.
+__global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
+                                                      int64_t ignore, int rows, int reduction,
+                                                      float* g, const Head* head, const Head* planes,
+                                                      Head* out) {
+  __shared__ float w[16];
+  __shared__ float all;
+  float top = 0.0f;
+  bool bad = false;
+  if (reduction == SMQ_REDUCE_NONE) {
+    for (int m = threadIdx.x; m < rows; m += 1024)
+      if (target[m] != ignore) {
+        top = fmaxf(top, fabsf(grad[m]));
+        bad |= !(fabsf(grad[m]) < __builtin_inff());
+      }
+  } else if (threadIdx.x == 0) {
+    // no row takes part: no gradient
+    const float v = reduction == SMQ_REDUCE_SUM ? *grad
+                    : head->count > 0.0         ? (float)((double)*grad / head->count) : 0.0f;
+    top = fabsf(v);
+    bad = !(top < __builtin_inff());
+  }
+  if (bad) top = __builtin_inff();
+  top = wave_max_dpp(top);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 16; k++) top = fmaxf(top, w[k]);
+    all = top;
+    out->scale_dh = ldexpf(top / kDlScale, planes ? -planes->exp_w : 0);
+    out->scale_dw = ldexpf(top / kDlScale, planes ? -planes->exp_h : 0);
+    out->scale_db = top / kDlScale;
+  }
+  __syncthreads();
+  top = all;
+  for (int m = threadIdx.x; m < rows; m += 1024) {
+    float v = 0.0f;
+    if (target[m] != ignore && top > 0.0f) {
+      if (reduction == SMQ_REDUCE_NONE) v = grad[m] / top;
+      else v = *grad < 0.0f ? -1.0f : 1.0f;
+    }
+    g[m] = v * kDlScale;
+  }
+}
+
+// dl of a piece from its logits, to `o` [rows, piece] and transposed to `ot` [piece, rows]; column
+// sums (the bias' gradient) per block of rows.
+struct DlEpi {
+  const int* exponent;
+  const float* bias;
+  const int64_t* target;
+  const float* lse;
+  const float* g;
+  int64_t first, vocab;  // the piece's first vocabulary entry
+  Mat o, ot;
+  float* sums;  // [blocks][piece] or NULL
+  template <int BM, int BN, int WM, int WN, int TM, int TN>
+  __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float* stage, int m0, int n0, int M,
+                                         int N, int im, int, int wm, int, int lane,
+                                         int64_t batch) const {
+    const int ex = exponent ? *exponent : 0;
+    float* sum = sums ? sums + (int64_t)(im * WM + wm) * N : nullptr;
+    stage_out<TM, TN>(
+        acc, stage, m0, n0, M, N, lane, batch, o, ot, true, sum != nullptr,
+        [&](int m, int n, float4 v) {
+          const float gm = g[m], ls = lse[m];
+          const int64_t t = target[m];
+          const bool known = t >= 0 && t < vocab;
+          const int64_t at = t - first - n;
+          float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            float l = ex ? ldexpf(w[k], ex) : w[k];
+            if (bias && n + k < N) l += bias[first + n + k];
+            const float p = exp_near(l - ls) - (at == k ? 1.0f : 0.0f);
+            w[k] = gm == 0.0f ? 0.0f : known ? p * gm : __builtin_nanf("");
+          }
+          return make_float4(w[0], w[1], w[2], w[3]);
+        },
+        [&](int n, float s) { sum[n] = s; });
+  }
+};
+
+__global__ __launch_bounds__(256) void bias_sum_kernel(const float* part, int blocks, int n,
+                                                       const Head* head, float* db) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= n) return;
+  double s = 0.0;
+  for (int k = 0; k < blocks; k++) s += (double)part[(int64_t)k * n + v];
+  db[v] = (float)(s * (double)head->scale_db);
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+struct Arena {
+  char* base;
+  size_t used = 0;
+  explicit Arena(void* p) : base(reinterpret_cast<char*>(p)) {}
+  template <typename T>
+  T* take(size_t count) {
+    used = (used + 255) & ~size_t(255);
+    T* p = reinterpret_cast<T*>(base + used);
+    used += count * sizeof(T);
+    return p;
+  }
+};
+
+struct Shape {
+  int64_t tokens, dim, vocab, piece;
+  int dtype;
+  bool split() const { return dtype == SMQ_DTYPE_F32; }
+  size_t size() const { return dtype == SMQ_DTYPE_F32 ? 4 : 2; }
+};
+
+constexpr int kMaxParts = 512;
+inline int absmax_grid(int64_t rows) { return (int)(rows < 4 * kMaxParts ? (rows + 3) / 4 : kMaxParts); }
+
+// A 16-bit tensor is an operand as it is when its rows are whole k tiles on 16-byte boundaries.
+inline bool direct(const void* p, int64_t ld, int64_t cols, int dtype) {
+  return dtype != SMQ_DTYPE_F32 && cols % 64 == 0 && ld % 8 == 0 && ld <= (1 << 21) &&
+         (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+inline int plane_fmt(int dtype) {
+  return dtype == SMQ_DTYPE_F32 ? kSplit : dtype == SMQ_DTYPE_F16 ? kF16 : kBF16;
+}
+inline int out_fmt(int dtype) {
+  return dtype == SMQ_DTYPE_F32 ? kF32 : dtype == SMQ_DTYPE_F16 ? kF16 : kBF16;
+}
+const Mat kNoMat = {nullptr, 0, 0, kNone, 0};
+
+void layout(const void* src, int dtype, int64_t ld, int64_t rows, int64_t cols, const int* exponent,
+            const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt, hipStream_t st) {
+  if (dtype == SMQ_DTYPE_F32)
+    launch_layout((const float*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st);
+  else if (dtype == SMQ_DTYPE_F16)
+    launch_layout((const _Float16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st);
+  else
+    launch_layout((const __bf16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st);
+}
+
+// exponents of both inputs' fp16 operands -> *head (part: room for 2 * kMaxParts floats)
+template <typename T>
+void exponents(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, float* part, Head* head,
+               hipStream_t st) {
+  const int gh = absmax_grid(s.tokens), gw = absmax_grid(s.vocab);
+  hipLaunchKernelGGL(absmax_kernel<T>, dim3(gh), dim3(256), 0, st, h, ldh, s.tokens, (int)s.dim, part);
+  hipLaunchKernelGGL(absmax_kernel<T>, dim3(gw), dim3(256), 0, st, w, ldw, s.vocab, (int)s.dim, part + kMaxParts);
+  hipLaunchKernelGGL(exponent_kernel, dim3(1), dim3(256), 0, st, part, gh, part + kMaxParts, gw, head);
+}
+
+template <typename Epi>
+void product(int dtype, int tile, const Operand& A, const Operand& B, int kt, int shares, const Epi& e,
+             hipStream_t st) {
+  if (dtype == SMQ_DTYPE_BF16) launch<__bf16, false>(tile, A, B, kt, 1, 0, shares, e, st);
+  else if (dtype == SMQ_DTYPE_F16) launch<_Float16, false>(tile, A, B, kt, 1, 0, shares, e, st);
+  else launch<_Float16, true>(tile, A, B, kt, 1, 0, shares, e, st);
+}
+
+// [rows, cols] in operand form: in place where it can be, else laid out in the workspace.
+Operand operand(Arena& ws, const void* p, int64_t ld, int64_t rows, int64_t cols, const Shape& s,
+                const int* exponent, bool run, hipStream_t st) {
+  if (direct(p, ld, cols, s.dtype)) return {p, ld, 0, (int)rows};
+  const int64_t to = operand_ld(cols, s.split());
+  _Float16* q = ws.take<_Float16>((size_t)(rows * to));
+  if (run)
+    layout(p, s.dtype, ld, rows, cols, exponent, nullptr, 0,
+           {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, kNoMat, st);
+  return {q, to, 0, (int)rows};
+}
+
+int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype,
+             const int64_t* target, int64_t tokens, int64_t dim, int64_t vocab, int reduction) {
+  if (dtype != SMQ_DTYPE_F32 && dtype != SMQ_DTYPE_F16 && dtype != SMQ_DTYPE_BF16) {
+    set_error("%s: dtype %d is not one of SMQ_DTYPE_F32/F16/BF16", who, dtype);
+    return SMQ_ERR_INVALID;
+  }
+  if (tokens < 1 || dim < 1 || vocab < 1 || tokens > (1 << 20) || dim > (1 << 20) || vocab > (1 << 21)) {
+    set_error("%s: needs 1 <= tokens, dim <= 2^20 and 1 <= vocab <= 2^21, got %lld, %lld, %lld", who,
+              (long long)tokens, (long long)dim, (long long)vocab);
+    return SMQ_ERR_INVALID;
+  }
+  if (!h || !w || !target || ldh < dim || ldw < dim) {
+    set_error("%s: hidden, weight and target must be non-NULL, row pitches at least dim", who);
+    return SMQ_ERR_INVALID;
+  }
+  if (reduction != SMQ_REDUCE_NONE && reduction != SMQ_REDUCE_MEAN && reduction != SMQ_REDUCE_SUM) {
+    set_error("%s: reduction %d invalid", who, reduction);
+    return SMQ_ERR_INVALID;
+  }
+  return SMQ_OK;
+}
+
+struct ForwardPlan {
+  size_t bytes;
+  int rc;
+};
+// Lays the workspace out; enqueues when `run`.
+ForwardPlan forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,
+                    const int64_t* target, const float* bias, int64_t ignore, int reduction,
+                    float* loss, float* lse, Head* head, void* ws, bool run, hipStream_t st) {
+  Arena a(ws);
+  const int tile = choose_tile(s.tokens, s.vocab, 1, 0);
+  const TileShape ts = shape_of(tile);
+  const int64_t tn = (s.vocab + ts.bn - 1) / ts.bn;
+  const int blocks = (int)(tn * ts.wn);
+  float2* part = a.take<float2>((size_t)blocks * s.tokens);
+  float* picked = a.take<float>(s.tokens);
+  float* rows = a.take<float>(s.tokens);
+  const int* exponent = nullptr;
+  const int *eh = nullptr, *ew = nullptr;
+  if (s.split()) {
+    float* top = a.take<float>(2 * kMaxParts);
+    exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
+    if (run) exponents((const float*)h, ldh, (const float*)w, ldw, s, top, head, st);
+  }
+  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, run, st);
+  const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, run, st);
+  if (run) {
+    const SoftmaxEpi e = {exponent, bias, target, part, picked};
+    product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + 63) / 64)), dim3(256), 0, st, part,
+                       blocks, (int)s.tokens, target, ignore, s.vocab, picked, lse, rows);
+    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
+                       reduction, s.split() ? 1 : 0, loss, head);
+  }
+  return {a.used, SMQ_OK};
+}
+
+// Shares of the k range of dh: enough workgroups to fill the chip where dh itself has few tiles.
+int dh_shares(const Shape& s, int tile, int kt) {
+  const int64_t wgs = tile_count(s.tokens, s.dim, tile, 0);
+  int64_t k = (512 + wgs - 1) / wgs;
+  if (k > kt / 8) k = kt / 8;
+  return (int)(k < 1 ? 1 : k > 32 ? 32 : k);
+}
+
+int64_t default_piece(const Shape& s) {
+  const int64_t planes = s.split() ? 2 : 1;
+  const int64_t per = 2 * planes * (2 * round_up(s.tokens, 64) + round_up(s.dim, 64));
+  int64_t p = (int64_t)(kPieceBytes / per);
+  p = p / 256 * 256;
+  return p < 256 ? 256 : p > (1 << 20) ? 1 << 20 : p;
+}
+
+size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s, const int64_t* target,
+                const float* bias, int64_t ignore, int reduction, const float* lse, const Head* head,
+                const float* grad, void* dh, void* dw, float* db, void* ws, bool run, hipStream_t st) {
+  Arena a(ws);
+  const bool sp = s.split();
+  const int fmt = sp ? kSplit : kF16;  // the gradient products' operands
+  const int grad_dtype = sp ? SMQ_DTYPE_F32 : SMQ_DTYPE_F16;
+  if (s.piece <= 0) s.piece = default_piece(s);
+  if (s.piece > s.vocab) s.piece = s.vocab;
+  const int64_t pieces = (s.vocab + s.piece - 1) / s.piece;
+  const int* exponent = sp ? &head->exp_out : nullptr;
+  float* g = a.take<float>(s.tokens);
+  Head* fac = a.take<Head>(1);
+  const Head* planes = sp ? head : nullptr;
+  if (s.dtype == SMQ_DTYPE_BF16) {
+    float* top = a.take<float>(2 * kMaxParts);
+    planes = fac;
+    if (run) exponents((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, fac, st);
+  }
+  const int* eh = planes ? &planes->exp_h : nullptr;
+  const int* ew = planes ? &planes->exp_w : nullptr;
+  if (run)
+    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
+                       (int)s.tokens, reduction, g, head, planes, fac);
+  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, run, st);
+  // h transposed: the operand of dw. Ignored rows are zeros, whatever they hold.
+  const int64_t ldt = operand_ld(s.tokens, sp);
+  const int padt = operand_pad(s.tokens, sp);
+  _Float16* ht = nullptr;
+  if (dw) {
+    ht = a.take<_Float16>((size_t)(s.dim * ldt));
+    if (run)
+      layout(h, s.dtype, ldh, s.tokens, s.dim, eh, target, ignore, kNoMat, {ht, ldt, 0, fmt, padt}, st);
+  }
+  const int64_t ldp = operand_ld(s.piece, sp);
+  _Float16* dl = a.take<_Float16>((size_t)(s.tokens * ldp));
+  _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
+  _Float16* wt = dh ? a.take<_Float16>((size_t)(s.dim * ldp)) : nullptr;
+  const int tile_l = choose_tile(s.tokens, s.piece, 1, 0);
+  const int row_blocks = (int)((s.tokens + shape_of(tile_l).bm - 1) / shape_of(tile_l).bm) *
+                         (tile_l == kSkinny ? 1 : 2);
+  float* sums = db ? a.take<float>((size_t)row_blocks * s.piece) : nullptr;
+  const int tile_h = choose_tile(s.tokens, s.dim, 1, 0) == kSkinny ? kSkinny : kT128;
+  const int tile_dh = choose_tile(s.tokens, s.dim, 1, 0) == kT256 ? kT256 : tile_h;
+  const int shares = dh_shares(s, tile_dh, operand_kt(s.piece, sp));
+  const int64_t ldacc = round_up(s.dim, 4);
+  const bool whole = pieces == 1 && shares == 1;
+  float* accum = dh && !whole ? a.take<float>((size_t)(shares * s.tokens * ldacc)) : nullptr;
+  const size_t wsize = s.size();
+  const size_t mark = a.used;
+  size_t most = mark;
+  for (int64_t i = 0; i < pieces; i++) {
+    a.used = mark;
+    const int64_t v0 = i * s.piece, n = s.vocab - v0 < s.piece ? s.vocab - v0 : s.piece;
+    const char* wp = reinterpret_cast<const char*>(w) + (size_t)(v0 * ldw) * wsize;
+    const Operand B = operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, run, st);
+    if (a.used > most) most = a.used;
+    if (!run) continue;
+    const int padn = operand_pad(n, sp);
+    const DlEpi e = {exponent, bias, target, lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
+                     {dlt, ldt, 0, fmt, padt}, sums};
+    product(s.dtype, tile_l, A, B, operand_kt(s.dim, sp), 1, e, st);
+    if (db)
+      hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, sums,
+                         row_blocks, (int)n, fac, db + v0);
+    if (dh) {
+      layout(wp, s.dtype, ldw, n, s.dim, ew, nullptr, 0, kNoMat, {wt, ldp, 0, fmt, padn}, st);
+      const Operand L = {dl, ldp, 0, (int)s.tokens}, W = {wt, ldp, 0, (int)s.dim};
+      StoreEpi se = {1.0f, 1.0f, whole ? &fac->scale_dh : nullptr, kNoMat, kNoMat, kNoMat, 0, s.tokens * ldacc};
+      se.o = whole ? Mat{dh, s.dim, 0, out_fmt(s.dtype), 0} : Mat{accum, ldacc, 0, kF32, 0};
+      if (i > 0) se.src = se.o;
+      product(grad_dtype, tile_dh, L, W, operand_kt(n, sp), shares, se, st);
+    }
+    if (dw) {
+      const Operand L = {dlt, ldt, 0, (int)n}, H = {ht, ldt, 0, (int)s.dim};
+      StoreEpi se = {1.0f, 0.0f, &fac->scale_dw, kNoMat, kNoMat, kNoMat, 0, 0};
+      se.o = {reinterpret_cast<char*>(dw) + (size_t)(v0 * s.dim) * wsize, s.dim, 0, out_fmt(s.dtype), 0};
+      product(grad_dtype, choose_tile(n, s.dim, 1, 0), L, H, operand_kt(s.tokens, sp), 1, se, st);
+    }
+  }
+  if (run && dh && !whole) {
+    const StoreEpi se = {1.0f, 0.0f, &fac->scale_dh, kNoMat, {dh, s.dim, 0, out_fmt(s.dtype), 0}, kNoMat, 0, 0};
+    hipLaunchKernelGGL(split_sum_kernel, dim3((unsigned)((s.dim + 63) / 64), (unsigned)((s.tokens + 63) / 64)),
+                       dim3(256), 0, st, accum, ldacc, s.tokens * ldacc, shares, (int64_t)0,
+                       (int)s.tokens, (int)s.dim, 0, se);
+  }
+  return most;
+}
+
+}  // namespace ce
+}  // namespace smq
+
+using namespace smq;
+using namespace smq::ce;
+
+extern "C" {
+
+size_t smq_linear_ce_workspace_bytes(const void* hidden, int64_t hidden_ld, const void* weight,
+                                     int64_t weight_ld, int dtype, int64_t tokens, int64_t dim,
+                                     int64_t vocab, int64_t piece, int grad_flags) {
+  const int64_t none = 0;
+  if (validate("linear_ce_workspace_bytes", hidden, hidden_ld, weight, weight_ld, dtype, &none, tokens,
+               dim, vocab, SMQ_REDUCE_SUM) != SMQ_OK)
+    return 0;
+  const Shape s = {tokens, dim, vocab, piece, dtype};
+  Head* head = nullptr;
+  if (!grad_flags)
+    return forward(hidden, hidden_ld, weight, weight_ld, s, nullptr, nullptr, 0, 0, nullptr, nullptr,
+                   head, nullptr, false, nullptr).bytes + 256;
+  char mark[1];
+  return backward(hidden, hidden_ld, weight, weight_ld, s, nullptr, nullptr, 0, 0, nullptr, head,
+                  nullptr, grad_flags & SMQ_CE_GRAD_HIDDEN ? mark : nullptr,
+                  grad_flags & SMQ_CE_GRAD_WEIGHT ? mark : nullptr,
+                  grad_flags & SMQ_CE_GRAD_BIAS ? reinterpret_cast<float*>(mark) : nullptr, nullptr,
+                  false, nullptr) + 256;
+}
+
+int smq_linear_ce_forward(const void* hidden, int64_t hidden_ld, const void* weight, int64_t weight_ld,
+                          int dtype, const int64_t* target, const float* bias, int64_t tokens,
+                          int64_t dim, int64_t vocab, int64_t ignore_index, int reduction, float* loss,
+                          float* lse, void* head, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  const int rc = validate("linear_ce_forward", hidden, hidden_ld, weight, weight_ld, dtype, target,
+                          tokens, dim, vocab, reduction);
+  if (rc != SMQ_OK) return rc;
+  if (!loss || !lse || !head) {
+    set_error("linear_ce_forward: loss, lse and head must be non-NULL");
+    return SMQ_ERR_INVALID;
+  }
+  const size_t need = smq_linear_ce_workspace_bytes(hidden, hidden_ld, weight, weight_ld, dtype,
+                                                    tokens, dim, vocab, 0, 0);
+  if (!workspace || workspace_bytes < need) {
+    set_error("linear_ce_forward: workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    return SMQ_ERR_WORKSPACE;
+  }
+  const Shape s = {tokens, dim, vocab, 0, dtype};
+  forward(hidden, hidden_ld, weight, weight_ld, s, target, bias, ignore_index, reduction, loss, lse,
+          reinterpret_cast<Head*>(head), workspace, true, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("linear_ce_forward");
+}
+
+int smq_linear_ce_backward(const void* hidden, int64_t hidden_ld, const void* weight,
+                           int64_t weight_ld, int dtype, const int64_t* target, const float* bias,
+                           int64_t tokens, int64_t dim, int64_t vocab, int64_t ignore_index,
+                           int reduction, const float* lse, const void* head, const float* grad_loss,
+                           void* grad_hidden, void* grad_weight, float* grad_bias, int64_t piece,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = validate("linear_ce_backward", hidden, hidden_ld, weight, weight_ld, dtype, target,
+                          tokens, dim, vocab, reduction);
+  if (rc != SMQ_OK) return rc;
+  if (!lse || !head || !grad_loss || (!grad_hidden && !grad_weight && !grad_bias) || piece < 0 ||
+      piece > (1 << 20)) {
+    set_error("linear_ce_backward: lse, head, grad_loss and one gradient must be non-NULL, "
+              "0 <= piece <= 2^20");
+    return SMQ_ERR_INVALID;
+  }
+  const int flags = (grad_hidden ? SMQ_CE_GRAD_HIDDEN : 0) | (grad_weight ? SMQ_CE_GRAD_WEIGHT : 0) |
+                    (grad_bias ? SMQ_CE_GRAD_BIAS : 0);
+  const size_t need = smq_linear_ce_workspace_bytes(hidden, hidden_ld, weight, weight_ld, dtype,
+                                                    tokens, dim, vocab, piece, flags);
+  if (!workspace || workspace_bytes < need) {
+    set_error("linear_ce_backward: workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+    return SMQ_ERR_WORKSPACE;
+  }
+  const Shape s = {tokens, dim, vocab, piece, dtype};
+  backward(hidden, hidden_ld, weight, weight_ld, s, target, bias, ignore_index, reduction, lse,
+           reinterpret_cast<const Head*>(head), grad_loss, grad_hidden, grad_weight, grad_bias,
+           workspace, true, reinterpret_cast<hipStream_t>(stream));
+  return check_launch("linear_ce_backward");
+}
+
+}  // extern "C"

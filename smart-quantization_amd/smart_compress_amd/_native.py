@@ -7,6 +7,7 @@ mirror include/smq.h field for field.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -48,6 +49,17 @@ SMQ_DTYPE_BF16 = 2
 SMQ_DTYPE_F64 = 3
 SMQ_ROUND_NEAREST = 0
 SMQ_ROUND_STOCHASTIC = 1
+SMQ_REDUCE_NONE = 0
+SMQ_REDUCE_MEAN = 1
+SMQ_REDUCE_SUM = 2
+SMQ_CE_GRAD_HIDDEN = 1
+SMQ_CE_GRAD_WEIGHT = 2
+SMQ_CE_GRAD_BIAS = 4
+SMQ_CE_HEAD_BYTES = 64
+SMQ_ACT_NONE = 0
+SMQ_ACT_RELU = 1
+SMQ_ACT_SILU = 2
+SMQ_ACT_GELU = 3
 
 
 class SmqSmaqParams(ctypes.Structure):
@@ -353,6 +365,32 @@ SIGNATURES = {
         _I32,
         [_P, _P, _I64, _I32, _I32, _P, _U64, _U64, _P, _P, _SZ, _U32, _I32],
     ),
+    "smq_linear_ce_workspace_bytes": (_SZ, [_P, _I64, _P, _I64, _I32, _I64, _I64, _I64, _I64,
+                                            _I32]),
+    "smq_linear_ce_forward": (
+        _I32,
+        [_P, _I64, _P, _I64, _I32, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _SZ, _P],
+    ),
+    "smq_linear_ce_backward": (
+        _I32,
+        [_P, _I64, _P, _I64, _I32, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P,
+         _I64, _P, _SZ, _P],
+    ),
+    "smq_group_norm_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I32]),
+    "smq_group_norm_act": (
+        _I32,
+        [_P, _I32, _P, _I64, _I64, _I64, _I64, _P, _P, ctypes.c_double, _I32, _P, _P, _P, _SZ, _P],
+    ),
+    "smq_group_norm_act_backward": (
+        _I32,
+        [_P, _P, _I32, _P, _I64, _I64, _I64, _I64, _P, _P, _I32, _P, _P, _P, _P, _P, _SZ, _P],
+    ),
+    "smq_orthogonalize_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I64]),
+    "smq_orthogonalize": (
+        _I32,
+        [_P, _I64, _I64, _I32, _P, _I64, _I64, _I64, _I32, ctypes.POINTER(ctypes.c_double),
+         ctypes.c_double, _P, _SZ, _P],
+    ),
 }
 
 _lib = None
@@ -521,6 +559,22 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is not None:
         return _raw_stream(device_index(device))
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (launches go to the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
+def call_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """A workspace for one call, from torch's allocator: returned to it in stream order when the
+    call's tensors go, and private to its graph during a capture."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 # ---- per (device, stream) workspaces (the library needs them neither zeroed nor reset) ----------

@@ -1,8 +1,12 @@
 """Layer-type selection for the compression callers (reference: util/pytorch/quantization.py:8-129,
 161-180: the ``*_LAYERS`` tables, ``LAYERS_TYPES``, ``DEFAULT_LAYER_TYPES``,
-``is_valid_layer_type``). Kept in its own module here; ``quantization`` re-exports it."""
+``is_valid_layer_type``). Kept in its own module here; ``quantization`` re-exports it. This package's
+own normalisation and loss modules stand in the tables beside torch's."""
 
 from torch import nn
+
+from .loss import LinearCrossEntropy
+from .norm import GroupNormAct
 
 SEQUENTIAL_LAYERS = [nn.Sequential, nn.ModuleList]
 DICT_LAYERS = [nn.ModuleDict]
@@ -20,14 +24,14 @@ ACTIVATION_LAYERS = [nn.ELU, nn.Hardshrink, nn.Hardtanh, nn.LeakyReLU, nn.LogSig
                      nn.Softsign, nn.Tanh, nn.Tanhshrink, nn.Threshold, nn.Softmin, nn.Softmax,
                      nn.Softmax2d, nn.LogSoftmax]
 NORM_LAYERS = [nn.BatchNorm1d, nn.BatchNorm2d, nn.BatchNorm3d, nn.GroupNorm, nn.InstanceNorm1d,
-               nn.InstanceNorm2d, nn.InstanceNorm3d, nn.LayerNorm, nn.LocalResponseNorm]
+               nn.InstanceNorm2d, nn.InstanceNorm3d, nn.LayerNorm, nn.LocalResponseNorm, GroupNormAct]
 LINEAR_LAYERS = [nn.Linear, nn.Bilinear]
 DROPOUT_LAYERS = [nn.Dropout, nn.Dropout2d, nn.Dropout3d, nn.AlphaDropout]
 LOSS_LAYERS = [nn.L1Loss, nn.MSELoss, nn.CrossEntropyLoss, nn.NLLLoss, nn.PoissonNLLLoss,
                nn.KLDivLoss, nn.BCELoss, nn.BCEWithLogitsLoss, nn.MarginRankingLoss,
                nn.HingeEmbeddingLoss, nn.MultiLabelMarginLoss, nn.SmoothL1Loss,
                nn.SoftMarginLoss, nn.MultiLabelSoftMarginLoss, nn.MultiMarginLoss,
-               nn.TripletMarginLoss]
+               nn.TripletMarginLoss, LinearCrossEntropy]
 
 LAYERS_TYPES = {
     "conv": CONV_LAYERS,

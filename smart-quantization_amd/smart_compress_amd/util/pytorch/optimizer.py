@@ -8,8 +8,8 @@ util/pytorch/hooks.py:22-34 (``wrap_optimizer``). Same constructor, same order o
   swap-in;
 * after the inner step: gradients again, then weights ``w <- Q(w)`` (groups without
   ``no_weight_compression``, every parameter of the group), then momenta (SGD ``momentum_buffer``
-  unless ``momentum == 0``; Adam/AdamW ``exp_avg`` and ``exp_avg_sq`` with ``all_positive=True``),
-  skipping ``no_momentum_compression`` groups.
+  unless ``momentum == 0``, and this package's ``Muon`` the same way; Adam/AdamW ``exp_avg`` and
+  ``exp_avg_sq`` with ``all_positive=True``), skipping ``no_momentum_compression`` groups.
 
 Fusion: when a quantiser is this package's ``SmartFP`` (wrapped by ``wrap_optimizer`` below), each
 of those loops becomes ONE ``SmaqMulti`` call (two launches) that
@@ -27,6 +27,7 @@ from torch.optim import SGD, Adam, AdamW, Optimizer
 from ... import _native as N
 from ...compress.smart import SmartFP
 from .multi import SmaqMulti
+from .muon import Muon
 
 __all__ = ["OptimLP", "TaggedQuant", "wrap_optimizer"]
 
@@ -80,12 +81,12 @@ class OptimLP(Optimizer):
         self.grad_quant = grad_quant
         self.momentum_quant = momentum_quant
         self.acc_quant = acc_quant
-        if isinstance(optim, SGD):
+        if isinstance(optim, (SGD, Muon)):
             self.momentum_keys: List[Tuple[str, Dict]] = [("momentum_buffer", {})]
         elif isinstance(optim, (Adam, AdamW)):
             self.momentum_keys = [("exp_avg", {}), ("exp_avg_sq", {"all_positive": True})]
         else:
-            raise NotImplementedError("Only supporting Adam and SGD for now. ")
+            raise NotImplementedError("Only supporting Adam, SGD and Muon for now. ")
         if acc_quant is not None:
             self.weight_acc = {p: p.detach().clone().type_as(p)
                                for g in self.param_groups for p in g["params"]}
@@ -187,7 +188,7 @@ class OptimLP(Optimizer):
             for g in self.param_groups:
                 if g.get("no_momentum_compression", False):
                     continue
-                if isinstance(self.optim, SGD) and g["momentum"] == 0:
+                if isinstance(self.optim, (SGD, Muon)) and g["momentum"] == 0:
                     continue
                 for p in g["params"]:
                     if not p.requires_grad or p.grad is None:

@@ -1,0 +1,310 @@
+"""linear_cross_entropy / LinearCrossEntropy on the GPU against the formula in float64.
+
+Tolerances. u = 2^-24, k = dim. A logit is a float32 sum of k products in runs of 16: off by at most
+e = (k / 16 + 24) u max_v sum|h w| (float32 inputs: each factor also off by 2^-23, the dropped product
+of the low planes by 2^-24: within the 24). The loss is off by 2 e + 8 u (|lse| + |logit|). dl = g (p - 1) is
+off by g p (2 e + 8 u) and rounds to an operand: half a step is 2^-11 (fp16, 10 stored bits) relative,
+or 2^-23 (two planes: what hi leaves is below 2^-11, of which lo's half step is 2^-12 at most), and
+2^-38 of the largest g absolute; the gradient products add (n / 16 + 24) u of their sums of magnitudes
+over n terms and round to the inputs' type by half a step."""
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from smart_compress_amd.util.pytorch.loss import LinearCrossEntropy, linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def make(tokens, dim, vocab, dtype, bias, ignored, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    h = torch.randn(tokens, dim, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(vocab, dim, generator=g, device="cuda") * 2 * dim ** -0.5).to(dtype)
+    b = torch.randn(vocab, generator=g, device="cuda") if bias else None
+    t = torch.randint(0, vocab, (tokens,), generator=g, device="cuda")
+    if ignored:
+        t[torch.rand(tokens, generator=g, device="cuda") < ignored] = -100
+    return h, w, b, t
+
+
+def reference(h, w, b, t, reduction, g, ignore=-100):
+    """float64 loss and gradients, and the bounds of their errors (module docstring)."""
+    H, W = h.double(), w.double()
+    keep = t != ignore
+    H = torch.where(keep[:, None], H, torch.zeros_like(H))
+    at = torch.where(keep, t, torch.zeros_like(t))
+    logits = H @ W.t()
+    size = (H.abs() @ W.abs().t()).amax(1)
+    if b is not None:
+        logits = logits + b.double()
+        size = size + b.double().abs().max()
+    lse = torch.logsumexp(logits, 1)
+    pick = logits.gather(1, at[:, None])[:, 0]
+    rows = torch.where(keep, lse - pick, torch.zeros_like(lse))
+    count = keep.sum().double()
+    e = (h.shape[1] / 16 + 24) * U * size
+    br = 2 * e + 8 * U * (lse.abs() + pick.abs())
+    if reduction == "none":
+        loss, bl = rows, br
+        gr = g.double() * keep
+    else:
+        div = count if reduction == "mean" else torch.ones_like(count)
+        loss, bl = rows.sum() / div, (br * keep).sum() / div
+        gr = g.double() / div * keep
+    p = torch.exp(logits - lse[:, None])
+    dl = p.clone()
+    dl[torch.arange(len(t)), at] -= 1
+    dl = dl * gr[:, None]
+    half = 2.0 ** -23 if h.dtype == torch.float32 else 2.0 ** -11
+    bdl = (gr.abs()[:, None] * p * (2 * e[:, None] + 8 * U) + dl.abs() * half
+           + gr.abs().max() * 2.0 ** -38)
+
+    def product(a, ba, c):
+        n = a.shape[1]
+        extra = 2.0 ** -23 * (a.abs() @ c.abs())  # planes of c, the scale's rounding
+        return a @ c, ba @ c.abs() + ((n / 16 + 24) * U) * (a.abs() @ c.abs()) + extra
+
+    dh, bh = product(dl, bdl, W)
+    dw, bw = product(dl.t().contiguous(), bdl.t().contiguous(), H)
+    db, bb = dl.sum(0), bdl.sum(0) + (len(t) / 8 + 24) * U * dl.abs().sum(0)
+    return loss, bl, (dh, dw, db), (bh, bw, bb)
+
+
+def close(got, want, bound, dtype):
+    step = torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal * \
+        torch.finfo(dtype).eps / 2
+    assert not torch.isnan(got).any()
+    over = ((got.double() - want).abs() - bound - step).max().item()
+    assert over <= 0, f"over the bound by {over:.3g}"
+
+
+def check(h, w, b, t, reduction, piece=0, seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    grad = (torch.randn(len(t), generator=g, device="cuda") if reduction == "none"
+            else torch.tensor(-1.7, device="cuda"))
+    leaves = [x.detach().requires_grad_() for x in (h, w, b) if x is not None]
+    loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2] if b is not None else None,
+                                reduction=reduction, vocab_piece=piece)
+    assert loss.dtype == torch.float32
+    got = torch.autograd.grad(loss, leaves, grad)
+    want, bl, grads, bounds = reference(h, w, b, t, reduction, grad)
+    close(loss, want, bl, torch.float32)
+    for x, e, bound, leaf in zip(got, grads, bounds, leaves):
+        assert x.shape == leaf.shape and x.dtype == leaf.dtype
+        close(x, e, bound, leaf.dtype)
+    return loss, got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,dim,vocab,bias,reduction,ignored,piece", [
+    (1, 64, 1000, True, "mean", 0, 0), (1, 1, 1, False, "sum", 0, 0), (2, 3, 5, True, "none", 0, 2),
+    (7, 33, 517, True, "none", 0.3, 0), (9, 64, 200, False, "mean", 0, 0),
+    (33, 64, 300, False, "sum", 0.3, 100), (130, 129, 2001, True, "none", 0.3, 500),
+    (257, 128, 4097, False, "mean", 0.1, 0), (600, 256, 5003, True, "mean", 0.3, 2048),
+    (1030, 72, 9000, True, "mean", 0.1, 9000)])
+def test_loss_and_gradients(tokens, dim, vocab, bias, reduction, ignored, piece, dtype):
+    check(*make(tokens, dim, vocab, dtype, bias, ignored, seed=tokens), reduction, piece)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_tiles(dtype):
+    check(*make(2100, 320, 20011, dtype, True, 0.2), "mean", 7001)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides(dtype):
+    h, w, b, t = make(40, 64, 333, dtype, True, 0.2, seed=4)
+    wide = torch.randn(40, 200, device="cuda").to(dtype)
+    wide[:, 3:67] = h
+    turned = w.t().contiguous().t()
+    tt = torch.stack([t, t], 1)[:, 0]
+    a = check(h, w, b, t, "mean")
+    c = check(wide[:, 3:67], turned, b, tt, "mean")
+    assert torch.equal(a[0], c[0])
+    check(h[:1].expand(40, 64), w, b, t, "sum")  # one row seen forty times
+
+
+def test_batched_hidden_and_views():
+    h, w, _, t = make(60, 32, 100, torch.float32, False, 0.1, seed=5)
+    leaf = h.view(3, 20, 32).detach().requires_grad_()
+    loss = linear_cross_entropy(leaf, w, t.view(3, 20), reduction="none")
+    assert loss.shape == (3, 20)
+    flat = linear_cross_entropy(h, w, t, reduction="none")
+    assert torch.equal(loss.view(-1), flat)
+    assert torch.autograd.grad(loss.sum(), leaf)[0].shape == leaf.shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ignored_rows_hold_anything(dtype):
+    h, w, b, t = make(70, 64, 400, dtype, True, 0.4, seed=6)
+    base = check(h, w, b, t, "mean")
+    dirty = h.clone()
+    rows = torch.nonzero(t == -100).view(-1)
+    dirty[rows[0]], dirty[rows[1]], dirty[rows[2:]] = float("nan"), float("inf"), 0.0
+    other = [x.detach().requires_grad_() for x in (dirty, w, b)]
+    loss = linear_cross_entropy(other[0], other[1], t, other[2])
+    grads = torch.autograd.grad(loss, other, torch.tensor(-1.7, device="cuda"))
+    if dtype == torch.float32:  # its scale is taken over all rows, inf among them
+        assert torch.isfinite(loss)
+    else:
+        assert torch.equal(loss, base[0])
+    assert (grads[0][rows] == 0).all()
+    for g in grads:
+        assert torch.isfinite(g.float()).all()
+
+
+def test_all_ignored():
+    h, w, b, t = make(5, 32, 50, torch.float32, True, 0)
+    t.fill_(-100)
+    leaves = [x.requires_grad_() for x in (h, w, b)]
+    loss = linear_cross_entropy(h, w, t, b)
+    assert torch.isnan(loss)
+    for g in torch.autograd.grad(loss, leaves):
+        assert (g == 0).all()
+    assert linear_cross_entropy(h, w, t, b, reduction="sum") == 0
+    assert (linear_cross_entropy(h, w, t, b, reduction="none") == 0).all()
+
+
+def test_target_out_of_range_is_nan_and_stays_in_its_row():
+    h, w, _, t = make(6, 32, 50, torch.float32, False, 0, seed=7)
+    t[2], t[4] = 50, -3
+    leaf = h.detach().requires_grad_()
+    rows = linear_cross_entropy(leaf, w, t, reduction="none")
+    bad = torch.tensor([False, False, True, False, True, False], device="cuda")
+    assert torch.equal(torch.isnan(rows), bad)
+    g = torch.autograd.grad(rows.sum(), leaf)[0]
+    assert torch.equal(torch.isnan(g).all(1), bad) and torch.equal(torch.isnan(g).any(1), bad)
+
+
+def test_other_ignore_index_and_masked_vocabulary():
+    h, w, b, t = make(50, 64, 300, torch.float32, True, 0, seed=8)
+    b[200:] = float("-inf")  # entries that can not be
+    t = t % 200
+    t[::7] = 5
+    want = F.cross_entropy((h.double() @ w.double().t() + b.double()), t, ignore_index=5)
+    leaves = [x.detach().requires_grad_() for x in (h, w)]
+    got = linear_cross_entropy(*leaves, t, b, ignore_index=5)
+    assert abs(got.item() - want.item()) <= 64 * U * 20
+    dw = torch.autograd.grad(got, leaves)[1]
+    assert (dw[200:] == 0).all() and torch.isfinite(dw).all()
+    low = b.clone()
+    low[200:] = torch.finfo(torch.float32).min  # the type's lowest value masks as well
+    assert torch.equal(linear_cross_entropy(h, w, t, low, ignore_index=5), got)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 1.0, 2.0 ** 40])
+def test_float32_range(scale):
+    """Float32 inputs of any size: the planes' exponents follow the largest magnitude."""
+    h, w, _, t = make(40, 96, 500, torch.float32, False, 0, seed=9)
+    a = check(h, w, None, t, "mean")
+    leaves = [(h * scale).requires_grad_(), (w / scale).requires_grad_()]
+    loss = linear_cross_entropy(*leaves, t)
+    assert torch.equal(loss, a[0])
+    dh = torch.autograd.grad(loss, leaves, torch.tensor(-1.7, device="cuda"))[0]
+    assert torch.equal(dh * scale, a[1][0])
+
+
+def test_selected_gradients():
+    h, w, b, t = make(70, 64, 400, torch.bfloat16, True, 0.2, seed=10)
+    _, full = check(h, w, b, t, "mean")
+    for pick in range(3):
+        leaves = [x.detach().requires_grad_(i == pick) for i, x in enumerate((h, w, b))]
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+        got = torch.autograd.grad(loss, leaves[pick], torch.tensor(-1.7, device="cuda"))[0]
+        assert torch.equal(got, full[pick])
+
+
+def test_pieces_agree():
+    h, w, b, t = make(300, 64, 3000, torch.bfloat16, True, 0.2, seed=11)
+    _, one = check(h, w, b, t, "mean", 3000)
+    for piece in (1, 255, 1024):
+        if piece == 1:
+            part = check(h, w[:9], b[:9], torch.where(t < 0, t, t % 9), "sum", 1)
+            assert torch.isfinite(part[0])
+            continue
+        _, got = check(h, w, b, t, "mean", piece)
+        assert torch.equal(got[1], one[1]) and torch.equal(got[2], one[2])
+
+
+def test_half_bias_and_module():
+    m = LinearCrossEntropy(64, 300, device="cuda", dtype=torch.bfloat16)
+    lin = torch.nn.Linear(64, 300, device="cuda", dtype=torch.bfloat16)
+    m.load_state_dict(lin.state_dict())
+    h, _, _, t = make(20, 64, 300, torch.bfloat16, False, 0.1, seed=12)
+    loss = m(h, t)
+    want, bl, _, _ = reference(h, lin.weight.detach(), lin.bias.detach().float(), t, "mean",
+                               torch.tensor(1.0, device="cuda"))
+    close(loss, want, bl, torch.float32)
+    loss.backward()
+    assert m.bias.grad.dtype == torch.bfloat16 and m.weight.grad.shape == (300, 64)
+
+
+def test_directional_difference():
+    h, w, b, t = make(12, 24, 70, torch.float32, True, 0.2, seed=13)
+    leaves = [x.detach().requires_grad_() for x in (h, w, b)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="sum")
+    grads = torch.autograd.grad(loss, leaves)
+    for i, grad in enumerate(grads):
+        d = torch.randn_like(leaves[i])
+        d /= d.norm()
+        s = 2.0 ** -6
+        f = [linear_cross_entropy(*[x + (s * k * d if j == i else 0) for j, x in
+                                    enumerate(leaves[:2])], t,
+                                  leaves[2] + (s * k * d if i == 2 else 0), reduction="sum").item()
+             for k in (1, -1)]
+        # rounding of two losses of ~60 over 2 s, and s^2 / 6 of a third derivative below 12 * |h|^3
+        assert abs((f[0] - f[1]) / (2 * s) - (grad * d).sum().item()) <= \
+            64 * 60 * U / s + s * s / 6 * 12 * h.norm(dim=1).max().item() ** 3 * 0.1
+
+
+def test_graph_replays():
+    h, w, b, t = make(300, 128, 5000, torch.bfloat16, True, 0.2, seed=14)
+    leaves = [x.detach().clone().requires_grad_() for x in (h, w, b)]
+
+    def call():
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], vocab_piece=2048)
+        return (loss.detach(), *torch.autograd.grad(loss, leaves))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for k in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(h * (k + 1) / 2)
+        t.copy_(t.roll(1))
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = call()
+        for _, out in graphs:
+            assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+def test_results_repeat():
+    runs = [check(*make(515, 192, 9001, torch.float32, True, 0.2, seed=15), "mean", 4000)
+            for _ in range(3)]
+    for loss, grads in runs[1:]:
+        assert torch.equal(loss, runs[0][0])
+        assert all(torch.equal(a, c) for a, c in zip(grads, runs[0][1]))
+
+
+def test_empty():
+    h = torch.empty(0, 16, device="cuda", requires_grad=True)
+    w = torch.randn(30, 16, device="cuda", requires_grad=True)
+    t = torch.empty(0, dtype=torch.int64, device="cuda")
+    assert torch.isnan(linear_cross_entropy(h, w, t))
+    total = linear_cross_entropy(h, w, t, reduction="sum")
+    total.backward()
+    assert total == 0 and (w.grad == 0).all()
+    assert linear_cross_entropy(h, w, t, reduction="none").shape == (0,)
