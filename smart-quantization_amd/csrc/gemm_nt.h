@@ -19,7 +19,11 @@
 // variables: the compiler then knows that a read of one does not wait for the loads into another.
 //
 // What bounds it: a wave's 128 x 64 part reads (128 + 64) * 16 * 2 bytes of LDS per 128 x 64 x 16
-// product, 75 % of the LDS rate at the full MFMA rate; 64 x 64 parts need 100 %.
+// product, 75 % of the LDS rate at the full MFMA rate; 64 x 64 parts need 100 %. Measured (fp16,
+// random data): 8192 x 8192 x 4096 at 1100 TFLOP/s with 256 x 256 tiles and 950 with 128 x 128 (1040
+// and 900 before the reads were spread between the MFMAs); two planes, which read LDS half as often
+// per MFMA, 4096^3 at 430 (1290 of single products). A large library product reaches 1250-1300 here.
+// Four waves of 128 x 128 parts measured 930, bands of 8 and 16 tile rows 1-3 % less than 4.
 #pragma once
 
 #include "smq_common.h"
@@ -162,7 +166,7 @@ __device__ __forceinline__ void store_n(const Mat& d, int64_t b, int64_t r, int6
 // XCD get consecutive tiles, in bands of kBand tile rows, so the tiles an XCD has in flight share
 // their rows of A and B. `tri`: only the tiles on and above the diagonal of a square tile grid (a
 // symmetric product; the epilogue writes the mirrored part).
-constexpr int kBand = 8;
+constexpr int kBand = 4;
 __device__ __forceinline__ void pick_tile(int tm, int tn, int tri, int& im, int& in) {
   const int total = tri ? tm * (tm + 1) / 2 : tm * tn;
   const int id = blockIdx.x, x = id & 7, q = total >> 3, rem = total & 7;
@@ -266,36 +270,56 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Oper
 #pragma unroll
       for (int j = 0; j < TN; j++) acc[i][j] = Frag<H>::mma(fb[j], fa[i], acc[i][j]);
   };
-  frag fa0[TM], fb0[TN], fa1[TM], fb1[TN];
+  frag fa0[TM], fb0[TN], fa1[TM], fb1[TN], fa2[TM], fb2[TN];
+  // One LDS read behind each MFMA: left to itself the compiler sinks a read to just before its use
+  // and waits there.
+  auto mix = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM + TN; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
   // One k tile in (la, lb), whose first fragments are in f0; (ma, mb) is the next tile's buffer.
   auto tile = [&](H* la, H* lb, H* ma, H* mb, int t) __attribute__((always_inline)) {
     if constexpr (!SPLIT) {
       read(la, lb, 1, fa1, fb1);
       mma(fa0, fb0);
+      mix();
       read(la, lb, 2, fa0, fb0);
       mma(fa1, fb1);
+      mix();
       read(la, lb, 3, fa1, fb1);
       mma(fa0, fb0);
+      mix();
     } else {
       // chunks 0-3 are hi, 4-7 are lo
       read(la, lb, 2, fa1, fb1);
       mma(fa0, fb0);
+      mix();
       mma(fa0, fb1);
+      read(la, lb, 1, fa2, fb2);
       mma(fa1, fb0);
-      read(la, lb, 1, fa0, fb0);
+      mix();
       read(la, lb, 3, fa1, fb1);
-      mma(fa0, fb0);
+      mma(fa2, fb2);
+      mix();
     }
     // every wave has its fragments of this tile, and the next tile has landed
+    __builtin_amdgcn_s_setprio(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     if (t + 2 < nk) fetch(la, lb, t + 2);
+    __builtin_amdgcn_s_setprio(1);
+    read(ma, mb, 0, fa0, fb0);
     if constexpr (!SPLIT) {
-      read(ma, mb, 0, fa0, fb0);
       mma(fa1, fb1);
+      mix();
     } else {
-      mma(fa0, fb1);
-      mma(fa1, fb0);
-      read(ma, mb, 0, fa0, fb0);
+      mma(fa2, fb1);
+      mma(fa1, fb2);
+      mix();
     }
   };
   if (nk > 0) {

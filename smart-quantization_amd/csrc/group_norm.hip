@@ -41,10 +41,20 @@ __device__ __forceinline__ void put(typename Pack<T, V>::type& v, int i, float f
   else v[i] = (T)f;
 }
 
+// 1 / (1 + exp(-z)) from the hardware's exp2 and reciprocal, each within 1 ulp: the product with log2(e) is
+// carried in two parts, so the result is within 4 ulp for every z (|z| is cut at 126 / log2(e), where
+// the result is 0 or 1 to the last bit); a library expf and an IEEE division cost three times the kernel.
+__device__ __forceinline__ float sigmoid(float z) {
+  const float x = z < -87.0f ? 87.0f : z > 87.0f ? -87.0f : -z;
+  const float t = x * 1.44269504f;
+  const float e = fmaf(x, 1.44269504f, -t) + x * 1.92596303e-8f;
+  const float p = __builtin_amdgcn_exp2f(t);
+  return __builtin_amdgcn_rcpf(1.0f + fmaf(p, e * 0.693147181f, p));
+}
 __device__ __forceinline__ float act_of(int act, float z) {
   switch (act) {
     case SMQ_ACT_RELU: return z < 0.0f ? 0.0f : z;
-    case SMQ_ACT_SILU: return z / (1.0f + expf(-z));
+    case SMQ_ACT_SILU: return z * sigmoid(z);
     case SMQ_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.707106781f));
     default: return z;
   }
@@ -53,11 +63,14 @@ __device__ __forceinline__ float slope_of(int act, float z) {
   switch (act) {
     case SMQ_ACT_RELU: return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
     case SMQ_ACT_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
+      const float s = sigmoid(z);
       return s * (1.0f + z * (1.0f - s));
     }
-    case SMQ_ACT_GELU:
-      return 0.5f * (1.0f + erff(z * 0.707106781f)) + z * expf(-0.5f * z * z) * 0.398942280f;
+    case SMQ_ACT_GELU: {
+      const float x = -0.5f * z * z;
+      const float p = __builtin_amdgcn_exp2f((x < -87.0f ? -87.0f : x) * 1.44269504f);
+      return 0.5f * (1.0f + erff(z * 0.707106781f)) + z * p * 0.398942280f;
+    }
     default: return 1.0f;
   }
 }

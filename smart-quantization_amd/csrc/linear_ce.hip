@@ -24,13 +24,12 @@ using namespace gemm;
 constexpr float kDlScale = 16384.0f;
 constexpr size_t kPieceBytes = size_t(1) << 30;  // default limit of a backward piece's buffers
 
-// Words the forward leaves for the backward (device): exponents of the two operands, the count of
-// rows that take part.
+// What a pass keeps on the device; the count is what the forward leaves for the backward.
 struct Head {
   int exp_h, exp_w;  // power-of-two exponents of the fp16 operands made of the inputs
   int exp_out;       // -(exp_h + exp_w)
   int pad;
-  double count;
+  double count;      // rows that take part
   float scale_dh, scale_dw, scale_db;  // backward: the factors of the gradients
 };
 
@@ -95,17 +94,18 @@ __device__ __forceinline__ float exp_near(float x) {
 }
 
 // ---- forward epilogue ---------------------------------------------------------------------------
-// Per row and per wave's block of columns: the maximum and the sum of exp(l - maximum); the target's
-// logit goes straight out (one lane of the grid owns it).
+// Per row and per tile's columns: the maximum and the sum of exp(l - maximum), joined over the tile's
+// waves in LDS; the target's logit goes straight out (one lane of the grid owns it).
 struct SoftmaxEpi {
   const int* exponent;
   const float* bias;
   const int64_t* target;
-  float2* part;  // [blocks][rows]
+  float2* part;  // [tiles][rows]
   float* picked;
   template <int BM, int BN, int WM, int WN, int TM, int TN>
   __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float*, int m0, int n0, int M, int N,
-                                         int, int in, int, int wn, int lane, int64_t) const {
+                                         int im, int in, int wm, int wn, int lane, int64_t) const {
+    __shared__ float2 joint[WN][BM];
     const int ex = exponent ? *exponent : 0;
     const float ninf = -__builtin_inff();
 #pragma unroll
@@ -142,37 +142,154 @@ struct SoftmaxEpi {
             picked[m] = acc[i][j][r];
         }
       sum += __shfl_xor(sum, 32, 64);
-      if (lane < 32 && m < M) part[(int64_t)(in * WN + wn) * M + m] = make_float2(top, sum);
+      if (lane < 32) joint[wn][wm * TM * 32 + i * 32 + lane] = make_float2(top, sum);
+    }
+    __syncthreads();
+    const int row = threadIdx.x;
+    if (row < BM && im * BM + row < M) {
+      float2 a = joint[0][row];
+#pragma unroll
+      for (int k = 1; k < WN; k++) {
+        const float2 b = joint[k][row];
+        const float t = fmaxf(a.x, b.x), at = t == ninf ? 0.0f : t;
+        a.y = a.y * exp_near(a.x - at) + b.y * exp_near(b.x - at);
+        a.x = t;
+      }
+      part[(int64_t)in * M + im * BM + row] = a;
     }
   }
 };
 
+// ---- forward of a few tokens ---------------------------------------------------------------------
+// Bound by the one read of the weight: each wave takes kRows vocabulary entries at a time straight from
+// memory in their own type (no fp16 planes are made), 16 bytes a lane, against up to NT rows of hidden
+// kept in LDS as fp32; a token's (maximum, sum) runs along in registers.
+constexpr int kRows = 4;
+template <typename T, int NT>
+__global__ __launch_bounds__(256) void few_kernel(const T* h, int64_t ldh, const T* w, int64_t ldw,
+                                                  int tokens, int dim, int vocab, const float* bias,
+                                                  const int64_t* target, float2* part, float* picked) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(V)));
+  extern __shared__ float hs[];  // [NT][dim]
+  __shared__ float2 joint[4][NT];
+  for (int i = threadIdx.x; i < NT * dim; i += 256) {
+    const int t = i / dim;
+    hs[i] = t < tokens ? (float)h[(int64_t)t * ldh + (i - t * dim)] : 0.0f;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float ninf = -__builtin_inff();
+  float top[NT], sum[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) top[t] = ninf, sum[t] = 0.0f;
+  for (int v0 = (blockIdx.x * 4 + wave) * kRows; v0 < vocab; v0 += gridDim.x * 4 * kRows) {
+    const T* p[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) p[r] = w + (int64_t)(v0 + r < vocab ? v0 + r : vocab - 1) * ldw;
+    float acc[kRows][NT];
+#pragma unroll
+    for (int r = 0; r < kRows; r++)
+#pragma unroll
+      for (int t = 0; t < NT; t++) acc[r][t] = 0.0f;
+#pragma unroll 2
+    for (int k = lane * V; k < dim; k += 64 * V) {
+      vec x[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; r++) x[r] = *reinterpret_cast<const vec*>(p[r] + k);
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float y[V];
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(hs + t * dim + k + i);
+          y[i] = q.x, y[i + 1] = q.y, y[i + 2] = q.z, y[i + 3] = q.w;
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; r++)
+#pragma unroll
+          for (int i = 0; i < V; i++) acc[r][t] = fmaf((float)x[r][i], y[i], acc[r][t]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      const int v = v0 + r;
+      const float b = bias && v < vocab ? bias[v] : 0.0f;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float s = acc[r][t];
+        s += dpp_f32<kDppXor1>(s);
+        s += dpp_f32<kDppXor2>(s);
+        s += dpp_f32<kDppHalfMirror>(s);
+        s += dpp_f32<kDppMirror>(s);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        acc[r][t] = v < vocab ? s + b : ninf;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      float m = top[t];
+#pragma unroll
+      for (int r = 0; r < kRows; r++) m = fmaxf(m, acc[r][t]);
+      const float at = m == ninf ? 0.0f : m;
+      float s = sum[t] * exp_near(top[t] - at);
+#pragma unroll
+      for (int r = 0; r < kRows; r++) s += exp_near(acc[r][t] - at);
+      top[t] = m, sum[t] = s;
+      const int64_t y = t < tokens ? target[t] : -1;
+      if (lane == 0 && y >= v0 && y < v0 + kRows && y < vocab) {
+#pragma unroll
+        for (int r = 0; r < kRows; r++)
+          if (y == v0 + r) picked[t] = acc[r][t];
+      }
+    }
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int t = 0; t < NT; t++) joint[wave][t] = make_float2(top[t], sum[t]);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < tokens) {
+    const int t = threadIdx.x;
+    float m = ninf, s = 0.0f;
+    for (int k = 0; k < 4; k++) m = fmaxf(m, joint[k][t].x);
+    const float at = m == ninf ? 0.0f : m;
+    for (int k = 0; k < 4; k++) s += joint[k][t].y * exp_near(joint[k][t].x - at);
+    part[(int64_t)blockIdx.x * tokens + t] = make_float2(m, s);
+  }
+}
+
 // ---- joining the blocks -------------------------------------------------------------------------
-// 64 rows a workgroup, 4 waves share the blocks; the joined statistics of a row by thread. A target
-// that is neither ignored nor in [0, vocab) gives NaN (nothing is read for it).
-__global__ __launch_bounds__(256) void join_kernel(const float2* part, int blocks, int rows,
+// R rows a workgroup (a power of two up to 16), 256 / R threads share a row's tiles. A target that is
+// neither ignored nor in [0, vocab) gives NaN (nothing is read for it).
+__global__ __launch_bounds__(256) void join_kernel(const float2* part, int blocks, int rows, int R,
                                                    const int64_t* target, int64_t ignore,
                                                    int64_t vocab, const float* picked, float* lse,
                                                    float* row_loss) {
-  const int m = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  float top = -__builtin_inff(), sum = 0.0f;
+  const int r = threadIdx.x & (R - 1), m = blockIdx.x * R + r;
+  const float ninf = -__builtin_inff();
+  float top = ninf, sum = 0.0f;
   if (m < rows)
-    for (int k = w; k < blocks; k += 4) {
+    for (int k = threadIdx.x / R; k < blocks; k += 256 / R) {
       const float2 p = part[(int64_t)k * rows + m];
-      const float t = fmaxf(top, p.x), at = t == -__builtin_inff() ? 0.0f : t;
-      sum = sum * expf(top - at) + p.y * expf(p.x - at);
+      const float t = fmaxf(top, p.x), at = t == ninf ? 0.0f : t;
+      sum = sum * exp_near(top - at) + p.y * exp_near(p.x - at);
       top = t;
     }
-  __shared__ float st[4][64], ss[4][64];
-  st[w][threadIdx.x & 63] = top, ss[w][threadIdx.x & 63] = sum;
-  __syncthreads();
-  if (w || m >= rows) return;
-  const int x = threadIdx.x;
-  const float t = fmaxf(fmaxf(st[0][x], st[1][x]), fmaxf(st[2][x], st[3][x]));
-  const float at = t == -__builtin_inff() ? 0.0f : t;
-  float s = 0.0f;
-  for (int k = 0; k < 4; k++) s += ss[k][x] * expf(st[k][x] - at);
-  const float l = at + logf(s);
+  __shared__ float2 sh[256];
+  sh[threadIdx.x] = make_float2(top, sum);
+  for (int h = 128; h >= R; h >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < h) {
+      const float2 a = sh[threadIdx.x], b = sh[threadIdx.x + h];
+      const float t = fmaxf(a.x, b.x), at = t == ninf ? 0.0f : t;
+      sh[threadIdx.x] = make_float2(t, a.y * exp_near(a.x - at) + b.y * exp_near(b.x - at));
+    }
+  }
+  if (threadIdx.x >= R || m >= rows) return;
+  const float2 a = sh[threadIdx.x];
+  const float l = (a.x == ninf ? 0.0f : a.x) + logf(a.y);
   lse[m] = l;
   const int64_t y = target[m];
   row_loss[m] = y == ignore ? 0.0f : y >= 0 && y < vocab ? l - picked[m] : __builtin_nanf("");
@@ -181,7 +298,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float2* part, int block
 // One workgroup: the loss over rows (fp64 sums in a fixed order) and the count of rows taking part.
 __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const int64_t* target,
                                                     int64_t ignore, int rows, int reduction,
-                                                    int planes, float* loss, Head* head) {
+                                                    float* loss, Head* head) {
   double s = 0.0, c = 0.0;
   for (int m = threadIdx.x; m < rows; m += 1024) {
     s += (double)row_loss[m];
@@ -196,7 +313,6 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
     s = c = 0.0;
     for (int k = 0; k < 16; k++) s += a[k], c += b[k];
     head->count = c;
-    if (!planes) head->exp_h = head->exp_w = head->exp_out = 0;
     if (reduction == SMQ_REDUCE_MEAN) *loss = (float)(s / c);
     if (reduction == SMQ_REDUCE_SUM) *loss = (float)s;
   }
@@ -395,40 +511,77 @@ int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t
   return SMQ_OK;
 }
 
-struct ForwardPlan {
-  size_t bytes;
-  int rc;
-};
-// Lays the workspace out; enqueues when `run`.
-ForwardPlan forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,
+// Few tokens: as many as the lanes' multiply-adds keep up with the read of the weight (a 4-byte weight
+// leaves time for 16, a 2-byte one for 4), whole 16-byte vectors, hidden within 64 KiB of LDS.
+int few_tokens(const void* h, const void* w, int64_t ldw, const Shape& s) {
+  const int v = (int)(16 / s.size());
+  const int nt = s.tokens <= 1 ? 1 : s.tokens <= 2 ? 2 : s.tokens <= 4 ? 4 : s.tokens <= 8 ? 8 : 16;
+  if (s.tokens > (s.split() ? 16 : 4) || s.dim % v || ldw % v || (reinterpret_cast<uintptr_t>(w) & 15) ||
+      nt * s.dim * 4 > 65536 - 1024)
+    return 0;
+  return nt;
+}
+int few_grid(const Shape& s) {
+  const int64_t g = (s.vocab + 4 * kRows - 1) / (4 * kRows);
+  return (int)(g < 2048 ? g : 2048);
+}
+template <typename T>
+void launch_few(int nt, const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,
+                const float* bias, const int64_t* target, float2* part, float* picked, hipStream_t st) {
+  const dim3 grid(few_grid(s)), block(256);
+  const size_t lds = (size_t)nt * s.dim * 4;
+  const T* a = reinterpret_cast<const T*>(h);
+  const T* b = reinterpret_cast<const T*>(w);
+  const int n = (int)s.tokens, d = (int)s.dim, v = (int)s.vocab;
+  if (nt == 1) hipLaunchKernelGGL((few_kernel<T, 1>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
+  else if (nt == 2) hipLaunchKernelGGL((few_kernel<T, 2>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
+  else if (nt == 4) hipLaunchKernelGGL((few_kernel<T, 4>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
+  else if constexpr (sizeof(T) == 4) {
+    if (nt == 8) hipLaunchKernelGGL((few_kernel<T, 8>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
+    else hipLaunchKernelGGL((few_kernel<T, 16>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
+  }
+}
+
+// Lays the workspace out; enqueues when `run`. Returns the bytes used.
+size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,
                     const int64_t* target, const float* bias, int64_t ignore, int reduction,
                     float* loss, float* lse, Head* head, void* ws, bool run, hipStream_t st) {
   Arena a(ws);
   const int tile = choose_tile(s.tokens, s.vocab, 1, 0);
   const TileShape ts = shape_of(tile);
   const int64_t tn = (s.vocab + ts.bn - 1) / ts.bn;
-  const int blocks = (int)(tn * ts.wn);
+  const int few = few_tokens(h, w, ldw, s);
+  const int blocks = few ? few_grid(s) : (int)tn;
   float2* part = a.take<float2>((size_t)blocks * s.tokens);
   float* picked = a.take<float>(s.tokens);
   float* rows = a.take<float>(s.tokens);
   const int* exponent = nullptr;
   const int *eh = nullptr, *ew = nullptr;
-  if (s.split()) {
+  if (s.split() && !few) {
     float* top = a.take<float>(2 * kMaxParts);
     exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
     if (run) exponents((const float*)h, ldh, (const float*)w, ldw, s, top, head, st);
   }
-  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, run, st);
-  const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, run, st);
-  if (run) {
+  if (few) {
+    if (run) {
+      if (s.dtype == SMQ_DTYPE_F32) launch_few<float>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
+      else if (s.dtype == SMQ_DTYPE_F16) launch_few<_Float16>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
+      else launch_few<__bf16>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
+    }
+  } else {
+    const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, run, st);
+    const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, run, st);
     const SoftmaxEpi e = {exponent, bias, target, part, picked};
-    product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + 63) / 64)), dim3(256), 0, st, part,
-                       blocks, (int)s.tokens, target, ignore, s.vocab, picked, lse, rows);
-    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
-                       reduction, s.split() ? 1 : 0, loss, head);
+    if (run) product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
   }
-  return {a.used, SMQ_OK};
+  if (run) {
+    const int per = s.tokens >= 2048 ? 16 : s.tokens >= 256 ? 4 : 1;
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + per - 1) / per)), dim3(256), 0, st, part,
+                       blocks, (int)s.tokens, per, target, ignore, s.vocab, picked, lse, rows);
+    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
+                       reduction, loss, head);
+  }
+  return a.used;
 }
 
 // Shares of the k range of dh: enough workgroups to fill the chip where dh itself has few tiles.
@@ -457,15 +610,15 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   if (s.piece <= 0) s.piece = default_piece(s);
   if (s.piece > s.vocab) s.piece = s.vocab;
   const int64_t pieces = (s.vocab + s.piece - 1) / s.piece;
-  const int* exponent = sp ? &head->exp_out : nullptr;
   float* g = a.take<float>(s.tokens);
   Head* fac = a.take<Head>(1);
-  const Head* planes = sp ? head : nullptr;
-  if (s.dtype == SMQ_DTYPE_BF16) {
+  const Head* planes = s.dtype == SMQ_DTYPE_F16 ? nullptr : fac;
+  if (planes) {
     float* top = a.take<float>(2 * kMaxParts);
-    planes = fac;
-    if (run) exponents((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, fac, st);
+    if (run && sp) exponents((const float*)h, ldh, (const float*)w, ldw, s, top, fac, st);
+    else if (run) exponents((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, fac, st);
   }
+  const int* exponent = sp ? &fac->exp_out : nullptr;
   const int* eh = planes ? &planes->exp_h : nullptr;
   const int* ew = planes ? &planes->exp_w : nullptr;
   if (run)
@@ -555,7 +708,7 @@ size_t smq_linear_ce_workspace_bytes(const void* hidden, int64_t hidden_ld, cons
   Head* head = nullptr;
   if (!grad_flags)
     return forward(hidden, hidden_ld, weight, weight_ld, s, nullptr, nullptr, 0, 0, nullptr, nullptr,
-                   head, nullptr, false, nullptr).bytes + 256;
+                   head, nullptr, false, nullptr) + 256;
   char mark[1];
   return backward(hidden, hidden_ld, weight, weight_ld, s, nullptr, nullptr, 0, 0, nullptr, head,
                   nullptr, grad_flags & SMQ_CE_GRAD_HIDDEN ? mark : nullptr,
