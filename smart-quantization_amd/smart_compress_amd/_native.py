@@ -476,6 +476,22 @@ def torch_fast():
     return _torch_fast
 
 
+_train_fast = None
+_train_fast_tried = False
+
+
+def train_fast():
+    """The at::Tensor-level binding of the training-step operators (csrc/trainfast.cpp), or None
+    (then their Python autograd Functions). SMQ_TORCHFAST=0 disables it too."""
+    global _train_fast, _train_fast_tried
+    if _train_fast_tried:
+        return _train_fast
+    if os.environ.get("SMQ_TORCHFAST", "1") != "0":
+        _train_fast = _load_binding("_smqtrain")
+    _train_fast_tried = True
+    return _train_fast
+
+
 def ws_getter(kind: str):
     """The workspace callback of the C hot paths: (device index, stream, nbytes) -> the
     (kind, device, stream) workspace of this table."""

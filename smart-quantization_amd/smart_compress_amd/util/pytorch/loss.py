@@ -144,9 +144,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         if bias is not None:
             empty = empty + 0.0 * bias.float().sum()
         return empty if reduction == "none" else getattr(empty, reduction)()
-    loss = _LinearCrossEntropy.apply(hidden.reshape(-1, hidden.shape[-1]), weight, bias,
-                                     target.reshape(-1), int(ignore_index), _REDUCTIONS[reduction],
-                                     int(vocab_piece))
+    fast = N.train_fast()
+    call = _LinearCrossEntropy.apply if fast is None else fast.linear_ce
+    loss = call(hidden.reshape(-1, hidden.shape[-1]), weight, bias, target.reshape(-1),
+                int(ignore_index), _REDUCTIONS[reduction], int(vocab_piece))
     return loss.view(target.shape) if reduction == "none" else loss
 
 

@@ -38,9 +38,12 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     if len(coefficients) != 3:
         raise ValueError(f"{who}: three coefficients expected, got {len(coefficients)}")
     x = update.detach()
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel() == 0:
-        return out
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    fast = N.train_fast()
+    if fast is not None:
+        return fast.orthogonalize(x, steps, *map(float, coefficients), float(eps))
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     x = x if x.dim() == 3 else x.unsqueeze(0)
     batch, rows, cols = x.shape
     if (cols > 1 and x.stride(2) != 1) or (rows > 1 and x.stride(1) < cols):

@@ -105,10 +105,11 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     value normalises to 0. No second derivative."""
     who = "group_norm_act"
     params = [t for t in (weight, bias) if t is not None]
+    device = x.device
     for t in (x, *params):
         N.require_device(t, who)
-        if t.device != x.device:
-            raise RuntimeError(f"{who}: tensors on {x.device} and {t.device}")
+        if t.device != device:
+            raise RuntimeError(f"{who}: tensors on {device} and {t.device}")
         if t.dtype not in N.DTYPE_CODES:
             raise TypeError(f"{who}: dtype {t.dtype} is not float32, float16 or bfloat16")
     if x.dim() < 2:
@@ -129,6 +130,10 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
         for t in params:
             out = out + 0.0 * t.sum().to(x.dtype)
         return out
+    fast = N.train_fast()
+    if fast is not None:
+        return fast.group_norm(x, weight, bias, int(num_groups), float(eps),
+                               _ACTIVATIONS[activation])
     return _GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps),
                                _ACTIVATIONS[activation])
 

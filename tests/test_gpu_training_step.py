@@ -123,3 +123,74 @@ def test_compressed_training_steps():
         for p, q in zip(ta, tb):
             assert torch.isfinite(p).all() and torch.equal(p, q)
     assert acts.stats()["saved_packed"] > 0
+
+
+def test_python_functions_equal_the_binding(monkeypatch):
+    """Without the C binding the Python autograd Functions give the same bits."""
+    from smart_compress_amd import _native as N
+    from smart_compress_amd.util.pytorch.loss import linear_cross_entropy
+    from smart_compress_amd.util.pytorch.muon import orthogonalize
+    from smart_compress_amd.util.pytorch.norm import group_norm_act
+
+    assert N.train_fast() is not None
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(2, 24, 9, 9, generator=g, device="cuda").to(torch.bfloat16)
+    w, b = (torch.randn(24, generator=g, device="cuda").half() for _ in range(2))
+    h = torch.randn(50, 40, generator=g, device="cuda")
+    v = torch.randn(300, 40, generator=g, device="cuda")
+    c = torch.randn(300, generator=g, device="cuda").to(torch.bfloat16)
+    t = torch.randint(0, 300, (50,), generator=g, device="cuda")
+    wide = torch.randn(3, 30, 70, generator=g, device="cuda")[:, :, 5:45]
+
+    def run():
+        out = []
+        leaves = [p.detach().requires_grad_() for p in (x, w, b)]
+        y = group_norm_act(leaves[0], 6, leaves[1], leaves[2], activation="gelu")
+        out += [y, *torch.autograd.grad(y.float().square().sum(), leaves)]
+        leaves = [p.detach().requires_grad_() for p in (h, v, c)]
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+        out += [loss, *torch.autograd.grad(loss.square().sum(), leaves)]
+        return out + [orthogonalize(wide), orthogonalize(wide[0].t())]
+
+    want = run()
+    monkeypatch.setattr(N, "_train_fast", None)
+    for a, e in zip(run(), want):
+        assert a.dtype == e.dtype and a.stride() == e.stride() and torch.equal(a, e)
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_no_second_derivative(binding, monkeypatch):
+    from smart_compress_amd import _native as N
+    from smart_compress_amd.util.pytorch.loss import linear_cross_entropy
+    from smart_compress_amd.util.pytorch.norm import group_norm_act
+
+    if not binding:
+        N.train_fast()
+        monkeypatch.setattr(N, "_train_fast", None)
+    x = torch.randn(2, 8, 4, 4, device="cuda", requires_grad=True)
+    h = torch.randn(5, 8, device="cuda", requires_grad=True)
+    t = torch.zeros(5, dtype=torch.int64, device="cuda")
+    for out, leaf in ((group_norm_act(x, 2).sum(), x),
+                      (linear_cross_entropy(h, torch.randn(9, 8, device="cuda"), t), h)):
+        with pytest.raises(RuntimeError):
+            grad = torch.autograd.grad(out, leaf, create_graph=True)[0]
+            torch.autograd.grad(grad.sum(), leaf)
+
+
+def test_autograd_keeps_only_what_is_said():
+    """The loss keeps a number a row, not the logits; the norm its input and two floats a group."""
+    from smart_compress_amd.util.pytorch.loss import linear_cross_entropy
+    from smart_compress_amd.util.pytorch.norm import group_norm_act
+
+    h = torch.randn(512, 64, device="cuda", requires_grad=True)
+    v = torch.randn(40000, 64, device="cuda", requires_grad=True)
+    t = torch.randint(0, 40000, (512,), device="cuda")
+    x = torch.randn(8, 64, 32, 32, device="cuda").contiguous(
+        memory_format=torch.channels_last).requires_grad_()
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    loss = linear_cross_entropy(h, v, t)
+    assert torch.cuda.memory_allocated() - base <= 16 * 1024
+    y = group_norm_act(x, 8, activation="silu")
+    assert torch.cuda.memory_allocated() - base <= 32 * 1024 + y.numel() * 4
+    del loss, y
