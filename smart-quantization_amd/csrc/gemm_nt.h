@@ -9,6 +9,8 @@
 //               Three products hi*hi + hi*lo + lo*hi per k step; the dropped lo*lo is below 2^-24 of
 //               the largest product. An fp32-class product at a third of the fp16 rate, where the
 //               fp32 MFMA runs at a sixteenth.
+//   twice       one plane in the layout of two, [32 x | 32 x] (kDup): against an operand of two planes
+//               the one-plane product gives (hi + lo) x.
 //
 // Kernel: a workgroup of WM x WN waves computes a BM x BN tile; a k tile of both operands (128 bytes
 // a row) goes from global memory straight into one of two LDS buffers (buffer_load ... lds, 16 bytes
@@ -61,7 +63,7 @@ struct Operand {
 };
 
 // Output / source formats of a matrix an epilogue reads or writes.
-enum Fmt : int { kNone = 0, kF32 = 1, kF16 = 2, kBF16 = 3, kSplit = 4 };
+enum Fmt : int { kNone = 0, kF32 = 1, kF16 = 2, kBF16 = 3, kSplit = 4, kDup = 5 };
 struct Mat {
   void* p;
   int64_t ld;
@@ -83,6 +85,10 @@ __device__ __forceinline__ float4 load4(const Mat& s, int64_t b, int64_t r, int6
     return make_float4((float)hi.x + (float)lo.x, (float)hi.y + (float)lo.y,
                        (float)hi.z + (float)lo.z, (float)hi.w + (float)lo.w);
   }
+  if (s.fmt == kDup) {
+    const h4 v = *reinterpret_cast<const h4*>(reinterpret_cast<const _Float16*>(s.p) + row + split_at(c));
+    return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w);
+  }
   if (s.fmt == kF16) {
     const h4 v = *reinterpret_cast<const h4*>(reinterpret_cast<const _Float16*>(s.p) + row + c);
     return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w);
@@ -100,6 +106,9 @@ __device__ __forceinline__ void store1(const Mat& d, int64_t row, int64_t c, flo
     const _Float16 hi = (_Float16)v;
     p[0] = hi;
     p[32] = (_Float16)(v - (float)hi);
+  } else if (d.fmt == kDup) {
+    _Float16* p = reinterpret_cast<_Float16*>(d.p) + row + split_at(c);
+    p[0] = p[32] = (_Float16)v;
   } else if (d.fmt == kF16) {
     reinterpret_cast<_Float16*>(d.p)[row + c] = (_Float16)v;
   } else if (d.fmt == kBF16) {
@@ -125,7 +134,7 @@ __device__ __forceinline__ void store_n(const Mat& d, int64_t b, int64_t r, int6
 #pragma unroll
   for (int i = 0; i < N; i++) w[i] = c + i < cols ? v[i] : 0.0f;
   const int size = d.fmt == kF32 ? 4 : 2, need = N * size < 16 ? N * size : 16;
-  const bool whole = c + N <= end && (d.fmt == kSplit ||
+  const bool whole = c + N <= end && (d.fmt == kSplit || d.fmt == kDup ||
                      ((reinterpret_cast<uintptr_t>(d.p) + (row + c) * size) & (need - 1)) == 0);
   if (!whole) {
     for (int i = 0; i < N; i++)
@@ -142,6 +151,13 @@ __device__ __forceinline__ void store_n(const Mat& d, int64_t b, int64_t r, int6
     _Float16* p = reinterpret_cast<_Float16*>(d.p) + row + split_at(c);
     *reinterpret_cast<hN*>(p) = hi;
     *reinterpret_cast<hN*>(p + 32) = lo;
+  } else if (d.fmt == kDup) {
+    hN h;
+#pragma unroll
+    for (int i = 0; i < N; i++) h[i] = (_Float16)w[i];
+    _Float16* p = reinterpret_cast<_Float16*>(d.p) + row + split_at(c);
+    *reinterpret_cast<hN*>(p) = h;
+    *reinterpret_cast<hN*>(p + 32) = h;
   } else if (d.fmt == kF16) {
     hN h;
 #pragma unroll
@@ -186,21 +202,17 @@ __device__ __forceinline__ void pick_tile(int tm, int tn, int tri, int& im, int&
   in = u / high;
 }
 
-template <typename H, int BM, int BN, int WM, int WN, bool SPLIT, typename Epi>
-__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Operand B, int kt,
-                                                                 int tm, int tn, int tri, Epi epi) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the buffer builtins' types do not exist in the host pass
+template <typename H, int BM, int BN, int WM, int WN, int STAGES, bool SPLIT, typename Epi>
+__device__ __forceinline__ void gemm_nt_body(const Operand& A, const Operand& B, int kt, int tm, int tn,
+                                             int tri, const Epi& epi, H* a0, H* b0, H* a1, H* b1, H* a2,
+                                             H* b2, H* a3, H* b3) {
   typedef typename Frag<H>::type frag;
   constexpr int kWaves = WM * WN;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
   constexpr int LA = BM / 8 / kWaves, LB = BN / 8 / kWaves;  // loads a wave issues per k tile
   static_assert(TM * WM * 32 == BM && TN * WN * 32 == BN, "tile");
   static_assert(LA * 8 * kWaves == BM && LB * 8 * kWaves == BN, "loads");
-  __shared__ __attribute__((aligned(1024))) H a0[BM * 64];
-  __shared__ __attribute__((aligned(1024))) H b0[BN * 64];
-  __shared__ __attribute__((aligned(1024))) H a1[BM * 64];
-  __shared__ __attribute__((aligned(1024))) H b1[BN * 64];
-
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -263,12 +275,33 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Oper
     for (int j = 0; j < TN; j++)
       fb[j] = *reinterpret_cast<const frag*>(lb + (wn * TN * 32 + j * 32 + fr) * 64 + at);
   };
+  // hi*lo and lo*hi in sums of their own: hi*hi then rounds a third as often (8e-8 instead of 1.4e-7 of
+  // a sum of 640 positive products). 256 x 256 tiles have no registers for them.
+  constexpr bool kApart = SPLIT && BM < 256;
+  f32x16 low[kApart ? TM : 1][kApart ? TN : 1];
+  if constexpr (kApart) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) low[i][j][r] = 0.0f;
+  }
   // operands swapped: a lane then holds runs of 4 consecutive n of one m
   auto mma = [&](const frag(&fa)[TM], const frag(&fb)[TN]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < TM; i++)
 #pragma unroll
       for (int j = 0; j < TN; j++) acc[i][j] = Frag<H>::mma(fb[j], fa[i], acc[i][j]);
+  };
+  auto cross = [&](const frag(&fa)[TM], const frag(&fb)[TN]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        if constexpr (kApart) low[i][j] = Frag<H>::mma(fb[j], fa[i], low[i][j]);
+        else acc[i][j] = Frag<H>::mma(fb[j], fa[i], acc[i][j]);
+      }
   };
   frag fa0[TM], fb0[TN], fa1[TM], fb1[TN], fa2[TM], fb2[TN];
   // One LDS read behind each MFMA: left to itself the compiler sinks a read to just before its use
@@ -279,6 +312,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Oper
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto landed = [&]() __attribute__((always_inline)) {
+    if constexpr (STAGES == 2)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * (LA + LB)) : "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
   // One k tile in (la, lb), whose first fragments are in f0; (ma, mb) is the next tile's buffer.
@@ -298,41 +338,68 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Oper
       read(la, lb, 2, fa1, fb1);
       mma(fa0, fb0);
       mix();
-      mma(fa0, fb1);
+      cross(fa0, fb1);
       read(la, lb, 1, fa2, fb2);
-      mma(fa1, fb0);
+      cross(fa1, fb0);
       mix();
       read(la, lb, 3, fa1, fb1);
       mma(fa2, fb2);
       mix();
     }
-    // every wave has its fragments of this tile, and the next tile has landed
+    // every wave has its fragments of this tile, and the next tile has landed (the ones behind it
+    // may still be on their way)
     __builtin_amdgcn_s_setprio(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    if (t + 2 < nk) fetch(la, lb, t + 2);
+    landed();
+    if constexpr (STAGES == 2) {
+      if (t + 2 < nk) fetch(la, lb, t + 2);
+    } else {  // always: `landed` counts the loads behind the next tile's
+      fetch(la, lb, t + STAGES < nk ? t + STAGES : nk - 1);
+    }
     __builtin_amdgcn_s_setprio(1);
     read(ma, mb, 0, fa0, fb0);
     if constexpr (!SPLIT) {
       mma(fa1, fb1);
       mix();
     } else {
-      mma(fa2, fb1);
-      mma(fa1, fb2);
+      cross(fa2, fb1);
+      cross(fa1, fb2);
       mix();
     }
   };
   if (nk > 0) {
+    // (a tile past the end is the last one again: the counts of loads in flight stay the same)
     fetch(a0, b0, 0);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (nk > 1) fetch(a1, b1, 1);
-    read(a0, b0, 0, fa0, fb0);
-    int t = 0;
-    for (; t + 1 < nk; t += 2) {
-      tile(a0, b0, a1, b1, t);
-      tile(a1, b1, a0, b0, t + 1);
+    fetch(a1, b1, nk > 1 ? 1 : 0);
+    if constexpr (STAGES == 4) {
+      fetch(a2, b2, nk > 2 ? 2 : 0);
+      fetch(a3, b3, nk > 3 ? 3 : 0);
     }
-    if (t < nk) tile(a0, b0, a1, b1, t);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * (LA + LB)) : "memory");
+    read(a0, b0, 0, fa0, fb0);
+    for (int t = 0;;) {
+      if constexpr (STAGES == 2) {
+        tile(a0, b0, a1, b1, t);
+        if (++t >= nk) break;
+        tile(a1, b1, a0, b0, t);
+        if (++t >= nk) break;
+      } else {
+        tile(a0, b0, a1, b1, t);
+        if (++t >= nk) break;
+        tile(a1, b1, a2, b2, t);
+        if (++t >= nk) break;
+        tile(a2, b2, a3, b3, t);
+        if (++t >= nk) break;
+        tile(a3, b3, a0, b0, t);
+        if (++t >= nk) break;
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads still in flight write the LDS
+  }
+  if constexpr (kApart) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] += low[i][j];
   }
   __syncthreads();  // the LDS buffers are free for the epilogue
 
@@ -352,8 +419,39 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Oper
   epi.template finish<BM, BN, WM, WN, TM, TN>(acc, stage, row_a + wm * TM * 32,
                                               row_b + wn * TN * 32, A.rows, B.rows, im, in, wm, wn,
                                               lane, batch);
+}
+#endif
+
+// The LDS buffers of each depth are variables of their own kernel: that is what the compiler tells
+// them apart by.
+#define SMQ_TILE_LDS(name, rows) __shared__ __attribute__((aligned(1024))) H name[(rows) * 64]
+template <typename H, int BM, int BN, int WM, int WN, bool SPLIT, typename Epi>
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_nt_kernel(Operand A, Operand B, int kt, int tm,
+                                                                 int tn, int tri, Epi epi) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  SMQ_TILE_LDS(a0, BM);
+  SMQ_TILE_LDS(b0, BN);
+  SMQ_TILE_LDS(a1, BM);
+  SMQ_TILE_LDS(b1, BN);
+  gemm_nt_body<H, BM, BN, WM, WN, 2, SPLIT>(A, B, kt, tm, tn, tri, epi, a0, b0, a1, b1, a0, b0, a1, b1);
 #endif
 }
+template <typename H, int BM, int BN, int WM, int WN, bool SPLIT, typename Epi>
+__global__ __launch_bounds__(WM* WN * 64, 1) void gemm_nt_deep_kernel(Operand A, Operand B, int kt,
+                                                                      int tm, int tn, int tri, Epi epi) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  SMQ_TILE_LDS(a0, BM);
+  SMQ_TILE_LDS(b0, BN);
+  SMQ_TILE_LDS(a1, BM);
+  SMQ_TILE_LDS(b1, BN);
+  SMQ_TILE_LDS(a2, BM);
+  SMQ_TILE_LDS(b2, BN);
+  SMQ_TILE_LDS(a3, BM);
+  SMQ_TILE_LDS(b3, BN);
+  gemm_nt_body<H, BM, BN, WM, WN, 4, SPLIT>(A, B, kt, tm, tn, tri, epi, a0, b0, a1, b1, a2, b2, a3, b3);
+#endif
+}
+#undef SMQ_TILE_LDS
 
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -426,26 +524,32 @@ __device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* st
   if (sums && (lane < kCols) && n0 + lane < N) colsum(n0 + lane, total);
 }
 
-// C = alpha * acc + beta * src, to `o` and / or transposed to `ot` (a symmetric product writes the
-// same matrix twice; its diagonal tiles once). `scale`: a factor of alpha in device memory, or NULL.
+// C = alpha * acc + beta * src + diag * I, to `o` and / or transposed to `ot` (a symmetric product
+// writes the same matrix twice; its diagonal tiles once). `scale`: a factor of alpha in device memory,
+// one per matrix of the batch, or NULL.
 // A launch split over k (gridDim.y shares) writes share y to o + y * share.
+__device__ __forceinline__ void add_diag(float4& v, int m, int n, float d) {
+  const int k = m - n;
+  v.x += k == 0 ? d : 0.0f, v.y += k == 1 ? d : 0.0f, v.z += k == 2 ? d : 0.0f, v.w += k == 3 ? d : 0.0f;
+}
 struct StoreEpi {
   float alpha, beta;
   const float* scale;
   Mat src, o, ot;
   int tri;
   int64_t share;
+  float diag;
   template <int BM, int BN, int WM, int WN, int TM, int TN>
   __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float* stage, int m0, int n0, int M,
                                          int N, int im, int in, int, int, int lane,
                                          int64_t batch) const {
-    const float al = scale ? alpha * *scale : alpha;
+    const float al = scale ? alpha * scale[batch] : alpha;
     Mat s = src, d = o;
     if (gridDim.y > 1) {
       d.p = reinterpret_cast<float*>(d.p) + blockIdx.y * share;
       if (s.fmt != kNone) s.p = reinterpret_cast<float*>(s.p) + blockIdx.y * share;
     }
-    const float be = beta;
+    const float be = beta, dg = diag;
     stage_out<TM, TN>(
         acc, stage, m0, n0, M, N, lane, batch, d, ot, ot.fmt != kNone && !(tri && im == in), false,
         [&](int m, int n, float4 v) {
@@ -454,74 +558,80 @@ struct StoreEpi {
             const float4 c = load4(s, batch, m, n);
             v.x += be * c.x, v.y += be * c.y, v.z += be * c.z, v.w += be * c.w;
           }
+          add_diag(v, m, n, dg);
           return v;
         },
         [](int, float) {});
   }
 };
 
-// The second half of a product split over k: C = alpha * sum over the shares + beta * src, 64 x 64 a
-// workgroup (the same walk as the product's own epilogue, with the tile in LDS from the start).
+// The second half of a product split over k: C = alpha * sum over the shares + beta * src + diag * I,
+// 32 x 32 a workgroup (the same walk as the product's own epilogue, with the tile in LDS).
 static __global__ __launch_bounds__(256) void split_sum_kernel(const float* part, int64_t ld,
                                                                int64_t share, int shares,
                                                                int64_t batch_stride, int M, int N,
                                                                int mirror, StoreEpi e) {
-  __shared__ float tile[64][68];
+  __shared__ float tile[32][36];
   const int im = blockIdx.y, in = blockIdx.x;
-  if (e.tri && in < im) return;
+  if (e.tri && in / 2 < im / 2) return;  // (the shares hold whole tiles of 64, so the diagonal's both halves)
   const int64_t batch = blockIdx.z;
-  const float al = e.scale ? e.alpha * *e.scale : e.alpha;
-  const int c = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
-  const bool turn = mirror && !(e.tri && im == in);
-#pragma unroll
-  for (int p = 0; p < 64; p += 16) {
-    const int m = im * 64 + p + r0, n = in * 64 + c;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (m < M) {
-      if (n < N) {
-        const float* q = part + batch * batch_stride + (int64_t)m * ld + n;
-        for (int k = 0; k < shares; k++) {
-          const float4 w = *reinterpret_cast<const float4*>(q + k * share);
-          v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-        }
-        v.x *= al, v.y *= al, v.z *= al, v.w *= al;
-        if (e.src.fmt != kNone) {
-          const float4 s = load4(e.src, batch, m, n);
-          v.x += e.beta * s.x, v.y += e.beta * s.y, v.z += e.beta * s.z, v.w += e.beta * s.w;
-        }
+  const float al = e.scale ? e.alpha * e.scale[batch] : e.alpha;
+  const int c = (threadIdx.x & 7) * 4, r = threadIdx.x >> 3;
+  const bool turn = mirror && !(e.tri && im / 2 == in / 2);
+  const int m = im * 32 + r, n = in * 32 + c;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (m < M) {
+    if (n < N) {
+      const float* q = part + batch * batch_stride + (int64_t)m * ld + n;
+#pragma unroll 4
+      for (int k = 0; k < shares; k++) {
+        const float4 w = *reinterpret_cast<const float4*>(q + k * share);
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
       }
-      const float w[4] = {v.x, v.y, v.z, v.w};
-      if (e.o.fmt != kNone) store_n<4>(e.o, batch, m, n, N, w);
+      v.x *= al, v.y *= al, v.z *= al, v.w *= al;
+      if (e.src.fmt != kNone) {
+        const float4 s = load4(e.src, batch, m, n);
+        v.x += e.beta * s.x, v.y += e.beta * s.y, v.z += e.beta * s.z, v.w += e.beta * s.w;
+      }
+      add_diag(v, m, n, e.diag);
     }
-    if (turn) *reinterpret_cast<float4*>(&tile[p + r0][c]) = v;
+    const float w[4] = {v.x, v.y, v.z, v.w};
+    if (e.o.fmt != kNone) store_n<4>(e.o, batch, m, n, N, w);
   }
   if (!turn) return;
+  *reinterpret_cast<float4*>(&tile[r][c]) = v;
   __syncthreads();
-  const int n = in * 64 + (threadIdx.x & 63), m0 = im * 64 + (threadIdx.x >> 6) * 16;
-  if (n < N) {
+  const int nt = in * 32 + (threadIdx.x & 31), m0 = im * 32 + (threadIdx.x >> 5) * 4;
+  if (nt < N) {
+    float w[4];
 #pragma unroll
-    for (int h = 0; h < 16; h += 8) {
-      float w[8];
-#pragma unroll
-      for (int k = 0; k < 8; k++)
-        w[k] = m0 + h + k < M ? tile[(threadIdx.x >> 6) * 16 + h + k][threadIdx.x & 63] : 0.0f;
-      store_n<8>(e.ot, batch, n, m0 + h, M, w);
-    }
+    for (int k = 0; k < 4; k++) w[k] = m0 + k < M ? tile[(threadIdx.x >> 5) * 4 + k][threadIdx.x & 31] : 0.0f;
+    store_n<4>(e.ot, batch, nt, m0, M, w);
   }
 }
+static inline void launch_split_sum(const float* part, int64_t ld, int64_t share, int shares,
+                                    int64_t batch_stride, int M, int N, int batch, int mirror,
+                                    const StoreEpi& e, hipStream_t st) {
+  // (whole 64-column pads of an operand: its padding is written here too)
+  hipLaunchKernelGGL(split_sum_kernel, dim3((N + 63) / 64 * 2, (M + 63) / 64 * 2, batch), dim3(256), 0, st,
+                     part, ld, share, shares, batch_stride, M, N, mirror, e);
+}
 
-// Tile shapes. 256 x 256 runs fastest per tile, but a grid below the CU count leaves CUs idle;
-// smaller tiles fill them. kSkinny: up to 32 rows of A, the product bounded by the read of B.
-enum Tile : int { kT256 = 0, kT128 = 1, kT64 = 2, kSkinny = 3 };
+// Tile shapes. 256 x 256 runs fastest per tile, but a grid below the CU count leaves CUs idle; smaller
+// tiles fill them. kT128 has two k tiles in LDS and leaves room for a second workgroup on the CU;
+// kDeep, kT64 and kSkinny have four on the way, for grids that give a CU only one workgroup to hide
+// the loads behind. kSkinny: up to 32 rows of A, the product bounded by the read of B.
+enum Tile : int { kT256 = 0, kT128 = 1, kT64 = 2, kSkinny = 3, kDeep = 4 };
 struct TileShape {
-  int bm, bn, wn, cols;  // cols: columns one wave holds
+  int bm, bn, wm;
 };
 static inline TileShape shape_of(int t) {
   switch (t) {
-    case kT256: return {256, 256, 4, 64};
-    case kT128: return {128, 128, 2, 64};
-    case kT64: return {64, 64, 2, 32};
-    default: return {32, 128, 4, 32};
+    case kT256: return {256, 256, 2};
+    case kT128: return {128, 128, 2};
+    case kDeep: return {128, 128, 2};
+    case kT64: return {64, 64, 2};
+    default: return {32, 128, 1};
   }
 }
 static inline int64_t tile_count(int64_t m, int64_t n, int t, int tri) {
@@ -529,31 +639,42 @@ static inline int64_t tile_count(int64_t m, int64_t n, int t, int tri) {
   const int64_t a = (m + s.bm - 1) / s.bm, b = (n + s.bn - 1) / s.bn;
   return tri ? a * (a + 1) / 2 : a * b;
 }
+// How full the last round of `wgs` workgroups on `slots` places is, over all rounds.
+static inline double fill_of(int64_t wgs, int64_t slots) {
+  return (double)wgs / (double)((wgs + slots - 1) / slots * slots);
+}
+// 256 x 256 or 128 x 128 (0.87 of its rate, two workgroups a CU) by how full their rounds are: 6 x 1024 x
+// 4096 x 1024 is 384 of the former in two rounds (81 us) and 1536 of the latter in three (74 us).
 static inline int choose_tile(int64_t m, int64_t n, int64_t batch, int tri) {
   if (m <= 32 && !tri) return kSkinny;
-  if (batch * tile_count(m, n, kT256, tri) >= 192) return kT256;
-  if (batch * tile_count(m, n, kT128, tri) >= 128) return kT128;
+  const int64_t big = batch * tile_count(m, n, kT256, tri), mid = batch * tile_count(m, n, kT128, tri);
+  if (big >= 128 && fill_of(big, 256) >= 0.87 * fill_of(mid, 512)) return kT256;
+  if (mid >= 384) return kT128;
+  if (mid >= 128) return kDeep;
   return kT64;
 }
-template <typename H, int BM, int BN, int WM, int WN, bool SPLIT, typename Epi>
+template <typename H, int BM, int BN, int WM, int WN, bool DEEP, bool SPLIT, typename Epi>
 static inline void launch_tile(const Operand& A, const Operand& B, int kt, int batch, int tri,
                                int shares, const Epi& epi, hipStream_t st) {
   const int tm = (A.rows + BM - 1) / BM, tn = (B.rows + BN - 1) / BN;
-  const int grid = tri ? tm * (tm + 1) / 2 : tm * tn;
-  hipLaunchKernelGGL((gemm_nt_kernel<H, BM, BN, WM, WN, SPLIT, Epi>), dim3(grid, shares, batch),
-                     dim3(WM * WN * 64), 0, st, A, B, kt, tm, tn, tri, epi);
+  const dim3 grid(tri ? tm * (tm + 1) / 2 : tm * tn, shares, batch), block(WM * WN * 64);
+  if constexpr (DEEP)
+    hipLaunchKernelGGL((gemm_nt_deep_kernel<H, BM, BN, WM, WN, SPLIT, Epi>), grid, block, 0, st, A, B, kt,
+                       tm, tn, tri, epi);
+  else
+    hipLaunchKernelGGL((gemm_nt_kernel<H, BM, BN, WM, WN, SPLIT, Epi>), grid, block, 0, st, A, B, kt, tm,
+                       tn, tri, epi);
 }
 template <typename H, bool SPLIT, typename Epi>
 static inline void launch(int tile, const Operand& A, const Operand& B, int kt, int batch, int tri,
                           int shares, const Epi& epi, hipStream_t st) {
-  if (tile == kT256)
-    launch_tile<H, 256, 256, 2, 4, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
-  else if (tile == kT128)
-    launch_tile<H, 128, 128, 2, 2, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
-  else if (tile == kT64)
-    launch_tile<H, 64, 64, 2, 2, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
-  else
-    launch_tile<H, 32, 128, 1, 4, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+  switch (tile) {
+    case kT256: return launch_tile<H, 256, 256, 2, 4, false, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+    case kT128: return launch_tile<H, 128, 128, 2, 2, false, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+    case kDeep: return launch_tile<H, 128, 128, 2, 2, true, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+    case kT64: return launch_tile<H, 64, 64, 2, 2, true, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+    default: return launch_tile<H, 32, 128, 1, 4, true, SPLIT>(A, B, kt, batch, tri, shares, epi, st);
+  }
 }
 
 // Layout pass: src [rows, cols] of type T, row pitch ld, times 2^*exponent (NULL: 1) times *factor

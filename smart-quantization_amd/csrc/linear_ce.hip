@@ -478,14 +478,21 @@ void product(int dtype, int tile, const Operand& A, const Operand& B, int kt, in
 }
 
 // [rows, cols] in operand form: in place where it can be, else laid out in the workspace.
+// `turned` (absent: fmt kNone) is written transposed along the way, in one pass over p where both go by
+// the same exponent (float32) or none.
 Operand operand(Arena& ws, const void* p, int64_t ld, int64_t rows, int64_t cols, const Shape& s,
-                const int* exponent, bool run, hipStream_t st) {
-  if (direct(p, ld, cols, s.dtype)) return {p, ld, 0, (int)rows};
+                const int* exponent, const int* turned_exponent, const Mat& turned, bool run,
+                hipStream_t st) {
+  const bool in_place = direct(p, ld, cols, s.dtype);
+  const bool once = !in_place && exponent == turned_exponent;
+  if (run && turned.fmt != kNone && !once)
+    layout(p, s.dtype, ld, rows, cols, turned_exponent, nullptr, 0, kNoMat, turned, st);
+  if (in_place) return {p, ld, 0, (int)rows};
   const int64_t to = operand_ld(cols, s.split());
   _Float16* q = ws.take<_Float16>((size_t)(rows * to));
   if (run)
     layout(p, s.dtype, ld, rows, cols, exponent, nullptr, 0,
-           {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, kNoMat, st);
+           {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, once ? turned : kNoMat, st);
   return {q, to, 0, (int)rows};
 }
 
@@ -569,8 +576,8 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
       else launch_few<__bf16>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
     }
   } else {
-    const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, run, st);
-    const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, run, st);
+    const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, kNoMat, run, st);
+    const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, kNoMat, run, st);
     const SoftmaxEpi e = {exponent, bias, target, part, picked};
     if (run) product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
   }
@@ -584,12 +591,30 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
   return a.used;
 }
 
-// Shares of the k range of dh: enough workgroups to fill the chip where dh itself has few tiles.
-int dh_shares(const Shape& s, int tile, int kt) {
-  const int64_t wgs = tile_count(s.tokens, s.dim, tile, 0);
-  int64_t k = (512 + wgs - 1) / wgs;
-  if (k > kt / 8) k = kt / 8;
-  return (int)(k < 1 ? 1 : k > 32 ? 32 : k);
+// dh has few tiles and a long k range: split over k until its workgroups fill the chip (two rounds of
+// 128 x 128 tiles, one of 256 x 256 where those come near a full one), at least 8 k tiles a share.
+struct DhPlan {
+  int tile, shares;
+};
+DhPlan dh_plan(const Shape& s, int kt) {
+  if (s.tokens <= 32) {
+    const int64_t wgs = tile_count(s.tokens, s.dim, kSkinny, 0);
+    const int64_t k = (512 + wgs - 1) / wgs, most = kt / 8 < 1 ? 1 : kt / 8;
+    return {kSkinny, (int)(k < most ? (k > 32 ? 32 : k) : (most > 32 ? 32 : most))};
+  }
+  const int64_t big = tile_count(s.tokens, s.dim, kT256, 0), mid = tile_count(s.tokens, s.dim, kT128, 0);
+  const int most = kt / 8 < 1 ? 1 : kt / 8 > 32 ? 32 : kt / 8;
+  auto best = [&](int64_t wgs, int64_t slots, double* fill) {
+    int k = 1;
+    *fill = 0.0;
+    for (int i = 1; i <= most && wgs * (i - 1) < 2 * slots; i++)
+      if (fill_of(wgs * i, slots) > *fill + 0.02) *fill = fill_of(wgs * i, slots), k = i;
+    return k;
+  };
+  double fb, fm;
+  const int kb = best(big, 256, &fb), km = best(mid, 512, &fm);
+  if (fb >= 0.87 * fm) return {kT256, kb};
+  return {kT128, km};
 }
 
 int64_t default_piece(const Shape& s) {
@@ -624,7 +649,7 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
                        (int)s.tokens, reduction, g, head, planes, fac);
-  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, run, st);
+  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, nullptr, kNoMat, run, st);
   // h transposed: the operand of dw. Ignored rows are zeros, whatever they hold.
   const int64_t ldt = operand_ld(s.tokens, sp);
   const int padt = operand_pad(s.tokens, sp);
@@ -639,12 +664,10 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
   _Float16* wt = dh ? a.take<_Float16>((size_t)(s.dim * ldp)) : nullptr;
   const int tile_l = choose_tile(s.tokens, s.piece, 1, 0);
-  const int row_blocks = (int)((s.tokens + shape_of(tile_l).bm - 1) / shape_of(tile_l).bm) *
-                         (tile_l == kSkinny ? 1 : 2);
+  const int row_blocks = (int)((s.tokens + shape_of(tile_l).bm - 1) / shape_of(tile_l).bm) * shape_of(tile_l).wm;
   float* sums = db ? a.take<float>((size_t)row_blocks * s.piece) : nullptr;
-  const int tile_h = choose_tile(s.tokens, s.dim, 1, 0) == kSkinny ? kSkinny : kT128;
-  const int tile_dh = choose_tile(s.tokens, s.dim, 1, 0) == kT256 ? kT256 : tile_h;
-  const int shares = dh_shares(s, tile_dh, operand_kt(s.piece, sp));
+  const DhPlan dp = dh_plan(s, operand_kt(s.piece, sp));
+  const int tile_dh = dp.tile, shares = dp.shares;
   const int64_t ldacc = round_up(s.dim, 4);
   const bool whole = pieces == 1 && shares == 1;
   float* accum = dh && !whole ? a.take<float>((size_t)(shares * s.tokens * ldacc)) : nullptr;
@@ -655,10 +678,11 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     a.used = mark;
     const int64_t v0 = i * s.piece, n = s.vocab - v0 < s.piece ? s.vocab - v0 : s.piece;
     const char* wp = reinterpret_cast<const char*>(w) + (size_t)(v0 * ldw) * wsize;
-    const Operand B = operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, run, st);
+    const int padn = operand_pad(n, sp);
+    const Operand B = operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew,
+                              dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat, run, st);
     if (a.used > most) most = a.used;
     if (!run) continue;
-    const int padn = operand_pad(n, sp);
     const DlEpi e = {exponent, bias, target, lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
                      {dlt, ldt, 0, fmt, padt}, sums};
     product(s.dtype, tile_l, A, B, operand_kt(s.dim, sp), 1, e, st);
@@ -666,25 +690,22 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
       hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, sums,
                          row_blocks, (int)n, fac, db + v0);
     if (dh) {
-      layout(wp, s.dtype, ldw, n, s.dim, ew, nullptr, 0, kNoMat, {wt, ldp, 0, fmt, padn}, st);
       const Operand L = {dl, ldp, 0, (int)s.tokens}, W = {wt, ldp, 0, (int)s.dim};
-      StoreEpi se = {1.0f, 1.0f, whole ? &fac->scale_dh : nullptr, kNoMat, kNoMat, kNoMat, 0, s.tokens * ldacc};
+      StoreEpi se = {1.0f, 1.0f, whole ? &fac->scale_dh : nullptr, kNoMat, kNoMat, kNoMat, 0, s.tokens * ldacc, 0.0f};
       se.o = whole ? Mat{dh, s.dim, 0, out_fmt(s.dtype), 0} : Mat{accum, ldacc, 0, kF32, 0};
       if (i > 0) se.src = se.o;
       product(grad_dtype, tile_dh, L, W, operand_kt(n, sp), shares, se, st);
     }
     if (dw) {
       const Operand L = {dlt, ldt, 0, (int)n}, H = {ht, ldt, 0, (int)s.dim};
-      StoreEpi se = {1.0f, 0.0f, &fac->scale_dw, kNoMat, kNoMat, kNoMat, 0, 0};
+      StoreEpi se = {1.0f, 0.0f, &fac->scale_dw, kNoMat, kNoMat, kNoMat, 0, 0, 0.0f};
       se.o = {reinterpret_cast<char*>(dw) + (size_t)(v0 * s.dim) * wsize, s.dim, 0, out_fmt(s.dtype), 0};
       product(grad_dtype, choose_tile(n, s.dim, 1, 0), L, H, operand_kt(s.tokens, sp), 1, se, st);
     }
   }
   if (run && dh && !whole) {
-    const StoreEpi se = {1.0f, 0.0f, &fac->scale_dh, kNoMat, {dh, s.dim, 0, out_fmt(s.dtype), 0}, kNoMat, 0, 0};
-    hipLaunchKernelGGL(split_sum_kernel, dim3((unsigned)((s.dim + 63) / 64), (unsigned)((s.tokens + 63) / 64)),
-                       dim3(256), 0, st, accum, ldacc, s.tokens * ldacc, shares, (int64_t)0,
-                       (int)s.tokens, (int)s.dim, 0, se);
+    const StoreEpi se = {1.0f, 0.0f, &fac->scale_dh, kNoMat, {dh, s.dim, 0, out_fmt(s.dtype), 0}, kNoMat, 0, 0, 0.0f};
+    launch_split_sum(accum, ldacc, s.tokens * ldacc, shares, 0, (int)s.tokens, (int)s.dim, 1, 0, se, st);
   }
   return most;
 }

@@ -1,20 +1,26 @@
 // orthogonalize.hip — the nearest semi-orthogonal matrix to an update, by Newton-Schulz products.
 //
 //   X = G / (|G|_F + eps), turned so that its m rows are the shorter side;
-//   steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X     (an odd polynomial of the singular values)
+//   steps times:  A = X X^T,  X <- (a I + b A + c A A) X     (an odd polynomial of the singular values)
 //
-// Every product runs on gemm_nt.h with both operands contiguous along k: A and B are symmetric, so
-// only their tiles on and above the diagonal are computed (the epilogue writes both), and X is kept
-// both ways round, as [m, n] (operand of A) and as [n, m] (operand of B X); the last product's
-// epilogue writes both again. 3 m^2 n + m^3 operations a step instead of 4 m^2 n + 2 m^3.
+// All factors are polynomials of one symmetric matrix, so they commute, and a stage of up to kStage
+// steps needs X only at its ends:
+//   A = X X^T;  each step:  Q = a I + b A + c A A,  P <- Q P,  A <- (Q A) Q;   X <- P X
+// The m x m products are symmetric: only the tiles on and above the diagonal are computed (the epilogue
+// writes both halves). A stage of r steps costs 3 m^2 n + (4 r - 3) m^3 operations instead of
+// r (4 m^2 n + 2 m^3): five steps as 3 + 2 6 m^2 n + 14 m^3, as 2 + 2 + 1 9 m^2 n + 11 m^3, instead of
+// 20 m^2 n + 10 m^3. X is kept both ways round, as [m, n] (operand of A) and as [n, m] (operand of P X):
+// all operands of gemm_nt.h are contiguous along k.
 //
-// Rounding. What is stored between products is fp16 at a power-of-two scale that keeps it in range
-// (the host bounds the singular values step by step), as two planes (hi + lo, 23 bits, three products
-// a multiply-add): float32-class. One plane would be off by 0.15 % on Gaussian matrices and by 1-4 %
-// where a few strong directions hide the rest (the polynomial raises the small singular values 3.4-fold
-// a step, and with them the error the large ones leave there); one bf16 plane by 1-11 %. The last two
-// steps no longer raise anything: for bf16 results, themselves off by 0.17 %, steps from the fourth on
-// keep one plane (0.05-0.2 % off), at a third of the operations.
+// Rounding. Between products a matrix is held as two fp16 planes (23 bits) at a power-of-two scale that
+// keeps it in range (the host bounds the singular values step by step). One plane would be off by 0.15 %
+// on Gaussian matrices and by 1-4 % where a few strong directions hide the rest. A stage squares the
+// ratio of the singular values once (A), so its length is limited. Simulated on matrices whose strong
+// directions are 5 to 200 times the rest, five steps are off by 0.5 - 1.2e-6 as 2 + 2 + 1, 1 - 6e-6 as
+// 3 + 2, up to 8e-5 as one stage of 5, and 1 - 20e-6 in plain float32 products: float32 takes stages of
+// 2, the 16-bit types, whose results round to 2^-11 and 2^-8, stages of 3. 16-bit inputs are exact in one
+// plane, so the first stage reads one plane of them; for bf16 results, which round to 2^-8, the last P X
+// takes one plane of each (0.03 - 0.3 % off, against the 0.17 % of the result's own rounding).
 #include <math.h>
 
 #include "gemm_nt.h"
@@ -24,7 +30,9 @@ namespace ortho {
 using namespace gemm;
 
 constexpr int kParts = 256;
-constexpr int kPlaneSteps = 3;  // bf16 results: steps that keep two planes
+
+__host__ __device__ constexpr int round32(int v) { return (v + 31) & ~31; }
+__host__ __device__ constexpr int round64(int v) { return (v + 63) & ~63; }
 
 // ---- the norm -----------------------------------------------------------------------------------
 template <typename T>
@@ -51,13 +59,357 @@ __global__ __launch_bounds__(256) void square_sum_kernel(const T* x, int64_t ld,
   __syncthreads();
   if (threadIdx.x == 0) part[blockIdx.y * gridDim.x + blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
 }
-// factor[batch] = scale / (norm + eps)
-__global__ __launch_bounds__(64) void norm_kernel(const double* part, int n, double eps, double scale,
-                                                  float* factor) {
+// Per matrix: pow2 = 2^e that brings the norm to [2^13, 2^14) (so the fp16 planes hold it: an element of
+// size norm / 2^27 still has full precision), rest = 1 / ((norm + eps) 2^e) and its square, which
+// the products with X take as a factor.
+__global__ __launch_bounds__(64) void norm_kernel(const double* part, int n, double eps, float* pow2,
+                                                  float* rest, float* rest2) {
   double s = 0.0;
   for (int i = threadIdx.x; i < n; i += 64) s += part[blockIdx.x * n + i];
   s = wave_sum(s);
-  if (threadIdx.x == 0) factor[blockIdx.x] = (float)(scale / (sqrt(s) + eps));
+  if (threadIdx.x == 0) {
+    const double norm = sqrt(s);
+    int e = 0;
+    if (norm > 0.0 && norm < 1e300) {
+      frexp(norm, &e);
+      e = 14 - e;
+      e = e > 120 ? 120 : e < -120 ? -120 : e;
+    }
+    const double r = 1.0 / ((norm + eps) * ldexp(1.0, e));
+    pow2[blockIdx.x] = ldexpf(1.0f, e);
+    rest[blockIdx.x] = (float)r;
+    rest2[blockIdx.x] = (float)(r * r);
+  }
+}
+
+// ---- one workgroup a matrix -----------------------------------------------------------------------
+// m <= 64: the products of a stage are too small to fill the chip and each launch costs more than it
+// computes, so one workgroup keeps A, Q and P of a matrix in LDS (as operands: two planes in the
+// tiles of gemm_nt.h) and registers (as fp32). With `whole`, where n is short or the stack deep, it also
+// forms A from X, applies P and goes through all stages; else it takes A from, and leaves P in, global
+// memory. 64 x 64 float32, 5 steps: 49 us a call (110 as 18 launches of gemm_nt.h). For m up to 128, on 16
+// waves, the same kernel was no faster than those launches.
+struct SmallStep {
+  float qa, qb, qc;  // coefficients a, b, c
+  float sa, sq, sw, sp;  // 2^e of A, Q, W = Q A and P as operands
+};
+struct SmallArgs {
+  SmallStep step[8];
+  int steps;         // of this launch (a stage, or all)
+  int stage;         // steps of a stage
+  int m, n, batch;
+  Mat x[2], xt[2];   // whole: X and X^T; the stages alternate
+  Mat y;             // whole: the result
+  int turned;
+  int fmt_x0, fmt_xt0, coarse;
+  const float* rest;
+  const float* rest2;
+  float ex[8];       // 2^-ex of X at each stage's start
+  float ey[8];       // 2^ey of X at each stage's end
+  Mat gram, p;       // not whole
+  float gram_scale, p_scale;  // 2^-ea, 2^ep
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+struct Small {
+  static constexpr int DIM = 64;
+  // one 32 x 32 block a wave
+  static constexpr int kWn = DIM / 32, kWaves = kWn * kWn;
+  static constexpr int TM = 1, TN = 1;
+  static constexpr int kTiles = DIM / 32;  // k tiles a region holds
+  static constexpr int kTileHalves = DIM * 64;
+  static constexpr int kLoads = DIM / 8 / kWaves;  // loads a wave issues per k tile
+  typedef f32x16 Block[TM][TN];
+  int lane, wave, wm, wn;
+
+  __device__ __forceinline__ void clear(Block& v) const {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) v[i][j][r] = 0.0f;
+  }
+  // k tile t of `rows` rows from row0 of a matrix -> region + slot (rows past the end: the last one)
+  __device__ __forceinline__ void fetch(const Mat& a, int64_t batch, int row0, int rows, int t,
+                                        _Float16* region, int slot) const {
+    const int have = rows - row0 < DIM ? rows - row0 : DIM;
+    const char* p = reinterpret_cast<const char*>(a.p) + 2 * (batch * a.batch + (int64_t)row0 * a.ld);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)((have - 1) * a.ld * 2 + (t + 1) * 128), 0x00027000);
+    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      const int r = (i * kWaves + wave) * 8 + (lane >> 3);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (lds_void*)(region + slot * kTileHalves + (i * kWaves + wave) * 512), 16,
+          (int)((r < have ? r : have - 1) * a.ld * 2) + chunk, t * 128, 0, 0);
+    }
+  }
+  template <int T>
+  __device__ __forceinline__ void read(const _Float16* tile, int base, int s, f16x8 (&f)[T]) const {
+    const int at = ((s * 2 + (lane >> 5)) ^ (lane & 7)) * 8;
+#pragma unroll
+    for (int i = 0; i < T; i++)
+      f[i] = *reinterpret_cast<const f16x8*>(tile + (base * T * 32 + i * 32 + (lane & 31)) * 64 + at);
+  }
+  // acc[i][j] += rows of `u` (runs of a lane) x rows of `v` (one a lane)
+  __device__ __forceinline__ void mma(const f16x8 (&u)[TN], const f16x8 (&v)[TM], Block& acc) const {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++) acc[i][j] = Frag<_Float16>::mma(u[j], v[i], acc[i][j]);
+  }
+  // acc += (rows of a: one a lane) x (rows of b: runs of 4) over `tiles` k tiles. A wave's block is
+  // (ba, bb).
+  __device__ __forceinline__ void product(const _Float16* a, const _Float16* b, int tiles, bool two, int ba,
+                                          int bb, Block& acc, Block& low) const {
+#pragma unroll 1
+    for (int t = 0; t < tiles; t++) {
+      const _Float16 *ta = a + t * kTileHalves, *tb = b + t * kTileHalves;
+      if (two) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          f16x8 ah[TM], al[TM], bh[TN], bl[TN];
+          read(ta, ba, s, ah);
+          read(tb, bb, s, bh);
+          read(ta, ba, s + 2, al);
+          read(tb, bb, s + 2, bl);
+          mma(bh, ah, acc);
+          mma(bl, ah, low);
+          mma(bh, al, low);
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+          f16x8 fa[TM], fb[TN];
+          read(ta, ba, s, fa);
+          read(tb, bb, s, fb);
+          mma(fb, fa, acc);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void sum(Block& acc, const Block& low, float scale) const {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][j][r] = (acc[i][j][r] + low[i][j][r]) * scale;
+  }
+  // f(i, j, r, row, col): the four values from register r on are columns col..col+3 of a row
+  template <typename F>
+  __device__ __forceinline__ void each(int br, int bc, F f) const {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          f(i, j, r, br * TM * 32 + i * 32 + (lane & 31), bc * TN * 32 + j * 32 + 2 * r + 4 * (lane >> 5));
+  }
+  // A symmetric matrix as an operand: v * scale, columns from m on are zeros.
+  __device__ __forceinline__ void put(_Float16* region, const Block& v, float scale, int m, bool two) const {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    each(wm, wn, [&](int i, int j, int r, int row, int col) {
+      h4 hi, lo;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float x = col + k < m ? v[i][j][r + k] * scale : 0.0f;
+        hi[k] = (_Float16)x;
+        lo[k] = (_Float16)(x - (float)hi[k]);
+      }
+      const int x7 = row & 7;
+      if (two) {
+        _Float16* t = region + (col >> 5) * kTileHalves + row * 64 + (col & 7);
+        const int c = (col & 31) >> 3;
+        *reinterpret_cast<h4*>(t + (c ^ x7) * 8) = hi;
+        *reinterpret_cast<h4*>(t + ((c + 4) ^ x7) * 8) = lo;
+      } else {
+        _Float16* t = region + (col >> 6) * kTileHalves + row * 64 + (col & 7);
+        *reinterpret_cast<h4*>(t + (((col & 63) >> 3) ^ x7) * 8) = hi;
+      }
+    });
+  }
+};
+#endif
+
+template <bool WHOLE>
+__global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef Small S;
+  constexpr int DIM = S::DIM;
+  typedef typename S::Block Block;
+  __shared__ __attribute__((aligned(1024))) _Float16 r0[DIM * DIM * 2];
+  __shared__ __attribute__((aligned(1024))) _Float16 r1[DIM * DIM * 2];
+  S s;
+  s.lane = threadIdx.x & 63;
+  s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  s.wm = s.wave / S::kWn, s.wn = s.wave % S::kWn;
+  const int64_t batch = blockIdx.x;
+  const int m = A.m, n = A.n, km = (m + 31) / 32;
+  constexpr int kAll = S::kTiles * S::kLoads;  // loads of a whole region
+  Block a, p, acc, low;
+  for (int done = 0, stage = 0; done < A.steps; stage++) {
+    const int r = A.steps - done < A.stage ? A.steps - done : A.stage;
+    const bool end = done + r == A.steps;
+    // ---- A = X X^T
+    if constexpr (WHOLE) {
+      Mat X = A.x[stage & 1];
+      if (stage == 0) X.fmt = A.fmt_x0;
+      else X.fmt = kSplit, X.ld = (int64_t)round32(n) * 2, X.batch = X.ld * m;
+      const bool two = X.fmt == kSplit;
+      const int kt = two ? (n + 31) / 32 : (n + 63) / 64;
+      auto load = [&](int first, _Float16* region) {
+#pragma unroll
+        for (int t = 0; t < S::kTiles; t++)
+          s.fetch(X, batch, 0, m, first + t < kt ? first + t : kt - 1, region, t);
+      };
+      s.clear(acc);
+      s.clear(low);
+      load(0, r0);
+#pragma unroll 1
+      for (int t = 0; t < kt; t += 2 * S::kTiles) {
+        auto half = [&](int first, _Float16* here, _Float16* there) {
+          load(first + S::kTiles, there);
+          asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kAll) : "memory");
+          if (first < kt)
+            s.product(here, here, kt - first < S::kTiles ? kt - first : S::kTiles, two, s.wm, s.wn, acc, low);
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        };
+        half(t, r0, r1);
+        half(t + S::kTiles, r1, r0);
+      }
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      const float f = A.ex[stage] * A.ex[stage] * (stage == 0 ? A.rest2[batch] : 1.0f);
+#pragma unroll
+      for (int i = 0; i < S::TM; i++)
+#pragma unroll
+        for (int j = 0; j < S::TN; j++)
+#pragma unroll
+          for (int q = 0; q < 16; q++) a[i][j][q] = (acc[i][j][q] + low[i][j][q]) * f;
+    } else {
+      s.each(s.wm, s.wn, [&](int i, int j, int q, int row, int col) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (row < m && col < A.gram.pad) v = load4(A.gram, batch, row, col);
+        a[i][j][q] = v.x * A.gram_scale, a[i][j][q + 1] = v.y * A.gram_scale;
+        a[i][j][q + 2] = v.z * A.gram_scale, a[i][j][q + 3] = v.w * A.gram_scale;
+      });
+    }
+    s.put(r0, a, A.step[done].sa, m, true);
+    __syncthreads();
+    // ---- P of the stage
+#pragma unroll 1
+    for (int i = 0; i < r; i++) {
+      const SmallStep& k = A.step[done + i];
+      const float ia = 1.0f / k.sa, iq = 1.0f / k.sq;
+      s.clear(acc);
+      s.clear(low);
+      s.product(r0, r0, km, true, s.wm, s.wn, acc, low);
+      s.sum(acc, low, ia * ia);
+      s.each(s.wm, s.wn, [&](int x, int y, int q, int row, int col) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          acc[x][y][q + e] = (row == col + e ? k.qa : 0.0f) + k.qb * a[x][y][q + e] + k.qc * acc[x][y][q + e];
+      });
+      s.put(r1, acc, k.sq, m, true);
+      if (i == 0) {
+#pragma unroll
+        for (int x = 0; x < S::TM; x++)
+#pragma unroll
+          for (int y = 0; y < S::TN; y++) p[x][y] = acc[x][y];
+      }
+      __syncthreads();
+      if (i + 1 < r) {
+        s.clear(acc);
+        s.clear(low);
+        s.product(r1, r0, km, true, s.wm, s.wn, acc, low);  // W = Q A
+        s.sum(acc, low, iq * ia);
+        __syncthreads();
+        s.put(r0, acc, k.sw, m, true);
+        __syncthreads();
+        s.clear(a);
+        s.clear(low);
+        s.product(r0, r1, km, true, s.wm, s.wn, a, low);  // A <- W Q
+        s.sum(a, low, iq / k.sw);
+        __syncthreads();
+      }
+      if (i > 0) {  // P <- Q P
+        if (i + 1 == r) __syncthreads();
+        s.put(r0, p, A.step[done + i - 1].sp, m, true);
+        __syncthreads();
+        s.clear(p);
+        s.clear(low);
+        s.product(r1, r0, km, true, s.wm, s.wn, p, low);
+        s.sum(p, low, iq / A.step[done + i - 1].sp);
+        __syncthreads();
+      }
+      if (i + 1 < r) {
+        s.put(r0, a, A.step[done + i + 1].sa, m, true);
+        __syncthreads();
+      }
+    }
+    // ---- X <- P X
+    if constexpr (!WHOLE) {
+      s.each(s.wm, s.wn, [&](int i, int j, int q, int row, int col) {
+        if (row < m) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[e] = p[i][j][q + e] * A.p_scale;
+          store_n<4>(A.p, batch, row, col, m, w);
+        }
+      });
+    } else {
+      Mat XT = A.xt[stage & 1];
+      XT.fmt = stage == 0 ? A.fmt_xt0 : end && A.coarse ? kF16 : kSplit;
+      const bool one = XT.fmt == kF16, two = XT.fmt == kSplit;
+      if (stage > 0) XT.ld = one ? (int64_t)round64(m) : (int64_t)round32(m) * 2;
+      if (stage > 0) XT.batch = XT.ld * n;
+      const float sp = A.step[done + r - 1].sp;
+      const float f = A.ex[stage] * (stage == 0 ? A.rest[batch] : 1.0f) * A.ey[stage] / sp;
+      __syncthreads();
+      s.put(r0, p, sp, m, !one);
+      const int tiles = one ? (m + 63) / 64 : km;
+      // the next stage's matrices
+      const bool next_coarse = A.steps - done - r <= A.stage && A.coarse;
+      Mat X2 = A.x[(stage + 1) & 1], XT2 = A.xt[(stage + 1) & 1];
+      X2.fmt = kSplit, X2.ld = (int64_t)round32(n) * 2, X2.batch = X2.ld * m, X2.pad = round32(n);
+      XT2.fmt = next_coarse ? kF16 : kSplit;
+      XT2.pad = next_coarse ? round64(m) : round32(m);
+      XT2.ld = next_coarse ? XT2.pad : 2 * XT2.pad, XT2.batch = XT2.ld * n;
+#pragma unroll 1
+      for (int c0 = 0; c0 < n; c0 += DIM) {
+        for (int t = 0; t < tiles; t++) s.fetch(XT, batch, c0, n, t, r1, t);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (!end || !A.turned) {
+          s.clear(acc);
+          s.clear(low);
+          s.product(r0, r1, tiles, two, s.wm, s.wn, acc, low);
+          s.sum(acc, low, f);
+          s.each(s.wm, s.wn, [&](int i, int j, int q, int row, int col) {
+            const float w[4] = {acc[i][j][q], acc[i][j][q + 1], acc[i][j][q + 2], acc[i][j][q + 3]};
+            if (row < m) store_n<4>(end ? A.y : X2, batch, row, c0 + col, n, w);
+          });
+        }
+        if (!end || A.turned) {  // the same product the other way round: runs along m
+          s.clear(acc);
+          s.clear(low);
+          s.product(r1, r0, tiles, two, s.wm, s.wn, acc, low);
+          s.sum(acc, low, f);
+          s.each(s.wm, s.wn, [&](int i, int j, int q, int row, int col) {
+            const float w[4] = {acc[i][j][q], acc[i][j][q + 1], acc[i][j][q + 2], acc[i][j][q + 3]};
+            if (c0 + row < n) store_n<4>(end ? A.y : XT2, batch, c0 + row, col, m, w);
+          });
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+      // this workgroup reads what it wrote
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    done += r;
+  }
+#endif
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -67,6 +419,13 @@ struct Plan {
   int dtype, steps;
   double a, b, c;
 };
+
+// Steps of a stage. A call bound by its launches (under 2^20 elements, not much longer than wide) takes
+// single steps: three launches each, where a longer stage makes 7 for two and 11 for three.
+int stage_of(const Plan& p) {
+  if (p.m > 64 && p.batch * p.m * p.n < (1 << 20) && p.n <= 4 * p.m) return 1;
+  return p.dtype == SMQ_DTYPE_F32 ? 2 : 3;
+}
 
 // Largest |a s + b s^3 + c s^5| over 0 <= s <= top.
 double grown(const Plan& p, double top) {
@@ -107,23 +466,28 @@ struct Arena {
   }
 };
 
-// Shares of the k range where the tiles alone leave CUs idle: at least 8 k tiles a share, at most 8
-// shares (their sum costs a pass over all of them).
+// Shares of the k range where the tiles alone leave CUs idle: at least 16 k tiles a share, at most 8
+// shares (their sum is a launch of its own, about 16 k tiles long).
 int shares_for(int64_t wgs, int kt) {
-  int64_t k = 256 / (wgs < 1 ? 1 : wgs);
-  if (k > kt / 8) k = kt / 8;
+  int64_t k = 288 / (wgs < 1 ? 1 : wgs);
+  if (k > kt / 16) k = kt / 16;
   return (int)(k < 1 ? 1 : k > 8 ? 8 : k);
 }
 
 struct Buffers {
-  _Float16 *x[2], *xt[2], *gram, *poly;
+  _Float16 *x[2], *xt[2], *gram[2], *q[2], *p[2], *w;
   float* part;  // shares of a product split over k
 };
 
 // One product, split over k or not.
-void product(bool split, const Operand& A, const Operand& B, int kt, int batch, const StoreEpi& e,
+void product(bool split, const Operand& A, const Operand& B, int kt, int batch, StoreEpi e,
              const Buffers& w, bool run, size_t* need, hipStream_t st) {
-  const int tile = choose_tile(A.rows, B.rows, batch, e.tri);
+  // A symmetric product whose whole grid of small tiles fits the chip at once is not halved: the mirrored
+  // store costs 2 us, the other half nothing. (Two planes in 256 x 256 tiles round more, gemm_nt.h, and
+  // are no faster at these lengths.)
+  if (e.tri && batch * tile_count(A.rows, B.rows, kT64, 0) <= 256) e.tri = 0, e.ot.fmt = kNone;
+  int tile = choose_tile(A.rows, B.rows, batch, e.tri);
+  if (split && tile == kT256) tile = kT128;
   const int shares = tile == kT256 ? 1 : shares_for(batch * tile_count(A.rows, B.rows, tile, e.tri), kt);
   const int64_t ld = round_up(B.rows, 4), per = (int64_t)A.rows * ld;
   if (shares > 1 && need) {
@@ -133,36 +497,29 @@ void product(bool split, const Operand& A, const Operand& B, int kt, int batch, 
   if (!run) return;
   StoreEpi d = e;
   if (shares > 1) {
-    d = {1.0f, 0.0f, nullptr, {}, {w.part, ld, per, kF32, 0}, {}, 0, batch * per};
+    d = {1.0f, 0.0f, nullptr, {}, {w.part, ld, per, kF32, 0}, {}, 0, batch * per, 0.0f};
   }
   if (split) launch<_Float16, true>(tile, A, B, kt, batch, e.tri, shares, d, st);
   else launch<_Float16, false>(tile, A, B, kt, batch, e.tri, shares, d, st);
   if (shares > 1)
-    hipLaunchKernelGGL(split_sum_kernel,
-                       dim3((unsigned)((B.rows + 63) / 64), (unsigned)((A.rows + 63) / 64), batch),
-                       dim3(256), 0, st, w.part, ld, batch * per, shares, per, A.rows, B.rows,
-                       e.ot.fmt != kNone ? 1 : 0, e);
-}
-
-// Small stacks, bound by their launches, keep two planes throughout: it costs them nothing.
-bool planes_at(const Plan& p, int step) {
-  return p.dtype != SMQ_DTYPE_BF16 || step < kPlaneSteps ||
-         (double)p.batch * p.m * p.m * p.n < (double)(1 << 28);
+    launch_split_sum(w.part, ld, batch * per, shares, per, A.rows, B.rows, batch,
+                     e.ot.fmt != kNone ? 1 : 0, e, st);
 }
 
 template <typename T>
-void first_layout(const Plan& p, const T* g, int64_t ld, int64_t stride, double eps, double scale,
-                  double* part, float* factor, const Mat& x, const Mat& xt, hipStream_t st) {
+void first_layout(const Plan& p, const T* g, int64_t ld, int64_t stride, double eps, double* part,
+                  float* pow2, float* rest, float* rest2, const Mat& x, const Mat& xt, hipStream_t st) {
   const int rows = (int)(p.turned ? p.n : p.m), cols = (int)(p.turned ? p.m : p.n);
   const int grid = rows < 4 * kParts ? (rows + 3) / 4 : kParts;
   hipLaunchKernelGGL(square_sum_kernel<T>, dim3(grid, (unsigned)p.batch), dim3(256), 0, st, g, ld, stride,
                      rows, cols, part);
-  hipLaunchKernelGGL(norm_kernel, dim3((unsigned)p.batch), dim3(64), 0, st, part, grid, eps, scale, factor);
-  launch_layout(g, ld, stride, rows, cols, (int)p.batch, nullptr, factor, nullptr, 0, p.turned ? xt : x,
+  hipLaunchKernelGGL(norm_kernel, dim3((unsigned)p.batch), dim3(64), 0, st, part, grid, eps, pow2, rest,
+                     rest2);
+  launch_layout(g, ld, stride, rows, cols, (int)p.batch, nullptr, pow2, nullptr, 0, p.turned ? xt : x,
                 p.turned ? x : xt, st);
 }
 
-// The products of one step of either format, walked without a launch: the floats their shares need.
+// The products of a call of either format, walked without a launch: the floats their shares need.
 size_t share_floats(const Plan& p) {
   size_t need = 0;
   for (int s = 0; s < 2; s++) {
@@ -174,8 +531,28 @@ size_t share_floats(const Plan& p) {
     product(sp, X, X, operand_kt(p.m, sp), (int)p.batch, e, {}, false, &need, nullptr);
     e.tri = 0;
     product(sp, X, XT, operand_kt(p.m, sp), (int)p.batch, e, {}, false, &need, nullptr);
+    product(false, X, XT, operand_kt(p.m, true), (int)p.batch, e, {}, false, &need, nullptr);
   }
   return need;
+}
+
+// The small kernel's steps first .. first + count of a call; *top is the bound of X's singular values
+// before and after them. `stage`: where P starts anew.
+void fill_steps(const Plan& p, int count, int stage, double* top, SmallArgs* a) {
+  double most = 1.0;
+  for (int i = 0; i < count; i++) {
+    if (i % stage == 0) most = 1.0;
+    const double t = *top * *top, lift = fabs(p.a) + fabs(p.b) * t + fabs(p.c) * t * t;
+    most *= lift;
+    a->step[i] = {(float)p.a, (float)p.b, (float)p.c, (float)ldexp(1.0, exponent_for(t)),
+                  (float)ldexp(1.0, exponent_for(lift)), (float)ldexp(1.0, exponent_for(lift * t)),
+                  (float)ldexp(1.0, exponent_for(most))};
+    *top = grown(p, *top);
+  }
+}
+template <bool WHOLE>
+void launch_small(const SmallArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL(small_kernel<WHOLE>, dim3(a.batch), dim3(256), 0, st, a);
 }
 
 // Lays the workspace out and, when `run`, enqueues the call. Returns the bytes used.
@@ -184,61 +561,136 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
   Arena a(ws);
   const int64_t bt = p.batch, m = p.m, n = p.n;
   const int batch = (int)bt;
-  // room for the larger of the two formats; two of each X (a step reads one and writes the other)
+  // room for the largest format; two of each X (a stage reads one and writes the other)
   const int64_t ldn = 2 * round_up(n, 64), ldm = 2 * round_up(m, 64);
   double* part = a.take<double>((size_t)(bt * kParts));
-  float* factor = a.take<float>((size_t)bt);
+  float* pow2 = a.take<float>((size_t)bt);
+  float* rest = a.take<float>((size_t)bt);
+  float* rest2 = a.take<float>((size_t)bt);
   Buffers w;
   for (int k = 0; k < 2; k++) {
     w.x[k] = a.take<_Float16>((size_t)(bt * m * ldn));
     w.xt[k] = a.take<_Float16>((size_t)(bt * n * ldm));
+    w.gram[k] = a.take<_Float16>((size_t)(bt * m * ldm));
+    w.q[k] = a.take<_Float16>((size_t)(bt * m * ldm));
+    w.p[k] = a.take<_Float16>((size_t)(bt * m * ldm));
   }
-  w.gram = a.take<_Float16>((size_t)(bt * m * ldm));
-  w.poly = a.take<_Float16>((size_t)(bt * m * ldm));
+  w.w = a.take<_Float16>((size_t)(bt * m * ldm));
   w.part = a.take<float>(share_floats(p));
   if (!run) return a.used;
 
-  auto mat = [&](_Float16* q, int64_t cols, int64_t rows, bool planes) {
-    const int64_t l = operand_ld(cols, planes);
-    return Mat{q, l, rows * l, planes ? kSplit : kF16, operand_pad(cols, planes)};
+  auto mat = [&](_Float16* q, int64_t cols, int64_t rows, int fmt) {
+    const bool two = fmt != kF16;
+    const int64_t l = operand_ld(cols, two);
+    return Mat{q, l, rows * l, fmt, operand_pad(cols, two)};
   };
   auto op = [](const Mat& q, int64_t rows) { return Operand{q.p, q.ld, q.batch, (int)rows}; };
   const Mat none = {nullptr, 0, 0, kNone, 0};
   const int out = p.dtype == SMQ_DTYPE_F32 ? kF32 : p.dtype == SMQ_DTYPE_F16 ? kF16 : kBF16;
-  double top = 1.0;  // bound of X's singular values
-  int ex = exponent_for(top);
-  Mat X = mat(w.x[0], n, m, planes_at(p, 0)), XT = mat(w.xt[0], m, n, planes_at(p, 0));
-  const double scale = ldexp(1.0, ex);
+  const bool coarse = p.dtype == SMQ_DTYPE_BF16;  // the last P X in one plane of each
+  const int longest = stage_of(p);
+  bool end = p.steps <= longest;                  // the stage at hand is the last one
+  Mat X = mat(w.x[0], n, m, p.dtype == SMQ_DTYPE_F32 ? kSplit : kF16);
+  Mat XT = mat(w.xt[0], m, n, p.dtype == SMQ_DTYPE_F32 ? kSplit : end && coarse ? kF16 : kDup);
   if (p.dtype == SMQ_DTYPE_F32)
-    first_layout(p, (const float*)g, ld, stride, eps, scale, part, factor, X, XT, st);
+    first_layout(p, (const float*)g, ld, stride, eps, part, pow2, rest, rest2, X, XT, st);
   else if (p.dtype == SMQ_DTYPE_F16)
-    first_layout(p, (const _Float16*)g, ld, stride, eps, scale, part, factor, X, XT, st);
+    first_layout(p, (const _Float16*)g, ld, stride, eps, part, pow2, rest, rest2, X, XT, st);
   else
-    first_layout(p, (const __bf16*)g, ld, stride, eps, scale, part, factor, X, XT, st);
-  for (int i = 0; i < p.steps; i++) {
-    const bool last = i + 1 == p.steps, sp = planes_at(p, i);
-    const double q = top * top;
-    const int ea = exponent_for(q), eb = exponent_for(fabs(p.b) * q + fabs(p.c) * q * q);
-    const Mat A = mat(w.gram, m, m, sp), P = mat(w.poly, m, m, sp);
+    first_layout(p, (const __bf16*)g, ld, stride, eps, part, pow2, rest, rest2, X, XT, st);
+
+  double top = 1.0;  // bound of X's singular values
+  const bool small = m <= 64;
+  // One workgroup a matrix also for the products with X: where they are short, or the stack fills the chip.
+  if (small && p.steps <= 8 && (n <= 256 || batch >= 128)) {
+    SmallArgs sa = {};
+    sa.steps = p.steps, sa.stage = longest, sa.m = (int)m, sa.n = (int)n, sa.batch = batch;
+    sa.x[0] = X, sa.xt[0] = XT, sa.x[1].p = w.x[1], sa.xt[1].p = w.xt[1];
+    sa.fmt_x0 = X.fmt, sa.fmt_xt0 = XT.fmt, sa.coarse = coarse ? 1 : 0, sa.turned = p.turned ? 1 : 0;
+    sa.y = {y, p.turned ? m : n, m * n, out, 0};
+    sa.rest = rest, sa.rest2 = rest2;
+    fill_steps(p, p.steps, longest, &top, &sa);
+    double bound = 1.0;
+    for (int s = 0, done = 0; done < p.steps; s++) {
+      sa.ex[s] = s == 0 ? 1.0f : 1.0f / sa.ey[s - 1];
+      for (int i = 0; i < longest && done < p.steps; i++, done++) bound = grown(p, bound);
+      sa.ey[s] = done == p.steps ? 1.0f : (float)ldexp(1.0, exponent_for(bound));
+    }
+    launch_small<true>(sa, st);
+    return a.used;
+  }
+  int ex = 0;  // X is held times 2^ex (in the first stage the factors `rest` say it)
+  const int km = operand_kt(m, true);
+  for (int done = 0, stage = 0; done < p.steps; stage++) {
+    const int r = p.steps - done < longest ? p.steps - done : longest;
+    done += r;
+    end = done == p.steps;
+    const int pfmt = end && coarse ? kF16 : kSplit;
     // A = X X^T
-    StoreEpi e = {(float)ldexp(1.0, ea - 2 * ex), 0.0f, nullptr, none, A, A, 1, 0};
-    product(sp, op(X, m), op(X, m), operand_kt(n, sp), batch, e, w, true, nullptr, st);
-    // B = b A + c A A
-    e = {(float)ldexp(p.c, eb - 2 * ea), (float)ldexp(p.b, eb - ea), nullptr, A, P, P, 1, 0};
-    product(sp, op(A, m), op(A, m), operand_kt(m, sp), batch, e, w, true, nullptr, st);
-    // X <- a X + B X
-    top = grown(p, top);
-    const int ey = last ? 0 : exponent_for(top);
+    int ea = exponent_for(top * top);
+    Mat A = mat(w.gram[0], m, m, kSplit);
+    StoreEpi e = {(float)ldexp(1.0, ea - 2 * ex), 0.0f, stage ? nullptr : rest2, none, A, A, 1, 0, 0.0f};
+    product(X.fmt == kSplit, op(X, m), op(X, m), operand_kt(n, X.fmt == kSplit), batch, e, w, true, nullptr, st);
+    Mat P = none;
+    int ep = 0;
+    if (small) {
+      SmallArgs sa = {};
+      sa.steps = sa.stage = r, sa.m = (int)m, sa.batch = batch;
+      sa.gram = A, sa.gram_scale = (float)ldexp(1.0, -ea);
+      fill_steps(p, r, r, &top, &sa);
+      P = mat(w.p[0], m, m, pfmt);
+      sa.p = P, sa.p_scale = sa.step[r - 1].sp;
+      frexpf(sa.p_scale, &ep);
+      ep -= 1;
+      launch_small<false>(sa, st);
+    }
+    double most = 1.0;  // bound of P
+    for (int i = 0; i < r && !small; i++) {
+      const double t = top * top, lift = fabs(p.a) + fabs(p.b) * t + fabs(p.c) * t * t;
+      const int eq = exponent_for(lift);
+      // Q = a I + b A + c A A
+      const Mat Q = mat(w.q[i & 1], m, m, r == 1 ? pfmt : kSplit);
+      e = {(float)ldexp(p.c, eq - 2 * ea), (float)ldexp(p.b, eq - ea), nullptr, A, Q, Q, 1, 0,
+           (float)ldexp(p.a, eq)};
+      product(true, op(A, m), op(A, m), km, batch, e, w, true, nullptr, st);
+      most *= lift;
+      if (i == 0) {
+        P = Q, ep = eq;
+      } else {
+        // P <- Q P
+        const int en = exponent_for(most);
+        const Mat P2 = mat(w.p[i & 1], m, m, i + 1 == r ? pfmt : kSplit);
+        e = {(float)ldexp(1.0, en - eq - ep), 0.0f, nullptr, none, P2, P2, 1, 0, 0.0f};
+        product(true, op(Q, m), op(P, m), km, batch, e, w, true, nullptr, st);
+        P = P2, ep = en;
+      }
+      const double next = grown(p, top);
+      if (i + 1 < r) {
+        // A <- (Q A) Q
+        const int ew = exponent_for(lift * t), en = exponent_for(next * next);
+        const Mat W = mat(w.w, m, m, kSplit), A2 = mat(w.gram[(i + 1) & 1], m, m, kSplit);
+        e = {(float)ldexp(1.0, ew - eq - ea), 0.0f, nullptr, none, W, W, 1, 0, 0.0f};
+        product(true, op(Q, m), op(A, m), km, batch, e, w, true, nullptr, st);
+        e = {(float)ldexp(1.0, en - ew - eq), 0.0f, nullptr, none, A2, A2, 1, 0, 0.0f};
+        product(true, op(W, m), op(Q, m), km, batch, e, w, true, nullptr, st);
+        A = A2, ea = en;
+      }
+      top = next;
+    }
+    // X <- P X
+    const int ey = end ? 0 : exponent_for(top);
     Mat X2, XT2;
-    if (!last) {
-      const bool np = planes_at(p, i + 1);
-      X2 = mat(w.x[(i + 1) & 1], n, m, np), XT2 = mat(w.xt[(i + 1) & 1], m, n, np);
+    if (!end) {
+      const bool last = p.steps - done <= longest;
+      X2 = mat(w.x[(stage + 1) & 1], n, m, kSplit);
+      XT2 = mat(w.xt[(stage + 1) & 1], m, n, last && coarse ? kF16 : kSplit);
     } else {
       const Mat Y = {y, p.turned ? m : n, m * n, out, 0};
       X2 = p.turned ? none : Y, XT2 = p.turned ? Y : none;
     }
-    e = {(float)ldexp(1.0, ey - eb - ex), (float)ldexp(p.a, ey - ex), nullptr, X, X2, XT2, 0, 0};
-    product(sp, op(P, m), op(XT, n), operand_kt(m, sp), batch, e, w, true, nullptr, st);
+    e = {(float)ldexp(1.0, ey - ep - ex), 0.0f, stage ? nullptr : rest, none, X2, XT2, 0, 0, 0.0f};
+    product(XT.fmt == kSplit, op(P, m), op(XT, n), XT.fmt == kF16 ? operand_kt(m, false) : km, batch, e, w,
+            true, nullptr, st);
     X = X2, XT = XT2, ex = ey;
   }
   return a.used;
