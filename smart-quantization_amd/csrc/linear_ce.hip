@@ -382,20 +382,23 @@ struct DlEpi {
                                          int64_t batch) const {
     const int ex = exponent ? *exponent : 0;
     float* sum = sums ? sums + (int64_t)(im * WM + wm) * N : nullptr;
-    stage_out<TM, TN>(
+    stage_out<TM, TN, true>(
         acc, stage, m0, n0, M, N, lane, batch, o, ot, true, sum != nullptr,
-        [&](int m, int n, float4 v) {
-          const float gm = g[m], ls = lse[m];
-          const int64_t t = target[m];
-          const bool known = t >= 0 && t < vocab;
-          const int64_t at = t - first - n;
+        [&](int m) {  // g, lse, the target's place in the piece (-1: elsewhere, -2: nowhere)
+          const int64_t t = target[m], at = t - first;
+          const int k = t < 0 || t >= vocab ? -2 : at >= 0 && at < N ? (int)at : -1;
+          return make_float4(g[m], lse[m], __builtin_bit_cast(float, k), 0.0f);
+        },
+        [&](int, int n, float4 v, float4 row) {
+          const int at = __builtin_bit_cast(int, row.z) - n;
+          const bool known = __builtin_bit_cast(int, row.z) != -2;
           float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; k++) {
             float l = ex ? ldexpf(w[k], ex) : w[k];
             if (bias && n + k < N) l += bias[first + n + k];
-            const float p = exp_near(l - ls) - (at == k ? 1.0f : 0.0f);
-            w[k] = gm == 0.0f ? 0.0f : known ? p * gm : __builtin_nanf("");
+            const float p = exp_near(l - row.y) - (at == k ? 1.0f : 0.0f);
+            w[k] = row.x == 0.0f ? 0.0f : known ? p * row.x : __builtin_nanf("");
           }
           return make_float4(w[0], w[1], w[2], w[3]);
         },

@@ -562,7 +562,7 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
   const int64_t bt = p.batch, m = p.m, n = p.n;
   const int batch = (int)bt;
   // room for the largest format; two of each X (a stage reads one and writes the other)
-  const int64_t ldn = 2 * round_up(n, 64), ldm = 2 * round_up(m, 64);
+  const int64_t ldn = 2 * round_up(n, 64) + 64, ldm = 2 * round_up(m, 64) + 64;
   double* part = a.take<double>((size_t)(bt * kParts));
   float* pow2 = a.take<float>((size_t)bt);
   float* rest = a.take<float>((size_t)bt);
