@@ -41,37 +41,45 @@ __device__ __forceinline__ void put(typename Pack<T, V>::type& v, int i, float f
   else v[i] = (T)f;
 }
 
-// 1 / (1 + exp(-z)) from the hardware's exp2 and reciprocal, each within 1 ulp: the product with log2(e) is
-// carried in two parts, so the result is within 4 ulp for every z (|z| is cut at 126 / log2(e), where
-// the result is 0 or 1 to the last bit); a library expf and an IEEE division cost three times the kernel.
+// 1 / (1 + exp(-z)) from the hardware's exp2 and reciprocal: off by (1 - s) |z| 2^-23 + 2 ulp relative, so
+// exact to float32's size wherever z s counts; 0 and 1 at the ends. A library expf and an IEEE division
+// cost three times the rest of the kernel (it is bound by these instructions, not by memory, otherwise).
 __device__ __forceinline__ float sigmoid(float z) {
-  const float x = z < -87.0f ? 87.0f : z > 87.0f ? -87.0f : -z;
-  const float t = x * 1.44269504f;
-  const float e = fmaf(x, 1.44269504f, -t) + x * 1.92596303e-8f;
-  const float p = __builtin_amdgcn_exp2f(t);
-  return __builtin_amdgcn_rcpf(1.0f + fmaf(p, e * 0.693147181f, p));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
 }
-__device__ __forceinline__ float act_of(int act, float z) {
-  switch (act) {
-    case SMQ_ACT_RELU: return z < 0.0f ? 0.0f : z;
-    case SMQ_ACT_SILU: return z * sigmoid(z);
-    case SMQ_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.707106781f));
-    default: return z;
+// The activation of V values, one branch for all of them.
+template <int V>
+__device__ __forceinline__ void act_of(int act, float (&z)[V]) {
+  if (act == SMQ_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] = z[i] < 0.0f ? 0.0f : z[i];
+  } else if (act == SMQ_ACT_SILU) {
+    // -inf stays 0 x -inf = NaN as z times its sigmoid is
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] *= sigmoid(z[i]);
+  } else if (act == SMQ_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] = 0.5f * z[i] * (1.0f + erff(z[i] * 0.707106781f));
   }
 }
-__device__ __forceinline__ float slope_of(int act, float z) {
-  switch (act) {
-    case SMQ_ACT_RELU: return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
-    case SMQ_ACT_SILU: {
-      const float s = sigmoid(z);
-      return s * (1.0f + z * (1.0f - s));
+// dy times the activation's slope at z.
+template <int V>
+__device__ __forceinline__ void slope_of(int act, const float (&z)[V], float (&dy)[V]) {
+  if (act == SMQ_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < V; i++) dy[i] = z[i] > 0.0f ? dy[i] : z[i] == z[i] ? 0.0f : z[i];
+  } else if (act == SMQ_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const float s = sigmoid(z[i]);
+      dy[i] *= fmaf(z[i] * s, 1.0f - s, s);
     }
-    case SMQ_ACT_GELU: {
-      const float x = -0.5f * z * z;
-      const float p = __builtin_amdgcn_exp2f((x < -87.0f ? -87.0f : x) * 1.44269504f);
-      return 0.5f * (1.0f + erff(z * 0.707106781f)) + z * p * 0.398942280f;
+  } else if (act == SMQ_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const float p = __builtin_amdgcn_exp2f(z[i] * z[i] * -0.721347520f);
+      dy[i] *= fmaf(z[i] * p, 0.398942280f, 0.5f + 0.5f * erff(z[i] * 0.707106781f));
     }
-    default: return 1.0f;
   }
 }
 
@@ -206,9 +214,12 @@ __global__ __launch_bounds__(1024) void resident_forward(Args A) {
     const int64_t r = row + (int64_t)k * rows;
     if (active && r < A.s) {
       vec o;
+      float z[V];
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        put<T, V>(o, i, act_of(A.act, fmaf(at<T, V>(v[k], i) - mean[i], mul[i], add[i])));
+      for (int i = 0; i < V; i++) z[i] = fmaf(at<T, V>(v[k], i) - mean[i], mul[i], add[i]);
+      act_of<V>(A.act, z);
+#pragma unroll
+      for (int i = 0; i < V; i++) put<T, V>(o, i, z[i]);
       *reinterpret_cast<vec*>(y + r * A.c) = o;
     }
   }
@@ -237,27 +248,40 @@ __global__ __launch_bounds__(1024) void resident_backward(Args A) {
       d[k] = *reinterpret_cast<const vec*>(dy + r * A.c);
     }
   }
-  float mean[V], rstd[V], w[V], b[V], p1[V], p2[V];
+  // d = x - mean; z = d mul + b; sums of dz and dz d (times rstd: dz xhat)
+  float mean[V], rstd[V], mul[V], b[V], p1[V], p2[V];
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int c = active ? c0 + col * V + i : 0;
     const int64_t g = (int64_t)blockIdx.y * A.groups + c / A.cg;
     mean[i] = A.mean[g], rstd[i] = A.rstd[g];
-    w[i] = A.weight ? A.weight[c] : 1.0f;
+    mul[i] = (A.weight ? A.weight[c] : 1.0f) * rstd[i];
     b[i] = A.bias ? A.bias[c] : 0.0f;
     p1[i] = p2[i] = 0.0f;
   }
+  auto slopes = [&](int k, float (&x0)[V], float (&dz)[V]) __attribute__((always_inline)) {
+    float z[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      x0[i] = at<T, V>(v[k], i) - mean[i];
+      z[i] = fmaf(x0[i], mul[i], b[i]);
+      dz[i] = at<T, V>(d[k], i);
+    }
+    slope_of<V>(A.act, z, dz);
+  };
 #pragma unroll
   for (int k = 0; k < R; k++)
     if (active && row + (int64_t)k * rows < A.s) {
+      float x0[V], dz[V];
+      slopes(k, x0, dz);
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float h = (at<T, V>(v[k], i) - mean[i]) * rstd[i];
-        const float dz = at<T, V>(d[k], i) * slope_of(A.act, fmaf(h, w[i], b[i]));
-        p1[i] += dz;
-        p2[i] = fmaf(dz, h, p2[i]);
+        p1[i] += dz[i];
+        p2[i] = fmaf(dz[i], x0[i], p2[i]);
       }
     }
+#pragma unroll
+  for (int i = 0; i < V; i++) p2[i] *= rstd[i];
   const float inv = 1.0f / ((float)A.s * (float)A.cg);
   const float* scale = A.weight ? A.weight + c0 : nullptr;
   float* chan = reinterpret_cast<float*>(A.chan + (int64_t)blockIdx.y * A.c + c0);
@@ -275,22 +299,21 @@ __global__ __launch_bounds__(1024) void resident_backward(Args A) {
     }
   }
   __syncthreads();
+  // dx = rstd (dz w - c1 - xhat c2) = dz mul - rstd c1 - d rstd^2 c2
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int g = (col * V + i) / A.cg;
-    p1[i] = stat[g], p2[i] = stat[groups + g];
+    p1[i] = -rstd[i] * stat[g], p2[i] = -rstd[i] * rstd[i] * stat[groups + g];
   }
 #pragma unroll
   for (int k = 0; k < R; k++) {
     const int64_t r = row + (int64_t)k * rows;
     if (active && r < A.s) {
       vec o;
+      float x0[V], dz[V];
+      slopes(k, x0, dz);
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        const float h = (at<T, V>(v[k], i) - mean[i]) * rstd[i];
-        const float dz = at<T, V>(d[k], i) * slope_of(A.act, fmaf(h, w[i], b[i]));
-        put<T, V>(o, i, rstd[i] * (dz * w[i] - p1[i] - h * p2[i]));
-      }
+      for (int i = 0; i < V; i++) put<T, V>(o, i, fmaf(dz[i], mul[i], fmaf(x0[i], p2[i], p1[i])));
       *reinterpret_cast<vec*>(dx + r * A.c) = o;
     }
   }
@@ -364,14 +387,23 @@ __global__ __launch_bounds__(256) void join_stats(Args A) {
   const int g = blockIdx.x, n = blockIdx.y, c0 = g * A.cg;
   const T* x = reinterpret_cast<const T*>(A.x) + (int64_t)n * A.s * A.c;
   double s = 0.0, q = 0.0;
-  for (int64_t id = threadIdx.x; id < (int64_t)A.cg * A.chunks; id += 256) {
-    const int c = c0 + (int)(id % A.cg), ch = (int)(id / A.cg);
-    const double k = (double)(float)x[c];
-    const double cnt = (double)(A.s * (ch + 1) / A.chunks - A.s * ch / A.chunks);
-    const float2 p = A.part[((int64_t)n * A.chunks + ch) * A.c + c];
-    s += (double)p.x + cnt * k;
-    q += (double)p.y + 2.0 * k * (double)p.x + cnt * k * k;
-  }
+  // a thread keeps to one channel where the group has at most 256
+  const int per = A.cg < 256 ? A.cg : 256, lanes = 256 / per;
+  const int first = threadIdx.x % per, at0 = threadIdx.x / per;
+  if (at0 < lanes)
+    for (int i = first; i < A.cg; i += per) {
+      const double k = (double)(float)x[c0 + i];
+      const float2* part = A.part + (int64_t)n * A.chunks * A.c + c0 + i;
+      double s1 = 0.0, s2 = 0.0, cnt = 0.0;
+#pragma unroll 4
+      for (int ch = at0; ch < A.chunks; ch += lanes) {
+        const float2 p = part[(int64_t)ch * A.c];
+        cnt += (double)(A.s * (ch + 1) / A.chunks - A.s * ch / A.chunks);
+        s1 += (double)p.x, s2 += (double)p.y;
+      }
+      s += s1 + cnt * k;
+      q += s2 + 2.0 * k * s1 + cnt * k * k;
+    }
   s = wave_sum(s), q = wave_sum(q);
   __shared__ double a[4], b[4];
   if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = s, b[threadIdx.x >> 6] = q;
@@ -405,9 +437,12 @@ __global__ __launch_bounds__(256) void stream_forward(Args A) {
   for (int64_t r = w.first + w.row; r < w.last; r += w.rows) {
     const vec v = *reinterpret_cast<const vec*>(x + r * A.c);
     vec o;
+    float z[V];
 #pragma unroll
-    for (int i = 0; i < V; i++)
-      put<T, V>(o, i, act_of(A.act, fmaf(at<T, V>(v, i) - mean[i], mul[i], add[i])));
+    for (int i = 0; i < V; i++) z[i] = fmaf(at<T, V>(v, i) - mean[i], mul[i], add[i]);
+    act_of<V>(A.act, z);
+#pragma unroll
+    for (int i = 0; i < V; i++) put<T, V>(o, i, z[i]);
     *reinterpret_cast<vec*>(y + r * A.c) = o;
   }
 }
@@ -424,26 +459,34 @@ __global__ __launch_bounds__(256) void stream_sums(Args A) {
     const int64_t base = (int64_t)blockIdx.z * A.s * A.c + w.c;
     const T* x = reinterpret_cast<const T*>(A.x) + base;
     const T* dy = reinterpret_cast<const T*>(A.dy) + base;
-    float mean[V], rstd[V], wt[V], b[V];
+    float mean[V], rstd[V], mul[V], b[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
       const int64_t g = (int64_t)blockIdx.z * A.groups + (w.c + i) / A.cg;
       mean[i] = A.mean[g], rstd[i] = A.rstd[g];
-      wt[i] = A.weight ? A.weight[w.c + i] : 1.0f;
+      mul[i] = (A.weight ? A.weight[w.c + i] : 1.0f) * rstd[i];
       b[i] = A.bias ? A.bias[w.c + i] : 0.0f;
     }
 #pragma unroll 4
     for (int64_t r = w.first + w.row; r < w.last; r += w.rows) {
       const vec v = *reinterpret_cast<const vec*>(x + r * A.c);
       const vec d = *reinterpret_cast<const vec*>(dy + r * A.c);
+      float x0[V], z[V], dz[V];
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float h = (at<T, V>(v, i) - mean[i]) * rstd[i];
-        const float dz = at<T, V>(d, i) * slope_of(A.act, fmaf(h, wt[i], b[i]));
-        p1[i] += dz;
-        p2[i] = fmaf(dz, h, p2[i]);
+        x0[i] = at<T, V>(v, i) - mean[i];
+        z[i] = fmaf(x0[i], mul[i], b[i]);
+        dz[i] = at<T, V>(d, i);
+      }
+      slope_of<V>(A.act, z, dz);
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        p1[i] += dz[i];
+        p2[i] = fmaf(dz[i], x0[i], p2[i]);
       }
     }
+#pragma unroll
+    for (int i = 0; i < V; i++) p2[i] *= rstd[i];
   }
   chunk_sums<V>(A, w, p1, p2, sh);
 }
@@ -484,48 +527,55 @@ __global__ __launch_bounds__(256) void stream_backward(Args A) {
   const T* x = reinterpret_cast<const T*>(A.x) + base;
   const T* dy = reinterpret_cast<const T*>(A.dy) + base;
   T* dx = reinterpret_cast<T*>(A.y) + base;
-  float mean[V], rstd[V], wt[V], b[V], c1[V], c2[V];
+  float mean[V], mul[V], b[V], c1[V], c2[V];
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int64_t g = (int64_t)blockIdx.z * A.groups + (w.c + i) / A.cg;
-    mean[i] = A.mean[g], rstd[i] = A.rstd[g];
-    wt[i] = A.weight ? A.weight[w.c + i] : 1.0f;
-    b[i] = A.bias ? A.bias[w.c + i] : 0.0f;
+    const float rstd = A.rstd[g];
     const float2 k = A.coef[g];
-    c1[i] = k.x, c2[i] = k.y;
+    mean[i] = A.mean[g];
+    mul[i] = (A.weight ? A.weight[w.c + i] : 1.0f) * rstd;
+    b[i] = A.bias ? A.bias[w.c + i] : 0.0f;
+    c1[i] = -rstd * k.x, c2[i] = -rstd * rstd * k.y;
   }
 #pragma unroll 4
   for (int64_t r = w.first + w.row; r < w.last; r += w.rows) {
     const vec v = *reinterpret_cast<const vec*>(x + r * A.c);
     const vec d = *reinterpret_cast<const vec*>(dy + r * A.c);
     vec o;
+    float x0[V], z[V], dz[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const float h = (at<T, V>(v, i) - mean[i]) * rstd[i];
-      const float dz = at<T, V>(d, i) * slope_of(A.act, fmaf(h, wt[i], b[i]));
-      put<T, V>(o, i, rstd[i] * (dz * wt[i] - c1[i] - h * c2[i]));
+      x0[i] = at<T, V>(v, i) - mean[i];
+      z[i] = fmaf(x0[i], mul[i], b[i]);
+      dz[i] = at<T, V>(d, i);
     }
+    slope_of<V>(A.act, z, dz);
+#pragma unroll
+    for (int i = 0; i < V; i++) put<T, V>(o, i, fmaf(dz[i], mul[i], fmaf(x0[i], c2[i], c1[i])));
     *reinterpret_cast<vec*>(dx + r * A.c) = o;
   }
 }
 
-// dweight, dbias: chan summed over n. 64 channels a workgroup, 4 waves share the samples.
-static __global__ __launch_bounds__(256) void param_sums(const float2* chan, int n, int c, float* dweight,
-                                                         float* dbias) {
-  const int ch = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+// dweight, dbias: chan summed over n. 64 channels a workgroup, 16 waves share the samples.
+static __global__ __launch_bounds__(1024) void param_sums(const float2* chan, int n, int c, float* dweight,
+                                                          float* dbias) {
+  const int t = threadIdx.x & 63, ch = blockIdx.x * 64 + t, w = threadIdx.x >> 6;
   double s1 = 0.0, s2 = 0.0;
-  if (ch < c)
-    for (int i = w; i < n; i += 4) {
+  if (ch < c) {
+#pragma unroll 4
+    for (int i = w; i < n; i += 16) {
       const float2 p = chan[(int64_t)i * c + ch];
       s1 += (double)p.x, s2 += (double)p.y;
     }
-  __shared__ double a[4][64], b[4][64];
-  a[w][threadIdx.x & 63] = s1, b[w][threadIdx.x & 63] = s2;
+  }
+  __shared__ double a[16][64], b[16][64];
+  a[w][t] = s1, b[w][t] = s2;
   __syncthreads();
   if (w == 0 && ch < c) {
-    const int t = threadIdx.x;
-    if (dbias) dbias[ch] = (float)((a[0][t] + a[1][t]) + (a[2][t] + a[3][t]));
-    if (dweight) dweight[ch] = (float)((b[0][t] + b[1][t]) + (b[2][t] + b[3][t]));
+    for (int i = 1; i < 16; i++) s1 += a[i][t], s2 += b[i][t];
+    if (dbias) dbias[ch] = (float)s1;
+    if (dweight) dweight[ch] = (float)s2;
   }
 }
 
@@ -565,13 +615,13 @@ Plan plan_of(int dtype, int v, int64_t n, int64_t s, int c, int cg, bool backwar
     int block = unit;
     while (block * size < 64 && c % (block * 2) == 0 && block * 2 / v <= 1024) block *= 2;
     const int cols = block / v;
-    // fewer, fuller threads first; more threads where the rows ask for them
+    // small workgroups of full threads first: several on a CU overlap their loads and their sums
     for (int t = 256; t <= 1024 && !p.r; t *= 2) {
       const int rows = t / cols;
       if (rows < 1) continue;
       const int64_t need = (s + rows - 1) / rows;
       for (int r = 1; r <= most; r *= 2)
-        if (need <= r && (r <= most / 2 || t == 1024)) {
+        if (need <= r) {
           p.r = r, p.threads = t, p.block = block;
           break;
         }
@@ -634,7 +684,7 @@ void backward(Args& A, const Plan& p, float* dweight, float* dbias, hipStream_t 
     SMQ_GN_V(T, SMQ_GN_STREAM, stream_backward, 0);
   }
   if (dweight || dbias)
-    hipLaunchKernelGGL(param_sums, dim3((A.c + 63) / 64), dim3(256), 0, st, A.chan, A.n, A.c, dweight, dbias);
+    hipLaunchKernelGGL(param_sums, dim3((A.c + 63) / 64), dim3(1024), 0, st, A.chan, A.n, A.c, dweight, dbias);
 }
 
 int validate(const char* who, int dtype, int64_t n, int64_t s, int64_t c, int64_t groups, int act) {
