@@ -93,7 +93,7 @@ struct Args {
   float* rstd;
   float2* part;  // streaming: [n, chunks, channels]
   float2* coef;  // streaming backward: [n, groups] (c1, c2)
-  float2* chan;  // backward: [n, channels] sums of dz, dz xhat
+  float2* chan;  // [n, channels]: streaming forward (mul, add) of z = x mul + add, backward sums of dz, dz xhat
   int64_t s;     // positions
   int n, c, groups, cg;
   int block;   // channels a workgroup covers
@@ -139,6 +139,19 @@ __device__ __forceinline__ float group_sum(const float* sh, const float* scale, 
   return s;
 }
 
+// Groups of adjacent channels, one division for all of them.
+struct Groups {
+  int g, left, cg;
+  __device__ __forceinline__ Groups(int channel, int cg_) : g(channel / cg_), cg(cg_) {
+    left = cg - (channel - g * cg);
+  }
+  __device__ __forceinline__ int next() {
+    const int at = g;
+    if (--left == 0) left = cg, g++;
+    return at;
+  }
+};
+
 // ---- resident -----------------------------------------------------------------------------------
 // Dynamic LDS: blockDim * V floats, then 2 floats per group of the block.
 template <typename T, int V, int R>
@@ -176,10 +189,14 @@ __global__ __launch_bounds__(1024) void resident_forward(Args A) {
     if (lane == 0) stat[g] = s * inv;
   }
   __syncthreads();
+  const Groups own(col * V, A.cg);
+  {
+    Groups at_group = own;
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    mean[i] = stat[(col * V + i) / A.cg];
-    sum[i] = 0.0f;
+    for (int i = 0; i < V; i++) {
+      mean[i] = stat[at_group.next()];
+      sum[i] = 0.0f;
+    }
   }
 #pragma unroll
   for (int k = 0; k < R; k++)
@@ -202,10 +219,11 @@ __global__ __launch_bounds__(1024) void resident_forward(Args A) {
   }
   __syncthreads();
   float mul[V], add[V];
+  Groups at_group = own;
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int c = c0 + col * V + i;
-    rstd[i] = stat[groups + (col * V + i) / A.cg];
+    rstd[i] = stat[groups + at_group.next()];
     mul[i] = (A.weight ? A.weight[active ? c : 0] : 1.0f) * rstd[i];
     add[i] = A.bias ? A.bias[active ? c : 0] : 0.0f;
   }
@@ -250,10 +268,12 @@ __global__ __launch_bounds__(1024) void resident_backward(Args A) {
   }
   // d = x - mean; z = d mul + b; sums of dz and dz d (times rstd: dz xhat)
   float mean[V], rstd[V], mul[V], b[V], p1[V], p2[V];
+  const Groups own(col * V, A.cg);
+  Groups at_group = own;
 #pragma unroll
   for (int i = 0; i < V; i++) {
     const int c = active ? c0 + col * V + i : 0;
-    const int64_t g = (int64_t)blockIdx.y * A.groups + c / A.cg;
+    const int64_t g = (int64_t)blockIdx.y * A.groups + c0 / A.cg + at_group.next();
     mean[i] = A.mean[g], rstd[i] = A.rstd[g];
     mul[i] = (A.weight ? A.weight[c] : 1.0f) * rstd[i];
     b[i] = A.bias ? A.bias[c] : 0.0f;
@@ -300,9 +320,10 @@ __global__ __launch_bounds__(1024) void resident_backward(Args A) {
   }
   __syncthreads();
   // dx = rstd (dz w - c1 - xhat c2) = dz mul - rstd c1 - d rstd^2 c2
+  at_group = own;
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const int g = (col * V + i) / A.cg;
+    const int g = at_group.next();
     p1[i] = -rstd[i] * stat[g], p2[i] = -rstd[i] * rstd[i] * stat[groups + g];
   }
 #pragma unroll
@@ -408,12 +429,20 @@ __global__ __launch_bounds__(256) void join_stats(Args A) {
   __shared__ double a[4], b[4];
   if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = s, b[threadIdx.x >> 6] = q;
   __syncthreads();
+  // every thread: the group's statistics, then its channels' mul = w rstd, add = b - mean mul (its rounding,
+  // 2^-24 |mean mul|, is that of the mean itself)
+  const double m = (double)A.s * A.cg;
+  s = ((a[0] + a[1]) + (a[2] + a[3])) / m;
+  q = ((b[0] + b[1]) + (b[2] + b[3])) / m - s * s;
+  const double rstd = 1.0 / sqrt((q < 0.0 ? 0.0 : q) + (double)A.eps);
   if (threadIdx.x == 0) {
-    const double m = (double)A.s * A.cg;
-    s = ((a[0] + a[1]) + (a[2] + a[3])) / m;
-    q = ((b[0] + b[1]) + (b[2] + b[3])) / m - s * s;
     A.mean[(int64_t)n * A.groups + g] = (float)s;
-    A.rstd[(int64_t)n * A.groups + g] = (float)(1.0 / sqrt((q < 0.0 ? 0.0 : q) + (double)A.eps));
+    A.rstd[(int64_t)n * A.groups + g] = (float)rstd;
+  }
+  for (int i = threadIdx.x; i < A.cg; i += 256) {
+    const float mul = (float)((A.weight ? (double)A.weight[c0 + i] : 1.0) * rstd);
+    A.chan[(int64_t)n * A.c + c0 + i] =
+        make_float2(mul, (float)((A.bias ? (double)A.bias[c0 + i] : 0.0) - s * (double)mul));
   }
 }
 
@@ -425,13 +454,16 @@ __global__ __launch_bounds__(256) void stream_forward(Args A) {
   const int64_t base = (int64_t)blockIdx.z * A.s * A.c + w.c;
   const T* x = reinterpret_cast<const T*>(A.x) + base;
   T* y = reinterpret_cast<T*>(A.y) + base;
-  float mean[V], mul[V], add[V];
+  float mul[V], add[V];
+  const float2* coef = A.chan + (int64_t)blockIdx.z * A.c + w.c;
+  if constexpr (V == 1) {
+    mul[0] = coef->x, add[0] = coef->y;
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; i++) {
-    const int64_t g = (int64_t)blockIdx.z * A.groups + (w.c + i) / A.cg;
-    mean[i] = A.mean[g];
-    mul[i] = (A.weight ? A.weight[w.c + i] : 1.0f) * A.rstd[g];
-    add[i] = A.bias ? A.bias[w.c + i] : 0.0f;
+    for (int i = 0; i < V; i += 2) {
+      const float4 q = *reinterpret_cast<const float4*>(coef + i);
+      mul[i] = q.x, add[i] = q.y, mul[i + 1] = q.z, add[i + 1] = q.w;
+    }
   }
 #pragma unroll 4
   for (int64_t r = w.first + w.row; r < w.last; r += w.rows) {
@@ -439,7 +471,7 @@ __global__ __launch_bounds__(256) void stream_forward(Args A) {
     vec o;
     float z[V];
 #pragma unroll
-    for (int i = 0; i < V; i++) z[i] = fmaf(at<T, V>(v, i) - mean[i], mul[i], add[i]);
+    for (int i = 0; i < V; i++) z[i] = fmaf(at<T, V>(v, i), mul[i], add[i]);
     act_of<V>(A.act, z);
 #pragma unroll
     for (int i = 0; i < V; i++) put<T, V>(o, i, z[i]);
@@ -460,9 +492,10 @@ __global__ __launch_bounds__(256) void stream_sums(Args A) {
     const T* x = reinterpret_cast<const T*>(A.x) + base;
     const T* dy = reinterpret_cast<const T*>(A.dy) + base;
     float mean[V], rstd[V], mul[V], b[V];
+    Groups at_group(w.c, A.cg);
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const int64_t g = (int64_t)blockIdx.z * A.groups + (w.c + i) / A.cg;
+      const int64_t g = (int64_t)blockIdx.z * A.groups + at_group.next();
       mean[i] = A.mean[g], rstd[i] = A.rstd[g];
       mul[i] = (A.weight ? A.weight[w.c + i] : 1.0f) * rstd[i];
       b[i] = A.bias ? A.bias[w.c + i] : 0.0f;
@@ -528,9 +561,10 @@ __global__ __launch_bounds__(256) void stream_backward(Args A) {
   const T* dy = reinterpret_cast<const T*>(A.dy) + base;
   T* dx = reinterpret_cast<T*>(A.y) + base;
   float mean[V], mul[V], b[V], c1[V], c2[V];
+  Groups at_group(w.c, A.cg);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const int64_t g = (int64_t)blockIdx.z * A.groups + (w.c + i) / A.cg;
+    const int64_t g = (int64_t)blockIdx.z * A.groups + at_group.next();
     const float rstd = A.rstd[g];
     const float2 k = A.coef[g];
     mean[i] = A.mean[g];
@@ -615,13 +649,15 @@ Plan plan_of(int dtype, int v, int64_t n, int64_t s, int c, int cg, bool backwar
     int block = unit;
     while (block * size < 64 && c % (block * 2) == 0 && block * 2 / v <= 1024) block *= 2;
     const int cols = block / v;
-    // small workgroups of full threads first: several on a CU overlap their loads and their sums
+    // Small workgroups of full threads first: several on a CU overlap their loads and their sums. A grid
+    // that leaves CUs idle takes large ones of short threads instead.
+    const bool few = n * (c / block) < 256;
     for (int t = 256; t <= 1024 && !p.r; t *= 2) {
       const int rows = t / cols;
       if (rows < 1) continue;
       const int64_t need = (s + rows - 1) / rows;
       for (int r = 1; r <= most; r *= 2)
-        if (need <= r) {
+        if (need <= r && (!few || r <= 2 || t == 1024)) {
           p.r = r, p.threads = t, p.block = block;
           break;
         }
@@ -720,7 +756,7 @@ size_t workspace(int dtype, int64_t n, int64_t s, int c, int cg, bool backward, 
   }
   parts = align_up(parts);
   const size_t coef = backward ? align_up((size_t)n * (c / cg) * sizeof(float2)) : 0;
-  const size_t chan = backward ? align_up((size_t)n * c * sizeof(float2)) : 0;
+  const size_t chan = backward || parts ? align_up((size_t)n * c * sizeof(float2)) : 0;
   if (A) {
     char* p = reinterpret_cast<char*>(ws);
     A->part = reinterpret_cast<float2*>(p);
