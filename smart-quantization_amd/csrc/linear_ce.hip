@@ -34,17 +34,23 @@ struct Head {
 };
 
 // ---- largest magnitude of a tensor -> exponent ---------------------------------------------------
+// Workgroups below gh take h [tokens, dim], the others w [vocab, dim].
 template <typename T>
-__global__ __launch_bounds__(256) void absmax_kernel(const T* x, int64_t ld, int64_t rows, int cols,
+__global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, int64_t tokens, const T* w,
+                                                     int64_t ldw, int64_t vocab, int cols, int gh,
                                                      float* part) {
   constexpr int V = 16 / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(V)));
+  const bool first = (int)blockIdx.x < gh;
+  const T* x = first ? h : w;
+  const int64_t ld = first ? ldh : ldw, rows = first ? tokens : vocab;
+  const int block = first ? blockIdx.x : blockIdx.x - gh, blocks = first ? gh : gridDim.x - gh;
   float top = 0.0f;
-  const int64_t stride = (int64_t)gridDim.x * 4;
   const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % V == 0;
   const int whole = wide ? cols / V * V : 0;
-  for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += stride) {
+  for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)blocks * 4) {
     const T* p = x + r * ld;
+#pragma unroll 2
     for (int k = (threadIdx.x & 63) * V; k < whole; k += 64 * V) {
       const vec v = *reinterpret_cast<const vec*>(p + k);
 #pragma unroll
@@ -53,10 +59,10 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* x, int64_t ld, int
     for (int k = whole + (threadIdx.x & 63); k < cols; k += 64) top = fmaxf(top, fabsf((float)p[k]));
   }
   top = wave_max_dpp(top);
-  __shared__ float w[4];
-  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = top;
+  __shared__ float m[4];
+  if ((threadIdx.x & 63) == 0) m[threadIdx.x >> 6] = top;
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 // Exponent e with max * 2^e in [2^13, 2^14): room for the fp16 planes and for sums of their products.
@@ -67,20 +73,24 @@ __device__ int plane_exponent(float top) {
   const int k = 14 - e;
   return k > 120 ? 120 : k;
 }
-__global__ __launch_bounds__(256) void exponent_kernel(const float* ph, int nh, const float* pw, int nw,
-                                                       Head* head) {
-  __shared__ float w[8];
+// The exponents of both tensors from their partial maxima (gh, then gw of them), by one workgroup of up to
+// 16 waves.
+__device__ void exponents_of(const float* part, int gh, int gw, Head* head) {
+  __shared__ float mh[16], mw[16];
   float a = 0.0f, b = 0.0f;
-  for (int i = threadIdx.x; i < nh; i += 256) a = fmaxf(a, ph[i]);
-  for (int i = threadIdx.x; i < nw; i += 256) b = fmaxf(b, pw[i]);
+  for (int i = threadIdx.x; i < gh; i += blockDim.x) a = fmaxf(a, part[i]);
+  for (int i = threadIdx.x; i < gw; i += blockDim.x) b = fmaxf(b, part[gh + i]);
   a = wave_max_dpp(a), b = wave_max_dpp(b);
-  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = a, w[4 + (threadIdx.x >> 6)] = b;
+  if ((threadIdx.x & 63) == 0) mh[threadIdx.x >> 6] = a, mw[threadIdx.x >> 6] = b;
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int eh = plane_exponent(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
-    const int ew = plane_exponent(fmaxf(fmaxf(w[4], w[5]), fmaxf(w[6], w[7])));
+    for (int k = 1; k < (int)(blockDim.x >> 6); k++) a = fmaxf(a, mh[k]), b = fmaxf(b, mw[k]);
+    const int eh = plane_exponent(a), ew = plane_exponent(b);
     head->exp_h = eh, head->exp_w = ew, head->exp_out = -(eh + ew);
   }
+}
+__global__ __launch_bounds__(256) void exponent_kernel(const float* part, int gh, int gw, Head* head) {
+  exponents_of(part, gh, gw, head);
 }
 
 // exp(x) for x <= about 0, within 2 ulp: the product with log2(e) is carried in two parts (a single
@@ -261,50 +271,52 @@ __global__ __launch_bounds__(256) void few_kernel(const T* h, int64_t ldh, const
 }
 
 // ---- joining the blocks -------------------------------------------------------------------------
-// R rows a workgroup (a power of two up to 16), 256 / R threads share a row's tiles. A target that is
-// neither ignored nor in [0, vocab) gives NaN (nothing is read for it).
-__global__ __launch_bounds__(256) void join_kernel(const float2* part, int blocks, int rows, int R,
-                                                   const int64_t* target, int64_t ignore,
-                                                   int64_t vocab, const float* picked, float* lse,
-                                                   float* row_loss) {
-  const int r = threadIdx.x & (R - 1), m = blockIdx.x * R + r;
+// A row's joined statistics: R rows a workgroup (a power of two), blockDim / R threads share a row's
+// blocks. Returns in the first R threads. A target that is neither ignored nor in [0, vocab) gives NaN
+// (nothing is read for it).
+__device__ __forceinline__ void join_row(const float2* part, int blocks, int rows, int R, int m,
+                                         const int64_t* target, int64_t ignore, int64_t vocab,
+                                         const float* picked, float2* sh, float* lse, float* loss) {
   const float ninf = -__builtin_inff();
+  const int share = blockDim.x / R;
   float top = ninf, sum = 0.0f;
-  if (m < rows)
-    for (int k = threadIdx.x / R; k < blocks; k += 256 / R) {
+  if (m < rows) {
+#pragma unroll 4
+    for (int k = threadIdx.x / R; k < blocks; k += share) {
       const float2 p = part[(int64_t)k * rows + m];
       const float t = fmaxf(top, p.x), at = t == ninf ? 0.0f : t;
       sum = sum * exp_near(top - at) + p.y * exp_near(p.x - at);
       top = t;
     }
-  __shared__ float2 sh[256];
+  }
   sh[threadIdx.x] = make_float2(top, sum);
-  for (int h = 128; h >= R; h >>= 1) {
+  for (int h = blockDim.x / 2; h >= R; h >>= 1) {
     __syncthreads();
-    if (threadIdx.x < h) {
+    if ((int)threadIdx.x < h) {
       const float2 a = sh[threadIdx.x], b = sh[threadIdx.x + h];
       const float t = fmaxf(a.x, b.x), at = t == ninf ? 0.0f : t;
       sh[threadIdx.x] = make_float2(t, a.y * exp_near(a.x - at) + b.y * exp_near(b.x - at));
     }
   }
-  if (threadIdx.x >= R || m >= rows) return;
+  if ((int)threadIdx.x >= R || m >= rows) return;
   const float2 a = sh[threadIdx.x];
   const float l = (a.x == ninf ? 0.0f : a.x) + logf(a.y);
-  lse[m] = l;
+  *lse = l;
   const int64_t y = target[m];
-  row_loss[m] = y == ignore ? 0.0f : y >= 0 && y < vocab ? l - picked[m] : __builtin_nanf("");
+  *loss = y == ignore ? 0.0f : y >= 0 && y < vocab ? l - picked[m] : __builtin_nanf("");
+}
+__global__ __launch_bounds__(256) void join_kernel(const float2* part, int blocks, int rows, int R,
+                                                   const int64_t* target, int64_t ignore,
+                                                   int64_t vocab, const float* picked, float* lse,
+                                                   float* row_loss) {
+  __shared__ float2 sh[256];
+  const int m = blockIdx.x * R + (threadIdx.x & (R - 1));
+  join_row(part, blocks, rows, R, m, target, ignore, vocab, picked, sh, lse + m, row_loss + m);
 }
 
-// One workgroup: the loss over rows (fp64 sums in a fixed order) and the count of rows taking part.
-__global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const int64_t* target,
-                                                    int64_t ignore, int rows, int reduction,
-                                                    float* loss, Head* head) {
-  double s = 0.0, c = 0.0;
-  for (int m = threadIdx.x; m < rows; m += 1024) {
-    s += (double)row_loss[m];
-    c += target[m] != ignore ? 1.0 : 0.0;
-    if (reduction == SMQ_REDUCE_NONE) loss[m] = row_loss[m];
-  }
+// The loss over rows (fp64 sums in a fixed order) and the count of rows taking part, from each thread's
+// sums; one workgroup of 16 waves.
+__device__ __forceinline__ void finish_loss(double s, double c, int reduction, float* loss, Head* head) {
   s = wave_sum(s), c = wave_sum(c);
   __shared__ double a[16], b[16];
   if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = s, b[threadIdx.x >> 6] = c;
@@ -317,51 +329,76 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
     if (reduction == SMQ_REDUCE_SUM) *loss = (float)s;
   }
 }
+__global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const int64_t* target,
+                                                    int64_t ignore, int rows, int reduction,
+                                                    float* loss, Head* head) {
+  double s = 0.0, c = 0.0;
+  for (int m = threadIdx.x; m < rows; m += 1024) {
+    s += (double)row_loss[m];
+    c += target[m] != ignore ? 1.0 : 0.0;
+    if (reduction == SMQ_REDUCE_NONE) loss[m] = row_loss[m];
+  }
+  finish_loss(s, c, reduction, loss, head);
+}
+// Both in one workgroup, where the partial statistics are few.
+__global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int blocks, int rows, int R,
+                                                         const int64_t* target, int64_t ignore,
+                                                         int64_t vocab, const float* picked, float* lse,
+                                                         int reduction, float* loss, Head* head) {
+  __shared__ float2 sh[1024];
+  const int m = threadIdx.x & (R - 1);
+  float l, value;
+  join_row(part, blocks, rows, R, m, target, ignore, vocab, picked, sh, &l, &value);
+  double s = 0.0, c = 0.0;
+  if ((int)threadIdx.x < R && m < rows) {
+    lse[m] = l;
+    if (reduction == SMQ_REDUCE_NONE) loss[m] = value;
+    s = (double)value;
+    c = target[m] != ignore ? 1.0 : 0.0;
+  }
+  finish_loss(s, c, reduction, loss, head);
+}
 
 // ---- backward -----------------------------------------------------------------------------------
-// One workgroup: the rows' factors relative to their largest magnitude, and what comes off again in
-// the epilogues. Ignored rows get 0.
+// One workgroup: the exponents of the operands (part: their maxima, NULL: none), the rows' factors relative
+// to their largest magnitude, and what comes off again in the epilogues. Ignored rows get 0, rows whose
+// gradient is not finite that gradient itself.
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
                                                       int64_t ignore, int rows, int reduction,
-                                                      float* g, const Head* head, const Head* planes,
-                                                      Head* out) {
+                                                      float* g, const Head* head, const float* part,
+                                                      int gh, int gw, Head* out) {
   __shared__ float w[16];
   __shared__ float all;
-  float top = 0.0f;
-  bool bad = false;
+  if (part) exponents_of(part, gh, gw, out);
+  const float inf = __builtin_inff();
+  float top = 0.0f, one = 0.0f;
   if (reduction == SMQ_REDUCE_NONE) {
-    for (int m = threadIdx.x; m < rows; m += 1024)
-      if (target[m] != ignore) {
-        top = fmaxf(top, fabsf(grad[m]));
-        bad |= !(fabsf(grad[m]) < __builtin_inff());
-      }
-  } else if (threadIdx.x == 0) {
+    for (int m = threadIdx.x; m < rows; m += 1024) {
+      const float a = fabsf(grad[m]);
+      if (target[m] != ignore && a < inf) top = fmaxf(top, a);
+    }
+  } else {
     // no row takes part: no gradient
-    const float v = reduction == SMQ_REDUCE_SUM ? *grad
-                    : head->count > 0.0         ? (float)((double)*grad / head->count) : 0.0f;
-    top = fabsf(v);
-    bad = !(top < __builtin_inff());
+    one = reduction == SMQ_REDUCE_SUM ? *grad
+          : head->count > 0.0         ? (float)((double)*grad / head->count) : 0.0f;
+    top = fabsf(one) < inf ? fabsf(one) : 0.0f;
   }
-  if (bad) top = __builtin_inff();
   top = wave_max_dpp(top);
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int k = 1; k < 16; k++) top = fmaxf(top, w[k]);
+    if (top == 0.0f) top = 1.0f;  // all zeros, or nothing finite
     all = top;
-    out->scale_dh = ldexpf(top / kDlScale, planes ? -planes->exp_w : 0);
-    out->scale_dw = ldexpf(top / kDlScale, planes ? -planes->exp_h : 0);
+    out->scale_dh = ldexpf(top / kDlScale, part ? -out->exp_w : 0);
+    out->scale_dw = ldexpf(top / kDlScale, part ? -out->exp_h : 0);
     out->scale_db = top / kDlScale;
   }
   __syncthreads();
   top = all;
   for (int m = threadIdx.x; m < rows; m += 1024) {
-    float v = 0.0f;
-    if (target[m] != ignore && top > 0.0f) {
-      if (reduction == SMQ_REDUCE_NONE) v = grad[m] / top;
-      else v = *grad < 0.0f ? -1.0f : 1.0f;
-    }
-    g[m] = v * kDlScale;
+    const float v = reduction == SMQ_REDUCE_NONE ? grad[m] : one;
+    g[m] = target[m] != ignore ? v / top * kDlScale : 0.0f;
   }
 }
 
@@ -462,14 +499,12 @@ void layout(const void* src, int dtype, int64_t ld, int64_t rows, int64_t cols, 
     launch_layout((const __bf16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st);
 }
 
-// exponents of both inputs' fp16 operands -> *head (part: room for 2 * kMaxParts floats)
+// The partial maxima of both inputs, absmax_grid of the tokens and of the vocabulary.
 template <typename T>
-void exponents(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, float* part, Head* head,
-               hipStream_t st) {
+void maxima(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, float* part, hipStream_t st) {
   const int gh = absmax_grid(s.tokens), gw = absmax_grid(s.vocab);
-  hipLaunchKernelGGL(absmax_kernel<T>, dim3(gh), dim3(256), 0, st, h, ldh, s.tokens, (int)s.dim, part);
-  hipLaunchKernelGGL(absmax_kernel<T>, dim3(gw), dim3(256), 0, st, w, ldw, s.vocab, (int)s.dim, part + kMaxParts);
-  hipLaunchKernelGGL(exponent_kernel, dim3(1), dim3(256), 0, st, part, gh, part + kMaxParts, gw, head);
+  hipLaunchKernelGGL(absmax_kernel<T>, dim3(gh + gw), dim3(256), 0, st, h, ldh, s.tokens, w, ldw, s.vocab,
+                     (int)s.dim, gh, part);
 }
 
 template <typename Epi>
@@ -481,20 +516,20 @@ void product(int dtype, int tile, const Operand& A, const Operand& B, int kt, in
 }
 
 // [rows, cols] in operand form: in place where it can be, else laid out in the workspace.
-// `turned` (absent: fmt kNone) is written transposed along the way, in one pass over p where both go by
+// Rows whose keep[row] is `skip` become zeros (keep NULL: none). `turned` (absent: fmt kNone) is written transposed along the way, in one pass over p where both go by
 // the same exponent (float32) or none.
 Operand operand(Arena& ws, const void* p, int64_t ld, int64_t rows, int64_t cols, const Shape& s,
-                const int* exponent, const int* turned_exponent, const Mat& turned, bool run,
-                hipStream_t st) {
+                const int* exponent, const int* turned_exponent, const int64_t* keep, int64_t skip,
+                const Mat& turned, bool run, hipStream_t st) {
   const bool in_place = direct(p, ld, cols, s.dtype);
   const bool once = !in_place && exponent == turned_exponent;
   if (run && turned.fmt != kNone && !once)
-    layout(p, s.dtype, ld, rows, cols, turned_exponent, nullptr, 0, kNoMat, turned, st);
+    layout(p, s.dtype, ld, rows, cols, turned_exponent, keep, skip, kNoMat, turned, st);
   if (in_place) return {p, ld, 0, (int)rows};
   const int64_t to = operand_ld(cols, s.split());
   _Float16* q = ws.take<_Float16>((size_t)(rows * to));
   if (run)
-    layout(p, s.dtype, ld, rows, cols, exponent, nullptr, 0,
+    layout(p, s.dtype, ld, rows, cols, exponent, keep, skip,
            {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, once ? turned : kNoMat, st);
   return {q, to, 0, (int)rows};
 }
@@ -570,7 +605,11 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
   if (s.split() && !few) {
     float* top = a.take<float>(2 * kMaxParts);
     exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
-    if (run) exponents((const float*)h, ldh, (const float*)w, ldw, s, top, head, st);
+    if (run) {
+      maxima((const float*)h, ldh, (const float*)w, ldw, s, top, st);
+      hipLaunchKernelGGL(exponent_kernel, dim3(1), dim3(256), 0, st, top, absmax_grid(s.tokens),
+                         absmax_grid(s.vocab), head);
+    }
   }
   if (few) {
     if (run) {
@@ -579,17 +618,24 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
       else launch_few<__bf16>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
     }
   } else {
-    const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, kNoMat, run, st);
-    const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, kNoMat, run, st);
+    const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, nullptr, 0, kNoMat, run, st);
+    const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, nullptr, 0, kNoMat, run, st);
     const SoftmaxEpi e = {exponent, bias, target, part, picked};
     if (run) product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
   }
   if (run) {
-    const int per = s.tokens >= 2048 ? 16 : s.tokens >= 256 ? 4 : 1;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + per - 1) / per)), dim3(256), 0, st, part,
-                       blocks, (int)s.tokens, per, target, ignore, s.vocab, picked, lse, rows);
-    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
-                       reduction, loss, head);
+    int per = 1;
+    if (s.tokens <= 1024 && s.tokens * blocks <= 16384) {
+      while (per < s.tokens) per *= 2;
+      hipLaunchKernelGGL(join_loss_kernel, dim3(1), dim3(1024), 0, st, part, blocks, (int)s.tokens, per,
+                         target, ignore, s.vocab, picked, lse, reduction, loss, head);
+    } else {
+      per = s.tokens >= 2048 ? 16 : s.tokens >= 256 ? 4 : 1;
+      hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + per - 1) / per)), dim3(256), 0, st, part,
+                         blocks, (int)s.tokens, per, target, ignore, s.vocab, picked, lse, rows);
+      hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
+                         reduction, loss, head);
+    }
   }
   return a.used;
 }
@@ -641,27 +687,26 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   float* g = a.take<float>(s.tokens);
   Head* fac = a.take<Head>(1);
   const Head* planes = s.dtype == SMQ_DTYPE_F16 ? nullptr : fac;
+  float* top = nullptr;
   if (planes) {
-    float* top = a.take<float>(2 * kMaxParts);
-    if (run && sp) exponents((const float*)h, ldh, (const float*)w, ldw, s, top, fac, st);
-    else if (run) exponents((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, fac, st);
+    top = a.take<float>(2 * kMaxParts);
+    if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, top, st);
+    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, st);
   }
   const int* exponent = sp ? &fac->exp_out : nullptr;
   const int* eh = planes ? &planes->exp_h : nullptr;
   const int* ew = planes ? &planes->exp_w : nullptr;
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
-                       (int)s.tokens, reduction, g, head, planes, fac);
-  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, nullptr, kNoMat, run, st);
-  // h transposed: the operand of dw. Ignored rows are zeros, whatever they hold.
+                       (int)s.tokens, reduction, g, head, top, absmax_grid(s.tokens),
+                       absmax_grid(s.vocab), fac);
+  // h, and transposed the operand of dw. Ignored rows are zeros, whatever they hold (where h is read in
+  // place its ignored rows' logits are not used).
   const int64_t ldt = operand_ld(s.tokens, sp);
   const int padt = operand_pad(s.tokens, sp);
-  _Float16* ht = nullptr;
-  if (dw) {
-    ht = a.take<_Float16>((size_t)(s.dim * ldt));
-    if (run)
-      layout(h, s.dtype, ldh, s.tokens, s.dim, eh, target, ignore, kNoMat, {ht, ldt, 0, fmt, padt}, st);
-  }
+  _Float16* ht = dw ? a.take<_Float16>((size_t)(s.dim * ldt)) : nullptr;
+  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, eh, target, ignore,
+                            dw ? Mat{ht, ldt, 0, fmt, padt} : kNoMat, run, st);
   const int64_t ldp = operand_ld(s.piece, sp);
   _Float16* dl = a.take<_Float16>((size_t)(s.tokens * ldp));
   _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
@@ -682,7 +727,7 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     const int64_t v0 = i * s.piece, n = s.vocab - v0 < s.piece ? s.vocab - v0 : s.piece;
     const char* wp = reinterpret_cast<const char*>(w) + (size_t)(v0 * ldw) * wsize;
     const int padn = operand_pad(n, sp);
-    const Operand B = operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew,
+    const Operand B = operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew, nullptr, 0,
                               dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat, run, st);
     if (a.used > most) most = a.used;
     if (!run) continue;
