@@ -647,20 +647,42 @@ static inline int64_t tile_count(int64_t m, int64_t n, int t, int tri) {
   const int64_t a = (m + s.bm - 1) / s.bm, b = (n + s.bn - 1) / s.bn;
   return tri ? a * (a + 1) / 2 : a * b;
 }
-// How full the last round of `wgs` workgroups on `slots` places is, over all rounds.
-static inline double fill_of(int64_t wgs, int64_t slots) {
-  return (double)wgs / (double)((wgs + slots - 1) / slots * slots);
+// Tile and shares of the k range for C [m, n] x batch over kt k tiles, by a cost in units of 28 ps: what a
+// CU needs for one element of C and one k tile at the rate of 256 x 256 tiles. A round of workgroups
+// costs its tile's area over the tile's relative rate (measured: 128 x 128 0.87 with two workgroups a CU,
+// 0.75 with one, 64 x 64 0.6 and 0.4, and so 32 x 128 by its area); rows and columns past the edge cost as
+// much as others, so a short m takes short tiles. Sharing k costs a pass over the partial sums (0.07 an
+// element and share) and a launch. 2048 x 768 over 938: 10 shares of 256 x 256 (24 tiles without);
+// 6 x 1024 x 4096 over 32: 128 x 128 in three full rounds (74 us) instead of 256 x 256 in two (81 us).
+struct Shared {
+  int tile, shares;
+};
+static inline Shared plan_product(int64_t m, int64_t n, int64_t kt, int64_t batch, int tri, bool share,
+                                  bool big = true) {
+  Shared best = {kT64, 1};
+  double least = -1.0;
+  const int most = !share || kt < 16 ? 1 : (int)(kt / 8 > 64 ? 64 : kt / 8);
+  auto look = [&](int tile, int64_t slots, double one, double both) {
+    const int64_t count = batch * tile_count(m, n, tile, tri);
+    for (int s = 1; s <= most; s++) {
+      const int64_t wgs = count * s;
+      const double rounds = wgs <= 256 ? one : both * (double)((wgs + slots - 1) / slots);
+      double cost = rounds * (double)((kt + s - 1) / s);
+      if (s > 1) cost += 0.07 * (double)s * (double)(batch * m * n) + 175e3;
+      if (least < 0.0 || cost < least) least = cost, best = {tile, s};
+      if (wgs >= 2 * slots) break;
+    }
+  };
+  if (big) look(kT256, 256, 65536.0, 65536.0);
+  look(kT128, 512, 21845.0, 37664.0);
+  if (best.tile == kT128 && batch * tile_count(m, n, kT128, tri) * best.shares <= 256) best.tile = kDeep;
+  const Shared before = best;
+  look(kT64, 512, 10240.0, 13650.0);
+  if (best.tile != kT64) best = before;
+  if (m <= 32 && !tri) look(kSkinny, 256, 10240.0, 10240.0);
+  return best;
 }
-// 256 x 256 or 128 x 128 (0.87 of its rate, two workgroups a CU) by how full their rounds are: 6 x 1024 x
-// 4096 x 1024 is 384 of the former in two rounds (81 us) and 1536 of the latter in three (74 us).
-static inline int choose_tile(int64_t m, int64_t n, int64_t batch, int tri) {
-  if (m <= 32 && !tri) return kSkinny;
-  const int64_t big = batch * tile_count(m, n, kT256, tri), mid = batch * tile_count(m, n, kT128, tri);
-  if (big >= 128 && fill_of(big, 256) >= 0.87 * fill_of(mid, 512)) return kT256;
-  if (mid >= 384) return kT128;
-  if (mid >= 128) return kDeep;
-  return kT64;
-}
+
 template <typename H, int BM, int BN, int WM, int WN, bool DEEP, bool SPLIT, typename Epi>
 static inline void launch_tile(const Operand& A, const Operand& B, int kt, int batch, int tri,
                                int shares, const Epi& epi, hipStream_t st) {

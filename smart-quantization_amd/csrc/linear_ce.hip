@@ -592,7 +592,7 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
                     const int64_t* target, const float* bias, int64_t ignore, int reduction,
                     float* loss, float* lse, Head* head, void* ws, bool run, hipStream_t st) {
   Arena a(ws);
-  const int tile = choose_tile(s.tokens, s.vocab, 1, 0);
+  const int tile = plan_product(s.tokens, s.vocab, operand_kt(s.dim, s.split()), 1, 0, false).tile;
   const TileShape ts = shape_of(tile);
   const int64_t tn = (s.vocab + ts.bn - 1) / ts.bn;
   const int few = few_tokens(h, w, ldw, s);
@@ -640,32 +640,6 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
   return a.used;
 }
 
-// dh has few tiles and a long k range: split over k until its workgroups fill the chip (two rounds of
-// 128 x 128 tiles, one of 256 x 256 where those come near a full one), at least 8 k tiles a share.
-struct DhPlan {
-  int tile, shares;
-};
-DhPlan dh_plan(const Shape& s, int kt) {
-  if (s.tokens <= 32) {
-    const int64_t wgs = tile_count(s.tokens, s.dim, kSkinny, 0);
-    const int64_t k = (512 + wgs - 1) / wgs, most = kt / 8 < 1 ? 1 : kt / 8;
-    return {kSkinny, (int)(k < most ? (k > 32 ? 32 : k) : (most > 32 ? 32 : most))};
-  }
-  const int64_t big = tile_count(s.tokens, s.dim, kT256, 0), mid = tile_count(s.tokens, s.dim, kT128, 0);
-  const int most = kt / 8 < 1 ? 1 : kt / 8 > 32 ? 32 : kt / 8;
-  auto best = [&](int64_t wgs, int64_t slots, double* fill) {
-    int k = 1;
-    *fill = 0.0;
-    for (int i = 1; i <= most && wgs * (i - 1) < 2 * slots; i++)
-      if (fill_of(wgs * i, slots) > *fill + 0.02) *fill = fill_of(wgs * i, slots), k = i;
-    return k;
-  };
-  double fb, fm;
-  const int kb = best(big, 256, &fb), km = best(mid, 512, &fm);
-  if (fb >= 0.87 * fm) return {kT256, kb};
-  return {kT128, km};
-}
-
 int64_t default_piece(const Shape& s) {
   const int64_t planes = s.split() ? 2 : 1;
   const int64_t per = 2 * planes * (2 * round_up(s.tokens, 64) + round_up(s.dim, 64));
@@ -711,10 +685,10 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   _Float16* dl = a.take<_Float16>((size_t)(s.tokens * ldp));
   _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
   _Float16* wt = dh ? a.take<_Float16>((size_t)(s.dim * ldp)) : nullptr;
-  const int tile_l = choose_tile(s.tokens, s.piece, 1, 0);
+  const int tile_l = plan_product(s.tokens, s.piece, operand_kt(s.dim, sp), 1, 0, false).tile;
   const int row_blocks = (int)((s.tokens + shape_of(tile_l).bm - 1) / shape_of(tile_l).bm) * shape_of(tile_l).wm;
   float* sums = db ? a.take<float>((size_t)row_blocks * s.piece) : nullptr;
-  const DhPlan dp = dh_plan(s, operand_kt(s.piece, sp));
+  const Shared dp = plan_product(s.tokens, s.dim, operand_kt(s.piece, sp), 1, 0, true);
   const int tile_dh = dp.tile, shares = dp.shares;
   const int64_t ldacc = round_up(s.dim, 4);
   const bool whole = pieces == 1 && shares == 1;
@@ -748,7 +722,7 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
       const Operand L = {dlt, ldt, 0, (int)n}, H = {ht, ldt, 0, (int)s.dim};
       StoreEpi se = {1.0f, 0.0f, &fac->scale_dw, kNoMat, kNoMat, kNoMat, 0, 0, 0.0f};
       se.o = {reinterpret_cast<char*>(dw) + (size_t)(v0 * s.dim) * wsize, s.dim, 0, out_fmt(s.dtype), 0};
-      product(grad_dtype, choose_tile(n, s.dim, 1, 0), L, H, operand_kt(s.tokens, sp), 1, se, st);
+      product(grad_dtype, plan_product(n, s.dim, operand_kt(s.tokens, sp), 1, 0, false).tile, L, H, operand_kt(s.tokens, sp), 1, se, st);
     }
   }
   if (run && dh && !whole) {

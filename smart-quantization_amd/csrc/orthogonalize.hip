@@ -466,14 +466,6 @@ struct Arena {
   }
 };
 
-// Shares of the k range where the tiles alone leave CUs idle: at least 16 k tiles a share, at most 8
-// shares (their sum is a launch of its own, about 16 k tiles long).
-int shares_for(int64_t wgs, int kt) {
-  int64_t k = 288 / (wgs < 1 ? 1 : wgs);
-  if (k > kt / 16) k = kt / 16;
-  return (int)(k < 1 ? 1 : k > 8 ? 8 : k);
-}
-
 struct Buffers {
   _Float16 *x[2], *xt[2], *gram[2], *q[2], *p[2], *w;
   float* part;  // shares of a product split over k
@@ -486,9 +478,8 @@ void product(bool split, const Operand& A, const Operand& B, int kt, int batch, 
   // store costs 2 us, the other half nothing. (Two planes in 256 x 256 tiles round more, gemm_nt.h, and
   // are no faster at these lengths.)
   if (e.tri && batch * tile_count(A.rows, B.rows, kT64, 0) <= 256) e.tri = 0, e.ot.fmt = kNone;
-  int tile = choose_tile(A.rows, B.rows, batch, e.tri);
-  if (split && tile == kT256) tile = kT128;
-  const int shares = tile == kT256 ? 1 : shares_for(batch * tile_count(A.rows, B.rows, tile, e.tri), kt);
+  const Shared plan = plan_product(A.rows, B.rows, kt, batch, e.tri, true, !split);
+  const int tile = plan.tile, shares = plan.shares;
   const int64_t ld = round_up(B.rows, 4), per = (int64_t)A.rows * ld;
   if (shares > 1 && need) {
     const size_t floats = (size_t)shares * batch * per;
