@@ -15,6 +15,8 @@
 // fp16 once scaled (what lies 2^-28 below the largest magnitude loses bits), in the transposed copies
 // that these products need anyway. dl is kept relative to the largest |g| and times 2^14, so that fp16
 // holds probabilities from 4e-9 up in full precision; the factors come off in the fp32 epilogues.
+#include <type_traits>
+
 #include "gemm_nt.h"
 
 namespace smq {
@@ -34,7 +36,8 @@ struct Head {
 };
 
 // ---- largest magnitude of a tensor -> exponent ---------------------------------------------------
-// Workgroups below gh take h [tokens, dim], the others w [vocab, dim].
+// Workgroups below gh take h [tokens, dim], the others w [vocab, dim]. Rows without gaps are read as one,
+// in whole vectors whatever the columns.
 template <typename T>
 __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, int64_t tokens, const T* w,
                                                      int64_t ldw, int64_t vocab, int cols, int gh,
@@ -45,18 +48,31 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, in
   const T* x = first ? h : w;
   const int64_t ld = first ? ldh : ldw, rows = first ? tokens : vocab;
   const int block = first ? blockIdx.x : blockIdx.x - gh, blocks = first ? gh : gridDim.x - gh;
+  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   float top = 0.0f;
-  const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % V == 0;
-  const int whole = wide ? cols / V * V : 0;
-  for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)blocks * 4) {
-    const T* p = x + r * ld;
-#pragma unroll 2
-    for (int k = (threadIdx.x & 63) * V; k < whole; k += 64 * V) {
-      const vec v = *reinterpret_cast<const vec*>(p + k);
+  if (ld == cols && aligned) {
+    const int64_t total = rows * cols, vecs = total / V, step = (int64_t)blocks * 256;
+    const vec* p = reinterpret_cast<const vec*>(x);
+#pragma unroll 4
+    for (int64_t k = block * 256 + threadIdx.x; k < vecs; k += step) {
+      const vec v = p[k];
 #pragma unroll
       for (int i = 0; i < V; i++) top = fmaxf(top, fabsf((float)v[i]));
     }
-    for (int k = whole + (threadIdx.x & 63); k < cols; k += 64) top = fmaxf(top, fabsf((float)p[k]));
+    if (block == 0 && (int)threadIdx.x < total - vecs * V)
+      top = fmaxf(top, fabsf((float)x[vecs * V + threadIdx.x]));
+  } else {
+    const int whole = aligned && ld % V == 0 ? cols / V * V : 0;
+    for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)blocks * 4) {
+      const T* p = x + r * ld;
+#pragma unroll 2
+      for (int k = (threadIdx.x & 63) * V; k < whole; k += 64 * V) {
+        const vec v = *reinterpret_cast<const vec*>(p + k);
+#pragma unroll
+        for (int i = 0; i < V; i++) top = fmaxf(top, fabsf((float)v[i]));
+      }
+      for (int k = whole + (threadIdx.x & 63); k < cols; k += 64) top = fmaxf(top, fabsf((float)p[k]));
+    }
   }
   top = wave_max_dpp(top);
   __shared__ float m[4];
@@ -170,103 +186,259 @@ struct SoftmaxEpi {
   }
 };
 
-// ---- forward of a few tokens ---------------------------------------------------------------------
-// Bound by the one read of the weight: each wave takes kRows vocabulary entries at a time straight from
-// memory in their own type (no fp16 planes are made), 16 bytes a lane, against up to NT rows of hidden
-// kept in LDS as fp32; a token's (maximum, sum) runs along in registers.
+// ---- few tokens -----------------------------------------------------------------------------------
+// Bound by reading the weight (and writing its gradient): each wave takes kRows vocabulary entries at a
+// time straight from memory in their own type (no fp16 planes, no transposed copies), V elements a lane,
+// against up to NT rows of hidden kept in LDS as fp32. Ignored rows are zeros there.
 constexpr int kRows = 4;
+template <typename T, int V> struct FewVec {
+  typedef T type __attribute__((ext_vector_type(V)));
+};
+template <typename T> struct FewVec<T, 1> {
+  typedef T type;
+};
+template <typename T, int V>
+__device__ __forceinline__ void few_load(const T* p, float (&x)[V]) {
+  const typename FewVec<T, V>::type v = *reinterpret_cast<const typename FewVec<T, V>::type*>(p);
+  if constexpr (V == 1) x[0] = (float)v;
+  else {
+#pragma unroll
+    for (int i = 0; i < V; i++) x[i] = (float)v[i];
+  }
+}
+template <int V>
+__device__ __forceinline__ void few_hidden(const float* p, float (&y)[V]) {
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(p + i);
+      y[i] = q.x, y[i + 1] = q.y, y[i + 2] = q.z, y[i + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) y[i] = p[i];
+  }
+}
 template <typename T, int NT>
-__global__ __launch_bounds__(256) void few_kernel(const T* h, int64_t ldh, const T* w, int64_t ldw,
-                                                  int tokens, int dim, int vocab, const float* bias,
-                                                  const int64_t* target, float2* part, float* picked) {
-  constexpr int V = 16 / sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(V)));
-  extern __shared__ float hs[];  // [NT][dim]
-  __shared__ float2 joint[4][NT];
-  for (int i = threadIdx.x; i < NT * dim; i += 256) {
+__device__ __forceinline__ void few_stage(const T* h, int64_t ldh, int tokens, int dim,
+                                          const int64_t* target, int64_t ignore, float* hs) {
+  for (int i = threadIdx.x; i < NT * dim; i += blockDim.x) {
     const int t = i / dim;
-    hs[i] = t < tokens ? (float)h[(int64_t)t * ldh + (i - t * dim)] : 0.0f;
+    hs[i] = t < tokens && target[t] != ignore ? (float)h[(int64_t)t * ldh + (i - t * dim)] : 0.0f;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float ninf = -__builtin_inff();
-  float top[NT], sum[NT];
+}
+// Which of a step's kRows x NT logits a lane ends with: number (r, t) = (n / NT, n % NT), n = lane >> kSame; its
+// 2^kSame neighbours hold the same one.
+template <int NT> struct FewLane {
+  static constexpr int kCount = kRows * NT;
+  static constexpr int kSame = kCount == 64 ? 0 : kCount == 32 ? 1 : kCount == 16 ? 2 : kCount == 8 ? 3 : 4;
+};
+template <int N, int D>
+__device__ __forceinline__ void fold_lanes(float* acc, int lane) {
+  if constexpr (N > 1) {
+    const bool up = (lane & D) != 0;
 #pragma unroll
-  for (int t = 0; t < NT; t++) top[t] = ninf, sum[t] = 0.0f;
-  for (int v0 = (blockIdx.x * 4 + wave) * kRows; v0 < vocab; v0 += gridDim.x * 4 * kRows) {
-    const T* p[kRows];
+    for (int i = 0; i < N / 2; i++) {
+      const float mine = up ? acc[i + N / 2] : acc[i], theirs = up ? acc[i] : acc[i + N / 2];
+      acc[i] = mine + __shfl_xor(theirs, D, 64);
+    }
+  } else {
+    acc[0] += __shfl_xor(acc[0], D, 64);
+  }
+  if constexpr (D > 1) fold_lanes<(N > 1 ? N / 2 : 1), D / 2>(acc, lane);
+}
+// The logits of entries v0 .. v0 + kRows - 1, one a lane (FewLane), without the bias. The sums over the
+// wave's lanes halve the values held at each exchange: 63 exchanges for 64 values, where a sum apiece in
+// all lanes takes 384, and what follows (exponentials) is done once instead of by all lanes.
+template <typename T, int V, int NT>
+__device__ __forceinline__ float few_logits(const T* w, int64_t ldw, int dim, int vocab, const float* hs,
+                                            int v0, int lane) {
+  constexpr int N = kRows * NT;
+  const T* p[kRows];
 #pragma unroll
-    for (int r = 0; r < kRows; r++) p[r] = w + (int64_t)(v0 + r < vocab ? v0 + r : vocab - 1) * ldw;
-    float acc[kRows][NT];
+  for (int r = 0; r < kRows; r++) p[r] = w + (int64_t)(v0 + r < vocab ? v0 + r : vocab - 1) * ldw;
+  float acc[N];
 #pragma unroll
-    for (int r = 0; r < kRows; r++)
-#pragma unroll
-      for (int t = 0; t < NT; t++) acc[r][t] = 0.0f;
+  for (int i = 0; i < N; i++) acc[i] = 0.0f;
 #pragma unroll 2
-    for (int k = lane * V; k < dim; k += 64 * V) {
-      vec x[kRows];
+  for (int k = lane * V; k < dim; k += 64 * V) {
+    float x[kRows][V];
 #pragma unroll
-      for (int r = 0; r < kRows; r++) x[r] = *reinterpret_cast<const vec*>(p[r] + k);
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        float y[V];
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-          const float4 q = *reinterpret_cast<const float4*>(hs + t * dim + k + i);
-          y[i] = q.x, y[i + 1] = q.y, y[i + 2] = q.z, y[i + 3] = q.w;
-        }
-#pragma unroll
-        for (int r = 0; r < kRows; r++)
-#pragma unroll
-          for (int i = 0; i < V; i++) acc[r][t] = fmaf((float)x[r][i], y[i], acc[r][t]);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; r++) {
-      const int v = v0 + r;
-      const float b = bias && v < vocab ? bias[v] : 0.0f;
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        float s = acc[r][t];
-        s += dpp_f32<kDppXor1>(s);
-        s += dpp_f32<kDppXor2>(s);
-        s += dpp_f32<kDppHalfMirror>(s);
-        s += dpp_f32<kDppMirror>(s);
-        s += __shfl_xor(s, 16, 64);
-        s += __shfl_xor(s, 32, 64);
-        acc[r][t] = v < vocab ? s + b : ninf;
-      }
-    }
+    for (int r = 0; r < kRows; r++) few_load<T, V>(p[r] + k, x[r]);
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      float m = top[t];
+      float y[V];
+      few_hidden<V>(hs + t * dim + k, y);
 #pragma unroll
-      for (int r = 0; r < kRows; r++) m = fmaxf(m, acc[r][t]);
-      const float at = m == ninf ? 0.0f : m;
-      float s = sum[t] * exp_near(top[t] - at);
+      for (int r = 0; r < kRows; r++)
 #pragma unroll
-      for (int r = 0; r < kRows; r++) s += exp_near(acc[r][t] - at);
-      top[t] = m, sum[t] = s;
-      const int64_t y = t < tokens ? target[t] : -1;
-      if (lane == 0 && y >= v0 && y < v0 + kRows && y < vocab) {
+        for (int i = 0; i < V; i++) acc[r * NT + t] = fmaf(x[r][i], y[i], acc[r * NT + t]);
+    }
+  }
+  fold_lanes<N, 32>(acc, lane);
+  return acc[0];
+}
+
+// Forward: each lane keeps the (maximum, sum of exponentials) of its token over its rows.
+template <typename T, int V, int NT>
+__global__ __launch_bounds__(1024) void few_kernel(const T* h, int64_t ldh, const T* w, int64_t ldw,
+                                                   int tokens, int dim, int vocab, const float* bias,
+                                                   const int64_t* target, int64_t ignore, float2* part,
+                                                   float* picked) {
+  extern __shared__ float hs[];  // [NT][dim]
+  __shared__ float2 joint[16][kRows * NT];
+  few_stage<T, NT>(h, ldh, tokens, dim, target, ignore, hs);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int n = lane >> FewLane<NT>::kSame, r = n / NT, t = n % NT;
+  const float ninf = -__builtin_inff();
+  const int64_t y = t < tokens ? target[t] : -1;
+  float top = ninf, sum = 0.0f;
+  for (int v0 = (blockIdx.x * waves + wave) * kRows; v0 < vocab; v0 += gridDim.x * waves * kRows) {
+    float l = few_logits<T, V, NT>(w, ldw, dim, vocab, hs, v0, lane);
+    const int v = v0 + r;
+    if (v < vocab) {
+      if (bias) l += bias[v];
+      if (y == v) picked[t] = l;
+      const float m = fmaxf(top, l), at = m == ninf ? 0.0f : m;
+      sum = sum * exp_near(top - at) + exp_near(l - at);
+      top = m;
+    }
+  }
+  joint[wave][n] = make_float2(top, sum);
+  __syncthreads();
+  if ((int)threadIdx.x < tokens) {
+    float m = ninf, s = 0.0f;
+    for (int k = 0; k < waves; k++)
+      for (int q = 0; q < kRows; q++) m = fmaxf(m, joint[k][q * NT + threadIdx.x].x);
+    const float at = m == ninf ? 0.0f : m;
+    for (int k = 0; k < waves; k++)
+      for (int q = 0; q < kRows; q++) {
+        const float2 b = joint[k][q * NT + threadIdx.x];
+        s += b.y * exp_near(b.x - at);
+      }
+    part[(int64_t)blockIdx.x * tokens + threadIdx.x] = make_float2(m, s);
+  }
+}
+
+// Backward, one read of the weight: dl [vocab, NT] in fp32 (for dh, NULL: not kept), the rows of dw, db.
+template <typename T, int V, int NT>
+__global__ __launch_bounds__(1024) void few_backward_kernel(const T* h, int64_t ldh, const T* w, int64_t ldw,
+                                                            int tokens, int dim, int vocab,
+                                                            const float* bias, const int64_t* target,
+                                                            int64_t ignore, int reduction, const float* lse,
+                                                            const float* grad, const Head* head, float* dl,
+                                                            T* dw, float* db) {
+  typedef typename FewVec<T, V>::type vec;
+  constexpr int kSame = FewLane<NT>::kSame;
+  extern __shared__ float hs[];  // [NT][dim]
+  few_stage<T, NT>(h, ldh, tokens, dim, target, ignore, hs);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int n = lane >> kSame, r = n / NT, t = n % NT;
+  // the lane's token: its factor (a bad target makes it NaN), lse and target
+  float g = 0.0f, ls = 0.0f;
+  int at = -1;
+  if (t < tokens && target[t] != ignore) {
+    g = reduction == SMQ_REDUCE_NONE ? grad[t]
+        : reduction == SMQ_REDUCE_SUM ? *grad : (float)((double)*grad / head->count);
+    ls = lse[t];
+    const int64_t y = target[t];
+    if (y >= 0 && y < vocab) at = (int)y;
+    else g = __builtin_nanf("");
+  }
+  for (int v0 = (blockIdx.x * waves + wave) * kRows; v0 < vocab; v0 += gridDim.x * waves * kRows) {
+    float l = few_logits<T, V, NT>(w, ldw, dim, vocab, hs, v0, lane);
+    const int v = v0 + r;
+    if (bias && v < vocab) l += bias[v];
+    const float p = exp_near(l - ls) - (at == v ? 1.0f : 0.0f);
+    const float d = g == 0.0f ? 0.0f : p * g;
+    if (dl && v < vocab && (lane & ((1 << kSame) - 1)) == 0) dl[(int64_t)v0 * NT + n] = d;
+    if (db) {
+      float total = d;
 #pragma unroll
-        for (int r = 0; r < kRows; r++)
-          if (y == v0 + r) picked[t] = acc[r][t];
+      for (int q = NT / 2; q >= 1; q >>= 1) total += __shfl_xor(total, q << kSame, 64);
+      if (t == 0 && v < vocab) db[v] = total;
+    }
+    if (!dw) continue;
+    float u[kRows][NT];  // wave-uniform
+#pragma unroll
+    for (int i = 0; i < kRows; i++)
+#pragma unroll
+      for (int q = 0; q < NT; q++)
+        u[i][q] = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, d), (i * NT + q) << kSame));
+    for (int k = lane * V; k < dim; k += 64 * V) {
+      float o[kRows][V];
+#pragma unroll
+      for (int i = 0; i < kRows; i++)
+#pragma unroll
+        for (int e = 0; e < V; e++) o[i][e] = 0.0f;
+#pragma unroll
+      for (int q = 0; q < NT; q++) {
+        float y[V];
+        few_hidden<V>(hs + q * dim + k, y);
+#pragma unroll
+        for (int i = 0; i < kRows; i++)
+#pragma unroll
+          for (int e = 0; e < V; e++) o[i][e] = fmaf(u[i][q], y[e], o[i][e]);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; i++)
+        if (v0 + i < vocab) {
+          vec x;
+          if constexpr (V == 1) x = (T)o[i][0];
+          else {
+#pragma unroll
+            for (int e = 0; e < V; e++) x[e] = (T)o[i][e];
+          }
+          *reinterpret_cast<vec*>(dw + (int64_t)(v0 + i) * dim + k) = x;
+        }
+    }
+  }
+}
+
+// dh of a chunk of the vocabulary: 64 V columns a workgroup, whose waves take turns at the chunk's
+// entries and are summed in LDS -> part [chunk][tokens][ld].
+template <typename T, int V, int NT>
+__global__ __launch_bounds__(256) void few_dh_kernel(const float* dl, const T* w, int64_t ldw, int tokens,
+                                                     int dim, int vocab, int64_t ld, float* part) {
+  __shared__ float sh[3][64 * V];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int k = (blockIdx.x * 64 + lane) * V;
+  const int first = (int)((int64_t)vocab * blockIdx.y / gridDim.y);
+  const int last = (int)((int64_t)vocab * (blockIdx.y + 1) / gridDim.y);
+  float acc[NT][V];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[t][i] = 0.0f;
+  if (k < dim) {
+#pragma unroll 4
+    for (int v = first + wave; v < last; v += 4) {
+      float x[V];
+      few_load<T, V>(w + (int64_t)v * ldw + k, x);
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const float d = dl[(int64_t)v * NT + t];
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[t][i] = fmaf(d, x[i], acc[t][i]);
       }
     }
   }
-  if (lane == 0) {
 #pragma unroll
-    for (int t = 0; t < NT; t++) joint[wave][t] = make_float2(top[t], sum[t]);
-  }
-  __syncthreads();
-  if ((int)threadIdx.x < tokens) {
-    const int t = threadIdx.x;
-    float m = ninf, s = 0.0f;
-    for (int k = 0; k < 4; k++) m = fmaxf(m, joint[k][t].x);
-    const float at = m == ninf ? 0.0f : m;
-    for (int k = 0; k < 4; k++) s += joint[k][t].y * exp_near(joint[k][t].x - at);
-    part[(int64_t)blockIdx.x * tokens + t] = make_float2(m, s);
+  for (int t = 0; t < NT; t++) {
+    __syncthreads();
+    if (wave) {
+#pragma unroll
+      for (int i = 0; i < V; i++) sh[wave - 1][lane * V + i] = acc[t][i];
+    }
+    __syncthreads();
+    if (wave == 0 && k < dim && t < tokens) {
+      float* o = part + ((int64_t)blockIdx.y * tokens + t) * ld + k;
+#pragma unroll
+      for (int i = 0; i < V; i++)
+        o[i] = (acc[t][i] + sh[0][lane * V + i]) + (sh[1][lane * V + i] + sh[2][lane * V + i]);
+    }
   }
 }
 
@@ -556,34 +728,86 @@ int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t
   return SMQ_OK;
 }
 
-// Few tokens: as many as the lanes' multiply-adds keep up with the read of the weight (a 4-byte weight
-// leaves time for 16, a 2-byte one for 4), whole 16-byte vectors, hidden within 64 KiB of LDS.
-int few_tokens(const void* h, const void* w, int64_t ldw, const Shape& s) {
-  const int v = (int)(16 / s.size());
+// Few tokens: up to 16, hidden within 128 KiB of LDS; 0: not few.
+struct Few {
+  int nt, v;
+  size_t lds;
+  int threads, grid;
+};
+Few few_tokens(const void* w, int64_t ldw, const Shape& s) {
+  if (s.tokens > 16) return {};
   const int nt = s.tokens <= 1 ? 1 : s.tokens <= 2 ? 2 : s.tokens <= 4 ? 4 : s.tokens <= 8 ? 8 : 16;
-  if (s.tokens > (s.split() ? 16 : 4) || s.dim % v || ldw % v || (reinterpret_cast<uintptr_t>(w) & 15) ||
-      nt * s.dim * 4 > 65536 - 1024)
-    return 0;
-  return nt;
+  const size_t lds = (size_t)nt * s.dim * 4;
+  if (lds > 128 * 1024) return {};
+  const int size = (int)s.size();
+  int v = 8 / size < 4 ? 4 : 8 / size;  // 4 elements a lane
+  while (v > 1 && (s.dim % v || ldw % v || (reinterpret_cast<uintptr_t>(w) & (v * size - 1)))) v /= 2;
+  // The more LDS a workgroup needs, the more waves share it; no more workgroups than are there at once
+  // (each stages hidden anew), but small ones.
+  const int threads = lds <= 16 * 1024 ? 256 : lds <= 40 * 1024 ? 512 : 1024;
+  const int64_t rows = threads / 64 * kRows, all = (s.vocab + rows - 1) / rows;
+  const int64_t fit = 160 * 1024 / (lds + 4096), room = 2048 / threads;
+  const int64_t most = lds <= 16 * 1024 ? 2048 : 256 * (fit < room ? fit : room);
+  return {nt, v, lds, threads, (int)(all < most ? all : most)};
 }
-int few_grid(const Shape& s) {
-  const int64_t g = (s.vocab + 4 * kRows - 1) / (4 * kRows);
-  return (int)(g < 2048 ? g : 2048);
+int few_chunks(const Shape& s, const Few& f) {
+  const int64_t cols = (s.dim + 64 * f.v - 1) / (64 * f.v);
+  int64_t c = (1024 + cols - 1) / cols;
+  if (c > s.vocab / 32) c = s.vocab / 32;
+  return (int)(c < 1 ? 1 : c > 128 ? 128 : c);
+}
+// kernel<T, V, NT> for a plan's v and nt
+template <typename T, int V, typename F>
+void few_tokens_case(int nt, F f) {
+  if (nt == 1) f(std::integral_constant<int, V>(), std::integral_constant<int, 1>());
+  else if (nt == 2) f(std::integral_constant<int, V>(), std::integral_constant<int, 2>());
+  else if (nt == 4) f(std::integral_constant<int, V>(), std::integral_constant<int, 4>());
+  else if (nt == 8) f(std::integral_constant<int, V>(), std::integral_constant<int, 8>());
+  else f(std::integral_constant<int, V>(), std::integral_constant<int, 16>());
+}
+template <typename T, typename F>
+void few_case(const Few& p, F f) {
+  if (p.v == 4) few_tokens_case<T, 4>(p.nt, f);
+  else if (p.v == 2) few_tokens_case<T, 2>(p.nt, f);
+  else few_tokens_case<T, 1>(p.nt, f);
+}
+// More than 64 KiB of dynamic LDS has to be asked for.
+template <typename K>
+void allow_lds(K kernel, size_t bytes) {
+  if (bytes > 48 * 1024)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
 }
 template <typename T>
-void launch_few(int nt, const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,
-                const float* bias, const int64_t* target, float2* part, float* picked, hipStream_t st) {
-  const dim3 grid(few_grid(s)), block(256);
-  const size_t lds = (size_t)nt * s.dim * 4;
-  const T* a = reinterpret_cast<const T*>(h);
-  const T* b = reinterpret_cast<const T*>(w);
-  const int n = (int)s.tokens, d = (int)s.dim, v = (int)s.vocab;
-  if (nt == 1) hipLaunchKernelGGL((few_kernel<T, 1>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
-  else if (nt == 2) hipLaunchKernelGGL((few_kernel<T, 2>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
-  else if (nt == 4) hipLaunchKernelGGL((few_kernel<T, 4>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
-  else if constexpr (sizeof(T) == 4) {
-    if (nt == 8) hipLaunchKernelGGL((few_kernel<T, 8>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
-    else hipLaunchKernelGGL((few_kernel<T, 16>), grid, block, lds, st, a, ldh, b, ldw, n, d, v, bias, target, part, picked);
+void launch_few(const Few& p, const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,
+                const float* bias, const int64_t* target, int64_t ignore, float2* part, float* picked,
+                hipStream_t st) {
+  few_case<T>(p, [&](auto v, auto nt) {
+    auto kernel = few_kernel<T, v.value, nt.value>;
+    allow_lds(kernel, p.lds);
+    hipLaunchKernelGGL(kernel, dim3(p.grid), dim3(p.threads), p.lds, st, reinterpret_cast<const T*>(h), ldh,
+                       reinterpret_cast<const T*>(w), ldw, (int)s.tokens, (int)s.dim, (int)s.vocab, bias,
+                       target, ignore, part, picked);
+  });
+}
+template <typename T>
+void launch_few_backward(const Few& p, const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,
+                         const float* bias, const int64_t* target, int64_t ignore, int reduction,
+                         const float* lse, const float* grad, const Head* head, float* dl, float* part,
+                         int64_t ld, int chunks, void* dh, void* dw, float* db, hipStream_t st) {
+  few_case<T>(p, [&](auto v, auto nt) {
+    auto kernel = few_backward_kernel<T, v.value, nt.value>;
+    allow_lds(kernel, p.lds);
+    hipLaunchKernelGGL(kernel, dim3(p.grid), dim3(p.threads), p.lds, st, reinterpret_cast<const T*>(h), ldh,
+                       reinterpret_cast<const T*>(w), ldw, (int)s.tokens, (int)s.dim, (int)s.vocab, bias,
+                       target, ignore, reduction, lse, grad, head, dl, reinterpret_cast<T*>(dw), db);
+    if (dh)
+      hipLaunchKernelGGL((few_dh_kernel<T, v.value, nt.value>),
+                         dim3((unsigned)((s.dim + 64 * p.v - 1) / (64 * p.v)), chunks), dim3(256), 0, st, dl,
+                         reinterpret_cast<const T*>(w), ldw, (int)s.tokens, (int)s.dim, (int)s.vocab, ld, part);
+  });
+  if (dh) {
+    const StoreEpi se = {1.0f, 0.0f, nullptr, kNoMat, {dh, s.dim, 0, out_fmt(s.dtype), 0}, kNoMat, 0, 0, 0.0f};
+    launch_split_sum(part, ld, s.tokens * ld, chunks, 0, (int)s.tokens, (int)s.dim, 1, 0, se, st);
   }
 }
 
@@ -595,14 +819,14 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
   const int tile = plan_product(s.tokens, s.vocab, operand_kt(s.dim, s.split()), 1, 0, false).tile;
   const TileShape ts = shape_of(tile);
   const int64_t tn = (s.vocab + ts.bn - 1) / ts.bn;
-  const int few = few_tokens(h, w, ldw, s);
-  const int blocks = few ? few_grid(s) : (int)tn;
+  const Few few = few_tokens(w, ldw, s);
+  const int blocks = few.nt ? few.grid : (int)tn;
   float2* part = a.take<float2>((size_t)blocks * s.tokens);
   float* picked = a.take<float>(s.tokens);
   float* rows = a.take<float>(s.tokens);
   const int* exponent = nullptr;
   const int *eh = nullptr, *ew = nullptr;
-  if (s.split() && !few) {
+  if (s.split() && !few.nt) {
     float* top = a.take<float>(2 * kMaxParts);
     exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
     if (run) {
@@ -611,11 +835,11 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
                          absmax_grid(s.vocab), head);
     }
   }
-  if (few) {
+  if (few.nt) {
     if (run) {
-      if (s.dtype == SMQ_DTYPE_F32) launch_few<float>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
-      else if (s.dtype == SMQ_DTYPE_F16) launch_few<_Float16>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
-      else launch_few<__bf16>(few, h, ldh, w, ldw, s, bias, target, part, picked, st);
+      if (s.dtype == SMQ_DTYPE_F32) launch_few<float>(few, h, ldh, w, ldw, s, bias, target, ignore, part, picked, st);
+      else if (s.dtype == SMQ_DTYPE_F16) launch_few<_Float16>(few, h, ldh, w, ldw, s, bias, target, ignore, part, picked, st);
+      else launch_few<__bf16>(few, h, ldh, w, ldw, s, bias, target, ignore, part, picked, st);
     }
   } else {
     const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, nullptr, 0, kNoMat, run, st);
@@ -652,6 +876,22 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
                 const float* bias, int64_t ignore, int reduction, const float* lse, const Head* head,
                 const float* grad, void* dh, void* dw, float* db, void* ws, bool run, hipStream_t st) {
   Arena a(ws);
+  if (const Few few = few_tokens(w, ldw, s); few.nt) {
+    const int chunks = few_chunks(s, few);
+    const int64_t ld = round_up(s.dim, 4);
+    float* dl = dh ? a.take<float>((size_t)(s.vocab * few.nt)) : nullptr;
+    float* part = dh ? a.take<float>((size_t)(chunks * s.tokens * ld)) : nullptr;
+    if (run) {
+      auto go = [&](auto type) {
+        launch_few_backward<decltype(type)>(few, h, ldh, w, ldw, s, bias, target, ignore, reduction, lse, grad,
+                                            head, dl, part, ld, chunks, dh, dw, db, st);
+      };
+      if (s.dtype == SMQ_DTYPE_F32) go(0.0f);
+      else if (s.dtype == SMQ_DTYPE_F16) go((_Float16)0);
+      else go((__bf16)0.0f);
+    }
+    return a.used;
+  }
   const bool sp = s.split();
   const int fmt = sp ? kSplit : kF16;  // the gradient products' operands
   const int grad_dtype = sp ? SMQ_DTYPE_F32 : SMQ_DTYPE_F16;

@@ -110,6 +110,42 @@ def test_loss_and_gradients(tokens, dim, vocab, bias, reduction, ignored, piece,
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,dim,vocab,ignored", [
+    (1, 68, 1003, 0), (2, 66, 50, 0), (3, 77, 5001, 0.3), (5, 2048, 400, 0.3), (8, 4096, 133, 0),
+    (11, 130, 3, 0.3), (16, 2048, 1001, 0.3), (16, 2049, 300, 0), (17, 64, 300, 0.3),
+    (4, 8192, 90, 0), (4, 8200, 90, 0)])
+def test_few_tokens(tokens, dim, vocab, ignored, dtype):
+    """Up to 16 tokens go without matrix cores while hidden fits the LDS: every vector width, row count
+    and both sides of the limits."""
+    for reduction in ("mean", "none"):
+        check(*make(tokens, dim, vocab, dtype, True, ignored, seed=dim), reduction)
+
+
+def test_few_tokens_take_strided_weights():
+    h, w, b, t = make(6, 48, 300, torch.float16, True, 0.2, seed=21)
+    base = check(h, w, b, t, "mean")
+    for pad in (1, 2, 4):
+        wide = torch.randn(300, 48 + 2 * pad, device="cuda").half()
+        wide[:, pad:pad + 48] = w
+        other = check(h, wide[:, pad:pad + 48], b, t, "mean")
+        assert abs(other[0].item() - base[0].item()) <= 64 * U * abs(base[0].item())
+
+
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_gradients_that_are_not_finite(tokens):
+    """A row's infinite gradient leaves the other rows of the hidden's gradient as they are."""
+    h, w, _, t = make(tokens, 64, 200, torch.float32, False, 0, seed=22)
+    g = torch.ones(tokens, device="cuda")
+    leaf = h.detach().requires_grad_()
+    want = torch.autograd.grad(linear_cross_entropy(leaf, w, t, reduction="none"), leaf, g)[0]
+    g[1] = float("inf")
+    got = torch.autograd.grad(linear_cross_entropy(leaf, w, t, reduction="none"), leaf, g)[0]
+    assert not torch.isfinite(got[1]).any()
+    got[1] = want[1]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_large_tiles(dtype):
     check(*make(2100, 320, 20011, dtype, True, 0.2), "mean", 7001)
 
