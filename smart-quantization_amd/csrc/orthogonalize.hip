@@ -3,24 +3,23 @@
 //   X = G / (|G|_F + eps), turned so that its m rows are the shorter side;
 //   steps times:  A = X X^T,  X <- (a I + b A + c A A) X     (an odd polynomial of the singular values)
 //
-// All factors are polynomials of one symmetric matrix, so they commute, and a stage of up to kStage
-// steps needs X only at its ends:
+// All factors are polynomials of one symmetric matrix, so they commute, and a stage of a few steps needs X
+// only at its ends:
 //   A = X X^T;  each step:  Q = a I + b A + c A A,  P <- Q P,  A <- (Q A) Q;   X <- P X
 // The m x m products are symmetric: only the tiles on and above the diagonal are computed (the epilogue
-// writes both halves). A stage of r steps costs 3 m^2 n + (4 r - 3) m^3 operations instead of
-// r (4 m^2 n + 2 m^3): five steps as 3 + 2 6 m^2 n + 14 m^3, as 2 + 2 + 1 9 m^2 n + 11 m^3, instead of
-// 20 m^2 n + 10 m^3. X is kept both ways round, as [m, n] (operand of A) and as [n, m] (operand of P X):
-// all operands of gemm_nt.h are contiguous along k.
+// writes both halves) where they fill the chip. A stage of r steps costs 3 m^2 n + (4 r - 3) m^3 operations
+// instead of r (3 m^2 n + m^3): five steps as 3 + 2 6 m^2 n + 14 m^3 instead of 15 m^2 n + 5 m^3. X is kept both
+// ways round, as [m, n] (operand of A) and as [n, m] (operand of P X): all operands of gemm_nt.h are
+// contiguous along k.
 //
 // Rounding. Between products a matrix is held as two fp16 planes (23 bits) at a power-of-two scale that
 // keeps it in range (the host bounds the singular values step by step). One plane would be off by 0.15 %
 // on Gaussian matrices and by 1-4 % where a few strong directions hide the rest. A stage squares the
-// ratio of the singular values once (A), so its length is limited. Simulated on matrices whose strong
-// directions are 5 to 200 times the rest, five steps are off by 0.5 - 1.2e-6 as 2 + 2 + 1, 1 - 6e-6 as
-// 3 + 2, up to 8e-5 as one stage of 5, and 1 - 20e-6 in plain float32 products: float32 takes stages of
-// 2, the 16-bit types, whose results round to 2^-11 and 2^-8, stages of 3. 16-bit inputs are exact in one
-// plane, so the first stage reads one plane of them; for bf16 results, which round to 2^-8, the last P X
-// takes one plane of each (0.03 - 0.3 % off, against the 0.17 % of the result's own rounding).
+// ratio of the singular values once more for each step behind its first: five steps measured 0.9 - 2.5e-6
+// off as single steps, 1.1 - 5.6e-6 as 2 + 2 + 1, 2 - 5e-6 as 3 + 2 (plain float32 products 0.6 - 3.4e-6).
+// float32 takes single steps; the 16-bit types, whose results round to 2^-11 and 2^-8, stages of 3. 16-bit
+// inputs are exact in one plane, so the first stage reads one plane of them; for bf16 results the last
+// P X takes one plane of each (0.03 - 0.3 % off, against the 0.17 % of the result's own rounding).
 #include <math.h>
 
 #include "gemm_nt.h"
@@ -420,11 +419,11 @@ struct Plan {
   double a, b, c;
 };
 
-// Steps of a stage. A call bound by its launches (under 2^20 elements, not much longer than wide) takes
-// single steps: three launches each, where a longer stage makes 7 for two and 11 for three.
+// Steps of a stage: one for float32 (rounding, above) and for calls bound by their launches (under 2^20
+// elements, not much longer than wide): a single step is three launches, three in a stage are eleven.
 int stage_of(const Plan& p) {
-  if (p.m > 64 && p.batch * p.m * p.n < (1 << 20) && p.n <= 4 * p.m) return 1;
-  return p.dtype == SMQ_DTYPE_F32 ? 2 : 3;
+  const bool launches = p.m > 64 && p.batch * p.m * p.n < (1 << 20) && p.n <= 4 * p.m;
+  return p.dtype == SMQ_DTYPE_F32 || launches ? 1 : 3;
 }
 
 // Largest |a s + b s^3 + c s^5| over 0 <= s <= top.
