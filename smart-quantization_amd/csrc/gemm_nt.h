@@ -9,6 +9,8 @@
 //               Three products hi*hi + hi*lo + lo*hi per k step; the dropped lo*lo is below 2^-24 of
 //               the largest product. An fp32-class product at a third of the fp16 rate, where the
 //               fp32 MFMA runs at a sixteenth.
+//   float32     as it is (Raw32), k padded to 32: the fp32 instructions, an eighth of the fp16 rate but no
+//               pass that makes planes; ld counts 16-bit units here too.
 //   twice       one plane in the layout of two, [32 x | 32 x] (kDup): against an operand of two planes
 //               the one-plane product gives (hi + lo) x.
 //
@@ -52,6 +54,22 @@ template <> struct Frag<_Float16> {
   typedef f16x8 type;
   static __device__ __forceinline__ f32x16 mma(type a, type b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// float32 as it is, on the fp32 matrix instructions: a row's k tile is 32 floats, the same 128 bytes. A
+// lane's 16 bytes are 4 columns, of which the four instructions take one each: which columns meet in
+// one instruction does not matter as long as both operands agree.
+struct Raw32 {
+  uint16_t half;
+};
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+template <> struct Frag<Raw32> {
+  typedef f32x4v type;
+  static __device__ __forceinline__ f32x16 mma(type a, type b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
   }
 };
 

@@ -30,18 +30,19 @@ constexpr size_t kPieceBytes = size_t(1) << 30;  // default limit of a backward 
 struct Head {
   int exp_h, exp_w;  // power-of-two exponents of the fp16 operands made of the inputs
   int exp_out;       // -(exp_h + exp_w)
-  int pad;
+  int known;         // forward: whether it needed, and left, the exponents
   double count;      // rows that take part
   float scale_dh, scale_dw, scale_db;  // backward: the factors of the gradients
 };
 
 // ---- largest magnitude of a tensor -> exponent ---------------------------------------------------
 // Workgroups below gh take h [tokens, dim], the others w [vocab, dim]. Rows without gaps are read as one,
-// in whole vectors whatever the columns.
+// in whole vectors whatever the columns. Nothing where the exponents are known already.
 template <typename T>
 __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, int64_t tokens, const T* w,
                                                      int64_t ldw, int64_t vocab, int cols, int gh,
-                                                     float* part) {
+                                                     float* part, const Head* known) {
+  if (known && known->known) return;
   constexpr int V = 16 / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(V)));
   const bool first = (int)blockIdx.x < gh;
@@ -488,7 +489,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float2* part, int block
 
 // The loss over rows (fp64 sums in a fixed order) and the count of rows taking part, from each thread's
 // sums; one workgroup of 16 waves.
-__device__ __forceinline__ void finish_loss(double s, double c, int reduction, float* loss, Head* head) {
+__device__ __forceinline__ void finish_loss(double s, double c, int reduction, int known, float* loss,
+                                            Head* head) {
   s = wave_sum(s), c = wave_sum(c);
   __shared__ double a[16], b[16];
   if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = s, b[threadIdx.x >> 6] = c;
@@ -496,13 +498,13 @@ __device__ __forceinline__ void finish_loss(double s, double c, int reduction, f
   if (threadIdx.x == 0) {
     s = c = 0.0;
     for (int k = 0; k < 16; k++) s += a[k], c += b[k];
-    head->count = c;
+    head->count = c, head->known = known;
     if (reduction == SMQ_REDUCE_MEAN) *loss = (float)(s / c);
     if (reduction == SMQ_REDUCE_SUM) *loss = (float)s;
   }
 }
 __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const int64_t* target,
-                                                    int64_t ignore, int rows, int reduction,
+                                                    int64_t ignore, int rows, int reduction, int known,
                                                     float* loss, Head* head) {
   double s = 0.0, c = 0.0;
   for (int m = threadIdx.x; m < rows; m += 1024) {
@@ -510,13 +512,13 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
     c += target[m] != ignore ? 1.0 : 0.0;
     if (reduction == SMQ_REDUCE_NONE) loss[m] = row_loss[m];
   }
-  finish_loss(s, c, reduction, loss, head);
+  finish_loss(s, c, reduction, known, loss, head);
 }
 // Both in one workgroup, where the partial statistics are few.
 __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int blocks, int rows, int R,
                                                          const int64_t* target, int64_t ignore,
                                                          int64_t vocab, const float* picked, float* lse,
-                                                         int reduction, float* loss, Head* head) {
+                                                         int reduction, int known, float* loss, Head* head) {
   __shared__ float2 sh[1024];
   const int m = threadIdx.x & (R - 1);
   float l, value;
@@ -528,20 +530,23 @@ __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int
     s = (double)value;
     c = target[m] != ignore ? 1.0 : 0.0;
   }
-  finish_loss(s, c, reduction, loss, head);
+  finish_loss(s, c, reduction, known, loss, head);
 }
 
 // ---- backward -----------------------------------------------------------------------------------
-// One workgroup: the exponents of the operands (part: their maxima, NULL: none), the rows' factors relative
+// One workgroup: the exponents of the operands (part: their maxima, NULL: none; `planes`: the forward may
+// have left them), the rows' factors relative
 // to their largest magnitude, and what comes off again in the epilogues. Ignored rows get 0, rows whose
 // gradient is not finite that gradient itself.
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
                                                       int64_t ignore, int rows, int reduction,
                                                       float* g, const Head* head, const float* part,
-                                                      int gh, int gw, Head* out) {
+                                                      int gh, int gw, int planes, Head* out) {
   __shared__ float w[16];
   __shared__ float all;
   if (part) exponents_of(part, gh, gw, out);
+  if (part && planes && head->known && threadIdx.x == 0)
+    out->exp_h = head->exp_h, out->exp_w = head->exp_w, out->exp_out = head->exp_out;
   const float inf = __builtin_inff();
   float top = 0.0f, one = 0.0f;
   if (reduction == SMQ_REDUCE_NONE) {
@@ -673,10 +678,11 @@ void layout(const void* src, int dtype, int64_t ld, int64_t rows, int64_t cols, 
 
 // The partial maxima of both inputs, absmax_grid of the tokens and of the vocabulary.
 template <typename T>
-void maxima(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, float* part, hipStream_t st) {
+void maxima(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, float* part, const Head* known,
+            hipStream_t st) {
   const int gh = absmax_grid(s.tokens), gw = absmax_grid(s.vocab);
   hipLaunchKernelGGL(absmax_kernel<T>, dim3(gh + gw), dim3(256), 0, st, h, ldh, s.tokens, w, ldw, s.vocab,
-                     (int)s.dim, gh, part);
+                     (int)s.dim, gh, part, known);
 }
 
 template <typename Epi>
@@ -726,6 +732,24 @@ int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t
     return SMQ_ERR_INVALID;
   }
   return SMQ_OK;
+}
+
+// float32 logits of up to 128 tokens, where both tensors are operands as they are: on the fp32 matrix
+// instructions straight from them. Making planes of the weight moves it three times more; with more tokens
+// the planes' eightfold rate pays for that (64 x 1024 x 30000: 272 us a step against 330 with planes, 256
+// tokens about even, 130 x 484 x 48351, whose rows would have to be copied, 573 against 411).
+bool in_place32(const void* p, int64_t ld, int64_t cols) {
+  return cols % 32 == 0 && ld % 4 == 0 && ld <= (1 << 20) && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+bool raw32(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s) {
+  return s.split() && s.tokens <= 128 && in_place32(h, ldh, s.dim) && in_place32(w, ldw, s.dim);
+}
+// The logits' product: by planes, one plane or raw float32.
+template <typename Epi>
+void logits(const Shape& s, bool raw, int tile, const Operand& A, const Operand& B, const Epi& e,
+            hipStream_t st) {
+  if (raw) launch<Raw32, false>(tile, A, B, (int)(round_up(s.dim, 32) / 32), 1, 0, 1, e, st);
+  else product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
 }
 
 // Few tokens: up to 16, hidden within 128 KiB of LDS; 0: not few.
@@ -826,11 +850,12 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
   float* rows = a.take<float>(s.tokens);
   const int* exponent = nullptr;
   const int *eh = nullptr, *ew = nullptr;
-  if (s.split() && !few.nt) {
+  const bool raw = raw32(h, ldh, w, ldw, s);
+  if (s.split() && !few.nt && !raw) {
     float* top = a.take<float>(2 * kMaxParts);
     exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
     if (run) {
-      maxima((const float*)h, ldh, (const float*)w, ldw, s, top, st);
+      maxima((const float*)h, ldh, (const float*)w, ldw, s, top, nullptr, st);
       hipLaunchKernelGGL(exponent_kernel, dim3(1), dim3(256), 0, st, top, absmax_grid(s.tokens),
                          absmax_grid(s.vocab), head);
     }
@@ -842,23 +867,25 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
       else launch_few<__bf16>(few, h, ldh, w, ldw, s, bias, target, ignore, part, picked, st);
     }
   } else {
-    const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, nullptr, 0, kNoMat, run, st);
-    const Operand B = operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, nullptr, 0, kNoMat, run, st);
+    const Operand A = raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
+                          : operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, nullptr, 0, kNoMat, run, st);
+    const Operand B = raw ? Operand{w, 2 * ldw, 0, (int)s.vocab}
+                          : operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, nullptr, 0, kNoMat, run, st);
     const SoftmaxEpi e = {exponent, bias, target, part, picked};
-    if (run) product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
+    if (run) logits(s, raw, tile, A, B, e, st);
   }
   if (run) {
     int per = 1;
     if (s.tokens <= 1024 && s.tokens * blocks <= 16384) {
       while (per < s.tokens) per *= 2;
       hipLaunchKernelGGL(join_loss_kernel, dim3(1), dim3(1024), 0, st, part, blocks, (int)s.tokens, per,
-                         target, ignore, s.vocab, picked, lse, reduction, loss, head);
+                         target, ignore, s.vocab, picked, lse, reduction, exponent ? 1 : 0, loss, head);
     } else {
       per = s.tokens >= 2048 ? 16 : s.tokens >= 256 ? 4 : 1;
       hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + per - 1) / per)), dim3(256), 0, st, part,
                          blocks, (int)s.tokens, per, target, ignore, s.vocab, picked, lse, rows);
       hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
-                         reduction, loss, head);
+                         reduction, exponent ? 1 : 0, loss, head);
     }
   }
   return a.used;
@@ -904,23 +931,27 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   float* top = nullptr;
   if (planes) {
     top = a.take<float>(2 * kMaxParts);
-    if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, top, st);
-    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, st);
+    if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, top, head, st);
+    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, nullptr, st);
   }
-  const int* exponent = sp ? &fac->exp_out : nullptr;
+  const bool raw = raw32(h, ldh, w, ldw, s);
+  const int* exponent = sp && !raw ? &fac->exp_out : nullptr;
   const int* eh = planes ? &planes->exp_h : nullptr;
   const int* ew = planes ? &planes->exp_w : nullptr;
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
                        (int)s.tokens, reduction, g, head, top, absmax_grid(s.tokens),
-                       absmax_grid(s.vocab), fac);
+                       absmax_grid(s.vocab), sp ? 1 : 0, fac);
   // h, and transposed the operand of dw. Ignored rows are zeros, whatever they hold (where h is read in
   // place its ignored rows' logits are not used).
   const int64_t ldt = operand_ld(s.tokens, sp);
   const int padt = operand_pad(s.tokens, sp);
   _Float16* ht = dw ? a.take<_Float16>((size_t)(s.dim * ldt)) : nullptr;
-  const Operand A = operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, eh, target, ignore,
-                            dw ? Mat{ht, ldt, 0, fmt, padt} : kNoMat, run, st);
+  const Mat turned_h = dw ? Mat{ht, ldt, 0, fmt, padt} : kNoMat;
+  if (run && raw && dw) layout(h, s.dtype, ldh, s.tokens, s.dim, eh, target, ignore, kNoMat, turned_h, st);
+  const Operand A =
+      raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
+          : operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, eh, target, ignore, turned_h, run, st);
   const int64_t ldp = operand_ld(s.piece, sp);
   _Float16* dl = a.take<_Float16>((size_t)(s.tokens * ldp));
   _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
@@ -941,13 +972,15 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     const int64_t v0 = i * s.piece, n = s.vocab - v0 < s.piece ? s.vocab - v0 : s.piece;
     const char* wp = reinterpret_cast<const char*>(w) + (size_t)(v0 * ldw) * wsize;
     const int padn = operand_pad(n, sp);
-    const Operand B = operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew, nullptr, 0,
-                              dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat, run, st);
+    const Mat turned_w = dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat;
+    if (run && raw && dh) layout(wp, s.dtype, ldw, n, s.dim, ew, nullptr, 0, kNoMat, turned_w, st);
+    const Operand B = raw ? Operand{wp, 2 * ldw, 0, (int)n}
+                          : operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew, nullptr, 0, turned_w, run, st);
     if (a.used > most) most = a.used;
     if (!run) continue;
     const DlEpi e = {exponent, bias, target, lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
                      {dlt, ldt, 0, fmt, padt}, sums};
-    product(s.dtype, tile_l, A, B, operand_kt(s.dim, sp), 1, e, st);
+    logits(s, raw, tile_l, A, B, e, st);
     if (db)
       hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, sums,
                          row_blocks, (int)n, fac, db + v0);
