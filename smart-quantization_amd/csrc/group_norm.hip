@@ -11,9 +11,8 @@
 //              transforms it: x is read once (forward 2 passes over memory, backward 3). Statistics by
 //              two passes over the registers (mean, then squared deviations).
 //   streaming  a launch for per-channel partial sums of row chunks, a small one that joins them, one
-//              that transforms: x is read twice. Statistics of the forward are sums of x - k and its
-//              square with k the channel's first value (no cancellation against a large mean), joined in
-//              fp64.
+//              that transforms: x is read twice. Statistics of the forward are means and squared
+//              deviations from them (no cancellation against a large mean), joined in fp64.
 // A thread owns V adjacent channels (16 bytes where the channel count allows) and walks rows, so its
 // parameters stay in registers. No atomics: the sums have a fixed order.
 #include "smq_common.h"
@@ -375,17 +374,25 @@ __device__ __forceinline__ void chunk_sums(const Args& A, const Walk& w, const f
   }
 }
 
+// A chunk's mean and squared deviations from it. A thread sums about its own first value, which is one of
+// those it sums: an outlier there costs no more than its own share of the variance (sums about the
+// channel's first value lost 10 % of it where that was the outlier). Threads are joined by their means.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void stream_stats(Args A) {
   typedef typename Pack<T, V>::type vec;
   __shared__ float2 sh[256 * V];
   const Walk w = walk_of<V>(A);
-  float s1[V], s2[V], k[V];
-#pragma unroll
-  for (int i = 0; i < V; i++) s1[i] = s2[i] = k[i] = 0.0f;
+  auto count = [&](int row) {
+    const int64_t left = w.last - w.first - row;
+    return left > 0 ? (int)((left + w.rows - 1) / w.rows) : 0;
+  };
   if (w.active) {
+    float s1[V], s2[V], k[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) s1[i] = s2[i] = k[i] = 0.0f;
     const T* x = reinterpret_cast<const T*>(A.x) + (int64_t)blockIdx.z * A.s * A.c + w.c;
-    const vec f = *reinterpret_cast<const vec*>(x);
+    const int n = count(w.row);
+    const vec f = *reinterpret_cast<const vec*>(x + (n ? w.first + w.row : 0) * A.c);
 #pragma unroll
     for (int i = 0; i < V; i++) k[i] = at<T, V>(f, i);
 #pragma unroll 4
@@ -398,32 +405,48 @@ __global__ __launch_bounds__(256) void stream_stats(Args A) {
         s2[i] = fmaf(d, d, s2[i]);
       }
     }
+    const float inv = n ? 1.0f / (float)n : 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const float m = s1[i] * inv, q = s2[i] - s1[i] * m;
+      sh[w.row * A.block + w.col * V + i] = make_float2(k[i] + m, q < 0.0f ? 0.0f : q);
+    }
   }
-  chunk_sums<V>(A, w, s1, s2, sh);
+  __syncthreads();
+  const int c0 = blockIdx.y * A.block;
+  for (int c = threadIdx.x; c < A.block && c0 + c < A.c; c += 256) {
+    float mean = 0.0f, q = 0.0f;
+    for (int r = 0; r < w.rows; r++) mean = fmaf((float)count(r), sh[r * A.block + c].x, mean);
+    mean /= (float)(w.last - w.first);
+    for (int r = 0; r < w.rows; r++) {
+      const float2 p = sh[r * A.block + c];
+      const float d = p.x - mean;
+      q += fmaf((float)count(r) * d, d, p.y);
+    }
+    A.part[((int64_t)blockIdx.z * A.chunks + blockIdx.x) * A.c + c0 + c] = make_float2(mean, q);
+  }
 }
 
-// One workgroup per (group, n): the chunks' sums of its channels -> mean, rstd.
+// One workgroup per (group, n): the chunks of its channels -> mean, rstd.
 template <typename T>
 __global__ __launch_bounds__(256) void join_stats(Args A) {
   const int g = blockIdx.x, n = blockIdx.y, c0 = g * A.cg;
   const T* x = reinterpret_cast<const T*>(A.x) + (int64_t)n * A.s * A.c;
-  double s = 0.0, q = 0.0;
+  double s = 0.0, q = 0.0;  // about k, the group's first value
+  const double k = (double)(float)x[c0];
   // a thread keeps to one channel where the group has at most 256
   const int per = A.cg < 256 ? A.cg : 256, lanes = 256 / per;
   const int first = threadIdx.x % per, at0 = threadIdx.x / per;
   if (at0 < lanes)
     for (int i = first; i < A.cg; i += per) {
-      const double k = (double)(float)x[c0 + i];
       const float2* part = A.part + (int64_t)n * A.chunks * A.c + c0 + i;
-      double s1 = 0.0, s2 = 0.0, cnt = 0.0;
 #pragma unroll 4
       for (int ch = at0; ch < A.chunks; ch += lanes) {
         const float2 p = part[(int64_t)ch * A.c];
-        cnt += (double)(A.s * (ch + 1) / A.chunks - A.s * ch / A.chunks);
-        s1 += (double)p.x, s2 += (double)p.y;
+        const double rows = (double)(A.s * (ch + 1) / A.chunks - A.s * ch / A.chunks);
+        const double d = (double)p.x - k;
+        s += rows * d, q += (double)p.y + rows * d * d;
       }
-      s += s1 + cnt * k;
-      q += s2 + 2.0 * k * s1 + cnt * k * k;
     }
   s = wave_sum(s), q = wave_sum(q);
   __shared__ double a[4], b[4];
@@ -434,6 +457,7 @@ __global__ __launch_bounds__(256) void join_stats(Args A) {
   const double m = (double)A.s * A.cg;
   s = ((a[0] + a[1]) + (a[2] + a[3])) / m;
   q = ((b[0] + b[1]) + (b[2] + b[3])) / m - s * s;
+  s += k;
   const double rstd = 1.0 / sqrt((q < 0.0 ? 0.0 : q) + (double)A.eps);
   if (threadIdx.x == 0) {
     A.mean[(int64_t)n * A.groups + g] = (float)s;

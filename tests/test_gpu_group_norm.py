@@ -259,3 +259,17 @@ def test_empty():
     assert y.shape == x.shape
     y.sum().backward()
     assert (w.grad == 0).all()
+
+
+@pytest.mark.parametrize("value", [-65504.0, 1e4])
+@pytest.mark.parametrize("shape", [(2, 32, 12, 12), (1, 32, 256, 256), (1, 6, 300, 211)])
+def test_outlier_in_the_first_place(shape, value):
+    """One value far off, where a channel's sums begin. The variance is a sum of non-negative terms of at
+    most 32 values a thread and 256 threads a chunk: off by 300 u relative at most and 50 u at these sizes
+    (4 + 32 values; 9 + 128 in the odd shape, of which all but a few are small against the outlier's own
+    term), rstd by half of it: 25 u |z| beside the 16 u of the bound."""
+    x, _, w, b = make(shape, torch.float32, seed=31)
+    x[:, :, 0, 0] = value
+    y = group_norm_act(x, 2, w, b)
+    want, bound, _ = reference(x, 2, w, b, 1e-5, "none")
+    close(y, want, 3 * bound, torch.float32)
