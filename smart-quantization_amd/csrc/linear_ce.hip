@@ -36,12 +36,18 @@ struct Head {
 };
 
 // ---- largest magnitude of a tensor -> exponent ---------------------------------------------------
-// Workgroups below gh take h [tokens, dim], the others w [vocab, dim]. Rows without gaps are read as one,
-// in whole vectors whatever the columns. Nothing where the exponents are known already.
+// Workgroups below gh take h [tokens, dim], the others w [vocab, dim]. A weight without gaps is read as
+// one row, in whole vectors whatever the columns. What is not finite and rows that are ignored leave the
+// scale to the rest. Nothing where the exponents are known already.
+__device__ __forceinline__ float finite_max(float top, float x) {
+  const float a = fabsf(x);
+  return a < __builtin_inff() ? fmaxf(top, a) : top;
+}
 template <typename T>
 __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, int64_t tokens, const T* w,
-                                                     int64_t ldw, int64_t vocab, int cols, int gh,
-                                                     float* part, const Head* known) {
+                                                     int64_t ldw, int64_t vocab, int cols,
+                                                     const int64_t* target, int64_t ignore, int gh, float* part,
+                                                     const Head* known) {
   if (known && known->known) return;
   constexpr int V = 16 / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(V)));
@@ -51,28 +57,29 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, in
   const int block = first ? blockIdx.x : blockIdx.x - gh, blocks = first ? gh : gridDim.x - gh;
   const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   float top = 0.0f;
-  if (ld == cols && aligned) {
+  if (!first && ld == cols && aligned) {
     const int64_t total = rows * cols, vecs = total / V, step = (int64_t)blocks * 256;
     const vec* p = reinterpret_cast<const vec*>(x);
 #pragma unroll 4
     for (int64_t k = block * 256 + threadIdx.x; k < vecs; k += step) {
       const vec v = p[k];
 #pragma unroll
-      for (int i = 0; i < V; i++) top = fmaxf(top, fabsf((float)v[i]));
+      for (int i = 0; i < V; i++) top = finite_max(top, (float)v[i]);
     }
     if (block == 0 && (int)threadIdx.x < total - vecs * V)
-      top = fmaxf(top, fabsf((float)x[vecs * V + threadIdx.x]));
+      top = finite_max(top, (float)x[vecs * V + threadIdx.x]);
   } else {
     const int whole = aligned && ld % V == 0 ? cols / V * V : 0;
     for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)blocks * 4) {
+      if (first && target[r] == ignore) continue;
       const T* p = x + r * ld;
 #pragma unroll 2
       for (int k = (threadIdx.x & 63) * V; k < whole; k += 64 * V) {
         const vec v = *reinterpret_cast<const vec*>(p + k);
 #pragma unroll
-        for (int i = 0; i < V; i++) top = fmaxf(top, fabsf((float)v[i]));
+        for (int i = 0; i < V; i++) top = finite_max(top, (float)v[i]);
       }
-      for (int k = whole + (threadIdx.x & 63); k < cols; k += 64) top = fmaxf(top, fabsf((float)p[k]));
+      for (int k = whole + (threadIdx.x & 63); k < cols; k += 64) top = finite_max(top, (float)p[k]);
     }
   }
   top = wave_max_dpp(top);
@@ -535,9 +542,8 @@ __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int
 
 // ---- backward -----------------------------------------------------------------------------------
 // One workgroup: the exponents of the operands (part: their maxima, NULL: none; `planes`: the forward may
-// have left them), the rows' factors relative
-// to their largest magnitude, and what comes off again in the epilogues. Ignored rows get 0, rows whose
-// gradient is not finite that gradient itself.
+// have left them), the rows' factors relative to their largest magnitude, and what comes off again in the
+// epilogues. Ignored rows get 0, rows whose gradient is not finite that gradient itself.
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
                                                       int64_t ignore, int rows, int reduction,
                                                       float* g, const Head* head, const float* part,
@@ -678,11 +684,11 @@ void layout(const void* src, int dtype, int64_t ld, int64_t rows, int64_t cols, 
 
 // The partial maxima of both inputs, absmax_grid of the tokens and of the vocabulary.
 template <typename T>
-void maxima(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, float* part, const Head* known,
-            hipStream_t st) {
+void maxima(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, const int64_t* target,
+            int64_t ignore, float* part, const Head* known, hipStream_t st) {
   const int gh = absmax_grid(s.tokens), gw = absmax_grid(s.vocab);
   hipLaunchKernelGGL(absmax_kernel<T>, dim3(gh + gw), dim3(256), 0, st, h, ldh, s.tokens, w, ldw, s.vocab,
-                     (int)s.dim, gh, part, known);
+                     (int)s.dim, target, ignore, gh, part, known);
 }
 
 template <typename Epi>
@@ -694,8 +700,8 @@ void product(int dtype, int tile, const Operand& A, const Operand& B, int kt, in
 }
 
 // [rows, cols] in operand form: in place where it can be, else laid out in the workspace.
-// Rows whose keep[row] is `skip` become zeros (keep NULL: none). `turned` (absent: fmt kNone) is written transposed along the way, in one pass over p where both go by
-// the same exponent (float32) or none.
+// Rows whose keep[row] is `skip` become zeros (keep NULL: none). `turned` (absent: fmt kNone) is written
+// transposed along the way, in one pass over p where both go by the same exponent (float32) or none.
 Operand operand(Arena& ws, const void* p, int64_t ld, int64_t rows, int64_t cols, const Shape& s,
                 const int* exponent, const int* turned_exponent, const int64_t* keep, int64_t skip,
                 const Mat& turned, bool run, hipStream_t st) {
@@ -721,6 +727,11 @@ int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t
   if (tokens < 1 || dim < 1 || vocab < 1 || tokens > (1 << 20) || dim > (1 << 20) || vocab > (1 << 21)) {
     set_error("%s: needs 1 <= tokens, dim <= 2^20 and 1 <= vocab <= 2^21, got %lld, %lld, %lld", who,
               (long long)tokens, (long long)dim, (long long)vocab);
+    return SMQ_ERR_INVALID;
+  }
+  if (tokens * vocab > ((int64_t)1 << 38)) {  // a launch has fewer than 2^32 threads
+    set_error("%s: tokens * vocab is limited to 2^38, got %lld * %lld", who, (long long)tokens,
+              (long long)vocab);
     return SMQ_ERR_INVALID;
   }
   if (!h || !w || !target || ldh < dim || ldw < dim) {
@@ -855,7 +866,7 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
     float* top = a.take<float>(2 * kMaxParts);
     exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
     if (run) {
-      maxima((const float*)h, ldh, (const float*)w, ldw, s, top, nullptr, st);
+      maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, nullptr, st);
       hipLaunchKernelGGL(exponent_kernel, dim3(1), dim3(256), 0, st, top, absmax_grid(s.tokens),
                          absmax_grid(s.vocab), head);
     }
@@ -931,8 +942,8 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   float* top = nullptr;
   if (planes) {
     top = a.take<float>(2 * kMaxParts);
-    if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, top, head, st);
-    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, top, nullptr, st);
+    if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, head, st);
+    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, nullptr, st);
   }
   const bool raw = raw32(h, ldh, w, ldw, s);
   const int* exponent = sp && !raw ? &fac->exp_out : nullptr;

@@ -111,7 +111,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     dtypes. ``reduction``: "mean" over the targets that are not ``ignore_index`` (NaN if there are
     none, as torch), "sum", or "none" (the shape of ``target``). Ignored rows take no part, whatever
     they hold, NaN included; a target outside the vocabulary makes its loss, and what depends on it,
-    NaN. Gradients reach ``hidden``, ``weight`` and ``bias``; there is no second derivative.
+    NaN. Up to 2^20 tokens and 2^21 vocabulary entries, 2^38 of their products, and ``dim`` up to 2^20.
+    Gradients reach ``hidden``, ``weight`` and ``bias``; there is no second derivative.
     ``vocab_piece``: vocabulary entries of one backward piece (0: what 1 GiB of buffers holds)."""
     who = "linear_cross_entropy"
     for t in (hidden, weight, target) + (() if bias is None else (bias,)):

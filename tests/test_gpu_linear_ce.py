@@ -344,3 +344,133 @@ def test_empty():
     total.backward()
     assert total == 0 and (w.grad == 0).all()
     assert linear_cross_entropy(h, w, t, reduction="none").shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ignored_rows_do_not_set_the_scale(dtype):
+    """Values far above the rest in rows that take no part: the others' results keep every bit."""
+    h, w, b, t = make(300, 96, 700, dtype, True, 0.4, seed=23)
+    zeroed = torch.where((t == -100)[:, None], torch.zeros_like(h), h)
+    huge = torch.full_like(h, 6e4 if dtype == torch.float16 else 1e30)
+    dirty = torch.where((t == -100)[:, None], huge, h)
+    base, other = check(zeroed, w, b, t, "mean"), check(dirty, w, b, t, "mean")
+    assert torch.equal(base[0], other[0])
+    assert all(torch.equal(x, y) for x, y in zip(base[1], other[1]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [9, 60, 300])
+def test_rows_that_are_not_finite_leave_the_others(tokens, dtype):
+    h, w, _, t = make(tokens, 96, 700, dtype, False, 0, seed=24)
+    h[1], h[4] = 0.0, 0.0
+    g = torch.randn(tokens, device="cuda")
+    got = []
+    for value in (0.0, float("inf"), float("nan")):
+        leaf = h.clone()
+        leaf[1], leaf[4, 5] = value, value
+        leaf.requires_grad_()
+        loss = linear_cross_entropy(leaf, w, t, reduction="none")
+        got.append((loss.detach(), torch.autograd.grad(loss, leaf, g)[0]))
+    rest = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    rest[1] = rest[4] = False
+    assert torch.isfinite(got[0][0]).all()
+    for loss, grad in got[1:]:
+        assert torch.isnan(loss[~rest]).all() and torch.isnan(grad[~rest]).all()
+        assert torch.equal(loss[rest], got[0][0][rest]) and torch.equal(grad[rest], got[0][1][rest])
+
+
+@pytest.mark.parametrize("tokens,dim,vocab,ignored,piece", [
+    (17, 32, 33, 0, 0), (100, 96, 4097, 0.3, 1000), (128, 160, 700, 0.1, 0), (129, 160, 700, 0.1, 0),
+    (64, 1024, 515, 0, 0), (90, 36, 517, 0, 0)])
+def test_float32_around_the_raw_products(tokens, dim, vocab, ignored, piece):
+    """Both sides of 128 tokens and of whole 128-byte rows."""
+    h, w, b, t = make(tokens, dim, vocab, torch.float32, True, ignored, seed=vocab)
+    check(h, w, b, t, "mean", piece)
+    wide = torch.randn(vocab, dim + 8, device="cuda")
+    for at in (4, 3):  # 16-byte rows, and not
+        wide[:, at:at + dim] = w
+        check(h, wide[:, at:at + dim], b, t, "none", piece)
+
+
+@pytest.mark.parametrize("tokens,dim,vocab,dtype", [
+    (1, 64, 300, torch.bfloat16), (16, 2048, 700, torch.float32), (64, 128, 5000, torch.float32),
+    (200, 100, 900, torch.float32)])
+def test_graph_replays_of_few_tokens(tokens, dim, vocab, dtype):
+    """The forms for few tokens (128 KiB of LDS among them) under capture, two graphs, replayed in turn."""
+    h, w, b, t = make(tokens, dim, vocab, dtype, True, 0, seed=25)
+    leaves = [x.detach().clone().requires_grad_() for x in (h, w, b)]
+
+    def call():
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+        return (loss.detach(), *torch.autograd.grad(loss, leaves))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for k in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(h * (k + 1) / 2)
+        t.copy_((t + 1) % vocab)
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        want = call()
+        for _, out in graphs:
+            assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+def test_backward_twice_and_two_calls_at_once():
+    h, w, b, t = make(200, 64, 900, torch.float32, True, 0.2, seed=26)
+    leaves = [x.detach().requires_grad_() for x in (h, w, b)]
+    one = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        two = linear_cross_entropy(leaves[0] * 2, leaves[1], t, leaves[2])
+        late = torch.autograd.grad(two, leaves[1], retain_graph=True)[0]
+    first = torch.autograd.grad(one, leaves, retain_graph=True)
+    again = torch.autograd.grad(one, leaves)
+    assert all(torch.equal(x, y) for x, y in zip(first, again))
+    torch.cuda.current_stream().wait_stream(other)
+    alone = linear_cross_entropy(leaves[0] * 2, leaves[1], t, leaves[2])
+    assert torch.equal(late, torch.autograd.grad(alone, leaves[1])[0])
+
+
+class HookError(Exception):
+    pass
+
+
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("tokens", [8, 60, 200])
+def test_saved_tensor_hooks(tokens, binding, monkeypatch):
+    """Saved tensors that come back elsewhere (other strides and alignment than the forward saw), and a
+    hook's own error."""
+    from smart_compress_amd import _native as N
+    if not binding:
+        monkeypatch.setattr(N, "train_fast", lambda: None)
+    h, w, b, t = make(tokens, 64, 500, torch.float32, True, 0.2, seed=27)
+    wide = torch.randn(500, 70, device="cuda")
+    wide[:, 3:67] = w
+    leaves = [x.detach().requires_grad_() for x in (h, wide[:, 3:67], b)]
+    with torch.autograd.graph.save_on_cpu():
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+    grad = torch.tensor(-1.7, device="cuda")
+    got = torch.autograd.grad(loss, leaves, grad)
+    want, bl, grads, bounds = reference(h, w, b, t, "mean", grad)
+    close(loss, want, bl, torch.float32)
+    for x, e, bound in zip(got, grads, bounds):
+        close(x, e, bound, torch.float32)
+
+    def refuse(_):
+        raise HookError("no")
+
+    with torch.autograd.graph.saved_tensors_hooks(refuse, lambda x: x), pytest.raises(HookError):
+        linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
