@@ -74,7 +74,8 @@ __global__ __launch_bounds__(64) void norm_kernel(const double* part, int n, dou
       e = 14 - e;
       e = e > 120 ? 120 : e < -120 ? -120 : e;
     }
-    const double r = 1.0 / ((norm + eps) * ldexp(1.0, e));
+    // a matrix of zeros stays one, however small eps (rest2 would leave fp32's range below 1e-19)
+    const double r = norm == 0.0 && eps > 0.0 ? 0.0 : 1.0 / ((norm + eps) * ldexp(1.0, e));
     pow2[blockIdx.x] = ldexpf(1.0f, e);
     rest[blockIdx.x] = (float)r;
     rest2[blockIdx.x] = (float)(r * r);

@@ -19,6 +19,7 @@
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -179,16 +180,12 @@ bool tensor_arg(PyObject* o, T* t, bool optional) {
   *t = THPVariable_Unpack(o);
   return true;
 }
+// Errors become Python's: what a saved-tensor hook raised as it is, no memory as OutOfMemoryError.
 template <typename F>
 PyObject* guarded(F f) {
-  try {
-    return THPVariable_Wrap(f());
-  } catch (const c10::Error& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-  }
-  return nullptr;
+  HANDLE_TH_ERRORS
+  return THPVariable_Wrap(f());
+  END_HANDLE_TH_ERRORS
 }
 
 PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {

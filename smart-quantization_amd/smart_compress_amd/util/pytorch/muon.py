@@ -83,9 +83,11 @@ class Muon(Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)} is not a matrix; "
-                                 "give it to another optimizer")
+            if p.dim() < 2 or p.dtype not in N.DTYPE_CODES:
+                self.param_groups.pop()
+                what = "not a matrix" if p.dim() < 2 else "not float32, float16 or bfloat16"
+                raise ValueError(f"Muon: a parameter of shape {tuple(p.shape)} and dtype {p.dtype} is "
+                                 f"{what}; give it to another optimizer")
 
     @torch.no_grad()
     def step(self, closure=None):

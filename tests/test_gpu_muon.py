@@ -234,3 +234,13 @@ def test_optim_lp_wraps_muon():
     assert tags == [{}] and (plain.optim.state[p]["momentum_buffer"] == 0).all()
     none = OptimLP(Muon([p], lr=0.1, momentum=0.0), momentum_quant=lambda t, **kw: 1 / 0)
     none.step()
+
+
+@pytest.mark.parametrize("shape", [(3, 20, 30), (2, 80, 100)])
+def test_zero_matrix_with_a_tiny_eps(shape):
+    """Zeros stay zeros for every eps above 0, beside matrices that are not."""
+    x = torch.randn(shape, device="cuda")
+    x[1] = 0.0
+    y = orthogonalize(x, eps=1e-30)
+    assert (y[1] == 0).all() and torch.isfinite(y).all()
+    assert torch.equal(y[0], orthogonalize(x[:1], eps=1e-30)[0])

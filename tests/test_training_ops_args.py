@@ -160,3 +160,20 @@ def test_backward_workspace_follows_the_piece():
     assert sizes[0] < full / 8
     big = lib.smq_linear_ce_workspace_bytes(p, 4096, p, 4096, 2, 8192, 4096, 131072, 0, 3)
     assert big < 1.5 * 2 ** 30
+
+
+def test_muon_keeps_no_refused_group():
+    opt = Muon([torch.nn.Parameter(torch.zeros(3, 4))])
+    with pytest.raises(ValueError, match="float32"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3, 4, dtype=torch.float64))]})
+    assert len(opt.param_groups) == 1
+
+
+def test_cross_entropy_limits_the_launch():
+    lib = N.lib()
+    one = ctypes.c_int(0)
+    p = ctypes.addressof(one)
+    for tokens, vocab, ok in ((1 << 18, 1 << 20, True), (1 << 19, 1 << 20, False), (1, 1 << 21, True)):
+        need = lib.smq_linear_ce_workspace_bytes(p, 64, p, 64, N.SMQ_DTYPE_BF16, tokens, 64, vocab, 0, 0)
+        assert (need > 0) == ok
+    assert "2^38" in err()
