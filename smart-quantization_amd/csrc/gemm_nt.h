@@ -136,25 +136,25 @@ __device__ __forceinline__ void store1(const Mat& d, int64_t row, int64_t c, flo
   }
 }
 
+// N elements of T at any element's address, in one access where the hardware has one for the size: rows of
+// an odd pitch cost little more than aligned ones that way.
+template <typename T, int N> struct Loose {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
 // N consecutive columns (N = 4 or 8, c a multiple of N) of row r; columns from `cols` on are padding
-// (zeros up to d.pad, nothing behind it). Padded matrices (d.pad >= cols rounded up to N) and rows
-// with whole vectors take vector stores.
+// (zeros up to d.pad, nothing behind it).
 template <int N>
 __device__ __forceinline__ void store_n(const Mat& d, int64_t b, int64_t r, int64_t c, int cols,
                                         const float (&v)[N]) {
   typedef _Float16 hN __attribute__((ext_vector_type(N)));
   typedef __bf16 bN __attribute__((ext_vector_type(N)));
-  typedef float fN __attribute__((ext_vector_type(4)));
   const int64_t row = b * d.batch + r * d.ld;
   const int end = d.pad > cols ? d.pad : cols;
   if (c >= end) return;
   float w[N];
 #pragma unroll
   for (int i = 0; i < N; i++) w[i] = c + i < cols ? v[i] : 0.0f;
-  const int size = d.fmt == kF32 ? 4 : 2, need = N * size < 16 ? N * size : 16;
-  const bool whole = c + N <= end && (d.fmt == kSplit || d.fmt == kDup ||
-                     ((reinterpret_cast<uintptr_t>(d.p) + (row + c) * size) & (need - 1)) == 0);
-  if (!whole) {
+  if (c + N > end) {
     for (int i = 0; i < N; i++)
       if (c + i < end) store1(d, row, c + i, w[i]);
     return;
@@ -180,18 +180,18 @@ __device__ __forceinline__ void store_n(const Mat& d, int64_t b, int64_t r, int6
     hN h;
 #pragma unroll
     for (int i = 0; i < N; i++) h[i] = (_Float16)w[i];
-    *reinterpret_cast<hN*>(reinterpret_cast<_Float16*>(d.p) + row + c) = h;
+    *reinterpret_cast<typename Loose<_Float16, N>::type*>(reinterpret_cast<_Float16*>(d.p) + row + c) = h;
   } else if (d.fmt == kBF16) {
     bN h;
 #pragma unroll
     for (int i = 0; i < N; i++) h[i] = (__bf16)w[i];
-    *reinterpret_cast<bN*>(reinterpret_cast<__bf16*>(d.p) + row + c) = h;
+    *reinterpret_cast<typename Loose<__bf16, N>::type*>(reinterpret_cast<__bf16*>(d.p) + row + c) = h;
   } else {
     float* p = reinterpret_cast<float*>(d.p) + row + c;
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      fN f = {w[i], w[i + 1], w[i + 2], w[i + 3]};
-      *reinterpret_cast<fN*>(p + i) = f;
+      const typename Loose<float, 4>::type f = {w[i], w[i + 1], w[i + 2], w[i + 3]};
+      *reinterpret_cast<typename Loose<float, 4>::type*>(p + i) = f;
     }
   }
 }
@@ -743,14 +743,13 @@ static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_
   const float fa = factor ? factor[batch] : 1.0f;
   const T* p = src + batch * batch_stride;
   const int q = threadIdx.x & 15, y = threadIdx.x >> 4;
-  const bool wide = (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && (ld & 3) == 0;
 #pragma unroll
   for (int i = 0; i < 64; i += 16) {
     const int r = r0 + y + i, c = c0 + q * 4;
     float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (r < rows && !(keep && keep[r] == skip)) {
-      typedef T t4 __attribute__((ext_vector_type(4)));
-      if (wide && c + 4 <= cols) {
+      typedef typename Loose<T, 4>::type t4;
+      if (c + 4 <= cols) {
         const t4 v = *reinterpret_cast<const t4*>(p + (int64_t)r * ld + c);
 #pragma unroll
         for (int k = 0; k < 4; k++) w[k] = (float)v[k];

@@ -50,14 +50,13 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, in
                                                      const Head* known) {
   if (known && known->known) return;
   constexpr int V = 16 / sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(V)));
+  typedef typename Loose<T, V>::type vec;
   const bool first = (int)blockIdx.x < gh;
   const T* x = first ? h : w;
   const int64_t ld = first ? ldh : ldw, rows = first ? tokens : vocab;
   const int block = first ? blockIdx.x : blockIdx.x - gh, blocks = first ? gh : gridDim.x - gh;
-  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   float top = 0.0f;
-  if (!first && ld == cols && aligned) {
+  if (!first && ld == cols) {
     const int64_t total = rows * cols, vecs = total / V, step = (int64_t)blocks * 256;
     const vec* p = reinterpret_cast<const vec*>(x);
 #pragma unroll 4
@@ -69,7 +68,7 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, in
     if (block == 0 && (int)threadIdx.x < total - vecs * V)
       top = finite_max(top, (float)x[vecs * V + threadIdx.x]);
   } else {
-    const int whole = aligned && ld % V == 0 ? cols / V * V : 0;
+    const int whole = cols / V * V;
     for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)blocks * 4) {
       if (first && target[r] == ignore) continue;
       const T* p = x + r * ld;

@@ -38,10 +38,9 @@ template <typename T>
 __global__ __launch_bounds__(256) void square_sum_kernel(const T* x, int64_t ld, int64_t batch_stride,
                                                          int rows, int cols, double* part) {
   constexpr int V = 16 / sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(V)));
+  typedef typename Loose<T, V>::type vec;
   const T* p = x + blockIdx.y * batch_stride;
-  const bool wide = (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % V == 0;
-  const int whole = wide ? cols / V * V : 0;
+  const int whole = cols / V * V;
   double s = 0.0;
   for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4) {
     const T* q = p + (int64_t)r * ld;
