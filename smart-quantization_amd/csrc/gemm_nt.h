@@ -78,6 +78,9 @@ struct Operand {
   int64_t ld;     // elements between rows
   int64_t batch;  // elements between matrices of a batch
   int rows;
+  // of A, where the host knows only the most there can be (device memory, NULL: what the host says):
+  const int* live = nullptr;   // rows
+  const int* depth = nullptr;  // columns
 };
 
 // Output / source formats of a matrix an epilogue reads or writes.
@@ -235,6 +238,16 @@ __device__ __forceinline__ void gemm_nt_body(const Operand& A, const Operand& B,
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int im, in;
+  int m_rows = A.rows;
+  if (A.live) {
+    m_rows = *A.live < m_rows ? *A.live : m_rows;
+    tm = (m_rows + BM - 1) / BM;
+    if ((int)blockIdx.x >= tm * tn) return;
+  }
+  if (A.depth) {
+    const int most = (*A.depth + (SPLIT ? 31 : 63)) / (SPLIT ? 32 : 64);
+    kt = most < kt ? most : kt;
+  }
   pick_tile(tm, tn, tri, im, in);
   const int row_a = im * BM, row_b = in * BN;
   const int64_t batch = blockIdx.z;
@@ -243,7 +256,7 @@ __device__ __forceinline__ void gemm_nt_body(const Operand& A, const Operand& B,
   const int k1 = (int)((int64_t)kt * (blockIdx.y + 1) / gridDim.y);
   const int nk = k1 - k0;
 
-  const int rows_a = A.rows - row_a < BM ? A.rows - row_a : BM;
+  const int rows_a = m_rows - row_a < BM ? m_rows - row_a : BM;
   const int rows_b = B.rows - row_b < BN ? B.rows - row_b : BN;
   const char* pa = reinterpret_cast<const char*>(A.p) + 2 * (batch * A.batch + (int64_t)row_a * A.ld) + (int64_t)k0 * 128;
   const char* pb = reinterpret_cast<const char*>(B.p) + 2 * (batch * B.batch + (int64_t)row_b * B.ld) + (int64_t)k0 * 128;
@@ -435,7 +448,7 @@ __device__ __forceinline__ void gemm_nt_body(const Operand& A, const Operand& B,
     else stage = reinterpret_cast<float*>(b1) + (w - kInA) * 32 * kPitch;
   }
   epi.template finish<BM, BN, WM, WN, TM, TN>(acc, stage, row_a + wm * TM * 32,
-                                              row_b + wn * TN * 32, A.rows, B.rows, im, in, wm, wn,
+                                              row_b + wn * TN * 32, m_rows, B.rows, im, in, wm, wn,
                                               lane, batch);
 }
 #endif
@@ -565,6 +578,9 @@ struct StoreEpi {
   int tri;
   int64_t share;
   float diag;
+  // split_sum_kernel only: row m goes to row map[m] of `o`, those from *live on as zeros (NULL: as they are)
+  const int* map = nullptr;
+  const int* live = nullptr;
   template <int BM, int BN, int WM, int WN, int TM, int TN>
   __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float* stage, int m0, int n0, int M,
                                          int N, int im, int in, int, int, int lane,
@@ -607,7 +623,7 @@ static __global__ __launch_bounds__(256) void split_sum_kernel(const float* part
   const int m = im * 32 + r, n = in * 32 + c;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (m < M) {
-    if (n < N) {
+    if (n < N && !(e.live && m >= *e.live)) {
       const float* q = part + batch * batch_stride + (int64_t)m * ld + n;
 #pragma unroll 4
       for (int k = 0; k < shares; k++) {
@@ -622,7 +638,7 @@ static __global__ __launch_bounds__(256) void split_sum_kernel(const float* part
       add_diag(v, m, n, e.diag);
     }
     const float w[4] = {v.x, v.y, v.z, v.w};
-    if (e.o.fmt != kNone) store_n<4>(e.o, batch, m, n, N, w);
+    if (e.o.fmt != kNone) store_n<4>(e.o, batch, e.map ? e.map[m] : m, n, N, w);
   }
   if (!turn) return;
   *reinterpret_cast<float4*>(&tile[r][c]) = v;
@@ -727,36 +743,38 @@ static inline void launch(int tile, const Operand& A, const Operand& B, int kt, 
 
 // Layout pass: src [rows, cols] of type T, row pitch ld, times 2^*exponent (NULL: 1) times *factor
 // (NULL: 1), to `d` row by row and / or to `dt` transposed (either may be absent), both zero padded.
-// Rows whose keep[row] equals `skip` are written as zeros (keep NULL: none). 64 x 64 a workgroup;
-// bound by its reads and writes of memory.
+// Rows whose keep[row] equals `skip` are written as zeros (keep NULL: none). With `map`, row r is src's row
+// map[r], and rows from *live on are zeros. 64 x 64 a workgroup; bound by its reads and writes of memory.
 template <typename T>
 static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_t ld,
                                                             int64_t batch_stride, int rows, int cols,
                                                             const int* exponent,
                                                             const float* factor,
                                                             const int64_t* keep, int64_t skip,
-                                                            Mat d, Mat dt) {
+                                                            const int* map, const int* live, Mat d,
+                                                            Mat dt) {
   __shared__ float tile[64][65];
   const int64_t batch = blockIdx.z;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   const int ex = exponent ? *exponent : 0;
   const float fa = factor ? factor[batch] : 1.0f;
   const T* p = src + batch * batch_stride;
-  const int q = threadIdx.x & 15, y = threadIdx.x >> 4;
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
 #pragma unroll
   for (int i = 0; i < 64; i += 16) {
-    const int r = r0 + y + i, c = c0 + q * 4;
+    const int r = r0 + y + i, c = c0 + x * 4;
     float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (r < rows && !(keep && keep[r] == skip)) {
+    if (r < rows && !(keep && keep[r] == skip) && !(map && r >= *live)) {
+      const T* q = p + (int64_t)(map ? map[r] : r) * ld;
       typedef typename Loose<T, 4>::type t4;
       if (c + 4 <= cols) {
-        const t4 v = *reinterpret_cast<const t4*>(p + (int64_t)r * ld + c);
+        const t4 v = *reinterpret_cast<const t4*>(q + c);
 #pragma unroll
         for (int k = 0; k < 4; k++) w[k] = (float)v[k];
       } else {
 #pragma unroll
         for (int k = 0; k < 4; k++)
-          if (c + k < cols) w[k] = (float)p[(int64_t)r * ld + c + k];
+          if (c + k < cols) w[k] = (float)q[c + k];
       }
 #pragma unroll
       for (int k = 0; k < 4; k++) w[k] = ldexpf(w[k] * fa, ex);
@@ -764,7 +782,7 @@ static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_
     if (d.fmt != kNone && r < rows) store_n<4>(d, batch, r, c, cols, w);
     if (dt.fmt != kNone) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) tile[y + i][q * 4 + k] = w[k];
+      for (int k = 0; k < 4; k++) tile[y + i][x * 4 + k] = w[k];
     }
   }
   if (dt.fmt == kNone) return;
@@ -786,9 +804,9 @@ template <typename T>
 static inline void launch_layout(const T* src, int64_t ld, int64_t batch_stride, int rows, int cols,
                                  int batch, const int* exponent, const float* factor,
                                  const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt,
-                                 hipStream_t st) {
+                                 hipStream_t st, const int* map = nullptr, const int* live = nullptr) {
   hipLaunchKernelGGL(layout_kernel<T>, dim3((cols + 63) / 64, (rows + 63) / 64, batch), dim3(256), 0,
-                     st, src, ld, batch_stride, rows, cols, exponent, factor, keep, skip, d, dt);
+                     st, src, ld, batch_stride, rows, cols, exponent, factor, keep, skip, map, live, d, dt);
 }
 
 static inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }

@@ -31,6 +31,7 @@ struct Head {
   int exp_h, exp_w;  // power-of-two exponents of the fp16 operands made of the inputs
   int exp_out;       // -(exp_h + exp_w)
   int known;         // forward: whether it needed, and left, the exponents
+  int rows, pad;     // rows that take part, where they are gathered (Kept)
   double count;      // rows that take part
   float scale_dh, scale_dw, scale_db;  // backward: the factors of the gradients
 };
@@ -112,8 +113,57 @@ __device__ void exponents_of(const float* part, int gh, int gw, Head* head) {
     head->exp_h = eh, head->exp_w = ew, head->exp_out = -(eh + ew);
   }
 }
-__global__ __launch_bounds__(256) void exponent_kernel(const float* part, int gh, int gw, Head* head) {
-  exponents_of(part, gh, gw, head);
+
+// ---- rows that take part, gathered --------------------------------------------------------------------
+// Padding and masked tokens are ignored rows. Where the products are long, the others are gathered and
+// only they are multiplied: their count stays on the device (gemm_nt.h's `live` and `depth`). map holds
+// the rows taking part in order, then the ignored ones; the other arrays are in the gathered order.
+struct Kept {
+  int* map;
+  int64_t* target;
+  float* lse;  // backward
+};
+// put(row, place, whether it takes part) for all rows, and their count; one workgroup of 16 waves.
+template <typename F>
+__device__ __forceinline__ void partition_rows(const int64_t* target, int64_t ignore, int rows, int* live,
+                                               F put) {
+  __shared__ int counts[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int total = 0;
+  for (int m = threadIdx.x; m < rows; m += 1024) total += target[m] != ignore ? 1 : 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+  if (lane == 0) counts[wave] = total;
+  __syncthreads();
+  total = 0;
+  for (int k = 0; k < 16; k++) total += counts[k];
+  int done = 0;
+  for (int base = 0; base < rows; base += 1024) {
+    const int m = base + threadIdx.x;
+    const bool keep = m < rows && target[m] != ignore;
+    const uint64_t mask = __ballot(keep);
+    __syncthreads();
+    if (lane == 0) counts[wave] = __popcll(mask);
+    __syncthreads();
+    int at = done + __popcll(mask & ((1ull << lane) - 1));
+    for (int k = 0; k < 16; k++) {
+      at += k < wave ? counts[k] : 0;
+      done += counts[k];
+    }
+    if (m < rows) put(m, keep ? at : total + (m - at), keep);
+  }
+  if (threadIdx.x == 0) *live = total;
+}
+// The exponents of the operands (part NULL: none are needed) and the gathered rows (map NULL: they are not).
+__global__ __launch_bounds__(1024) void prepare_kernel(const float* part, int gh, int gw, Head* head,
+                                                       const int64_t* target, int64_t ignore, int rows,
+                                                       Kept kept) {
+  if (part) exponents_of(part, gh, gw, head);
+  if (kept.map)
+    partition_rows(target, ignore, rows, &head->rows, [&](int m, int at, bool keep) {
+      kept.map[at] = m;
+      if (keep) kept.target[at] = target[m];
+    });
 }
 
 // exp(x) for x <= about 0, within 2 ulp: the product with log2(e) is carried in two parts (a single
@@ -484,13 +534,16 @@ __device__ __forceinline__ void join_row(const float2* part, int blocks, int row
   const int64_t y = target[m];
   *loss = y == ignore ? 0.0f : y >= 0 && y < vocab ? l - picked[m] : __builtin_nanf("");
 }
+// (live: the gathered rows' count, map their rows; the ignored ones get 0)
 __global__ __launch_bounds__(256) void join_kernel(const float2* part, int blocks, int rows, int R,
                                                    const int64_t* target, int64_t ignore,
-                                                   int64_t vocab, const float* picked, float* lse,
-                                                   float* row_loss) {
+                                                   int64_t vocab, const float* picked, const int* map,
+                                                   const int* live, float* lse, float* row_loss) {
   __shared__ float2 sh[256];
-  const int m = blockIdx.x * R + (threadIdx.x & (R - 1));
-  join_row(part, blocks, rows, R, m, target, ignore, vocab, picked, sh, lse + m, row_loss + m);
+  const int m = blockIdx.x * R + (threadIdx.x & (R - 1)), n = map ? *live : rows;
+  const int to = map && m < rows ? map[m] : m;
+  join_row(part, blocks, n, R, m, target, ignore, vocab, picked, sh, lse + to, row_loss + to);
+  if ((int)threadIdx.x < R && m >= n && m < rows) lse[to] = row_loss[to] = 0.0f;
 }
 
 // The loss over rows (fp64 sums in a fixed order) and the count of rows taking part, from each thread's
@@ -542,11 +595,13 @@ __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int
 // ---- backward -----------------------------------------------------------------------------------
 // One workgroup: the exponents of the operands (part: their maxima, NULL: none; `planes`: the forward may
 // have left them), the rows' factors relative to their largest magnitude, and what comes off again in the
-// epilogues. Ignored rows get 0, rows whose gradient is not finite that gradient itself.
+// epilogues. Ignored rows get 0 or are left out (Kept), rows whose gradient is not finite that gradient
+// itself.
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
                                                       int64_t ignore, int rows, int reduction,
                                                       float* g, const Head* head, const float* part,
-                                                      int gh, int gw, int planes, Head* out) {
+                                                      int gh, int gw, int planes, const float* lse, Kept kept,
+                                                      Head* out) {
   __shared__ float w[16];
   __shared__ float all;
   if (part) exponents_of(part, gh, gw, out);
@@ -578,10 +633,15 @@ __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const i
   }
   __syncthreads();
   top = all;
-  for (int m = threadIdx.x; m < rows; m += 1024) {
-    const float v = reduction == SMQ_REDUCE_NONE ? grad[m] : one;
-    g[m] = target[m] != ignore ? v / top * kDlScale : 0.0f;
+  auto factor = [&](int m) { return (reduction == SMQ_REDUCE_NONE ? grad[m] : one) / top * kDlScale; };
+  if (kept.map) {
+    partition_rows(target, ignore, rows, &out->rows, [&](int m, int at, bool keep) {
+      kept.map[at] = m;
+      if (keep) kept.target[at] = target[m], kept.lse[at] = lse[m], g[at] = factor(m);
+    });
+    return;
   }
+  for (int m = threadIdx.x; m < rows; m += 1024) g[m] = target[m] != ignore ? factor(m) : 0.0f;
 }
 
 // dl of a piece from its logits, to `o` [rows, piece] and transposed to `ot` [piece, rows]; column
@@ -600,6 +660,9 @@ struct DlEpi {
                                          int N, int im, int, int wm, int, int lane,
                                          int64_t batch) const {
     const int ex = exponent ? *exponent : 0;
+    Mat ot = this->ot;  // padded to whole k tiles of the rows there are
+    const int tile = ot.fmt == kSplit ? 32 : 64;
+    ot.pad = (M + tile - 1) / tile * tile;
     float* sum = sums ? sums + (int64_t)(im * WM + wm) * N : nullptr;
     stage_out<TM, TN, true>(
         acc, stage, m0, n0, M, N, lane, batch, o, ot, true, sum != nullptr,
@@ -625,11 +688,13 @@ struct DlEpi {
   }
 };
 
-__global__ __launch_bounds__(256) void bias_sum_kernel(const float* part, int blocks, int n,
-                                                       const Head* head, float* db) {
+// (live: `per` blocks for each `high` of the rows there are)
+__global__ __launch_bounds__(256) void bias_sum_kernel(const float* part, int blocks, int n, const int* live,
+                                                       int high, int per, const Head* head, float* db) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= n) return;
   double s = 0.0;
+  if (live) blocks = (*live + high - 1) / high * per;
   for (int k = 0; k < blocks; k++) s += (double)part[(int64_t)k * n + v];
   db[v] = (float)(s * (double)head->scale_db);
 }
@@ -672,13 +737,14 @@ inline int out_fmt(int dtype) {
 const Mat kNoMat = {nullptr, 0, 0, kNone, 0};
 
 void layout(const void* src, int dtype, int64_t ld, int64_t rows, int64_t cols, const int* exponent,
-            const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt, hipStream_t st) {
+            const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt, hipStream_t st,
+            const int* map = nullptr, const int* live = nullptr) {
   if (dtype == SMQ_DTYPE_F32)
-    launch_layout((const float*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st);
+    launch_layout((const float*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st, map, live);
   else if (dtype == SMQ_DTYPE_F16)
-    launch_layout((const _Float16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st);
+    launch_layout((const _Float16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st, map, live);
   else
-    launch_layout((const __bf16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st);
+    launch_layout((const __bf16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st, map, live);
 }
 
 // The partial maxima of both inputs, absmax_grid of the tokens and of the vocabulary.
@@ -698,23 +764,33 @@ void product(int dtype, int tile, const Operand& A, const Operand& B, int kt, in
   else launch<_Float16, true>(tile, A, B, kt, 1, 0, shares, e, st);
 }
 
-// [rows, cols] in operand form: in place where it can be, else laid out in the workspace.
-// Rows whose keep[row] is `skip` become zeros (keep NULL: none). `turned` (absent: fmt kNone) is written
-// transposed along the way, in one pass over p where both go by the same exponent (float32) or none.
+// Which rows of h an operand is made of: those with keep[row] != skip (the others zeros; keep NULL: all), or
+// with `map` the first *live that it names, gathered.
+struct Pick {
+  const int64_t* keep = nullptr;
+  int64_t skip = 0;
+  const int* map = nullptr;
+  const int* live = nullptr;
+};
+// [rows, cols] in operand form: in place where it can be, else laid out in the workspace. `turned` (absent:
+// fmt kNone) is written transposed along the way, in one pass over p where both go by the same exponent
+// (float32) or none.
 Operand operand(Arena& ws, const void* p, int64_t ld, int64_t rows, int64_t cols, const Shape& s,
-                const int* exponent, const int* turned_exponent, const int64_t* keep, int64_t skip,
-                const Mat& turned, bool run, hipStream_t st) {
-  const bool in_place = direct(p, ld, cols, s.dtype);
+                const int* exponent, const int* turned_exponent, const Pick& pick, const Mat& turned, bool run,
+                hipStream_t st) {
+  const bool in_place = direct(p, ld, cols, s.dtype) && !pick.map;
   const bool once = !in_place && exponent == turned_exponent;
   if (run && turned.fmt != kNone && !once)
-    layout(p, s.dtype, ld, rows, cols, turned_exponent, keep, skip, kNoMat, turned, st);
+    layout(p, s.dtype, ld, rows, cols, turned_exponent, pick.keep, pick.skip, kNoMat, turned, st, pick.map,
+           pick.live);
   if (in_place) return {p, ld, 0, (int)rows};
   const int64_t to = operand_ld(cols, s.split());
   _Float16* q = ws.take<_Float16>((size_t)(rows * to));
   if (run)
-    layout(p, s.dtype, ld, rows, cols, exponent, keep, skip,
-           {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, once ? turned : kNoMat, st);
-  return {q, to, 0, (int)rows};
+    layout(p, s.dtype, ld, rows, cols, exponent, pick.keep, pick.skip,
+           {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, once ? turned : kNoMat, st, pick.map,
+           pick.live);
+  return {q, to, 0, (int)rows, pick.live};
 }
 
 int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype,
@@ -753,6 +829,11 @@ bool in_place32(const void* p, int64_t ld, int64_t cols) {
 }
 bool raw32(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s) {
   return s.split() && s.tokens <= 128 && in_place32(h, ldh, s.dim) && in_place32(w, ldw, s.dim);
+}
+// Whether the rows that take part are gathered: where a product is long (2^35 multiplications, 70 us at the
+// full 16-bit rate) against the copy of h and the launch that finds them.
+bool gathered(const Shape& s) {
+  return s.tokens > 128 && s.tokens * s.vocab >= ((int64_t)1 << 35) / s.dim;
 }
 // The logits' product: by planes, one plane or raw float32.
 template <typename Epi>
@@ -860,16 +941,23 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
   float* rows = a.take<float>(s.tokens);
   const int* exponent = nullptr;
   const int *eh = nullptr, *ew = nullptr;
-  const bool raw = raw32(h, ldh, w, ldw, s);
+  const bool raw = raw32(h, ldh, w, ldw, s), gather = !few.nt && gathered(s);
+  float* top = nullptr;
   if (s.split() && !few.nt && !raw) {
-    float* top = a.take<float>(2 * kMaxParts);
+    top = a.take<float>(2 * kMaxParts);
     exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
-    if (run) {
-      maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, nullptr, st);
-      hipLaunchKernelGGL(exponent_kernel, dim3(1), dim3(256), 0, st, top, absmax_grid(s.tokens),
-                         absmax_grid(s.vocab), head);
-    }
+    if (run) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, nullptr, st);
   }
+  Kept kept = {};
+  Pick pick;
+  if (gather) {
+    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), nullptr};
+    pick.map = kept.map, pick.live = &head->rows;
+  }
+  const int64_t* at = gather ? kept.target : target;
+  if (run && (top || gather))
+    hipLaunchKernelGGL(prepare_kernel, dim3(1), dim3(1024), 0, st, top, absmax_grid(s.tokens),
+                       absmax_grid(s.vocab), head, target, ignore, (int)s.tokens, kept);
   if (few.nt) {
     if (run) {
       if (s.dtype == SMQ_DTYPE_F32) launch_few<float>(few, h, ldh, w, ldw, s, bias, target, ignore, part, picked, st);
@@ -878,22 +966,22 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
     }
   } else {
     const Operand A = raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
-                          : operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, nullptr, 0, kNoMat, run, st);
+                          : operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, pick, kNoMat, run, st);
     const Operand B = raw ? Operand{w, 2 * ldw, 0, (int)s.vocab}
-                          : operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, nullptr, 0, kNoMat, run, st);
-    const SoftmaxEpi e = {exponent, bias, target, part, picked};
+                          : operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, {}, kNoMat, run, st);
+    const SoftmaxEpi e = {exponent, bias, at, part, picked};
     if (run) logits(s, raw, tile, A, B, e, st);
   }
   if (run) {
     int per = 1;
-    if (s.tokens <= 1024 && s.tokens * blocks <= 16384) {
+    if (!gather && s.tokens <= 1024 && s.tokens * blocks <= 16384) {
       while (per < s.tokens) per *= 2;
       hipLaunchKernelGGL(join_loss_kernel, dim3(1), dim3(1024), 0, st, part, blocks, (int)s.tokens, per,
                          target, ignore, s.vocab, picked, lse, reduction, exponent ? 1 : 0, loss, head);
     } else {
       per = s.tokens >= 2048 ? 16 : s.tokens >= 256 ? 4 : 1;
       hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + per - 1) / per)), dim3(256), 0, st, part,
-                         blocks, (int)s.tokens, per, target, ignore, s.vocab, picked, lse, rows);
+                         blocks, (int)s.tokens, per, at, ignore, s.vocab, picked, pick.map, pick.live, lse, rows);
       hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
                          reduction, exponent ? 1 : 0, loss, head);
     }
@@ -937,6 +1025,15 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   const int64_t pieces = (s.vocab + s.piece - 1) / s.piece;
   float* g = a.take<float>(s.tokens);
   Head* fac = a.take<Head>(1);
+  const bool gather = gathered(s);
+  Kept kept = {};
+  Pick pick;
+  pick.keep = target, pick.skip = ignore;
+  if (gather) {
+    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), a.take<float>(s.tokens)};
+    pick = Pick();
+    pick.map = kept.map, pick.live = &fac->rows;
+  }
   const Head* planes = s.dtype == SMQ_DTYPE_F16 ? nullptr : fac;
   float* top = nullptr;
   if (planes) {
@@ -951,17 +1048,17 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
                        (int)s.tokens, reduction, g, head, top, absmax_grid(s.tokens),
-                       absmax_grid(s.vocab), sp ? 1 : 0, fac);
-  // h, and transposed the operand of dw. Ignored rows are zeros, whatever they hold (where h is read in
-  // place its ignored rows' logits are not used).
+                       absmax_grid(s.vocab), sp ? 1 : 0, lse, kept, fac);
+  // h, and transposed the operand of dw. Ignored rows are left out or zeros, whatever they hold (where h is
+  // read in place its ignored rows' logits are not used).
   const int64_t ldt = operand_ld(s.tokens, sp);
   const int padt = operand_pad(s.tokens, sp);
   _Float16* ht = dw ? a.take<_Float16>((size_t)(s.dim * ldt)) : nullptr;
   const Mat turned_h = dw ? Mat{ht, ldt, 0, fmt, padt} : kNoMat;
-  if (run && raw && dw) layout(h, s.dtype, ldh, s.tokens, s.dim, eh, target, ignore, kNoMat, turned_h, st);
+  if (run && raw && dw) layout(h, s.dtype, ldh, s.tokens, s.dim, eh, target, ignore, kNoMat, turned_h, st);  // (not gathered)
   const Operand A =
       raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
-          : operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, eh, target, ignore, turned_h, run, st);
+          : operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, eh, pick, turned_h, run, st);
   const int64_t ldp = operand_ld(s.piece, sp);
   _Float16* dl = a.take<_Float16>((size_t)(s.tokens * ldp));
   _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
@@ -972,7 +1069,7 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   const Shared dp = plan_product(s.tokens, s.dim, operand_kt(s.piece, sp), 1, 0, true);
   const int tile_dh = dp.tile, shares = dp.shares;
   const int64_t ldacc = round_up(s.dim, 4);
-  const bool whole = pieces == 1 && shares == 1;
+  const bool whole = pieces == 1 && shares == 1 && !gather;
   float* accum = dh && !whole ? a.take<float>((size_t)(shares * s.tokens * ldacc)) : nullptr;
   const size_t wsize = s.size();
   const size_t mark = a.used;
@@ -985,31 +1082,32 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     const Mat turned_w = dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat;
     if (run && raw && dh) layout(wp, s.dtype, ldw, n, s.dim, ew, nullptr, 0, kNoMat, turned_w, st);
     const Operand B = raw ? Operand{wp, 2 * ldw, 0, (int)n}
-                          : operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew, nullptr, 0, turned_w, run, st);
+                          : operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew, {}, turned_w, run, st);
     if (a.used > most) most = a.used;
     if (!run) continue;
-    const DlEpi e = {exponent, bias, target, lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
+    const DlEpi e = {exponent, bias, gather ? kept.target : target, gather ? kept.lse : lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
                      {dlt, ldt, 0, fmt, padt}, sums};
     logits(s, raw, tile_l, A, B, e, st);
     if (db)
       hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, sums,
-                         row_blocks, (int)n, fac, db + v0);
+                         row_blocks, (int)n, pick.live, shape_of(tile_l).bm, shape_of(tile_l).wm, fac, db + v0);
     if (dh) {
-      const Operand L = {dl, ldp, 0, (int)s.tokens}, W = {wt, ldp, 0, (int)s.dim};
+      const Operand L = {dl, ldp, 0, (int)s.tokens, pick.live}, W = {wt, ldp, 0, (int)s.dim};
       StoreEpi se = {1.0f, 1.0f, whole ? &fac->scale_dh : nullptr, kNoMat, kNoMat, kNoMat, 0, s.tokens * ldacc, 0.0f};
       se.o = whole ? Mat{dh, s.dim, 0, out_fmt(s.dtype), 0} : Mat{accum, ldacc, 0, kF32, 0};
       if (i > 0) se.src = se.o;
       product(grad_dtype, tile_dh, L, W, operand_kt(n, sp), shares, se, st);
     }
     if (dw) {
-      const Operand L = {dlt, ldt, 0, (int)n}, H = {ht, ldt, 0, (int)s.dim};
+      const Operand L = {dlt, ldt, 0, (int)n, nullptr, pick.live}, H = {ht, ldt, 0, (int)s.dim};
       StoreEpi se = {1.0f, 0.0f, &fac->scale_dw, kNoMat, kNoMat, kNoMat, 0, 0, 0.0f};
       se.o = {reinterpret_cast<char*>(dw) + (size_t)(v0 * s.dim) * wsize, s.dim, 0, out_fmt(s.dtype), 0};
       product(grad_dtype, plan_product(n, s.dim, operand_kt(s.tokens, sp), 1, 0, false).tile, L, H, operand_kt(s.tokens, sp), 1, se, st);
     }
   }
   if (run && dh && !whole) {
-    const StoreEpi se = {1.0f, 0.0f, &fac->scale_dh, kNoMat, {dh, s.dim, 0, out_fmt(s.dtype), 0}, kNoMat, 0, 0, 0.0f};
+    StoreEpi se = {1.0f, 0.0f, &fac->scale_dh, kNoMat, {dh, s.dim, 0, out_fmt(s.dtype), 0}, kNoMat, 0, 0, 0.0f};
+    se.map = pick.map, se.live = pick.live;
     launch_split_sum(accum, ldacc, s.tokens * ldacc, shares, 0, (int)s.tokens, (int)s.dim, 1, 0, se, st);
   }
   return most;

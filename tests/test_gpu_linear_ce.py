@@ -474,3 +474,54 @@ def test_saved_tensor_hooks(tokens, binding, monkeypatch):
 
     with torch.autograd.graph.saved_tensors_hooks(refuse, lambda x: x), pytest.raises(HookError):
         linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+
+
+GATHERED = (520, 704, 100003)  # long enough for the rows that take part to be gathered
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ignored,reduction,piece", [(0.5, "mean", 0), (0.1, "none", 40000), (0, "sum", 0)])
+def test_gathered_rows(ignored, reduction, piece, dtype):
+    h, w, b, t = make(*GATHERED, dtype, True, ignored, seed=28)
+    h = torch.where((t == -100)[:, None], torch.full_like(h, float("nan")), h)
+    check(h, w, b, t, reduction, piece)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kept", [0, 1, 63, 64, 65, 257])
+def test_few_gathered_rows(kept, dtype):
+    h, w, b, t = make(*GATHERED, dtype, True, 0, seed=29)
+    t[torch.randperm(len(t), device="cuda")[kept:]] = -100
+    if kept:
+        check(h, w, b, t, "sum")
+    else:
+        leaves = [x.requires_grad_() for x in (h, w, b)]
+        loss = linear_cross_entropy(h, w, t, b, reduction="none")
+        assert (loss == 0).all()
+        for x in torch.autograd.grad(loss.sum(), leaves):
+            assert (x == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_graph_replays_with_other_ignored_rows(dtype):
+    h, w, b, t = make(*GATHERED, dtype, True, 0, seed=30)
+    leaves = [x.detach().clone().requires_grad_() for x in (h, w, b)]
+
+    def call():
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+        return (loss.detach(), *torch.autograd.grad(loss, leaves))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for k in range(4):
+        t[:: k + 2] = -100
+        t[1:: k + 3] = k
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, call()))
