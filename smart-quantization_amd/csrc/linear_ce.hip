@@ -830,10 +830,13 @@ bool in_place32(const void* p, int64_t ld, int64_t cols) {
 bool raw32(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s) {
   return s.split() && s.tokens <= 128 && in_place32(h, ldh, s.dim) && in_place32(w, ldw, s.dim);
 }
-// Whether the rows that take part are gathered: where a product is long (2^35 multiplications, 70 us at the
-// full 16-bit rate) against the copy of h and the launch that finds them.
+// Whether the rows that take part are gathered: where a product is long against the copy of h (which float32
+// makes anyway) and the launch that finds them. Training, none / 15 % / 40 % ignored, gathered against not:
+// float32 512 x 768 x 30000 499 / 471 / 441 us against 491 / 488 / 484 (256 tokens 382 / 357 / 341, 375 /
+// 365 / 366), fp16 1024 x 1024 x 32000 478 / 447 / 392 against 466 / 464 / 461 (768 x 30000 383 / 360 / 328,
+// 365 / 362 / 361), fp16 2048 x 1024 x 50000 1300 / 1122 / 893 against 1282 / 1278 / 1271.
 bool gathered(const Shape& s) {
-  return s.tokens > 128 && s.tokens * s.vocab >= ((int64_t)1 << 35) / s.dim;
+  return s.tokens > 128 && s.tokens * s.vocab >= ((int64_t)1 << (s.split() ? 33 : 35)) / s.dim;
 }
 // The logits' product: by planes, one plane or raw float32.
 template <typename Epi>
