@@ -503,6 +503,8 @@ __global__ __launch_bounds__(256) void stream_forward(Args A) {
   }
 }
 
+// One row at a time: with four in flight the eight channels' coefficients and sums took 165 registers, 3
+// waves a SIMD (4 x 256 x 256 x 256 bf16 silu: 72 us, 62 now; its 268 MB take 52 at the rate of a copy).
 template <typename T, int V>
 __global__ __launch_bounds__(256) void stream_sums(Args A) {
   typedef typename Pack<T, V>::type vec;
@@ -524,7 +526,7 @@ __global__ __launch_bounds__(256) void stream_sums(Args A) {
       mul[i] = (A.weight ? A.weight[w.c + i] : 1.0f) * rstd[i];
       b[i] = A.bias ? A.bias[w.c + i] : 0.0f;
     }
-#pragma unroll 4
+#pragma unroll 1
     for (int64_t r = w.first + w.row; r < w.last; r += w.rows) {
       const vec v = *reinterpret_cast<const vec*>(x + r * A.c);
       const vec d = *reinterpret_cast<const vec*>(dy + r * A.c);
@@ -596,7 +598,7 @@ __global__ __launch_bounds__(256) void stream_backward(Args A) {
     b[i] = A.bias ? A.bias[w.c + i] : 0.0f;
     c1[i] = -rstd * k.x, c2[i] = -rstd * rstd * k.y;
   }
-#pragma unroll 4
+#pragma unroll 2
   for (int64_t r = w.first + w.row; r < w.last; r += w.rows) {
     const vec v = *reinterpret_cast<const vec*>(x + r * A.c);
     const vec d = *reinterpret_cast<const vec*>(dy + r * A.c);
