@@ -9,6 +9,16 @@
 // again, dl is written once as the 16-bit operand of the two gradient products, row by row and
 // transposed, and used up. Only lse is kept between the two passes.
 //
+// By size and type:
+//   up to 16 tokens        no matrix cores: the weight is read as it is, once in the forward and twice in the
+//                          backward (1 x 768 x 30000 float32 forward: 23 us, 18 at the rate of a copy)
+//   float32, to 128        the logits on the fp32 matrix instructions from the inputs in place, where their rows
+//                          allow (64 x 1024 x 30000: forward 47 us, both directions 267)
+//   the rest               16-bit matrix products; long ones over the rows that take part only (Kept).
+// Measured, forward and backward: 8192 x 4096 x 131072 bf16 33.5 ms (8 N V D operations with the logits'
+// second computation: 1050 TFLOP/s), 2048 x 768 x 30000 float32 1.29 ms, 777 x 1001 x 50001 fp16 with a third
+// of the rows ignored 0.63 ms. What bounds the large ones is the product itself, then dl's two copies.
+//
 // float32 inputs run as two fp16 planes (gemm_nt.h) scaled by a power of two per tensor; bf16 and fp16
 // inputs as they are. In the gradient products every 16-bit operand is fp16: dl rounded to 11 bits
 // (8 bits of bf16 were off by up to 2e-3 in the gradient of a target's row), and bf16 inputs, exact in
@@ -246,7 +256,8 @@ struct SoftmaxEpi {
 // ---- few tokens -----------------------------------------------------------------------------------
 // Bound by reading the weight (and writing its gradient): each wave takes kRows vocabulary entries at a
 // time straight from memory in their own type (no fp16 planes, no transposed copies), V elements a lane,
-// against up to NT rows of hidden kept in LDS as fp32. Ignored rows are zeros there.
+// against up to NT rows of hidden kept in LDS as fp32. Ignored rows are zeros there. Where there are fewer
+// rows than NT the last one stands for the missing, whose results go nowhere and whose factors are 0.
 constexpr int kRows = 4;
 template <typename T, int V> struct FewVec {
   typedef T type __attribute__((ext_vector_type(V)));
@@ -276,12 +287,12 @@ __device__ __forceinline__ void few_hidden(const float* p, float (&y)[V]) {
     for (int i = 0; i < V; i++) y[i] = p[i];
   }
 }
-template <typename T, int NT>
+template <typename T>
 __device__ __forceinline__ void few_stage(const T* h, int64_t ldh, int tokens, int dim,
                                           const int64_t* target, int64_t ignore, float* hs) {
-  for (int i = threadIdx.x; i < NT * dim; i += blockDim.x) {
+  for (int i = threadIdx.x; i < tokens * dim; i += blockDim.x) {
     const int t = i / dim;
-    hs[i] = t < tokens && target[t] != ignore ? (float)h[(int64_t)t * ldh + (i - t * dim)] : 0.0f;
+    hs[i] = target[t] != ignore ? (float)h[(int64_t)t * ldh + (i - t * dim)] : 0.0f;
   }
   __syncthreads();
 }
@@ -309,8 +320,8 @@ __device__ __forceinline__ void fold_lanes(float* acc, int lane) {
 // wave's lanes halve the values held at each exchange: 63 exchanges for 64 values, where a sum apiece in
 // all lanes takes 384, and what follows (exponentials) is done once instead of by all lanes.
 template <typename T, int V, int NT>
-__device__ __forceinline__ float few_logits(const T* w, int64_t ldw, int dim, int vocab, const float* hs,
-                                            int v0, int lane) {
+__device__ __forceinline__ float few_logits(const T* w, int64_t ldw, int tokens, int dim, int vocab,
+                                            const float* hs, int v0, int lane) {
   constexpr int N = kRows * NT;
   const T* p[kRows];
 #pragma unroll
@@ -326,7 +337,7 @@ __device__ __forceinline__ float few_logits(const T* w, int64_t ldw, int dim, in
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       float y[V];
-      few_hidden<V>(hs + t * dim + k, y);
+      few_hidden<V>(hs + (t < tokens ? t : tokens - 1) * dim + k, y);
 #pragma unroll
       for (int r = 0; r < kRows; r++)
 #pragma unroll
@@ -343,16 +354,16 @@ __global__ __launch_bounds__(1024) void few_kernel(const T* h, int64_t ldh, cons
                                                    int tokens, int dim, int vocab, const float* bias,
                                                    const int64_t* target, int64_t ignore, float2* part,
                                                    float* picked) {
-  extern __shared__ float hs[];  // [NT][dim]
+  extern __shared__ float hs[];  // [tokens][dim]
   __shared__ float2 joint[16][kRows * NT];
-  few_stage<T, NT>(h, ldh, tokens, dim, target, ignore, hs);
+  few_stage<T>(h, ldh, tokens, dim, target, ignore, hs);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int n = lane >> FewLane<NT>::kSame, r = n / NT, t = n % NT;
   const float ninf = -__builtin_inff();
   const int64_t y = t < tokens ? target[t] : -1;
   float top = ninf, sum = 0.0f;
   for (int v0 = (blockIdx.x * waves + wave) * kRows; v0 < vocab; v0 += gridDim.x * waves * kRows) {
-    float l = few_logits<T, V, NT>(w, ldw, dim, vocab, hs, v0, lane);
+    float l = few_logits<T, V, NT>(w, ldw, tokens, dim, vocab, hs, v0, lane);
     const int v = v0 + r;
     if (v < vocab) {
       if (bias) l += bias[v];
@@ -388,8 +399,8 @@ __global__ __launch_bounds__(1024) void few_backward_kernel(const T* h, int64_t 
                                                             T* dw, float* db) {
   typedef typename FewVec<T, V>::type vec;
   constexpr int kSame = FewLane<NT>::kSame;
-  extern __shared__ float hs[];  // [NT][dim]
-  few_stage<T, NT>(h, ldh, tokens, dim, target, ignore, hs);
+  extern __shared__ float hs[];  // [tokens][dim]
+  few_stage<T>(h, ldh, tokens, dim, target, ignore, hs);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int n = lane >> kSame, r = n / NT, t = n % NT;
   // the lane's token: its factor (a bad target makes it NaN), lse and target
@@ -404,7 +415,7 @@ __global__ __launch_bounds__(1024) void few_backward_kernel(const T* h, int64_t 
     else g = __builtin_nanf("");
   }
   for (int v0 = (blockIdx.x * waves + wave) * kRows; v0 < vocab; v0 += gridDim.x * waves * kRows) {
-    float l = few_logits<T, V, NT>(w, ldw, dim, vocab, hs, v0, lane);
+    float l = few_logits<T, V, NT>(w, ldw, tokens, dim, vocab, hs, v0, lane);
     const int v = v0 + r;
     if (bias && v < vocab) l += bias[v];
     const float p = exp_near(l - ls) - (at == v ? 1.0f : 0.0f);
@@ -433,7 +444,7 @@ __global__ __launch_bounds__(1024) void few_backward_kernel(const T* h, int64_t 
 #pragma unroll
       for (int q = 0; q < NT; q++) {
         float y[V];
-        few_hidden<V>(hs + q * dim + k, y);
+        few_hidden<V>(hs + (q < tokens ? q : tokens - 1) * dim + k, y);
 #pragma unroll
         for (int i = 0; i < kRows; i++)
 #pragma unroll
@@ -846,7 +857,8 @@ void logits(const Shape& s, bool raw, int tile, const Operand& A, const Operand&
   else product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
 }
 
-// Few tokens: up to 16, hidden within 128 KiB of LDS; 0: not few.
+// Few tokens: up to 16, hidden within 148 KiB of LDS; 0: not few.
+constexpr size_t kFewLds = 148 * 1024;
 struct Few {
   int nt, v;
   size_t lds;
@@ -855,8 +867,8 @@ struct Few {
 Few few_tokens(const void* w, int64_t ldw, const Shape& s) {
   if (s.tokens > 16) return {};
   const int nt = s.tokens <= 1 ? 1 : s.tokens <= 2 ? 2 : s.tokens <= 4 ? 4 : s.tokens <= 8 ? 8 : 16;
-  const size_t lds = (size_t)nt * s.dim * 4;
-  if (lds > 128 * 1024) return {};
+  const size_t lds = (size_t)s.tokens * s.dim * 4;
+  if (lds > kFewLds) return {};
   const int size = (int)s.size();
   int v = 8 / size < 4 ? 4 : 8 / size;  // 4 elements a lane
   while (v > 1 && (s.dim % v || ldw % v || (reinterpret_cast<uintptr_t>(w) & (v * size - 1)))) v /= 2;
@@ -893,7 +905,7 @@ void few_case(const Few& p, F f) {
 template <typename K>
 void allow_lds(K kernel, size_t bytes) {
   if (bytes > 48 * 1024)
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)kFewLds);
 }
 template <typename T>
 void launch_few(const Few& p, const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& s,

@@ -525,3 +525,11 @@ def test_graph_replays_with_other_ignored_rows(dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, call()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,dim", [(16, 2368), (16, 2369), (13, 2542), (9, 4209), (5, 7577), (3, 12629),
+                                        (1, 37888), (1, 37889)])
+def test_few_tokens_to_the_last_of_the_lds(tokens, dim, dtype):
+    # (a single row takes part: the mean over none is NaN)
+    check(*make(tokens, dim, 77, dtype, True, 0.2 if tokens > 1 else 0, seed=tokens), "mean")
