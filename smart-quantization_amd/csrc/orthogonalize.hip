@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64) void norm_kernel(const double* part, int n, dou
 // computes, so one workgroup keeps A, Q and P of a matrix in LDS (as operands: two planes in the
 // tiles of gemm_nt.h) and registers (as fp32). With `whole`, where n is short or the stack deep, it also
 // forms A from X, applies P and goes through all stages; else it takes A from, and leaves P in, global
-// memory. 64 x 64 float32, 5 steps: 49 us a call (110 as 18 launches of gemm_nt.h). For m up to 128, on 16
+// memory. 64 x 64 float32, 5 steps: 52 us a call (110 as 18 launches of gemm_nt.h). For m up to 128, on 16
 // waves, the same kernel was no faster than those launches.
 struct SmallStep {
   float qa, qb, qc;  // coefficients a, b, c
