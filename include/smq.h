@@ -685,14 +685,16 @@ int smq_cpu_smaq_decompress_f64(const void* packed, double* y, int64_t n, int n_
  * keeping less than the operations it replaces (no normalised copy, no logits, one momentum). They
  * have no counterpart among the reference's plugins. Device pointers; dtype SMQ_DTYPE_F32 / _F16 /
  * _BF16; sums, statistics and gradients of parameters in fp32 or wider. Results do not depend on
- * timing: no floating-point atomics. Workspaces need no initialisation. */
+ * timing: no floating-point atomics. Workspaces need no initialisation and start on 16-byte
+ * boundaries, as the gradients of the cross entropy do. */
 
 /* Softmax cross entropy of a linear head over a vocabulary:
  *   logits[m, v] = hidden[m] . weight[v] + bias[v], loss[m] = log sum_v exp logits[m, v] - logits[m, target[m]].
  * hidden [tokens, dim] and weight [vocab, dim] have unit column stride and the given row pitches
  * (elements); bias [vocab] fp32 or NULL. The logits are never stored: the forward keeps lse [tokens]
  * and `head` (SMQ_CE_HEAD_BYTES of device memory, 8-byte aligned), the backward computes them again for
- * `piece` vocabulary entries at a time (0: as many as 1 GiB of workspace allows). Rows whose target is
+ * `piece` vocabulary entries at a time (0: as many as 1 GiB of workspace allows). tokens, dim <= 2^20,
+ * vocab <= 2^21, tokens * vocab <= 2^38. Rows whose target is
  * ignore_index have loss and gradient 0, whatever they hold; any other target outside [0, vocab) makes
  * its loss and gradient NaN. loss: one fp32 (mean over the rows taking part, NaN if there are none;
  * sum) or [tokens] (none); grad_loss the same shape. Gradients are written whole, in the inputs' dtype

@@ -820,8 +820,8 @@ int smq_group_norm_act(const void* x, int dtype, void* y, int64_t n, int64_t pos
   const int v = width_of(dtype, c, ptrs, 2);
   Args A = {};
   const size_t need = gn::workspace(dtype, n, positions, c, cg, false, &A, workspace);
-  if (!workspace || workspace_bytes < need) {
-    set_error("group_norm_act: workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+    set_error("group_norm_act: workspace: need %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
     return SMQ_ERR_WORKSPACE;
   }
   const Plan p = plan_of(dtype, v, n, positions, c, cg, false);
@@ -851,8 +851,8 @@ int smq_group_norm_act_backward(const void* x, const void* dy, int dtype, void* 
   const int v = width_of(dtype, c, ptrs, 3);
   Args A = {};
   const size_t need = gn::workspace(dtype, n, positions, c, cg, true, &A, workspace);
-  if (!workspace || workspace_bytes < need) {
-    set_error("group_norm_act_backward: workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+    set_error("group_norm_act_backward: workspace: need %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
     return SMQ_ERR_WORKSPACE;
   }
   const Plan p = plan_of(dtype, v, n, positions, c, cg, true);

@@ -1170,8 +1170,8 @@ int smq_linear_ce_forward(const void* hidden, int64_t hidden_ld, const void* wei
   }
   const size_t need = smq_linear_ce_workspace_bytes(hidden, hidden_ld, weight, weight_ld, dtype,
                                                     tokens, dim, vocab, 0, 0);
-  if (!workspace || workspace_bytes < need) {
-    set_error("linear_ce_forward: workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+    set_error("linear_ce_forward: workspace: need %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
     return SMQ_ERR_WORKSPACE;
   }
   const Shape s = {tokens, dim, vocab, 0, dtype};
@@ -1199,9 +1199,13 @@ int smq_linear_ce_backward(const void* hidden, int64_t hidden_ld, const void* we
                     (grad_bias ? SMQ_CE_GRAD_BIAS : 0);
   const size_t need = smq_linear_ce_workspace_bytes(hidden, hidden_ld, weight, weight_ld, dtype,
                                                     tokens, dim, vocab, piece, flags);
-  if (!workspace || workspace_bytes < need) {
-    set_error("linear_ce_backward: workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+    set_error("linear_ce_backward: workspace: need %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
     return SMQ_ERR_WORKSPACE;
+  }
+  if ((reinterpret_cast<uintptr_t>(grad_hidden) | reinterpret_cast<uintptr_t>(grad_weight)) & 15) {
+    set_error("linear_ce_backward: gradients have to start on 16-byte boundaries");
+    return SMQ_ERR_INVALID;
   }
   const Shape s = {tokens, dim, vocab, piece, dtype};
   backward(hidden, hidden_ld, weight, weight_ld, s, target, bias, ignore_index, reduction, lse,

@@ -743,8 +743,8 @@ int smq_orthogonalize(const void* x, int64_t ld, int64_t batch_stride, int dtype
     return SMQ_ERR_INVALID;
   }
   const size_t need = smq_orthogonalize_workspace_bytes(dtype, batch, rows, cols);
-  if (!workspace || workspace_bytes < need) {
-    set_error("orthogonalize: workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)) {
+    set_error("orthogonalize: workspace: need %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
     return SMQ_ERR_WORKSPACE;
   }
   enqueue(p, x, ld, batch_stride, y, eps, workspace, true, reinterpret_cast<hipStream_t>(stream));

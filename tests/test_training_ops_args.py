@@ -177,3 +177,20 @@ def test_cross_entropy_limits_the_launch():
         need = lib.smq_linear_ce_workspace_bytes(p, 64, p, 64, N.SMQ_DTYPE_BF16, tokens, 64, vocab, 0, 0)
         assert (need > 0) == ok
     assert "2^38" in err()
+
+
+def test_c_abi_refuses_bad_alignment():
+    lib = N.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 63) & ~63
+    shape, tail = (p, 8, p, 8, 0), (p, None, 4, 8, 9, -100, 1)
+    big = 1 << 30
+    assert lib.smq_linear_ce_forward(*shape, *tail, p, p, p, p + 8, big, None) == -2 and "16-byte" in err()
+    assert lib.smq_linear_ce_backward(*shape, *tail, p, p, p, p, None, None, 0, p + 4, big, None) == -2
+    assert lib.smq_linear_ce_backward(*shape, *tail, p, p, p, p + 4, None, None, 0, p, big, None) == -1
+    assert lib.smq_linear_ce_backward(*shape, *tail, p, p, p, None, p + 8, None, 0, p, big, None) == -1
+    assert "boundaries" in err()
+    gn = (p, 0, p, 1, 4, 8, 2, None, None, 1e-5, 0, p, p)
+    assert lib.smq_group_norm_act(*gn, p + 4, big, None) == -2
+    c = (ctypes.c_double * 3)(3.4445, -4.7750, 2.0315)
+    assert lib.smq_orthogonalize(p, 6, 24, 0, p, 1, 4, 6, 5, c, 1e-7, p + 8, big, None) == -2
