@@ -9,7 +9,7 @@
 //               Three products hi*hi + hi*lo + lo*hi per k step; the dropped lo*lo is below 2^-24 of
 //               the largest product. An fp32-class product at a third of the fp16 rate, where the
 //               fp32 MFMA runs at a sixteenth.
-//   float32     as it is (Raw32), k padded to 32: the fp32 instructions, an eighth of the fp16 rate but no
+//   float32     as it is (Raw32), k padded to 32: the fp32 instructions, a sixteenth of the fp16 rate but no
 //               pass that makes planes; ld counts 16-bit units here too.
 //   twice       one plane in the layout of two, [32 x | 32 x] (kDup): against an operand of two planes
 //               the one-plane product gives (hi + lo) x.

@@ -833,7 +833,7 @@ int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t
 
 // float32 logits of up to 128 tokens, where both tensors are operands as they are: on the fp32 matrix
 // instructions straight from them. Making planes of the weight moves it three times more; with more tokens
-// the planes' eightfold rate pays for that (64 x 1024 x 30000: 272 us a step against 330 with planes, 256
+// the planes' fivefold rate pays for that (64 x 1024 x 30000: 272 us a step against 330 with planes, 256
 // tokens about even, 130 x 484 x 48351, whose rows would have to be copied, 573 against 411).
 bool in_place32(const void* p, int64_t ld, int64_t cols) {
   return cols % 32 == 0 && ld % 4 == 0 && ld <= (1 << 20) && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
