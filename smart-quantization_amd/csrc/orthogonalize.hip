@@ -88,6 +88,9 @@ __global__ __launch_bounds__(64) void norm_kernel(const double* part, int n, dou
 // forms A from X, applies P and goes through all stages; else it takes A from, and leaves P in, global
 // memory. 64 x 64 float32, 5 steps: 52 us a call (110 as 18 launches of gemm_nt.h). For m up to 128, on 16
 // waves, the same kernel was no faster than those launches.
+//
+// The workgroups of a stack do not wait for one another, and the buffers of X change their format between the
+// stages: a matrix keeps to its own part of them, at one stride (x[k].batch, xt[k].batch) whatever the format.
 struct SmallStep {
   float qa, qb, qc;  // coefficients a, b, c
   float sa, sq, sw, sp;  // 2^e of A, Q, W = Q A and P as operands
@@ -97,7 +100,7 @@ struct SmallArgs {
   int steps;         // of this launch (a stage, or all)
   int stage;         // steps of a stage
   int m, n, batch;
-  Mat x[2], xt[2];   // whole: X and X^T; the stages alternate
+  Mat x[2], xt[2];   // whole: X and X^T; the stages alternate (batch: room for a matrix in every format)
   Mat y;             // whole: the result
   int turned;
   int fmt_x0, fmt_xt0, coarse;
@@ -257,7 +260,7 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
     if constexpr (WHOLE) {
       Mat X = A.x[stage & 1];
       if (stage == 0) X.fmt = A.fmt_x0;
-      else X.fmt = kSplit, X.ld = (int64_t)round32(n) * 2, X.batch = X.ld * m;
+      else X.fmt = kSplit, X.ld = (int64_t)round32(n) * 2;
       const bool two = X.fmt == kSplit;
       const int kt = two ? (n + 31) / 32 : (n + 63) / 64;
       auto load = [&](int first, _Float16* region) {
@@ -364,7 +367,6 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
       XT.fmt = stage == 0 ? A.fmt_xt0 : end && A.coarse ? kF16 : kSplit;
       const bool one = XT.fmt == kF16, two = XT.fmt == kSplit;
       if (stage > 0) XT.ld = one ? (int64_t)round64(m) : (int64_t)round32(m) * 2;
-      if (stage > 0) XT.batch = XT.ld * n;
       const float sp = A.step[done + r - 1].sp;
       const float f = A.ex[stage] * (stage == 0 ? A.rest[batch] : 1.0f) * A.ey[stage] / sp;
       __syncthreads();
@@ -373,10 +375,10 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
       // the next stage's matrices
       const bool next_coarse = A.steps - done - r <= A.stage && A.coarse;
       Mat X2 = A.x[(stage + 1) & 1], XT2 = A.xt[(stage + 1) & 1];
-      X2.fmt = kSplit, X2.ld = (int64_t)round32(n) * 2, X2.batch = X2.ld * m, X2.pad = round32(n);
+      X2.fmt = kSplit, X2.ld = (int64_t)round32(n) * 2, X2.pad = round32(n);
       XT2.fmt = next_coarse ? kF16 : kSplit;
       XT2.pad = next_coarse ? round64(m) : round32(m);
-      XT2.ld = next_coarse ? XT2.pad : 2 * XT2.pad, XT2.batch = XT2.ld * n;
+      XT2.ld = next_coarse ? XT2.pad : 2 * XT2.pad;
 #pragma unroll 1
       for (int c0 = 0; c0 < n; c0 += DIM) {
         for (int t = 0; t < tiles; t++) s.fetch(XT, batch, c0, n, t, r1, t);
@@ -569,10 +571,10 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
   w.part = a.take<float>(share_floats(p));
   if (!run) return a.used;
 
+  // (a matrix's place in its buffer is the same in every format, small_kernel)
   auto mat = [&](_Float16* q, int64_t cols, int64_t rows, int fmt) {
     const bool two = fmt != kF16;
-    const int64_t l = operand_ld(cols, two);
-    return Mat{q, l, rows * l, fmt, operand_pad(cols, two)};
+    return Mat{q, operand_ld(cols, two), rows * (cols == n ? ldn : ldm), fmt, operand_pad(cols, two)};
   };
   auto op = [](const Mat& q, int64_t rows) { return Operand{q.p, q.ld, q.batch, (int)rows}; };
   const Mat none = {nullptr, 0, 0, kNone, 0};
@@ -596,6 +598,7 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
     SmallArgs sa = {};
     sa.steps = p.steps, sa.stage = longest, sa.m = (int)m, sa.n = (int)n, sa.batch = batch;
     sa.x[0] = X, sa.xt[0] = XT, sa.x[1].p = w.x[1], sa.xt[1].p = w.xt[1];
+    sa.x[1].batch = X.batch, sa.xt[1].batch = XT.batch;
     sa.fmt_x0 = X.fmt, sa.fmt_xt0 = XT.fmt, sa.coarse = coarse ? 1 : 0, sa.turned = p.turned ? 1 : 0;
     sa.y = {y, p.turned ? m : n, m * n, out, 0};
     sa.rest = rest, sa.rest2 = rest2;

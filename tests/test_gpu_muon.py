@@ -244,3 +244,26 @@ def test_zero_matrix_with_a_tiny_eps(shape):
     y = orthogonalize(x, eps=1e-30)
     assert (y[1] == 0).all() and torch.isfinite(y).all()
     assert torch.equal(y[0], orthogonalize(x[:1], eps=1e-30)[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steps", [5, 7, 8])
+@pytest.mark.parametrize("m,n", [(32, 64), (48, 40), (64, 96)])
+def test_deep_stacks_of_small_matrices(m, n, steps, dtype):
+    """Far more matrices than the chip holds at once: each is what it is alone, bit for bit. The stages of a
+    call change the format of the buffers that all its matrices share."""
+    g = torch.Generator(device="cuda").manual_seed(steps)
+    x = torch.randn(3000, m, n, generator=g, device="cuda").to(dtype)
+    y = orthogonalize(x, steps=steps)
+    assert torch.equal(y, orthogonalize(x.flip(0), steps=steps).flip(0))
+    for k in (0, 1, 2, 255, 256, 1024, 1500, 2047, 2998, 2999):
+        assert torch.equal(y[k], orthogonalize(x[k], steps=steps))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n", [(32, 512), (20, 1000), (1024, 17), (32, 480), (50, 513)])
+def test_stacks_of_long_small_matrices(m, n, dtype):
+    """At least 128 matrices, some with rows of whole 2 KiB as planes (which are padded)."""
+    x = matrix(130, m, n, 4.0, seed=n).to(dtype).cuda()
+    y = check(x, 4.0)
+    assert torch.equal(y, orthogonalize(x.flip(0)).flip(0))
