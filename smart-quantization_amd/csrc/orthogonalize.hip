@@ -18,8 +18,9 @@
 // ratio of the singular values once more for each step behind its first: five steps measured 0.9 - 2.5e-6
 // off as single steps, 1.1 - 5.6e-6 as 2 + 2 + 1, 2 - 5e-6 as 3 + 2 (plain float32 products 0.6 - 3.4e-6).
 // float32 takes single steps; the 16-bit types, whose results round to 2^-11 and 2^-8, stages of 3. 16-bit
-// inputs are exact in one plane, so the first stage reads one plane of them; for bf16 results the last
-// P X takes one plane of each (0.03 - 0.3 % off, against the 0.17 % of the result's own rounding).
+// inputs are exact in one plane, so the first stage reads one plane of them. (One plane of each operand in the
+// last P X of bf16 results would save 80 us of 1156 at 6 x 1024 x 4096 and be 0.03 - 0.3 % off, against
+// the 0.17 % of the result's own rounding.)
 #include <math.h>
 
 #include "gemm_nt.h"
@@ -31,7 +32,6 @@ using namespace gemm;
 constexpr int kParts = 256;
 
 __host__ __device__ constexpr int round32(int v) { return (v + 31) & ~31; }
-__host__ __device__ constexpr int round64(int v) { return (v + 63) & ~63; }
 
 // ---- the norm -----------------------------------------------------------------------------------
 template <typename T>
@@ -103,7 +103,7 @@ struct SmallArgs {
   Mat x[2], xt[2];   // whole: X and X^T; the stages alternate (batch: room for a matrix in every format)
   Mat y;             // whole: the result
   int turned;
-  int fmt_x0, fmt_xt0, coarse;
+  int fmt_x0, fmt_xt0;
   const float* rest;
   const float* rest2;
   float ex[8];       // 2^-ex of X at each stage's start
@@ -211,8 +211,8 @@ struct Small {
         for (int r = 0; r < 16; r += 4)
           f(i, j, r, br * TM * 32 + i * 32 + (lane & 31), bc * TN * 32 + j * 32 + 2 * r + 4 * (lane >> 5));
   }
-  // A symmetric matrix as an operand: v * scale, columns from m on are zeros.
-  __device__ __forceinline__ void put(_Float16* region, const Block& v, float scale, int m, bool two) const {
+  // A symmetric matrix as an operand of two planes: v * scale, columns from m on are zeros.
+  __device__ __forceinline__ void put(_Float16* region, const Block& v, float scale, int m) const {
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
     each(wm, wn, [&](int i, int j, int r, int row, int col) {
       h4 hi, lo;
@@ -222,16 +222,10 @@ struct Small {
         hi[k] = (_Float16)x;
         lo[k] = (_Float16)(x - (float)hi[k]);
       }
-      const int x7 = row & 7;
-      if (two) {
-        _Float16* t = region + (col >> 5) * kTileHalves + row * 64 + (col & 7);
-        const int c = (col & 31) >> 3;
-        *reinterpret_cast<h4*>(t + (c ^ x7) * 8) = hi;
-        *reinterpret_cast<h4*>(t + ((c + 4) ^ x7) * 8) = lo;
-      } else {
-        _Float16* t = region + (col >> 6) * kTileHalves + row * 64 + (col & 7);
-        *reinterpret_cast<h4*>(t + (((col & 63) >> 3) ^ x7) * 8) = hi;
-      }
+      const int x7 = row & 7, c = (col & 31) >> 3;
+      _Float16* t = region + (col >> 5) * kTileHalves + row * 64 + (col & 7);
+      *reinterpret_cast<h4*>(t + (c ^ x7) * 8) = hi;
+      *reinterpret_cast<h4*>(t + ((c + 4) ^ x7) * 8) = lo;
     });
   }
 };
@@ -299,7 +293,7 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
         a[i][j][q + 2] = v.z * A.gram_scale, a[i][j][q + 3] = v.w * A.gram_scale;
       });
     }
-    s.put(r0, a, A.step[done].sa, m, true);
+    s.put(r0, a, A.step[done].sa, m);
     __syncthreads();
     // ---- P of the stage
 #pragma unroll 1
@@ -315,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
         for (int e = 0; e < 4; e++)
           acc[x][y][q + e] = (row == col + e ? k.qa : 0.0f) + k.qb * a[x][y][q + e] + k.qc * acc[x][y][q + e];
       });
-      s.put(r1, acc, k.sq, m, true);
+      s.put(r1, acc, k.sq, m);
       if (i == 0) {
 #pragma unroll
         for (int x = 0; x < S::TM; x++)
@@ -329,7 +323,7 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
         s.product(r1, r0, km, true, s.wm, s.wn, acc, low);  // W = Q A
         s.sum(acc, low, iq * ia);
         __syncthreads();
-        s.put(r0, acc, k.sw, m, true);
+        s.put(r0, acc, k.sw, m);
         __syncthreads();
         s.clear(a);
         s.clear(low);
@@ -339,7 +333,7 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
       }
       if (i > 0) {  // P <- Q P
         if (i + 1 == r) __syncthreads();
-        s.put(r0, p, A.step[done + i - 1].sp, m, true);
+        s.put(r0, p, A.step[done + i - 1].sp, m);
         __syncthreads();
         s.clear(p);
         s.clear(low);
@@ -348,7 +342,7 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
         __syncthreads();
       }
       if (i + 1 < r) {
-        s.put(r0, a, A.step[done + i + 1].sa, m, true);
+        s.put(r0, a, A.step[done + i + 1].sa, m);
         __syncthreads();
       }
     }
@@ -364,29 +358,25 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
       });
     } else {
       Mat XT = A.xt[stage & 1];
-      XT.fmt = stage == 0 ? A.fmt_xt0 : end && A.coarse ? kF16 : kSplit;
-      const bool one = XT.fmt == kF16, two = XT.fmt == kSplit;
-      if (stage > 0) XT.ld = one ? (int64_t)round64(m) : (int64_t)round32(m) * 2;
+      XT.fmt = stage == 0 ? A.fmt_xt0 : kSplit;
+      const bool two = XT.fmt == kSplit;
+      if (stage > 0) XT.ld = (int64_t)round32(m) * 2;
       const float sp = A.step[done + r - 1].sp;
       const float f = A.ex[stage] * (stage == 0 ? A.rest[batch] : 1.0f) * A.ey[stage] / sp;
       __syncthreads();
-      s.put(r0, p, sp, m, !one);
-      const int tiles = one ? (m + 63) / 64 : km;
+      s.put(r0, p, sp, m);
       // the next stage's matrices
-      const bool next_coarse = A.steps - done - r <= A.stage && A.coarse;
       Mat X2 = A.x[(stage + 1) & 1], XT2 = A.xt[(stage + 1) & 1];
       X2.fmt = kSplit, X2.ld = (int64_t)round32(n) * 2, X2.pad = round32(n);
-      XT2.fmt = next_coarse ? kF16 : kSplit;
-      XT2.pad = next_coarse ? round64(m) : round32(m);
-      XT2.ld = next_coarse ? XT2.pad : 2 * XT2.pad;
+      XT2.fmt = kSplit, XT2.ld = (int64_t)round32(m) * 2, XT2.pad = round32(m);
 #pragma unroll 1
       for (int c0 = 0; c0 < n; c0 += DIM) {
-        for (int t = 0; t < tiles; t++) s.fetch(XT, batch, c0, n, t, r1, t);
+        for (int t = 0; t < km; t++) s.fetch(XT, batch, c0, n, t, r1, t);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (!end || !A.turned) {
           s.clear(acc);
           s.clear(low);
-          s.product(r0, r1, tiles, two, s.wm, s.wn, acc, low);
+          s.product(r0, r1, km, two, s.wm, s.wn, acc, low);
           s.sum(acc, low, f);
           s.each(s.wm, s.wn, [&](int i, int j, int q, int row, int col) {
             const float w[4] = {acc[i][j][q], acc[i][j][q + 1], acc[i][j][q + 2], acc[i][j][q + 3]};
@@ -396,7 +386,7 @@ __global__ __launch_bounds__(256, 2) void small_kernel(SmallArgs A) {
         if (!end || A.turned) {  // the same product the other way round: runs along m
           s.clear(acc);
           s.clear(low);
-          s.product(r1, r0, tiles, two, s.wm, s.wn, acc, low);
+          s.product(r1, r0, km, two, s.wm, s.wn, acc, low);
           s.sum(acc, low, f);
           s.each(s.wm, s.wn, [&](int i, int j, int q, int row, int col) {
             const float w[4] = {acc[i][j][q], acc[i][j][q + 1], acc[i][j][q + 2], acc[i][j][q + 3]};
@@ -514,17 +504,14 @@ void first_layout(const Plan& p, const T* g, int64_t ld, int64_t stride, double 
 // The products of a call of either format, walked without a launch: the floats their shares need.
 size_t share_floats(const Plan& p) {
   size_t need = 0;
-  for (int s = 0; s < 2; s++) {
-    const bool sp = s == 0;
-    const Operand X = {nullptr, 0, 0, (int)p.m}, XT = {nullptr, 0, 0, (int)p.n};
-    StoreEpi e = {};
-    e.tri = 1;
-    product(sp, X, X, operand_kt(p.n, sp), (int)p.batch, e, {}, false, &need, nullptr);
-    product(sp, X, X, operand_kt(p.m, sp), (int)p.batch, e, {}, false, &need, nullptr);
-    e.tri = 0;
-    product(sp, X, XT, operand_kt(p.m, sp), (int)p.batch, e, {}, false, &need, nullptr);
-    product(false, X, XT, operand_kt(p.m, true), (int)p.batch, e, {}, false, &need, nullptr);
-  }
+  const Operand X = {nullptr, 0, 0, (int)p.m}, XT = {nullptr, 0, 0, (int)p.n};
+  const int km = operand_kt(p.m, true), batch = (int)p.batch;
+  StoreEpi e = {};
+  e.tri = 1;
+  product(true, X, X, km, batch, e, {}, false, &need, nullptr);
+  for (int s = 0; s < 2; s++) product(s == 0, X, X, operand_kt(p.n, s == 0), batch, e, {}, false, &need, nullptr);
+  e.tri = 0;
+  for (int s = 0; s < 2; s++) product(s == 0, X, XT, km, batch, e, {}, false, &need, nullptr);
   return need;
 }
 
@@ -579,11 +566,9 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
   auto op = [](const Mat& q, int64_t rows) { return Operand{q.p, q.ld, q.batch, (int)rows}; };
   const Mat none = {nullptr, 0, 0, kNone, 0};
   const int out = p.dtype == SMQ_DTYPE_F32 ? kF32 : p.dtype == SMQ_DTYPE_F16 ? kF16 : kBF16;
-  const bool coarse = p.dtype == SMQ_DTYPE_BF16;  // the last P X in one plane of each
   const int longest = stage_of(p);
-  bool end = p.steps <= longest;                  // the stage at hand is the last one
   Mat X = mat(w.x[0], n, m, p.dtype == SMQ_DTYPE_F32 ? kSplit : kF16);
-  Mat XT = mat(w.xt[0], m, n, p.dtype == SMQ_DTYPE_F32 ? kSplit : end && coarse ? kF16 : kDup);
+  Mat XT = mat(w.xt[0], m, n, p.dtype == SMQ_DTYPE_F32 ? kSplit : kDup);
   if (p.dtype == SMQ_DTYPE_F32)
     first_layout(p, (const float*)g, ld, stride, eps, part, pow2, rest, rest2, X, XT, st);
   else if (p.dtype == SMQ_DTYPE_F16)
@@ -599,7 +584,7 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
     sa.steps = p.steps, sa.stage = longest, sa.m = (int)m, sa.n = (int)n, sa.batch = batch;
     sa.x[0] = X, sa.xt[0] = XT, sa.x[1].p = w.x[1], sa.xt[1].p = w.xt[1];
     sa.x[1].batch = X.batch, sa.xt[1].batch = XT.batch;
-    sa.fmt_x0 = X.fmt, sa.fmt_xt0 = XT.fmt, sa.coarse = coarse ? 1 : 0, sa.turned = p.turned ? 1 : 0;
+    sa.fmt_x0 = X.fmt, sa.fmt_xt0 = XT.fmt, sa.turned = p.turned ? 1 : 0;
     sa.y = {y, p.turned ? m : n, m * n, out, 0};
     sa.rest = rest, sa.rest2 = rest2;
     fill_steps(p, p.steps, longest, &top, &sa);
@@ -617,8 +602,7 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
   for (int done = 0, stage = 0; done < p.steps; stage++) {
     const int r = p.steps - done < longest ? p.steps - done : longest;
     done += r;
-    end = done == p.steps;
-    const int pfmt = end && coarse ? kF16 : kSplit;
+    const bool end = done == p.steps;
     // A = X X^T
     int ea = exponent_for(top * top);
     Mat A = mat(w.gram[0], m, m, kSplit);
@@ -631,7 +615,7 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
       sa.steps = sa.stage = r, sa.m = (int)m, sa.batch = batch;
       sa.gram = A, sa.gram_scale = (float)ldexp(1.0, -ea);
       fill_steps(p, r, r, &top, &sa);
-      P = mat(w.p[0], m, m, pfmt);
+      P = mat(w.p[0], m, m, kSplit);
       sa.p = P, sa.p_scale = sa.step[r - 1].sp;
       frexpf(sa.p_scale, &ep);
       ep -= 1;
@@ -642,7 +626,7 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
       const double t = top * top, lift = fabs(p.a) + fabs(p.b) * t + fabs(p.c) * t * t;
       const int eq = exponent_for(lift);
       // Q = a I + b A + c A A
-      const Mat Q = mat(w.q[i & 1], m, m, r == 1 ? pfmt : kSplit);
+      const Mat Q = mat(w.q[i & 1], m, m, kSplit);
       e = {(float)ldexp(p.c, eq - 2 * ea), (float)ldexp(p.b, eq - ea), nullptr, A, Q, Q, 1, 0,
            (float)ldexp(p.a, eq)};
       product(true, op(A, m), op(A, m), km, batch, e, w, true, nullptr, st);
@@ -652,7 +636,7 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
       } else {
         // P <- Q P
         const int en = exponent_for(most);
-        const Mat P2 = mat(w.p[i & 1], m, m, i + 1 == r ? pfmt : kSplit);
+        const Mat P2 = mat(w.p[i & 1], m, m, kSplit);
         e = {(float)ldexp(1.0, en - eq - ep), 0.0f, nullptr, none, P2, P2, 1, 0, 0.0f};
         product(true, op(Q, m), op(P, m), km, batch, e, w, true, nullptr, st);
         P = P2, ep = en;
@@ -674,16 +658,14 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
     const int ey = end ? 0 : exponent_for(top);
     Mat X2, XT2;
     if (!end) {
-      const bool last = p.steps - done <= longest;
       X2 = mat(w.x[(stage + 1) & 1], n, m, kSplit);
-      XT2 = mat(w.xt[(stage + 1) & 1], m, n, last && coarse ? kF16 : kSplit);
+      XT2 = mat(w.xt[(stage + 1) & 1], m, n, kSplit);
     } else {
       const Mat Y = {y, p.turned ? m : n, m * n, out, 0};
       X2 = p.turned ? none : Y, XT2 = p.turned ? Y : none;
     }
     e = {(float)ldexp(1.0, ey - ep - ex), 0.0f, stage ? nullptr : rest, none, X2, XT2, 0, 0, 0.0f};
-    product(XT.fmt == kSplit, op(P, m), op(XT, n), XT.fmt == kF16 ? operand_kt(m, false) : km, batch, e, w,
-            true, nullptr, st);
+    product(XT.fmt == kSplit, op(P, m), op(XT, n), km, batch, e, w, true, nullptr, st);
     X = X2, XT = XT2, ex = ey;
   }
   return a.used;

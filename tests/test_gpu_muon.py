@@ -267,3 +267,40 @@ def test_stacks_of_long_small_matrices(m, n, dtype):
     x = matrix(130, m, n, 4.0, seed=n).to(dtype).cuda()
     y = check(x, 4.0)
     assert torch.equal(y, orthogonalize(x.flip(0)).flip(0))
+
+
+def tight(length):
+    """Float32-class: per step six operands rounded to two planes (2^-23 each) and a sum of length / 16
+    float32 roundings, all independent, each step's error growing by 1.5 in those behind it; twice that
+    for the worst of a few. One fp16 plane in place of two is 1e-3 to 6e-3 off."""
+    step = 2.0 ** -24 * (6 * 4 + length / 16) ** 0.5
+    return 2 * step * ((1.5 ** 10 - 1) / (1.5 ** 2 - 1)) ** 0.5
+
+
+def shapes():
+    g = torch.Generator().manual_seed(5)
+    yield "gauss", torch.randn(8, 1024, 1536, generator=g)
+    yield "tall", torch.randn(1, 900, 300, generator=g)
+    for ratio in (64.0, 1000.0):
+        yield f"ratio{ratio:.0f}", matrix(2, 200, 320, ratio, seed=3)
+    yield "small", matrix(3, 48, 80, 4.0, seed=7)
+    yield "square", matrix(1, 64, 64, 64.0, seed=3)
+    yield "long", matrix(2, 40, 900, 8.0, seed=8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_16_bit_results_round_once(dtype):
+    """What a result is off beyond half a step of its own type is float32-class: of a stage of three steps,
+    whose powers of the Gram matrix keep less of its small singular values, four times tight(). (The
+    last product in one plane of each operand, emulated: 6e-5 to 1.7e-4 of the norm beyond half a step.)"""
+    for name, x in shapes():
+        x = x.to(dtype)
+        y = orthogonalize(x.cuda())
+        for k in (0, len(x) - 1):
+            want, got = reference(x[k]), y[k].double().cpu()
+            bits = 11 if dtype == torch.float16 else 8
+            lowest = -14 if dtype == torch.float16 else -126
+            half = torch.ldexp(torch.ones_like(got), torch.frexp(got)[1].clamp(min=lowest + 1) - bits - 1)
+            over = ((got - want).abs() - half).clamp(min=0).norm() / want.norm()
+            print(name, k, over.item(), flush=True)
+            assert over <= 4 * tight(max(x.shape[-2:])), (name, over)
