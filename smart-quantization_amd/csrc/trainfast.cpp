@@ -16,7 +16,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/ops/empty_strided.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -55,6 +55,17 @@ void only_once(const char* who) {
 }
 
 // ---- group norm -----------------------------------------------------------------------------------
+// A new tensor of x's shape in channels-last memory. No view: autograd refuses to change a view that a
+// custom function returns in place, and what follows a normalisation often does (out += identity).
+at::Tensor channels_last_like(const at::Tensor& x) {
+  at::DimVector strides(x.dim());
+  int64_t step = x.size(1);
+  strides[1] = 1;
+  for (int64_t d = x.dim() - 1; d > 1; d--) strides[d] = step, step *= x.size(d);
+  strides[0] = step;
+  return at::empty_strided(x.sizes(), strides, x.options());
+}
+
 struct GroupNorm : Function<GroupNorm> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const MaybeTensor& weight_,
                             const MaybeTensor& bias_, int64_t groups, double eps, int64_t act) {
@@ -62,7 +73,7 @@ struct GroupNorm : Function<GroupNorm> {
     const at::Tensor xl = x.detach().movedim(1, -1).contiguous();
     const int64_t n = xl.size(0), c = xl.size(-1), s = xl.numel() / (n * c);
     const c10::DeviceGuard guard(x.device());
-    at::Tensor y = at::empty_like(xl);
+    at::Tensor y = channels_last_like(x);
     at::Tensor stats = at::empty({2, n, groups}, x.options().dtype(at::kFloat));
     const size_t need = smq_group_norm_workspace_bytes(code_of(x), n, s, c, groups, 0);
     const at::Tensor ws = buffer(x, need, "group_norm_act"), w = f32(weight), b = f32(bias);
@@ -73,7 +84,7 @@ struct GroupNorm : Function<GroupNorm> {
     ctx->save_for_backward({x, weight, bias, stats});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["act"] = act;
-    return y.movedim(-1, 1);
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     only_once("group_norm_act");
@@ -83,7 +94,7 @@ struct GroupNorm : Function<GroupNorm> {
     const at::Tensor xl = x.detach().movedim(1, -1).contiguous(), dl = grads[0].movedim(1, -1).contiguous();
     const int64_t n = xl.size(0), c = xl.size(-1), s = xl.numel() / (n * c);
     const c10::DeviceGuard guard(x.device());
-    at::Tensor dx = at::empty_like(xl), dw, db;
+    at::Tensor dx = channels_last_like(x), dw, db;
     const auto fopt = x.options().dtype(at::kFloat);
     // (edges are counted over the tensors that are there)
     if (weight.defined() && ctx->needs_input_grad(1)) dw = at::empty({c}, fopt);
@@ -98,7 +109,7 @@ struct GroupNorm : Function<GroupNorm> {
        "group_norm_act backward");
     if (dw.defined()) dw = dw.to(weight.scalar_type());
     if (db.defined()) db = db.to(bias.scalar_type());
-    return {dx.movedim(-1, 1), dw, db, at::Tensor(), at::Tensor(), at::Tensor()};
+    return {dx, dw, db, at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 

@@ -28,6 +28,18 @@ def _channels_last(t: torch.Tensor) -> torch.Tensor:
     return t.movedim(1, -1).contiguous()
 
 
+def _channels_last_like(x: torch.Tensor) -> torch.Tensor:
+    """A new tensor of x's shape in channels-last memory. No view: autograd refuses to change a view that
+    a custom function returns in place, and what follows a normalisation often does (out += identity)."""
+    strides, step = [0] * x.dim(), x.shape[1]
+    strides[1] = 1
+    for d in range(x.dim() - 1, 1, -1):
+        strides[d] = step
+        step *= x.shape[d]
+    strides[0] = step
+    return torch.empty_strided(x.shape, strides, dtype=x.dtype, device=x.device)
+
+
 def _float_ptr(t: Optional[torch.Tensor]):
     """The parameter as contiguous fp32 and its address (the tensor has to outlive the launch)."""
     if t is None:
@@ -43,7 +55,7 @@ class _GroupNormAct(Function):
         n, c = xl.shape[0], xl.shape[-1]
         s = xl.numel() // (n * c)
         dev = x.device
-        y = torch.empty_like(xl)
+        y = _channels_last_like(x)
         stats = torch.empty(2, n, groups, dtype=torch.float32, device=dev)
         with N.on_device(dev):
             lib = N.lib()
@@ -60,7 +72,7 @@ class _GroupNormAct(Function):
                 N.stream_ptr(dev)), "group_norm_act")
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.args = (groups, activation)
-        return y.movedim(-1, 1)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -71,7 +83,7 @@ class _GroupNormAct(Function):
         n, c = xl.shape[0], xl.shape[-1]
         s = xl.numel() // (n * c)
         dev = x.device
-        dx = torch.empty_like(xl)
+        dx = _channels_last_like(x)
         need_w, need_b = ctx.needs_input_grad[1:3]
         dw = torch.empty(c, dtype=torch.float32, device=dev) if need_w else None
         db = torch.empty(c, dtype=torch.float32, device=dev) if need_b else None
@@ -89,7 +101,7 @@ class _GroupNormAct(Function):
                 activation, stats.data_ptr(), stats.data_ptr() + 4 * n * groups,
                 None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
                 ws.data_ptr(), need, N.stream_ptr(dev)), "group_norm_act backward")
-        return (dx.movedim(-1, 1) if ctx.needs_input_grad[0] else None,
+        return (dx if ctx.needs_input_grad[0] else None,
                 None if dw is None else dw.to(weight.dtype),
                 None if db is None else db.to(bias.dtype), None, None, None)
 

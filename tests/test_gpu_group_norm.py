@@ -273,3 +273,27 @@ def test_outlier_in_the_first_place(shape, value):
     y = group_norm_act(x, 2, w, b)
     want, bound, _ = reference(x, 2, w, b, 1e-5, "none")
     close(y, want, 3 * bound, torch.float32)
+
+
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("shape", [(6, 32), (2, 24, 10), (2, 32, 9, 7), (2, 16, 4, 6, 5), (2, 8, 1, 1)])
+def test_result_can_be_changed_in_place(shape, binding, monkeypatch):
+    """As a residual block does (out += identity, an in-place relu): same values and gradients as out of
+    place, and a result in channels-last memory that is no view."""
+    from smart_compress_amd import _native as N
+    if not binding:
+        monkeypatch.setattr(N, "train_fast", lambda: None)
+    x, dy, w, b = make(shape, torch.float32, seed=41)
+    got = []
+    for inplace in (True, False):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = group_norm_act(leaves[0], 4, leaves[1], leaves[2])
+        assert not y._is_view() and y.movedim(1, -1).is_contiguous()
+        if inplace:
+            y += x
+            y.mul_(2.0)
+            torch.nn.ReLU(inplace=True)(y)
+        else:
+            y = torch.relu((y + x) * 2.0)
+        got.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
+    assert all(torch.equal(a, c) for a, c in zip(*got))
