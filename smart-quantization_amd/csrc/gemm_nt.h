@@ -741,14 +741,20 @@ static inline void launch(int tile, const Operand& A, const Operand& B, int kt, 
   }
 }
 
-// Layout pass: src [rows, cols] of type T, row pitch ld, times 2^*exponent (NULL: 1) times *factor
-// (NULL: 1), to `d` row by row and / or to `dt` transposed (either may be absent), both zero padded.
+// Power-of-two exponents of a matrix' rows: e[r], or (each 0) *e for all of them; e NULL: 0.
+struct Exponents {
+  const int* e = nullptr;
+  int each = 0;
+  __device__ __forceinline__ int at(int r) const { return e ? e[each ? r : 0] : 0; }
+};
+// Layout pass: src [rows, cols] of type T, row pitch ld, times *factor (NULL: 1), to `d` row by row, times
+// 2^exponent of the row, and / or to `dt` transposed, times 2^turned (either may be absent), zero padded.
 // Rows whose keep[row] equals `skip` are written as zeros (keep NULL: none). With `map`, row r is src's row
 // map[r], and rows from *live on are zeros. 64 x 64 a workgroup; bound by its reads and writes of memory.
 template <typename T>
 static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_t ld,
                                                             int64_t batch_stride, int rows, int cols,
-                                                            const int* exponent,
+                                                            Exponents exponent, Exponents turned,
                                                             const float* factor,
                                                             const int64_t* keep, int64_t skip,
                                                             const int* map, const int* live, Mat d,
@@ -756,10 +762,17 @@ static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_
   __shared__ float tile[64][65];
   const int64_t batch = blockIdx.z;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  const int ex = exponent ? *exponent : 0;
   const float fa = factor ? factor[batch] : 1.0f;
   const T* p = src + batch * batch_stride;
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+  int er[4] = {}, et[4] = {};
+  if (exponent.e || turned.e) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int r = r0 + y + i * 16 < rows ? r0 + y + i * 16 : 0;
+      er[i] = exponent.at(r), et[i] = turned.at(r);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 64; i += 16) {
     const int r = r0 + y + i, c = c0 + x * 4;
@@ -777,12 +790,16 @@ static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_
           if (c + k < cols) w[k] = (float)q[c + k];
       }
 #pragma unroll
-      for (int k = 0; k < 4; k++) w[k] = ldexpf(w[k] * fa, ex);
+      for (int k = 0; k < 4; k++) w[k] *= fa;
     }
-    if (d.fmt != kNone && r < rows) store_n<4>(d, batch, r, c, cols, w);
     if (dt.fmt != kNone) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) tile[y + i][x * 4 + k] = w[k];
+      for (int k = 0; k < 4; k++) tile[y + i][x * 4 + k] = ldexpf(w[k], et[i / 16]);
+    }
+    if (d.fmt != kNone && r < rows) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) w[k] = ldexpf(w[k], er[i / 16]);
+      store_n<4>(d, batch, r, c, cols, w);
     }
   }
   if (dt.fmt == kNone) return;
@@ -802,11 +819,12 @@ static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_
 }
 template <typename T>
 static inline void launch_layout(const T* src, int64_t ld, int64_t batch_stride, int rows, int cols,
-                                 int batch, const int* exponent, const float* factor,
-                                 const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt,
+                                 int batch, const Exponents& exponent, const Exponents& turned,
+                                 const float* factor, const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt,
                                  hipStream_t st, const int* map = nullptr, const int* live = nullptr) {
   hipLaunchKernelGGL(layout_kernel<T>, dim3((cols + 63) / 64, (rows + 63) / 64, batch), dim3(256), 0,
-                     st, src, ld, batch_stride, rows, cols, exponent, factor, keep, skip, map, live, d, dt);
+                     st, src, ld, batch_stride, rows, cols, exponent, turned, factor, keep, skip, map, live, d,
+                     dt);
 }
 
 static inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }

@@ -19,8 +19,9 @@
 // second computation: 1050 TFLOP/s), 2048 x 768 x 30000 float32 1.29 ms, 777 x 1001 x 50001 fp16 with a third
 // of the rows ignored 0.63 ms. What bounds the large ones is the product itself, then dl's two copies.
 //
-// float32 inputs run as two fp16 planes (gemm_nt.h) scaled by a power of two per tensor; bf16 and fp16
-// inputs as they are. In the gradient products every 16-bit operand is fp16: dl rounded to 11 bits
+// float32 inputs run as two fp16 planes (gemm_nt.h), in the logits each row scaled by a power of two of its
+// own, taken off in the epilogue: every row is as exact as if it were alone, whatever the others' size. bf16 and
+// fp16 inputs run as they are. In the gradient products every 16-bit operand is fp16: dl rounded to 11 bits
 // (8 bits of bf16 were off by up to 2e-3 in the gradient of a target's row), and bf16 inputs, exact in
 // fp16 once scaled (what lies 2^-28 below the largest magnitude loses bits), in the transposed copies
 // that these products need anyway. dl is kept relative to the largest |g| and times 2^14, so that fp16
@@ -38,36 +39,43 @@ constexpr size_t kPieceBytes = size_t(1) << 30;  // default limit of a backward 
 
 // What a pass keeps on the device; the count is what the forward leaves for the backward.
 struct Head {
-  int exp_h, exp_w;  // power-of-two exponents of the fp16 operands made of the inputs
-  int exp_out;       // -(exp_h + exp_w)
-  int known;         // forward: whether it needed, and left, the exponents
+  int exp_h, exp_w;  // backward: exponents of the transposed fp16 operands
   int rows, pad;     // rows that take part, where they are gathered (Kept)
   double count;      // rows that take part
   float scale_dh, scale_dw, scale_db;  // backward: the factors of the gradients
 };
 
-// ---- largest magnitude of a tensor -> exponent ---------------------------------------------------
-// Workgroups below gh take h [tokens, dim], the others w [vocab, dim]. A weight without gaps is read as
-// one row, in whole vectors whatever the columns. What is not finite and rows that are ignored leave the
-// scale to the rest. Nothing where the exponents are known already.
+// ---- largest magnitudes -> exponents -------------------------------------------------------------
 __device__ __forceinline__ float finite_max(float top, float x) {
   const float a = fabsf(x);
   return a < __builtin_inff() ? fmaxf(top, a) : top;
 }
+// Exponent e with max * 2^e in [2^13, 2^14): room for the fp16 planes and for sums of their products.
+__device__ int plane_exponent(float top) {
+  if (!(top > 0.0f) || !(top < __builtin_inff())) return 0;
+  int e;
+  frexpf(top, &e);
+  const int k = 14 - e;
+  return k > 120 ? 120 : k;
+}
+// Workgroups below gh take h [tokens, dim], the others w [vocab, dim]: the largest magnitude of what each
+// reads, to part, and the exponents of the rows, to eh and ew (NULL: not wanted). 2^k lanes read a row, as many
+// as its vectors keep busy. A weight without gaps whose rows' exponents are not wanted is read as one row, in
+// whole vectors whatever the columns. What is not finite, and rows that are ignored, set no scale.
 template <typename T>
 __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, int64_t tokens, const T* w,
                                                      int64_t ldw, int64_t vocab, int cols,
                                                      const int64_t* target, int64_t ignore, int gh, float* part,
-                                                     const Head* known) {
-  if (known && known->known) return;
+                                                     int* eh, int* ew) {
   constexpr int V = 16 / sizeof(T);
   typedef typename Loose<T, V>::type vec;
   const bool first = (int)blockIdx.x < gh;
   const T* x = first ? h : w;
+  int* e = first ? eh : ew;
   const int64_t ld = first ? ldh : ldw, rows = first ? tokens : vocab;
   const int block = first ? blockIdx.x : blockIdx.x - gh, blocks = first ? gh : gridDim.x - gh;
   float top = 0.0f;
-  if (!first && ld == cols) {
+  if (!first && ld == cols && !e) {
     const int64_t total = rows * cols, vecs = total / V, step = (int64_t)blocks * 256;
     const vec* p = reinterpret_cast<const vec*>(x);
 #pragma unroll 4
@@ -80,16 +88,26 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, in
       top = finite_max(top, (float)x[vecs * V + threadIdx.x]);
   } else {
     const int whole = cols / V * V;
-    for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)blocks * 4) {
-      if (first && target[r] == ignore) continue;
-      const T* p = x + r * ld;
-#pragma unroll 2
-      for (int k = (threadIdx.x & 63) * V; k < whole; k += 64 * V) {
-        const vec v = *reinterpret_cast<const vec*>(p + k);
+    int shift = 6;
+    while (shift > 2 && V << (shift - 1) >= cols) shift--;
+    const int lanes = 1 << shift, at = threadIdx.x & (lanes - 1);
+    for (int64_t r = ((int64_t)block * 256 + threadIdx.x) >> shift; r < rows; r += ((int64_t)blocks * 256) >> shift) {
+      float m = 0.0f;
+      if (!(first && target[r] == ignore)) {
+        const T* p = x + r * ld;
+#pragma unroll 4
+        for (int k = at * V; k < whole; k += lanes * V) {
+          const vec v = *reinterpret_cast<const vec*>(p + k);
 #pragma unroll
-        for (int i = 0; i < V; i++) top = finite_max(top, (float)v[i]);
+          for (int i = 0; i < V; i++) m = finite_max(m, (float)v[i]);
+        }
+        for (int k = whole + at; k < cols; k += lanes) m = finite_max(m, (float)p[k]);
       }
-      for (int k = whole + (threadIdx.x & 63); k < cols; k += 64) top = finite_max(top, (float)p[k]);
+      if (e) {  // (a row's lanes are here together)
+        for (int o = lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if (at == 0) e[r] = plane_exponent(m);
+      }
+      top = fmaxf(top, m);
     }
   }
   top = wave_max_dpp(top);
@@ -99,14 +117,6 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, in
   if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// Exponent e with max * 2^e in [2^13, 2^14): room for the fp16 planes and for sums of their products.
-__device__ int plane_exponent(float top) {
-  if (!(top > 0.0f) || !(top < __builtin_inff())) return 0;
-  int e;
-  frexpf(top, &e);
-  const int k = 14 - e;
-  return k > 120 ? 120 : k;
-}
 // The exponents of both tensors from their partial maxima (gh, then gw of them), by one workgroup of up to
 // 16 waves.
 __device__ void exponents_of(const float* part, int gh, int gw, Head* head) {
@@ -120,7 +130,7 @@ __device__ void exponents_of(const float* part, int gh, int gw, Head* head) {
   if (threadIdx.x == 0) {
     for (int k = 1; k < (int)(blockDim.x >> 6); k++) a = fmaxf(a, mh[k]), b = fmaxf(b, mw[k]);
     const int eh = plane_exponent(a), ew = plane_exponent(b);
-    head->exp_h = eh, head->exp_w = ew, head->exp_out = -(eh + ew);
+    head->exp_h = eh, head->exp_w = ew;
   }
 }
 
@@ -131,6 +141,7 @@ __device__ void exponents_of(const float* part, int gh, int gw, Head* head) {
 struct Kept {
   int* map;
   int64_t* target;
+  int* exp;    // float32: the rows' exponents, else NULL
   float* lse;  // backward
 };
 // put(row, place, whether it takes part) for all rows, and their count; one workgroup of 16 waves.
@@ -164,16 +175,14 @@ __device__ __forceinline__ void partition_rows(const int64_t* target, int64_t ig
   }
   if (threadIdx.x == 0) *live = total;
 }
-// The exponents of the operands (part NULL: none are needed) and the gathered rows (map NULL: they are not).
-__global__ __launch_bounds__(1024) void prepare_kernel(const float* part, int gh, int gw, Head* head,
-                                                       const int64_t* target, int64_t ignore, int rows,
-                                                       Kept kept) {
-  if (part) exponents_of(part, gh, gw, head);
-  if (kept.map)
-    partition_rows(target, ignore, rows, &head->rows, [&](int m, int at, bool keep) {
-      kept.map[at] = m;
-      if (keep) kept.target[at] = target[m];
-    });
+// eh: the exponents of all rows (kept.exp NULL: none).
+__global__ __launch_bounds__(1024) void gather_kernel(const int64_t* target, int64_t ignore, int rows,
+                                                      const int* eh, Head* head, Kept kept) {
+  partition_rows(target, ignore, rows, &head->rows, [&](int m, int at, bool keep) {
+    kept.map[at] = m;
+    if (keep) kept.target[at] = target[m];
+    if (keep && kept.exp) kept.exp[at] = eh[m];
+  });
 }
 
 // exp(x) for x <= about 0, within 2 ulp: the product with log2(e) is carried in two parts (a single
@@ -189,8 +198,9 @@ __device__ __forceinline__ float exp_near(float x) {
 // ---- forward epilogue ---------------------------------------------------------------------------
 // Per row and per tile's columns: the maximum and the sum of exp(l - maximum), joined over the tile's
 // waves in LDS; the target's logit goes straight out (one lane of the grid owns it).
+template <bool PLANES>
 struct SoftmaxEpi {
-  const int* exponent;
+  const int *eh, *ew;  // PLANES: exponents that come off a row and a column
   const float* bias;
   const int64_t* target;
   float2* part;  // [tiles][rows]
@@ -199,7 +209,12 @@ struct SoftmaxEpi {
   __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float*, int m0, int n0, int M, int N,
                                          int im, int in, int wm, int wn, int lane, int64_t) const {
     __shared__ float2 joint[WN][BM];
-    const int ex = exponent ? *exponent : 0;
+    int em[TM];
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const int m = m0 + i * 32 + (lane & 31);
+      em[i] = PLANES && m < M ? eh[m] : 0;
+    }
     const float ninf = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < TN; j++)
@@ -207,9 +222,10 @@ struct SoftmaxEpi {
       for (int r = 0; r < 16; r++) {
         const int n = n0 + j * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
         const float b = bias && n < N ? bias[n] : 0.0f;
+        const int en = PLANES ? ew[n] : 0;  // (past N: its padding)
 #pragma unroll
         for (int i = 0; i < TM; i++) {
-          const float l = ex ? ldexpf(acc[i][j][r], ex) : acc[i][j][r];
+          const float l = PLANES ? ldexpf(acc[i][j][r], -(em[i] + en)) : acc[i][j][r];
           acc[i][j][r] = n < N ? l + b : ninf;
         }
       }
@@ -559,8 +575,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float2* part, int block
 
 // The loss over rows (fp64 sums in a fixed order) and the count of rows taking part, from each thread's
 // sums; one workgroup of 16 waves.
-__device__ __forceinline__ void finish_loss(double s, double c, int reduction, int known, float* loss,
-                                            Head* head) {
+__device__ __forceinline__ void finish_loss(double s, double c, int reduction, float* loss, Head* head) {
   s = wave_sum(s), c = wave_sum(c);
   __shared__ double a[16], b[16];
   if ((threadIdx.x & 63) == 0) a[threadIdx.x >> 6] = s, b[threadIdx.x >> 6] = c;
@@ -568,27 +583,27 @@ __device__ __forceinline__ void finish_loss(double s, double c, int reduction, i
   if (threadIdx.x == 0) {
     s = c = 0.0;
     for (int k = 0; k < 16; k++) s += a[k], c += b[k];
-    head->count = c, head->known = known;
+    head->count = c;
     if (reduction == SMQ_REDUCE_MEAN) *loss = (float)(s / c);
     if (reduction == SMQ_REDUCE_SUM) *loss = (float)s;
   }
 }
 __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const int64_t* target,
-                                                    int64_t ignore, int rows, int reduction, int known,
-                                                    float* loss, Head* head) {
+                                                    int64_t ignore, int rows, int reduction, float* loss,
+                                                    Head* head) {
   double s = 0.0, c = 0.0;
   for (int m = threadIdx.x; m < rows; m += 1024) {
     s += (double)row_loss[m];
     c += target[m] != ignore ? 1.0 : 0.0;
     if (reduction == SMQ_REDUCE_NONE) loss[m] = row_loss[m];
   }
-  finish_loss(s, c, reduction, known, loss, head);
+  finish_loss(s, c, reduction, loss, head);
 }
 // Both in one workgroup, where the partial statistics are few.
 __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int blocks, int rows, int R,
                                                          const int64_t* target, int64_t ignore,
                                                          int64_t vocab, const float* picked, float* lse,
-                                                         int reduction, int known, float* loss, Head* head) {
+                                                         int reduction, float* loss, Head* head) {
   __shared__ float2 sh[1024];
   const int m = threadIdx.x & (R - 1);
   float l, value;
@@ -600,24 +615,21 @@ __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int
     s = (double)value;
     c = target[m] != ignore ? 1.0 : 0.0;
   }
-  finish_loss(s, c, reduction, known, loss, head);
+  finish_loss(s, c, reduction, loss, head);
 }
 
 // ---- backward -----------------------------------------------------------------------------------
-// One workgroup: the exponents of the operands (part: their maxima, NULL: none; `planes`: the forward may
-// have left them), the rows' factors relative to their largest magnitude, and what comes off again in the
-// epilogues. Ignored rows get 0 or are left out (Kept), rows whose gradient is not finite that gradient
-// itself.
+// One workgroup: the exponents of the transposed operands (part: the inputs' maxima, NULL: none), the rows'
+// factors relative to their largest magnitude, and what comes off again in the epilogues. Ignored rows get
+// 0 or are left out (Kept), rows whose gradient is not finite that gradient itself. eh: as gather_kernel's.
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
                                                       int64_t ignore, int rows, int reduction,
                                                       float* g, const Head* head, const float* part,
-                                                      int gh, int gw, int planes, const float* lse, Kept kept,
+                                                      int gh, int gw, const float* lse, const int* eh, Kept kept,
                                                       Head* out) {
   __shared__ float w[16];
   __shared__ float all;
   if (part) exponents_of(part, gh, gw, out);
-  if (part && planes && head->known && threadIdx.x == 0)
-    out->exp_h = head->exp_h, out->exp_w = head->exp_w, out->exp_out = head->exp_out;
   const float inf = __builtin_inff();
   float top = 0.0f, one = 0.0f;
   if (reduction == SMQ_REDUCE_NONE) {
@@ -649,6 +661,7 @@ __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const i
     partition_rows(target, ignore, rows, &out->rows, [&](int m, int at, bool keep) {
       kept.map[at] = m;
       if (keep) kept.target[at] = target[m], kept.lse[at] = lse[m], g[at] = factor(m);
+      if (keep && kept.exp) kept.exp[at] = eh[m];
     });
     return;
   }
@@ -657,8 +670,9 @@ __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const i
 
 // dl of a piece from its logits, to `o` [rows, piece] and transposed to `ot` [piece, rows]; column
 // sums (the bias' gradient) per block of rows.
+template <bool PLANES>
 struct DlEpi {
-  const int* exponent;
+  const int *eh, *ew;  // as SoftmaxEpi's
   const float* bias;
   const int64_t* target;
   const float* lse;
@@ -670,17 +684,23 @@ struct DlEpi {
   __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float* stage, int m0, int n0, int M,
                                          int N, int im, int, int wm, int, int lane,
                                          int64_t batch) const {
-    const int ex = exponent ? *exponent : 0;
+    // a lane's four columns are the same in all of stage_out's rows
+    int en[4] = {};
+    if (PLANES) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) en[k] = ew[n0 + lane % (TN * 8) * 4 + k];  // (past N: its padding)
+    }
     Mat ot = this->ot;  // padded to whole k tiles of the rows there are
     const int tile = ot.fmt == kSplit ? 32 : 64;
     ot.pad = (M + tile - 1) / tile * tile;
     float* sum = sums ? sums + (int64_t)(im * WM + wm) * N : nullptr;
     stage_out<TM, TN, true>(
         acc, stage, m0, n0, M, N, lane, batch, o, ot, true, sum != nullptr,
-        [&](int m) {  // g, lse, the target's place in the piece (-1: elsewhere, -2: nowhere)
+        [&](int m) {  // g, lse, the target's place in the piece (-1: elsewhere, -2: nowhere), the exponent
           const int64_t t = target[m], at = t - first;
           const int k = t < 0 || t >= vocab ? -2 : at >= 0 && at < N ? (int)at : -1;
-          return make_float4(g[m], lse[m], __builtin_bit_cast(float, k), 0.0f);
+          return make_float4(g[m], lse[m], __builtin_bit_cast(float, k),
+                             __builtin_bit_cast(float, PLANES ? eh[m] : 0));
         },
         [&](int, int n, float4 v, float4 row) {
           const int at = __builtin_bit_cast(int, row.z) - n;
@@ -688,7 +708,7 @@ struct DlEpi {
           float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            float l = ex ? ldexpf(w[k], ex) : w[k];
+            float l = PLANES ? ldexpf(w[k], -(__builtin_bit_cast(int, row.w) + en[k])) : w[k];
             if (bias && n + k < N) l += bias[first + n + k];
             const float p = exp_near(l - row.y) - (at == k ? 1.0f : 0.0f);
             w[k] = row.x == 0.0f ? 0.0f : known ? p * row.x : __builtin_nanf("");
@@ -731,8 +751,10 @@ struct Shape {
   size_t size() const { return dtype == SMQ_DTYPE_F32 ? 4 : 2; }
 };
 
-constexpr int kMaxParts = 512;
+constexpr int kMaxParts = 1024;
 inline int absmax_grid(int64_t rows) { return (int)(rows < 4 * kMaxParts ? (rows + 3) / 4 : kMaxParts); }
+// Entries of the array of a weight's exponents: the epilogues read whole tiles of columns.
+inline size_t exponent_room(int64_t vocab) { return (size_t)vocab + 256; }
 
 // A 16-bit tensor is an operand as it is when its rows are whole k tiles on 16-byte boundaries.
 inline bool direct(const void* p, int64_t ld, int64_t cols, int dtype) {
@@ -747,32 +769,34 @@ inline int out_fmt(int dtype) {
 }
 const Mat kNoMat = {nullptr, 0, 0, kNone, 0};
 
-void layout(const void* src, int dtype, int64_t ld, int64_t rows, int64_t cols, const int* exponent,
-            const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt, hipStream_t st,
+void layout(const void* src, int dtype, int64_t ld, int64_t rows, int64_t cols, const Exponents& exponent,
+            const Exponents& turned, const int64_t* keep, int64_t skip, const Mat& d, const Mat& dt, hipStream_t st,
             const int* map = nullptr, const int* live = nullptr) {
   if (dtype == SMQ_DTYPE_F32)
-    launch_layout((const float*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st, map, live);
+    launch_layout((const float*)src, ld, 0, (int)rows, (int)cols, 1, exponent, turned, nullptr, keep, skip, d, dt,
+                  st, map, live);
   else if (dtype == SMQ_DTYPE_F16)
-    launch_layout((const _Float16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st, map, live);
+    launch_layout((const _Float16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, turned, nullptr, keep, skip, d, dt,
+                  st, map, live);
   else
-    launch_layout((const __bf16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, nullptr, keep, skip, d, dt, st, map, live);
+    launch_layout((const __bf16*)src, ld, 0, (int)rows, (int)cols, 1, exponent, turned, nullptr, keep, skip, d, dt,
+                  st, map, live);
 }
 
-// The partial maxima of both inputs, absmax_grid of the tokens and of the vocabulary.
+// The partial maxima of both inputs, absmax_grid of the tokens and of the vocabulary, and their rows' exponents.
 template <typename T>
 void maxima(const T* h, int64_t ldh, const T* w, int64_t ldw, const Shape& s, const int64_t* target,
-            int64_t ignore, float* part, const Head* known, hipStream_t st) {
+            int64_t ignore, float* part, int* eh, int* ew, hipStream_t st) {
   const int gh = absmax_grid(s.tokens), gw = absmax_grid(s.vocab);
   hipLaunchKernelGGL(absmax_kernel<T>, dim3(gh + gw), dim3(256), 0, st, h, ldh, s.tokens, w, ldw, s.vocab,
-                     (int)s.dim, target, ignore, gh, part, known);
+                     (int)s.dim, target, ignore, gh, part, eh, ew);
 }
 
-template <typename Epi>
-void product(int dtype, int tile, const Operand& A, const Operand& B, int kt, int shares, const Epi& e,
+// A gradient's product, of two planes or one of fp16.
+void product(bool split, int tile, const Operand& A, const Operand& B, int kt, int shares, const StoreEpi& e,
              hipStream_t st) {
-  if (dtype == SMQ_DTYPE_BF16) launch<__bf16, false>(tile, A, B, kt, 1, 0, shares, e, st);
-  else if (dtype == SMQ_DTYPE_F16) launch<_Float16, false>(tile, A, B, kt, 1, 0, shares, e, st);
-  else launch<_Float16, true>(tile, A, B, kt, 1, 0, shares, e, st);
+  if (split) launch<_Float16, true>(tile, A, B, kt, 1, 0, shares, e, st);
+  else launch<_Float16, false>(tile, A, B, kt, 1, 0, shares, e, st);
 }
 
 // Which rows of h an operand is made of: those with keep[row] != skip (the others zeros; keep NULL: all), or
@@ -784,23 +808,20 @@ struct Pick {
   const int* live = nullptr;
 };
 // [rows, cols] in operand form: in place where it can be, else laid out in the workspace. `turned` (absent:
-// fmt kNone) is written transposed along the way, in one pass over p where both go by the same exponent
-// (float32) or none.
+// fmt kNone) is written transposed along the way.
 Operand operand(Arena& ws, const void* p, int64_t ld, int64_t rows, int64_t cols, const Shape& s,
-                const int* exponent, const int* turned_exponent, const Pick& pick, const Mat& turned, bool run,
-                hipStream_t st) {
-  const bool in_place = direct(p, ld, cols, s.dtype) && !pick.map;
-  const bool once = !in_place && exponent == turned_exponent;
-  if (run && turned.fmt != kNone && !once)
-    layout(p, s.dtype, ld, rows, cols, turned_exponent, pick.keep, pick.skip, kNoMat, turned, st, pick.map,
-           pick.live);
-  if (in_place) return {p, ld, 0, (int)rows};
+                const Exponents& exponent, const Exponents& turned_exponent, const Pick& pick, const Mat& turned,
+                bool run, hipStream_t st) {
+  if (direct(p, ld, cols, s.dtype) && !pick.map) {
+    if (run && turned.fmt != kNone)
+      layout(p, s.dtype, ld, rows, cols, {}, turned_exponent, pick.keep, pick.skip, kNoMat, turned, st);
+    return {p, ld, 0, (int)rows};
+  }
   const int64_t to = operand_ld(cols, s.split());
   _Float16* q = ws.take<_Float16>((size_t)(rows * to));
   if (run)
-    layout(p, s.dtype, ld, rows, cols, exponent, pick.keep, pick.skip,
-           {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, once ? turned : kNoMat, st, pick.map,
-           pick.live);
+    layout(p, s.dtype, ld, rows, cols, exponent, turned_exponent, pick.keep, pick.skip,
+           {q, to, 0, plane_fmt(s.dtype), operand_pad(cols, s.split())}, turned, st, pick.map, pick.live);
   return {q, to, 0, (int)rows, pick.live};
 }
 
@@ -849,12 +870,15 @@ bool raw32(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& 
 bool gathered(const Shape& s) {
   return s.tokens > 128 && s.tokens * s.vocab >= ((int64_t)1 << (s.split() ? 33 : 35)) / s.dim;
 }
-// The logits' product: by planes, one plane or raw float32.
-template <typename Epi>
-void logits(const Shape& s, bool raw, int tile, const Operand& A, const Operand& B, const Epi& e,
-            hipStream_t st) {
-  if (raw) launch<Raw32, false>(tile, A, B, (int)(round_up(s.dim, 32) / 32), 1, 0, 1, e, st);
-  else product(s.dtype, tile, A, B, operand_kt(s.dim, s.split()), 1, e, st);
+// The logits' product: by planes, one plane or raw float32, with the epilogue make(planes).
+template <typename F>
+void logits(const Shape& s, bool raw, int tile, const Operand& A, const Operand& B, F make, hipStream_t st) {
+  const int kt = operand_kt(s.dim, s.split());
+  const auto one = make(std::false_type());
+  if (raw) launch<Raw32, false>(tile, A, B, (int)(round_up(s.dim, 32) / 32), 1, 0, 1, one, st);
+  else if (s.dtype == SMQ_DTYPE_BF16) launch<__bf16, false>(tile, A, B, kt, 1, 0, 1, one, st);
+  else if (s.dtype == SMQ_DTYPE_F16) launch<_Float16, false>(tile, A, B, kt, 1, 0, 1, one, st);
+  else launch<_Float16, true>(tile, A, B, kt, 1, 0, 1, make(std::true_type()), st);
 }
 
 // Few tokens: up to 16, hidden within 148 KiB of LDS; 0: not few.
@@ -954,25 +978,23 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
   float2* part = a.take<float2>((size_t)blocks * s.tokens);
   float* picked = a.take<float>(s.tokens);
   float* rows = a.take<float>(s.tokens);
-  const int* exponent = nullptr;
-  const int *eh = nullptr, *ew = nullptr;
+  int *eh = nullptr, *ew = nullptr;
   const bool raw = raw32(h, ldh, w, ldw, s), gather = !few.nt && gathered(s);
-  float* top = nullptr;
   if (s.split() && !few.nt && !raw) {
-    top = a.take<float>(2 * kMaxParts);
-    exponent = &head->exp_out, eh = &head->exp_h, ew = &head->exp_w;
-    if (run) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, nullptr, st);
+    float* top = a.take<float>(2 * kMaxParts);
+    eh = a.take<int>(s.tokens), ew = a.take<int>(exponent_room(s.vocab));
+    if (run) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, eh, ew, st);
   }
   Kept kept = {};
   Pick pick;
   if (gather) {
-    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), nullptr};
+    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), eh ? a.take<int>(s.tokens) : nullptr, nullptr};
     pick.map = kept.map, pick.live = &head->rows;
+    if (run)
+      hipLaunchKernelGGL(gather_kernel, dim3(1), dim3(1024), 0, st, target, ignore, (int)s.tokens, eh, head, kept);
+    eh = kept.exp;
   }
   const int64_t* at = gather ? kept.target : target;
-  if (run && (top || gather))
-    hipLaunchKernelGGL(prepare_kernel, dim3(1), dim3(1024), 0, st, top, absmax_grid(s.tokens),
-                       absmax_grid(s.vocab), head, target, ignore, (int)s.tokens, kept);
   if (few.nt) {
     if (run) {
       if (s.dtype == SMQ_DTYPE_F32) launch_few<float>(few, h, ldh, w, ldw, s, bias, target, ignore, part, picked, st);
@@ -981,24 +1003,25 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
     }
   } else {
     const Operand A = raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
-                          : operand(a, h, ldh, s.tokens, s.dim, s, eh, nullptr, pick, kNoMat, run, st);
+                          : operand(a, h, ldh, s.tokens, s.dim, s, {eh, 1}, {}, pick, kNoMat, run, st);
     const Operand B = raw ? Operand{w, 2 * ldw, 0, (int)s.vocab}
-                          : operand(a, w, ldw, s.vocab, s.dim, s, ew, nullptr, {}, kNoMat, run, st);
-    const SoftmaxEpi e = {exponent, bias, at, part, picked};
-    if (run) logits(s, raw, tile, A, B, e, st);
+                          : operand(a, w, ldw, s.vocab, s.dim, s, {ew, 1}, {}, {}, kNoMat, run, st);
+    if (run)
+      logits(s, raw, tile, A, B,
+             [&](auto planes) { return SoftmaxEpi<planes.value>{eh, ew, bias, at, part, picked}; }, st);
   }
   if (run) {
     int per = 1;
     if (!gather && s.tokens <= 1024 && s.tokens * blocks <= 16384) {
       while (per < s.tokens) per *= 2;
       hipLaunchKernelGGL(join_loss_kernel, dim3(1), dim3(1024), 0, st, part, blocks, (int)s.tokens, per,
-                         target, ignore, s.vocab, picked, lse, reduction, exponent ? 1 : 0, loss, head);
+                         target, ignore, s.vocab, picked, lse, reduction, loss, head);
     } else {
       per = s.tokens >= 2048 ? 16 : s.tokens >= 256 ? 4 : 1;
       hipLaunchKernelGGL(join_kernel, dim3((unsigned)((s.tokens + per - 1) / per)), dim3(256), 0, st, part,
                          blocks, (int)s.tokens, per, at, ignore, s.vocab, picked, pick.map, pick.live, lse, rows);
       hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, rows, target, ignore, (int)s.tokens,
-                         reduction, exponent ? 1 : 0, loss, head);
+                         reduction, loss, head);
     }
   }
   return a.used;
@@ -1034,7 +1057,6 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   }
   const bool sp = s.split();
   const int fmt = sp ? kSplit : kF16;  // the gradient products' operands
-  const int grad_dtype = sp ? SMQ_DTYPE_F32 : SMQ_DTYPE_F16;
   if (s.piece <= 0) s.piece = default_piece(s);
   if (s.piece > s.vocab) s.piece = s.vocab;
   const int64_t pieces = (s.vocab + s.piece - 1) / s.piece;
@@ -1045,35 +1067,37 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   Pick pick;
   pick.keep = target, pick.skip = ignore;
   if (gather) {
-    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), a.take<float>(s.tokens)};
+    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), sp ? a.take<int>(s.tokens) : nullptr,
+            a.take<float>(s.tokens)};
     pick = Pick();
     pick.map = kept.map, pick.live = &fac->rows;
   }
-  const Head* planes = s.dtype == SMQ_DTYPE_F16 ? nullptr : fac;
+  const bool raw = raw32(h, ldh, w, ldw, s), scaled = s.dtype != SMQ_DTYPE_F16;
+  // rows' exponents of the logits' operands, and one each for the transposed ones
+  int* eh = sp && !raw ? a.take<int>(s.tokens) : nullptr;
+  int* ew = sp && !raw ? a.take<int>(exponent_room(s.vocab)) : nullptr;
   float* top = nullptr;
-  if (planes) {
+  if (scaled) {
     top = a.take<float>(2 * kMaxParts);
-    if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, head, st);
-    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, nullptr, st);
+    if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, eh, ew, st);
+    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, nullptr, nullptr, st);
   }
-  const bool raw = raw32(h, ldh, w, ldw, s);
-  const int* exponent = sp && !raw ? &fac->exp_out : nullptr;
-  const int* eh = planes ? &planes->exp_h : nullptr;
-  const int* ew = planes ? &planes->exp_w : nullptr;
+  const Exponents turned_eh = {scaled ? &fac->exp_h : nullptr, 0}, turned_ew = {scaled ? &fac->exp_w : nullptr, 0};
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
                        (int)s.tokens, reduction, g, head, top, absmax_grid(s.tokens),
-                       absmax_grid(s.vocab), sp ? 1 : 0, lse, kept, fac);
+                       absmax_grid(s.vocab), lse, eh, kept, fac);
+  if (gather) eh = kept.exp;
   // h, and transposed the operand of dw. Ignored rows are left out or zeros, whatever they hold (where h is
   // read in place its ignored rows' logits are not used).
   const int64_t ldt = operand_ld(s.tokens, sp);
   const int padt = operand_pad(s.tokens, sp);
   _Float16* ht = dw ? a.take<_Float16>((size_t)(s.dim * ldt)) : nullptr;
   const Mat turned_h = dw ? Mat{ht, ldt, 0, fmt, padt} : kNoMat;
-  if (run && raw && dw) layout(h, s.dtype, ldh, s.tokens, s.dim, eh, target, ignore, kNoMat, turned_h, st);  // (not gathered)
+  if (run && raw && dw) layout(h, s.dtype, ldh, s.tokens, s.dim, {}, turned_eh, target, ignore, kNoMat, turned_h, st);  // (not gathered)
   const Operand A =
       raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
-          : operand(a, h, ldh, s.tokens, s.dim, s, sp ? eh : nullptr, eh, pick, turned_h, run, st);
+          : operand(a, h, ldh, s.tokens, s.dim, s, {eh, 1}, turned_eh, pick, turned_h, run, st);
   const int64_t ldp = operand_ld(s.piece, sp);
   _Float16* dl = a.take<_Float16>((size_t)(s.tokens * ldp));
   _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
@@ -1095,14 +1119,16 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     const char* wp = reinterpret_cast<const char*>(w) + (size_t)(v0 * ldw) * wsize;
     const int padn = operand_pad(n, sp);
     const Mat turned_w = dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat;
-    if (run && raw && dh) layout(wp, s.dtype, ldw, n, s.dim, ew, nullptr, 0, kNoMat, turned_w, st);
+    if (run && raw && dh) layout(wp, s.dtype, ldw, n, s.dim, {}, turned_ew, nullptr, 0, kNoMat, turned_w, st);
     const Operand B = raw ? Operand{wp, 2 * ldw, 0, (int)n}
-                          : operand(a, wp, ldw, n, s.dim, s, sp ? ew : nullptr, ew, {}, turned_w, run, st);
+                          : operand(a, wp, ldw, n, s.dim, s, {ew ? ew + v0 : nullptr, 1}, turned_ew, {}, turned_w, run, st);
     if (a.used > most) most = a.used;
     if (!run) continue;
-    const DlEpi e = {exponent, bias, gather ? kept.target : target, gather ? kept.lse : lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
-                     {dlt, ldt, 0, fmt, padt}, sums};
-    logits(s, raw, tile_l, A, B, e, st);
+    logits(s, raw, tile_l, A, B, [&](auto planes) {
+      return DlEpi<planes.value>{eh, ew ? ew + v0 : nullptr, bias, gather ? kept.target : target,
+                                 gather ? kept.lse : lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
+                                 {dlt, ldt, 0, fmt, padt}, sums};
+    }, st);
     if (db)
       hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, sums,
                          row_blocks, (int)n, pick.live, shape_of(tile_l).bm, shape_of(tile_l).wm, fac, db + v0);
@@ -1111,13 +1137,14 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
       StoreEpi se = {1.0f, 1.0f, whole ? &fac->scale_dh : nullptr, kNoMat, kNoMat, kNoMat, 0, s.tokens * ldacc, 0.0f};
       se.o = whole ? Mat{dh, s.dim, 0, out_fmt(s.dtype), 0} : Mat{accum, ldacc, 0, kF32, 0};
       if (i > 0) se.src = se.o;
-      product(grad_dtype, tile_dh, L, W, operand_kt(n, sp), shares, se, st);
+      product(sp, tile_dh, L, W, operand_kt(n, sp), shares, se, st);
     }
     if (dw) {
       const Operand L = {dlt, ldt, 0, (int)n, nullptr, pick.live}, H = {ht, ldt, 0, (int)s.dim};
       StoreEpi se = {1.0f, 0.0f, &fac->scale_dw, kNoMat, kNoMat, kNoMat, 0, 0, 0.0f};
       se.o = {reinterpret_cast<char*>(dw) + (size_t)(v0 * s.dim) * wsize, s.dim, 0, out_fmt(s.dtype), 0};
-      product(grad_dtype, plan_product(n, s.dim, operand_kt(s.tokens, sp), 1, 0, false).tile, L, H, operand_kt(s.tokens, sp), 1, se, st);
+      const int kt = operand_kt(s.tokens, sp);
+      product(sp, plan_product(n, s.dim, kt, 1, 0, false).tile, L, H, kt, 1, se, st);
     }
   }
   if (run && dh && !whole) {

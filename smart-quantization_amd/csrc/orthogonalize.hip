@@ -497,7 +497,7 @@ void first_layout(const Plan& p, const T* g, int64_t ld, int64_t stride, double 
                      rows, cols, part);
   hipLaunchKernelGGL(norm_kernel, dim3((unsigned)p.batch), dim3(64), 0, st, part, grid, eps, pow2, rest,
                      rest2);
-  launch_layout(g, ld, stride, rows, cols, (int)p.batch, nullptr, pow2, nullptr, 0, p.turned ? xt : x,
+  launch_layout(g, ld, stride, rows, cols, (int)p.batch, {}, {}, pow2, nullptr, 0, p.turned ? xt : x,
                 p.turned ? x : xt, st);
 }
 

@@ -533,3 +533,22 @@ def test_graph_replays_with_other_ignored_rows(dtype):
 def test_few_tokens_to_the_last_of_the_lds(tokens, dim, dtype):
     # (a single row takes part: the mean over none is NaN)
     check(*make(tokens, dim, 77, dtype, True, 0.2 if tokens > 1 else 0, seed=tokens), "mean")
+
+
+@pytest.mark.parametrize("power", [16, 24, 40])
+@pytest.mark.parametrize("tokens,dim,vocab,ignored", [(9, 64, 500, 0), (60, 36, 500, 0.2), (100, 64, 500, 0),
+                                                      (200, 100, 900, 0), (*GATHERED, 0.5)])
+def test_a_large_row_leaves_the_others_losses(tokens, dim, vocab, ignored, power):
+    """One finite row of hidden, or of the weight (masked by its bias), far above the rest: float32 losses of
+    the other rows keep every bit, at every number of tokens."""
+    h, w, b, t = make(tokens, dim, vocab, torch.float32, True, ignored, seed=31)
+    b[7], t[t == 7], t[3] = float("-inf"), 8, 5
+    rest = torch.arange(tokens, device="cuda") != 3
+    base = linear_cross_entropy(h, w, t, b, reduction="none")
+    want, bl, _, _ = reference(h, w, b.clamp(min=-1e30), t, "none", torch.ones(tokens, device="cuda"))
+    large_h, large_w = h.clone(), w.clone()
+    large_h[3] *= 2.0 ** power
+    large_w[7] *= 2.0 ** power
+    assert torch.equal(linear_cross_entropy(large_h, w, t, b, reduction="none")[rest], base[rest])
+    assert torch.equal(linear_cross_entropy(h, large_w, t, b, reduction="none"), base)
+    assert torch.isfinite(base).all()
