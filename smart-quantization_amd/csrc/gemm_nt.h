@@ -493,12 +493,13 @@ __device__ __forceinline__ void wave_sync() {
 // Walks a wave's part of C through its LDS stage, 32 rows at a time: `f(m, n, v)` turns four
 // consecutive accumulators of row m into the values to be written, which go to `o` row by row and,
 // where `ot` is set, to `ot` transposed. `colsum(n, v)`, where given, gets the sum over the part's
-// rows of column n. Lanes past the edges call neither. `prep(m)`: what f needs of a row, four words, read
-// once per row into the stage's spare columns (f's fourth argument).
-template <int TM, int TN, bool ROWS, typename P, typename F, typename S>
+// rows of column n. Lanes past the edges call neither. `prep(m)` (ROWS): what f needs of a row, four words, read
+// once per row into the stage's spare columns (f's fourth argument): the first is a factor of the row in the
+// transposed copy, `weigh(v, last)` makes the term of a column's sum of the copy's value and the row's last word.
+template <int TM, int TN, bool ROWS, typename P, typename F, typename W, typename S>
 __device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* stage, int m0, int n0,
                                           int M, int N, int lane, int64_t batch, const Mat& o,
-                                          const Mat& ot, bool mirror, bool sums, P prep, F f, S colsum) {
+                                          const Mat& ot, bool mirror, bool sums, P prep, F f, W weigh, S colsum) {
   constexpr int kCols = TN * 32, kPitch = kCols + 4;
   constexpr int kPer = kCols / 4, kRows = 64 / kPer;  // row phase: lanes a row, rows a pass
   float total = 0.0f;
@@ -523,14 +524,21 @@ __device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* st
         float* at = stage + r * kPitch + c;
         float4 v = *reinterpret_cast<const float4*>(at);
         if (mb + r < M) {
+          float factor = 1.0f;
           if (n0 + c < N) {
-            if constexpr (ROWS) v = f(mb + r, n0 + c, v, *reinterpret_cast<const float4*>(stage + r * kPitch + kCols));
-            else v = f(mb + r, n0 + c, v);
+            if constexpr (ROWS) {
+              const float4 row = *reinterpret_cast<const float4*>(stage + r * kPitch + kCols);
+              v = f(mb + r, n0 + c, v, row);
+              factor = row.x;
+            } else {
+              v = f(mb + r, n0 + c, v);
+            }
           }
           if (o.fmt != kNone) {
             const float w[4] = {v.x, v.y, v.z, v.w};
             store_n<4>(o, batch, mb + r, n0 + c, N, w);
           }
+          if constexpr (ROWS) v.x *= factor, v.y *= factor, v.z *= factor, v.w *= factor;
           if (mirror || sums) *reinterpret_cast<float4*>(at) = v;
         }
       }
@@ -543,9 +551,13 @@ __device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* st
             for (int r = 0; r < 32; r += 8) {
               float w[8];
 #pragma unroll
-              for (int k = 0; k < 8; k++) {
-                w[k] = mb + r + k < M ? stage[(r + k) * kPitch + lane % kCols] : 0.0f;
-                total += w[k];
+              for (int k = 0; k < 8; k++) w[k] = mb + r + k < M ? stage[(r + k) * kPitch + lane % kCols] : 0.0f;
+              if constexpr (ROWS) {
+                if (sums) {
+#pragma unroll
+                  for (int k = 0; k < 8; k++)
+                    if (mb + r + k < M) total += weigh(w[k], stage[(r + k) * kPitch + kCols + 3]);
+                }
               }
               if (mirror) store_n<8>(ot, batch, n, mb + r, M, w);
             }
@@ -563,7 +575,7 @@ __device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* st
   if (sums && (lane < kCols) && n0 + lane < N) colsum(n0 + lane, total);
 }
 
-// C = alpha * acc + beta * src + diag * I, to `o` and / or transposed to `ot` (a symmetric product
+// C = (alpha * acc + beta * src + diag * I) * rows[m], to `o` and / or transposed to `ot` (a symmetric product
 // writes the same matrix twice; its diagonal tiles once). `scale`: a factor of alpha in device memory,
 // one per matrix of the batch, or NULL.
 // A launch split over k (gridDim.y shares) writes share y to o + y * share.
@@ -581,6 +593,8 @@ struct StoreEpi {
   // split_sum_kernel only: row m goes to row map[m] of `o`, those from *live on as zeros (NULL: as they are)
   const int* map = nullptr;
   const int* live = nullptr;
+  const float* rows = nullptr;  // a factor per row, `row_step` apart (NULL: none)
+  int row_step = 1;
   template <int BM, int BN, int WM, int WN, int TM, int TN>
   __device__ __forceinline__ void finish(f32x16 (&acc)[TM][TN], float* stage, int m0, int n0, int M,
                                          int N, int im, int in, int, int, int lane,
@@ -601,13 +615,17 @@ struct StoreEpi {
             v.x += be * c.x, v.y += be * c.y, v.z += be * c.z, v.w += be * c.w;
           }
           add_diag(v, m, n, dg);
+          if (rows) {
+            const float f = rows[(int64_t)m * row_step];
+            v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+          }
           return v;
         },
-        [](int, float) {});
+        0, [](int, float) {});
   }
 };
 
-// The second half of a product split over k: C = alpha * sum over the shares + beta * src + diag * I,
+// The second half of a product split over k: C = (alpha * sum over the shares + beta * src + diag * I) * rows[m],
 // 32 x 32 a workgroup (the same walk as the product's own epilogue, with the tile in LDS).
 static __global__ __launch_bounds__(256) void split_sum_kernel(const float* part, int64_t ld,
                                                                int64_t share, int shares,
@@ -636,6 +654,10 @@ static __global__ __launch_bounds__(256) void split_sum_kernel(const float* part
         v.x += e.beta * s.x, v.y += e.beta * s.y, v.z += e.beta * s.z, v.w += e.beta * s.w;
       }
       add_diag(v, m, n, e.diag);
+      if (e.rows) {
+        const float f = e.rows[(int64_t)m * e.row_step];
+        v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+      }
     }
     const float w[4] = {v.x, v.y, v.z, v.w};
     if (e.o.fmt != kNone) store_n<4>(e.o, batch, e.map ? e.map[m] : m, n, N, w);
@@ -741,11 +763,12 @@ static inline void launch(int tile, const Operand& A, const Operand& B, int kt, 
   }
 }
 
-// Power-of-two exponents of a matrix' rows: e[r], or (each 0) *e for all of them; e NULL: 0.
+// Power-of-two exponents of a matrix' rows: e[step * r] (step 0: *e for all of them); e NULL: 0.
 struct Exponents {
   const int* e = nullptr;
-  int each = 0;
-  __device__ __forceinline__ int at(int r) const { return e ? e[each ? r : 0] : 0; }
+  int step = 0;
+  __device__ __forceinline__ int all() const { return e && step == 0 ? *e : 0; }
+  __device__ __forceinline__ int at(int r) const { return step ? e[step * r] : all(); }
 };
 // Layout pass: src [rows, cols] of type T, row pitch ld, times *factor (NULL: 1), to `d` row by row, times
 // 2^exponent of the row, and / or to `dt` transposed, times 2^turned (either may be absent), zero padded.
@@ -765,8 +788,10 @@ static __global__ __launch_bounds__(256) void layout_kernel(const T* src, int64_
   const float fa = factor ? factor[batch] : 1.0f;
   const T* p = src + batch * batch_stride;
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-  int er[4] = {}, et[4] = {};
-  if (exponent.e || turned.e) {
+  int er[4], et[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) er[i] = exponent.all(), et[i] = turned.all();
+  if (exponent.step | turned.step) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int r = r0 + y + i * 16 < rows ? r0 + y + i * 16 : 0;

@@ -23,9 +23,14 @@
 // own, taken off in the epilogue: every row is as exact as if it were alone, whatever the others' size. bf16 and
 // fp16 inputs run as they are. In the gradient products every 16-bit operand is fp16: dl rounded to 11 bits
 // (8 bits of bf16 were off by up to 2e-3 in the gradient of a target's row), and bf16 inputs, exact in
-// fp16 once scaled (what lies 2^-28 below the largest magnitude loses bits), in the transposed copies
-// that these products need anyway. dl is kept relative to the largest |g| and times 2^14, so that fp16
-// holds probabilities from 4e-9 up in full precision; the factors come off in the fp32 epilogues.
+// fp16 once scaled (what lies 2^-28 below a row's largest magnitude loses bits), in the transposed copies
+// that these products need anyway. dl is kept times 2^14, so that fp16 holds probabilities from 4e-9 up in
+// full precision, and the powers of two come off in the fp32 epilogues. A row's gradient g stays out of dl's
+// copy for dh, whose epilogue takes it: a row of dh is as exact as if it were alone. The sum over the rows in dw
+// has one scale, that of the largest |g| |h| of a row; a row 2^-k of it (float32, bf16) has half of k taken off
+// dl's transposed copy and half off h's, so that both stay in fp16's range (Row).
+#include <limits.h>
+
 #include <type_traits>
 
 #include "gemm_nt.h"
@@ -39,11 +44,21 @@ constexpr size_t kPieceBytes = size_t(1) << 30;  // default limit of a backward 
 
 // What a pass keeps on the device; the count is what the forward leaves for the backward.
 struct Head {
-  int exp_h, exp_w;  // backward: exponents of the transposed fp16 operands
-  int rows, pad;     // rows that take part, where they are gathered (Kept)
-  double count;      // rows that take part
-  float scale_dh, scale_dw, scale_db;  // backward: the factors of the gradients
+  int exp_w;     // backward: exponent of the transposed weight
+  int rows;      // rows that take part, where they are gathered (Kept)
+  double count;  // rows that take part
+  int exp_dw;    // backward: the largest exponent of a row's g times its h
+  float scale_dh, scale_dw;  // the factors of the gradients
 };
+// What the backward keeps of a row. Where its |g| |h| is 2^-k of the largest row's, h's transposed copy has
+// 2^-half of it, dl's the rest: t is below 2^(half - k) in magnitude.
+struct Row {
+  float g;     // its gradient (ignored: 0)
+  float t;     // the factor of dl's transposed copy, g 2^(-exp_dw - turned)
+  int exp;     // exponent of its h, whose largest magnitude it brings to [2^13, 2^14) (fp16: 0)
+  int turned;  // exponent of h's transposed copy, exp - half
+};
+
 
 // ---- largest magnitudes -> exponents -------------------------------------------------------------
 __device__ __forceinline__ float finite_max(float top, float x) {
@@ -52,7 +67,7 @@ __device__ __forceinline__ float finite_max(float top, float x) {
 }
 // Exponent e with max * 2^e in [2^13, 2^14): room for the fp16 planes and for sums of their products.
 __device__ int plane_exponent(float top) {
-  if (!(top > 0.0f) || !(top < __builtin_inff())) return 0;
+  if (!(top > 0.0f)) return 120;  // zeros: like the smallest
   int e;
   frexpf(top, &e);
   const int k = 14 - e;
@@ -117,21 +132,14 @@ __global__ __launch_bounds__(256) void absmax_kernel(const T* h, int64_t ldh, in
   if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// The exponents of both tensors from their partial maxima (gh, then gw of them), by one workgroup of up to
-// 16 waves.
-__device__ void exponents_of(const float* part, int gh, int gw, Head* head) {
-  __shared__ float mh[16], mw[16];
-  float a = 0.0f, b = 0.0f;
-  for (int i = threadIdx.x; i < gh; i += blockDim.x) a = fmaxf(a, part[i]);
-  for (int i = threadIdx.x; i < gw; i += blockDim.x) b = fmaxf(b, part[gh + i]);
-  a = wave_max_dpp(a), b = wave_max_dpp(b);
-  if ((threadIdx.x & 63) == 0) mh[threadIdx.x >> 6] = a, mw[threadIdx.x >> 6] = b;
+// The largest of one value a thread, in all threads of a workgroup of 16 waves.
+__device__ float largest_of(float v, float* sh) {
+  v = wave_max_dpp(v);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < (int)(blockDim.x >> 6); k++) a = fmaxf(a, mh[k]), b = fmaxf(b, mw[k]);
-    const int eh = plane_exponent(a), ew = plane_exponent(b);
-    head->exp_h = eh, head->exp_w = ew;
-  }
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  for (int k = 0; k < 16; k++) v = fmaxf(v, sh[k]);
+  return v;
 }
 
 // ---- rows that take part, gathered --------------------------------------------------------------------
@@ -141,7 +149,7 @@ __device__ void exponents_of(const float* part, int gh, int gw, Head* head) {
 struct Kept {
   int* map;
   int64_t* target;
-  int* exp;    // float32: the rows' exponents, else NULL
+  int* exp;    // forward, float32: the rows' exponents, else NULL
   float* lse;  // backward
 };
 // put(row, place, whether it takes part) for all rows, and their count; one workgroup of 16 waves.
@@ -619,64 +627,73 @@ __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int
 }
 
 // ---- backward -----------------------------------------------------------------------------------
-// One workgroup: the exponents of the transposed operands (part: the inputs' maxima, NULL: none), the rows'
-// factors relative to their largest magnitude, and what comes off again in the epilogues. Ignored rows get
-// 0 or are left out (Kept), rows whose gradient is not finite that gradient itself. eh: as gather_kernel's.
+// One workgroup: the transposed weight's exponent (part: gw partial maxima, NULL: none), the rows' factors, and
+// what comes off again in the epilogues. Ignored rows get 0 or are left out (Kept), rows whose gradient is not
+// finite that gradient itself. eh: the exponents of all rows of h (NULL: as they are).
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
                                                       int64_t ignore, int rows, int reduction,
-                                                      float* g, const Head* head, const float* part,
-                                                      int gh, int gw, const float* lse, const int* eh, Kept kept,
-                                                      Head* out) {
-  __shared__ float w[16];
-  __shared__ float all;
-  if (part) exponents_of(part, gh, gw, out);
-  const float inf = __builtin_inff();
-  float top = 0.0f, one = 0.0f;
-  if (reduction == SMQ_REDUCE_NONE) {
-    for (int m = threadIdx.x; m < rows; m += 1024) {
-      const float a = fabsf(grad[m]);
-      if (target[m] != ignore && a < inf) top = fmaxf(top, a);
-    }
-  } else {
-    // no row takes part: no gradient
-    one = reduction == SMQ_REDUCE_SUM ? *grad
-          : head->count > 0.0         ? (float)((double)*grad / head->count) : 0.0f;
-    top = fabsf(one) < inf ? fabsf(one) : 0.0f;
+                                                      const Head* head, const float* part, int gw,
+                                                      const float* lse, const int* eh, Kept kept, Row* out,
+                                                      Head* fac) {
+  __shared__ float sh[16];
+  int exp_w = 0;
+  if (part) {
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < gw; i += 1024) top = fmaxf(top, part[i]);
+    exp_w = plane_exponent(largest_of(top, sh));
   }
-  top = wave_max_dpp(top);
-  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = top;
-  __syncthreads();
+  // (no row takes part: no gradient)
+  const float one = reduction == SMQ_REDUCE_NONE  ? 0.0f
+                    : reduction == SMQ_REDUCE_SUM ? *grad
+                    : head->count > 0.0           ? (float)((double)*grad / head->count) : 0.0f;
+  auto size = [&](int m, float g) {  // the exponent of |g| |h|; g is finite and not 0
+    int e;
+    frexpf(g, &e);
+    return e - (eh ? eh[m] : 0);
+  };
+  auto counts = [&](float g) { return g != 0.0f && fabsf(g) < __builtin_inff(); };
+  const float none = (float)INT_MIN;
+  float top = none;
+  for (int m = threadIdx.x; m < rows; m += 1024) {
+    const float g = reduction == SMQ_REDUCE_NONE ? grad[m] : one;
+    if (target[m] != ignore && counts(g)) top = fmaxf(top, (float)size(m, g));
+  }
+  top = largest_of(top, sh);
+  const int most = top == none ? 0 : (int)top;
   if (threadIdx.x == 0) {
-    for (int k = 1; k < 16; k++) top = fmaxf(top, w[k]);
-    if (top == 0.0f) top = 1.0f;  // all zeros, or nothing finite
-    all = top;
-    out->scale_dh = ldexpf(top / kDlScale, part ? -out->exp_w : 0);
-    out->scale_dw = ldexpf(top / kDlScale, part ? -out->exp_h : 0);
-    out->scale_db = top / kDlScale;
+    fac->exp_w = exp_w, fac->exp_dw = most;
+    fac->scale_dh = ldexpf(1.0f / kDlScale, -exp_w);
+    fac->scale_dw = ldexpf(1.0f / kDlScale, most < 141 ? most : 141);  // (finite: its products with 0 are 0)
   }
-  __syncthreads();
-  top = all;
-  auto factor = [&](int m) { return (reduction == SMQ_REDUCE_NONE ? grad[m] : one) / top * kDlScale; };
+  auto row = [&](int m, bool keep) {
+    const float g = !keep ? 0.0f : reduction == SMQ_REDUCE_NONE ? grad[m] : one;
+    const int e = eh ? eh[m] : 0;
+    int turned = e;
+    if (!counts(g)) return Row{g, g, e, turned};
+    const int k = most - size(m, g);
+    if (eh) turned -= k > 100 ? k - 50 : k >> 1;  // (both copies of so small a row are 0; t stays normal)
+    return Row{g, ldexpf(g, -most - turned), e, turned};
+  };
   if (kept.map) {
-    partition_rows(target, ignore, rows, &out->rows, [&](int m, int at, bool keep) {
+    partition_rows(target, ignore, rows, &fac->rows, [&](int m, int at, bool keep) {
       kept.map[at] = m;
-      if (keep) kept.target[at] = target[m], kept.lse[at] = lse[m], g[at] = factor(m);
-      if (keep && kept.exp) kept.exp[at] = eh[m];
+      if (keep) kept.target[at] = target[m], kept.lse[at] = lse[m], out[at] = row(m, true);
     });
     return;
   }
-  for (int m = threadIdx.x; m < rows; m += 1024) g[m] = target[m] != ignore ? factor(m) : 0.0f;
+  for (int m = threadIdx.x; m < rows; m += 1024) out[m] = row(m, target[m] != ignore);
 }
 
-// dl of a piece from its logits, to `o` [rows, piece] and transposed to `ot` [piece, rows]; column
-// sums (the bias' gradient) per block of rows.
+// dl of a piece from its logits, to `o` [rows, piece], without the rows' gradients, and transposed, with them
+// (Row::t), to `ot` [piece, rows]; column sums (the bias' gradient) per block of rows.
 template <bool PLANES>
 struct DlEpi {
-  const int *eh, *ew;  // as SoftmaxEpi's
+  const int* ew;  // as SoftmaxEpi's
   const float* bias;
   const int64_t* target;
   const float* lse;
-  const float* g;
+  const Row* row;
+  const Head* fac;
   int64_t first, vocab;  // the piece's first vocabulary entry
   Mat o, ot;
   float* sums;  // [blocks][piece] or NULL
@@ -694,40 +711,46 @@ struct DlEpi {
     const int tile = ot.fmt == kSplit ? 32 : 64;
     ot.pad = (M + tile - 1) / tile * tile;
     float* sum = sums ? sums + (int64_t)(im * WM + wm) * N : nullptr;
+    const int back = fac->exp_dw - 14;
     stage_out<TM, TN, true>(
         acc, stage, m0, n0, M, N, lane, batch, o, ot, true, sum != nullptr,
-        [&](int m) {  // g, lse, the target's place in the piece (-1: elsewhere, -2: nowhere), the exponent
+        // the factor of the transposed copy, lse, the target's place in the piece (-1: elsewhere, -2: nowhere,
+        // -3: the row has no gradient), its two exponents
+        [&](int m) {
+          const Row q = row[m];
           const int64_t t = target[m], at = t - first;
-          const int k = t < 0 || t >= vocab ? -2 : at >= 0 && at < N ? (int)at : -1;
-          return make_float4(g[m], lse[m], __builtin_bit_cast(float, k),
-                             __builtin_bit_cast(float, PLANES ? eh[m] : 0));
+          const int k = q.g == 0.0f ? -3 : t < 0 || t >= vocab ? -2 : at >= 0 && at < N ? (int)at : -1;
+          return make_float4(q.t, lse[m], __builtin_bit_cast(float, k),
+                             __builtin_bit_cast(float, (int)((unsigned)q.turned << 16 | (q.exp & 0xffff))));
         },
         [&](int, int n, float4 v, float4 row) {
-          const int at = __builtin_bit_cast(int, row.z) - n;
-          const bool known = __builtin_bit_cast(int, row.z) != -2;
+          const int k0 = __builtin_bit_cast(int, row.z), at = k0 - n;
+          const int er = (int16_t)__builtin_bit_cast(int, row.w);
           float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            float l = PLANES ? ldexpf(w[k], -(__builtin_bit_cast(int, row.w) + en[k])) : w[k];
+            float l = PLANES ? ldexpf(w[k], -(er + en[k])) : w[k];
             if (bias && n + k < N) l += bias[first + n + k];
-            const float p = exp_near(l - row.y) - (at == k ? 1.0f : 0.0f);
-            w[k] = row.x == 0.0f ? 0.0f : known ? p * row.x : __builtin_nanf("");
+            const float p = fmaf(exp_near(l - row.y), kDlScale, at == k ? -kDlScale : 0.0f);
+            w[k] = k0 == -3 ? 0.0f : k0 == -2 ? __builtin_nanf("") : p;
           }
           return make_float4(w[0], w[1], w[2], w[3]);
         },
+        // p g from kDlScale p g 2^(-exp_dw - turned)
+        [&](float v, float w) { return ldexpf(v, back + (__builtin_bit_cast(int, w) >> 16)); },
         [&](int n, float s) { sum[n] = s; });
   }
 };
 
 // (live: `per` blocks for each `high` of the rows there are)
 __global__ __launch_bounds__(256) void bias_sum_kernel(const float* part, int blocks, int n, const int* live,
-                                                       int high, int per, const Head* head, float* db) {
+                                                       int high, int per, float* db) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= n) return;
   double s = 0.0;
   if (live) blocks = (*live + high - 1) / high * per;
   for (int k = 0; k < blocks; k++) s += (double)part[(int64_t)k * n + v];
-  db[v] = (float)(s * (double)head->scale_db);
+  db[v] = (float)s;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -1003,9 +1026,9 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
     }
   } else {
     const Operand A = raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
-                          : operand(a, h, ldh, s.tokens, s.dim, s, {eh, 1}, {}, pick, kNoMat, run, st);
+                          : operand(a, h, ldh, s.tokens, s.dim, s, eh ? Exponents{eh, 1} : Exponents(), {}, pick, kNoMat, run, st);
     const Operand B = raw ? Operand{w, 2 * ldw, 0, (int)s.vocab}
-                          : operand(a, w, ldw, s.vocab, s.dim, s, {ew, 1}, {}, {}, kNoMat, run, st);
+                          : operand(a, w, ldw, s.vocab, s.dim, s, ew ? Exponents{ew, 1} : Exponents(), {}, {}, kNoMat, run, st);
     if (run)
       logits(s, raw, tile, A, B,
              [&](auto planes) { return SoftmaxEpi<planes.value>{eh, ew, bias, at, part, picked}; }, st);
@@ -1060,34 +1083,33 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   if (s.piece <= 0) s.piece = default_piece(s);
   if (s.piece > s.vocab) s.piece = s.vocab;
   const int64_t pieces = (s.vocab + s.piece - 1) / s.piece;
-  float* g = a.take<float>(s.tokens);
+  Row* row = a.take<Row>(s.tokens);
   Head* fac = a.take<Head>(1);
   const bool gather = gathered(s);
   Kept kept = {};
   Pick pick;
   pick.keep = target, pick.skip = ignore;
   if (gather) {
-    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), sp ? a.take<int>(s.tokens) : nullptr,
-            a.take<float>(s.tokens)};
+    kept = {a.take<int>(s.tokens), a.take<int64_t>(s.tokens), nullptr, a.take<float>(s.tokens)};
     pick = Pick();
     pick.map = kept.map, pick.live = &fac->rows;
   }
   const bool raw = raw32(h, ldh, w, ldw, s), scaled = s.dtype != SMQ_DTYPE_F16;
-  // rows' exponents of the logits' operands, and one each for the transposed ones
-  int* eh = sp && !raw ? a.take<int>(s.tokens) : nullptr;
+  // exponents of h's rows, of w's rows (the logits' operand) and of w (the transposed one)
+  int* eh = scaled ? a.take<int>(s.tokens) : nullptr;
   int* ew = sp && !raw ? a.take<int>(exponent_room(s.vocab)) : nullptr;
   float* top = nullptr;
   if (scaled) {
     top = a.take<float>(2 * kMaxParts);
     if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, eh, ew, st);
-    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, nullptr, nullptr, st);
+    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, eh, nullptr, st);
   }
-  const Exponents turned_eh = {scaled ? &fac->exp_h : nullptr, 0}, turned_ew = {scaled ? &fac->exp_w : nullptr, 0};
+  const Exponents turned_eh = scaled ? Exponents{&row->turned, 4} : Exponents();
+  const Exponents turned_ew = {scaled ? &fac->exp_w : nullptr, 0};
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
-                       (int)s.tokens, reduction, g, head, top, absmax_grid(s.tokens),
-                       absmax_grid(s.vocab), lse, eh, kept, fac);
-  if (gather) eh = kept.exp;
+                       (int)s.tokens, reduction, head, top ? top + absmax_grid(s.tokens) : nullptr,
+                       absmax_grid(s.vocab), lse, eh, kept, row, fac);
   // h, and transposed the operand of dw. Ignored rows are left out or zeros, whatever they hold (where h is
   // read in place its ignored rows' logits are not used).
   const int64_t ldt = operand_ld(s.tokens, sp);
@@ -1097,7 +1119,8 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   if (run && raw && dw) layout(h, s.dtype, ldh, s.tokens, s.dim, {}, turned_eh, target, ignore, kNoMat, turned_h, st);  // (not gathered)
   const Operand A =
       raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
-          : operand(a, h, ldh, s.tokens, s.dim, s, {eh, 1}, turned_eh, pick, turned_h, run, st);
+          : operand(a, h, ldh, s.tokens, s.dim, s, sp ? Exponents{&row->exp, 4} : Exponents(), turned_eh, pick,
+                    turned_h, run, st);
   const int64_t ldp = operand_ld(s.piece, sp);
   _Float16* dl = a.take<_Float16>((size_t)(s.tokens * ldp));
   _Float16* dlt = a.take<_Float16>((size_t)(s.piece * ldt));
@@ -1121,22 +1144,24 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     const Mat turned_w = dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat;
     if (run && raw && dh) layout(wp, s.dtype, ldw, n, s.dim, {}, turned_ew, nullptr, 0, kNoMat, turned_w, st);
     const Operand B = raw ? Operand{wp, 2 * ldw, 0, (int)n}
-                          : operand(a, wp, ldw, n, s.dim, s, {ew ? ew + v0 : nullptr, 1}, turned_ew, {}, turned_w, run, st);
+                          : operand(a, wp, ldw, n, s.dim, s, ew ? Exponents{ew + v0, 1} : Exponents(), turned_ew, {},
+                                    turned_w, run, st);
     if (a.used > most) most = a.used;
     if (!run) continue;
     logits(s, raw, tile_l, A, B, [&](auto planes) {
-      return DlEpi<planes.value>{eh, ew ? ew + v0 : nullptr, bias, gather ? kept.target : target,
-                                 gather ? kept.lse : lse, g, v0, s.vocab, {dl, ldp, 0, fmt, padn},
+      return DlEpi<planes.value>{ew ? ew + v0 : nullptr, bias, gather ? kept.target : target,
+                                 gather ? kept.lse : lse, row, fac, v0, s.vocab, {dl, ldp, 0, fmt, padn},
                                  {dlt, ldt, 0, fmt, padt}, sums};
     }, st);
     if (db)
       hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, sums,
-                         row_blocks, (int)n, pick.live, shape_of(tile_l).bm, shape_of(tile_l).wm, fac, db + v0);
+                         row_blocks, (int)n, pick.live, shape_of(tile_l).bm, shape_of(tile_l).wm, db + v0);
     if (dh) {
       const Operand L = {dl, ldp, 0, (int)s.tokens, pick.live}, W = {wt, ldp, 0, (int)s.dim};
       StoreEpi se = {1.0f, 1.0f, whole ? &fac->scale_dh : nullptr, kNoMat, kNoMat, kNoMat, 0, s.tokens * ldacc, 0.0f};
       se.o = whole ? Mat{dh, s.dim, 0, out_fmt(s.dtype), 0} : Mat{accum, ldacc, 0, kF32, 0};
       if (i > 0) se.src = se.o;
+      if (whole) se.rows = &row->g, se.row_step = 4;
       product(sp, tile_dh, L, W, operand_kt(n, sp), shares, se, st);
     }
     if (dw) {
@@ -1149,7 +1174,7 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   }
   if (run && dh && !whole) {
     StoreEpi se = {1.0f, 0.0f, &fac->scale_dh, kNoMat, {dh, s.dim, 0, out_fmt(s.dtype), 0}, kNoMat, 0, 0, 0.0f};
-    se.map = pick.map, se.live = pick.live;
+    se.map = pick.map, se.live = pick.live, se.rows = &row->g, se.row_step = 4;
     launch_split_sum(accum, ldacc, s.tokens * ldacc, shares, 0, (int)s.tokens, (int)s.dim, 1, 0, se, st);
   }
   return most;

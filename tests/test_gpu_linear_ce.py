@@ -552,3 +552,59 @@ def test_a_large_row_leaves_the_others_losses(tokens, dim, vocab, ignored, power
     assert torch.equal(linear_cross_entropy(large_h, w, t, b, reduction="none")[rest], base[rest])
     assert torch.equal(linear_cross_entropy(h, large_w, t, b, reduction="none"), base)
     assert torch.isfinite(base).all()
+
+
+SPREAD = [(9, 64, 500, 0), (60, 36, 500, 0.2), (100, 64, 500, 0), (200, 100, 900, 0), (*GATHERED, 0.5)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,dim,vocab,ignored", SPREAD)
+def test_a_large_gradient_leaves_the_others(tokens, dim, vocab, ignored, dtype):
+    """One finite gradient of a loss, or one finite row of hidden, far above the rest: the other rows of
+    hidden's gradient keep every bit."""
+    h, w, b, t = make(tokens, dim, vocab, dtype, True, ignored, seed=32)
+    t[3] = 5
+    rest = torch.arange(tokens, device="cuda") != 3
+    g = torch.randn(tokens, device="cuda")
+
+    def run(h, g):
+        leaf = h.detach().requires_grad_()
+        return torch.autograd.grad(linear_cross_entropy(leaf, w, t, b, reduction="none"), leaf, g)[0]
+
+    base = run(h, g)
+    assert (base[rest & (t != -100)] != 0).any(1).all()
+    large = g.clone()
+    for power in (24, 40, -40):
+        large[3] = 2.0 ** power
+        assert torch.equal(run(h, large)[rest], base[rest])
+    if dtype != torch.float16:
+        for power in (24, 40):
+            spread = h.clone()
+            spread[3] *= 2.0 ** power
+            assert torch.equal(run(spread, g)[rest], base[rest])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("power", [24, 40])
+@pytest.mark.parametrize("tokens,dim,vocab,ignored", SPREAD)
+def test_the_weights_gradient_beside_large_rows(tokens, dim, vocab, ignored, power, dtype):
+    """Rows of hidden 2^k above the others, each sure of one entry: the weight's and the bias' gradients of
+    the other entries are those of the small rows alone. Both operands of such a sum have half of k taken off,
+    which leaves them 2^(k / 2 - 38) of a row's largest product."""
+    h, w, b, t = make(tokens, dim, vocab, dtype, True, ignored, seed=33)
+    t[::50] = 5
+    large = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    large[::50] = True
+    h[large] *= 2.0 ** power
+    g = torch.randn(tokens, device="cuda")
+    leaves = [x.detach().requires_grad_() for x in (h, w, b)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+    dw, db = torch.autograd.grad(loss, leaves[1:], g)
+    others = torch.ones(vocab, dtype=torch.bool, device="cuda")
+    others[5] = False
+    others[(h[large].double() @ w.double().t() + b.double()).argmax(1)] = False
+    small = ~large
+    _, _, want, bounds = reference(h[small], w, b, t[small], "none", g[small])
+    size = (g.abs() * h.abs().amax(1) * (t != -100))[small].double().sum() * 2.0 ** ((power + 4) / 2 - 37)
+    close(dw[others], want[1][others], bounds[1][others] + size, dtype)
+    close(db[others], want[2][others], bounds[2][others], torch.float32)
