@@ -495,11 +495,13 @@ __device__ __forceinline__ void wave_sync() {
 // where `ot` is set, to `ot` transposed. `colsum(n, v)`, where given, gets the sum over the part's
 // rows of column n. Lanes past the edges call neither. `prep(m)` (ROWS): what f needs of a row, four words, read
 // once per row into the stage's spare columns (f's fourth argument): the first is a factor of the row in the
-// transposed copy, `weigh(v, last)` makes the term of a column's sum of the copy's value and the row's last word.
-template <int TM, int TN, bool ROWS, typename P, typename F, typename W, typename S>
+// transposed copy, `weigh(v, last)` makes the term of a column's sum of the copy's value and the row's last word,
+// `out(v)` what goes to `o`.
+template <int TM, int TN, bool ROWS, typename P, typename F, typename O, typename W, typename S>
 __device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* stage, int m0, int n0,
                                           int M, int N, int lane, int64_t batch, const Mat& o,
-                                          const Mat& ot, bool mirror, bool sums, P prep, F f, W weigh, S colsum) {
+                                          const Mat& ot, bool mirror, bool sums, P prep, F f, O out, W weigh,
+                                          S colsum) {
   constexpr int kCols = TN * 32, kPitch = kCols + 4;
   constexpr int kPer = kCols / 4, kRows = 64 / kPer;  // row phase: lanes a row, rows a pass
   float total = 0.0f;
@@ -535,7 +537,9 @@ __device__ __forceinline__ void stage_out(const f32x16 (&acc)[TM][TN], float* st
             }
           }
           if (o.fmt != kNone) {
-            const float w[4] = {v.x, v.y, v.z, v.w};
+            float4 u = v;
+            if constexpr (ROWS) u = out(v);
+            const float w[4] = {u.x, u.y, u.z, u.w};
             store_n<4>(o, batch, mb + r, n0 + c, N, w);
           }
           if constexpr (ROWS) v.x *= factor, v.y *= factor, v.z *= factor, v.w *= factor;
@@ -621,7 +625,7 @@ struct StoreEpi {
           }
           return v;
         },
-        0, [](int, float) {});
+        0, 0, [](int, float) {});
   }
 };
 
@@ -763,12 +767,22 @@ static inline void launch(int tile, const Operand& A, const Operand& B, int kt, 
   }
 }
 
-// Power-of-two exponents of a matrix' rows: e[step * r] (step 0: *e for all of them); e NULL: 0.
+// In a sum whose largest terms have scale 2^0 a term of 2^-k has this part of k taken off one of its factors and
+// the rest off the other, so that both stay in fp16's range. (Past 100 both are 0 there; the other factor's part
+// stays a normal float.)
+__device__ __forceinline__ int half_of(int k) { return k > 100 ? k - 50 : k >> 1; }
+// Power-of-two exponents of a matrix' rows: e[step * r] (step 0: *e for all of them); e NULL: 0. With `least`, the
+// smallest of them, half of the difference comes off.
 struct Exponents {
   const int* e = nullptr;
   int step = 0;
+  const int* least = nullptr;
   __device__ __forceinline__ int all() const { return e && step == 0 ? *e : 0; }
-  __device__ __forceinline__ int at(int r) const { return step ? e[step * r] : all(); }
+  __device__ __forceinline__ int at(int r) const {
+    if (!step) return all();
+    const int v = e[step * r];
+    return least ? v - half_of(v - *least) : v;
+  }
 };
 // Layout pass: src [rows, cols] of type T, row pitch ld, times *factor (NULL: 1), to `d` row by row, times
 // 2^exponent of the row, and / or to `dt` transposed, times 2^turned (either may be absent), zero padded.

@@ -28,7 +28,8 @@
 // full precision, and the powers of two come off in the fp32 epilogues. A row's gradient g stays out of dl's
 // copy for dh, whose epilogue takes it: a row of dh is as exact as if it were alone. The sum over the rows in dw
 // has one scale, that of the largest |g| |h| of a row; a row 2^-k of it (float32, bf16) has half of k taken off
-// dl's transposed copy and half off h's, so that both stay in fp16's range (Row).
+// dl's transposed copy and half off h's, so that both stay in fp16's range (Row); dh's sum over float32 entries the
+// same of the largest |w|.
 #include <limits.h>
 
 #include <type_traits>
@@ -671,7 +672,7 @@ __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const i
     int turned = e;
     if (!counts(g)) return Row{g, g, e, turned};
     const int k = most - size(m, g);
-    if (eh) turned -= k > 100 ? k - 50 : k >> 1;  // (both copies of so small a row are 0; t stays normal)
+    if (eh) turned -= half_of(k);
     return Row{g, ldexpf(g, -most - turned), e, turned};
   };
   if (kept.map) {
@@ -686,9 +687,9 @@ __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const i
 
 // dl of a piece from its logits, to `o` [rows, piece], without the rows' gradients, and transposed, with them
 // (Row::t), to `ot` [piece, rows]; column sums (the bias' gradient) per block of rows.
-template <bool PLANES>
+template <bool PLANES, bool F32>
 struct DlEpi {
-  const int* ew;  // as SoftmaxEpi's
+  const int* ew;  // F32: the exponents of w's rows; PLANES: they come off the logits, as the rows' do
   const float* bias;
   const int64_t* target;
   const float* lse;
@@ -703,9 +704,15 @@ struct DlEpi {
                                          int64_t batch) const {
     // a lane's four columns are the same in all of stage_out's rows
     int en[4] = {};
-    if (PLANES) {
+    float part[4] = {};  // of an entry 2^-k of the largest what stays with dl
+    if constexpr (F32) {
+      const int least = fac->exp_w;
 #pragma unroll
-      for (int k = 0; k < 4; k++) en[k] = ew[n0 + lane % (TN * 8) * 4 + k];  // (past N: its padding)
+      for (int k = 0; k < 4; k++) {
+        en[k] = ew[n0 + lane % (TN * 8) * 4 + k];  // (past N: its padding)
+        const int d = en[k] - least;
+        part[k] = ldexpf(1.0f, half_of(d) - d);
+      }
     }
     Mat ot = this->ot;  // padded to whole k tiles of the rows there are
     const int tile = ot.fmt == kSplit ? 32 : 64;
@@ -735,6 +742,9 @@ struct DlEpi {
             w[k] = k0 == -3 ? 0.0f : k0 == -2 ? __builtin_nanf("") : p;
           }
           return make_float4(w[0], w[1], w[2], w[3]);
+        },
+        [&](float4 v) {
+          return F32 ? make_float4(v.x * part[0], v.y * part[1], v.z * part[2], v.w * part[3]) : v;
         },
         // p g from kDlScale p g 2^(-exp_dw - turned)
         [&](float v, float w) { return ldexpf(v, back + (__builtin_bit_cast(int, w) >> 16)); },
@@ -893,15 +903,16 @@ bool raw32(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& 
 bool gathered(const Shape& s) {
   return s.tokens > 128 && s.tokens * s.vocab >= ((int64_t)1 << (s.split() ? 33 : 35)) / s.dim;
 }
-// The logits' product: by planes, one plane or raw float32, with the epilogue make(planes).
+// The logits' product: by planes, one plane or raw float32, with the epilogue make(planes, float32).
 template <typename F>
 void logits(const Shape& s, bool raw, int tile, const Operand& A, const Operand& B, F make, hipStream_t st) {
   const int kt = operand_kt(s.dim, s.split());
-  const auto one = make(std::false_type());
-  if (raw) launch<Raw32, false>(tile, A, B, (int)(round_up(s.dim, 32) / 32), 1, 0, 1, one, st);
-  else if (s.dtype == SMQ_DTYPE_BF16) launch<__bf16, false>(tile, A, B, kt, 1, 0, 1, one, st);
-  else if (s.dtype == SMQ_DTYPE_F16) launch<_Float16, false>(tile, A, B, kt, 1, 0, 1, one, st);
-  else launch<_Float16, true>(tile, A, B, kt, 1, 0, 1, make(std::true_type()), st);
+  const std::true_type yes;
+  const std::false_type no;
+  if (raw) launch<Raw32, false>(tile, A, B, (int)(round_up(s.dim, 32) / 32), 1, 0, 1, make(no, yes), st);
+  else if (s.dtype == SMQ_DTYPE_BF16) launch<__bf16, false>(tile, A, B, kt, 1, 0, 1, make(no, no), st);
+  else if (s.dtype == SMQ_DTYPE_F16) launch<_Float16, false>(tile, A, B, kt, 1, 0, 1, make(no, no), st);
+  else launch<_Float16, true>(tile, A, B, kt, 1, 0, 1, make(yes, yes), st);
 }
 
 // Few tokens: up to 16, hidden within 148 KiB of LDS; 0: not few.
@@ -1031,7 +1042,7 @@ size_t forward(const void* h, int64_t ldh, const void* w, int64_t ldw, const Sha
                           : operand(a, w, ldw, s.vocab, s.dim, s, ew ? Exponents{ew, 1} : Exponents(), {}, {}, kNoMat, run, st);
     if (run)
       logits(s, raw, tile, A, B,
-             [&](auto planes) { return SoftmaxEpi<planes.value>{eh, ew, bias, at, part, picked}; }, st);
+             [&](auto planes, auto) { return SoftmaxEpi<planes.value>{eh, ew, bias, at, part, picked}; }, st);
   }
   if (run) {
     int per = 1;
@@ -1095,9 +1106,9 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     pick.map = kept.map, pick.live = &fac->rows;
   }
   const bool raw = raw32(h, ldh, w, ldw, s), scaled = s.dtype != SMQ_DTYPE_F16;
-  // exponents of h's rows, of w's rows (the logits' operand) and of w (the transposed one)
+  // exponents of h's rows, and of float32 w's
   int* eh = scaled ? a.take<int>(s.tokens) : nullptr;
-  int* ew = sp && !raw ? a.take<int>(exponent_room(s.vocab)) : nullptr;
+  int* ew = sp ? a.take<int>(exponent_room(s.vocab)) : nullptr;
   float* top = nullptr;
   if (scaled) {
     top = a.take<float>(2 * kMaxParts);
@@ -1105,7 +1116,6 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, eh, nullptr, st);
   }
   const Exponents turned_eh = scaled ? Exponents{&row->turned, 4} : Exponents();
-  const Exponents turned_ew = {scaled ? &fac->exp_w : nullptr, 0};
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
                        (int)s.tokens, reduction, head, top ? top + absmax_grid(s.tokens) : nullptr,
@@ -1142,16 +1152,17 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     const char* wp = reinterpret_cast<const char*>(w) + (size_t)(v0 * ldw) * wsize;
     const int padn = operand_pad(n, sp);
     const Mat turned_w = dh ? Mat{wt, ldp, 0, fmt, padn} : kNoMat;
+    const Exponents of_w = ew ? Exponents{ew + v0, 1} : Exponents();
+    const Exponents turned_ew = ew ? Exponents{ew + v0, 1, &fac->exp_w} : Exponents{scaled ? &fac->exp_w : nullptr, 0};
     if (run && raw && dh) layout(wp, s.dtype, ldw, n, s.dim, {}, turned_ew, nullptr, 0, kNoMat, turned_w, st);
     const Operand B = raw ? Operand{wp, 2 * ldw, 0, (int)n}
-                          : operand(a, wp, ldw, n, s.dim, s, ew ? Exponents{ew + v0, 1} : Exponents(), turned_ew, {},
-                                    turned_w, run, st);
+                          : operand(a, wp, ldw, n, s.dim, s, of_w, turned_ew, {}, turned_w, run, st);
     if (a.used > most) most = a.used;
     if (!run) continue;
-    logits(s, raw, tile_l, A, B, [&](auto planes) {
-      return DlEpi<planes.value>{ew ? ew + v0 : nullptr, bias, gather ? kept.target : target,
-                                 gather ? kept.lse : lse, row, fac, v0, s.vocab, {dl, ldp, 0, fmt, padn},
-                                 {dlt, ldt, 0, fmt, padt}, sums};
+    logits(s, raw, tile_l, A, B, [&](auto planes, auto f32) {
+      return DlEpi<planes.value, f32.value>{ew ? ew + v0 : nullptr, bias, gather ? kept.target : target,
+                                            gather ? kept.lse : lse, row, fac, v0, s.vocab,
+                                            {dl, ldp, 0, fmt, padn}, {dlt, ldt, 0, fmt, padt}, sums};
     }, st);
     if (db)
       hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, sums,

@@ -608,3 +608,25 @@ def test_the_weights_gradient_beside_large_rows(tokens, dim, vocab, ignored, pow
     size = (g.abs() * h.abs().amax(1) * (t != -100))[small].double().sum() * 2.0 ** ((power + 4) / 2 - 37)
     close(dw[others], want[1][others], bounds[1][others] + size, dtype)
     close(db[others], want[2][others], bounds[2][others], torch.float32)
+
+
+@pytest.mark.parametrize("power", [24, 40])
+@pytest.mark.parametrize("tokens,dim,vocab,ignored", SPREAD)
+def test_hiddens_gradient_beside_a_large_entry(tokens, dim, vocab, ignored, power):
+    """An entry of the weight 2^k above the others, masked by its bias: float32 gradients of hidden are those of
+    the other entries alone, whose factors in the sum have half of k taken off each: every term is off by
+    2^(k / 2 - 38) of its largest, and they add up as a random walk."""
+    h, w, b, t = make(tokens, dim, vocab, torch.float32, True, ignored, seed=34)
+    t = torch.where(t == -100, t, t % (vocab - 1))
+    b[-1] = float("-inf")
+    g = torch.randn(tokens, device="cuda")
+    large = w.clone()
+    large[-1] *= 2.0 ** power
+    leaves = [h.requires_grad_(), b.requires_grad_()]
+    loss = linear_cross_entropy(h, large, t, b, reduction="none")
+    dh, db = torch.autograd.grad(loss, leaves, g)
+    _, _, want, bounds = reference(h.detach(), w[:-1], b.detach()[:-1], t, "none", g)
+    size = (g.abs() * (t != -100))[:, None].double() * w[:-1].abs().max() * 2.0 ** ((power + 4) / 2 - 37)
+    close(dh, want[0], bounds[0] + size * min(vocab, 8 * vocab ** 0.5), torch.float32)
+    close(db[:-1], want[2], bounds[2], torch.float32)
+    assert db[-1] == 0
