@@ -54,7 +54,7 @@ struct Head {
 // What the backward keeps of a row. Where its |g| |h| is 2^-k of the largest row's, h's transposed copy has
 // 2^-half of it, dl's the rest: t is below 2^(half - k) in magnitude.
 struct Row {
-  float g;     // its gradient (ignored: 0)
+  float g;     // its gradient (ignored: 0, a bad target: NaN)
   float t;     // the factor of dl's transposed copy, g 2^(-exp_dw - turned)
   int exp;     // exponent of its h, whose largest magnitude it brings to [2^13, 2^14) (fp16: 0)
   int turned;  // exponent of h's transposed copy, exp - half
@@ -630,9 +630,9 @@ __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int
 // ---- backward -----------------------------------------------------------------------------------
 // One workgroup: the transposed weight's exponent (part: gw partial maxima, NULL: none), the rows' factors, and
 // what comes off again in the epilogues. Ignored rows get 0 or are left out (Kept), rows whose gradient is not
-// finite that gradient itself. eh: the exponents of all rows of h (NULL: as they are).
+// finite that gradient itself, rows whose target is no entry NaN. eh: the exponents of all rows of h (NULL: as they are).
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
-                                                      int64_t ignore, int rows, int reduction,
+                                                      int64_t ignore, int rows, int64_t vocab, int reduction,
                                                       const Head* head, const float* part, int gw,
                                                       const float* lse, const int* eh, Kept kept, Row* out,
                                                       Head* fac) {
@@ -667,7 +667,9 @@ __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const i
     fac->scale_dw = ldexpf(1.0f / kDlScale, most < 141 ? most : 141);  // (finite: its products with 0 are 0)
   }
   auto row = [&](int m, bool keep) {
-    const float g = !keep ? 0.0f : reduction == SMQ_REDUCE_NONE ? grad[m] : one;
+    const float g = !keep                                ? 0.0f
+                    : target[m] < 0 || target[m] >= vocab ? __builtin_nanf("")
+                    : reduction == SMQ_REDUCE_NONE        ? grad[m] : one;
     const int e = eh ? eh[m] : 0;
     int turned = e;
     if (!counts(g)) return Row{g, g, e, turned};
@@ -695,7 +697,7 @@ struct DlEpi {
   const float* lse;
   const Row* row;
   const Head* fac;
-  int64_t first, vocab;  // the piece's first vocabulary entry
+  int64_t first;  // the piece's first vocabulary entry
   Mat o, ot;
   float* sums;  // [blocks][piece] or NULL
   template <int BM, int BN, int WM, int WN, int TM, int TN>
@@ -721,12 +723,12 @@ struct DlEpi {
     const int back = fac->exp_dw - 14;
     stage_out<TM, TN, true>(
         acc, stage, m0, n0, M, N, lane, batch, o, ot, true, sum != nullptr,
-        // the factor of the transposed copy, lse, the target's place in the piece (-1: elsewhere, -2: nowhere,
-        // -3: the row has no gradient), its two exponents
+        // the factor of the transposed copy, lse, the target's place in the piece (-1: elsewhere, -2: the row
+        // has no gradient), its two exponents
         [&](int m) {
           const Row q = row[m];
-          const int64_t t = target[m], at = t - first;
-          const int k = q.g == 0.0f ? -3 : t < 0 || t >= vocab ? -2 : at >= 0 && at < N ? (int)at : -1;
+          const int64_t at = target[m] - first;
+          const int k = q.g == 0.0f ? -2 : at >= 0 && at < N ? (int)at : -1;
           return make_float4(q.t, lse[m], __builtin_bit_cast(float, k),
                              __builtin_bit_cast(float, (int)((unsigned)q.turned << 16 | (q.exp & 0xffff))));
         },
@@ -739,7 +741,7 @@ struct DlEpi {
             float l = PLANES ? ldexpf(w[k], -(er + en[k])) : w[k];
             if (bias && n + k < N) l += bias[first + n + k];
             const float p = fmaf(exp_near(l - row.y), kDlScale, at == k ? -kDlScale : 0.0f);
-            w[k] = k0 == -3 ? 0.0f : k0 == -2 ? __builtin_nanf("") : p;
+            w[k] = k0 == -2 ? 0.0f : p;
           }
           return make_float4(w[0], w[1], w[2], w[3]);
         },
@@ -1118,7 +1120,7 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   const Exponents turned_eh = scaled ? Exponents{&row->turned, 4} : Exponents();
   if (run)
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, st, grad, target, ignore,
-                       (int)s.tokens, reduction, head, top ? top + absmax_grid(s.tokens) : nullptr,
+                       (int)s.tokens, s.vocab, reduction, head, top ? top + absmax_grid(s.tokens) : nullptr,
                        absmax_grid(s.vocab), lse, eh, kept, row, fac);
   // h, and transposed the operand of dw. Ignored rows are left out or zeros, whatever they hold (where h is
   // read in place its ignored rows' logits are not used).
@@ -1161,7 +1163,7 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
     if (!run) continue;
     logits(s, raw, tile_l, A, B, [&](auto planes, auto f32) {
       return DlEpi<planes.value, f32.value>{ew ? ew + v0 : nullptr, bias, gather ? kept.target : target,
-                                            gather ? kept.lse : lse, row, fac, v0, s.vocab,
+                                            gather ? kept.lse : lse, row, fac, v0,
                                             {dl, ldp, 0, fmt, padn}, {dlt, ldt, 0, fmt, padt}, sums};
     }, st);
     if (db)

@@ -630,3 +630,22 @@ def test_hiddens_gradient_beside_a_large_entry(tokens, dim, vocab, ignored, powe
     close(dh, want[0], bounds[0] + size * min(vocab, 8 * vocab ** 0.5), torch.float32)
     close(db[:-1], want[2], bounds[2], torch.float32)
     assert db[-1] == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,dim,vocab,ignored", SPREAD)
+def test_bad_targets_under_a_zero_gradient(tokens, dim, vocab, ignored, dtype):
+    """A target outside the vocabulary makes its row's gradient NaN, and what sums over the rows, whatever the
+    gradient of its loss: 0 times NaN."""
+    h, w, b, t = make(tokens, dim, vocab, dtype, True, ignored, seed=35)
+    t[3], t[5] = vocab, -7
+    g = torch.ones(tokens, device="cuda")
+    g[3] = 0.0
+    leaves = [x.detach().requires_grad_() for x in (h, w, b)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+    dh, dw, db = torch.autograd.grad(loss, leaves, g)
+    bad = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    bad[3] = bad[5] = True
+    assert torch.equal(torch.isnan(loss), bad)
+    assert torch.isnan(dh[bad]).all() and torch.isfinite(dh[~bad]).all()
+    assert torch.isnan(dw).all() and torch.isnan(db).all()
