@@ -457,7 +457,7 @@ struct Arena {
   }
 };
 
-struct Buffers {
+struct Buffers {  // (those a call does not use are NULL)
   _Float16 *x[2], *xt[2], *gram[2], *q[2], *p[2], *w;
   float* part;  // shares of a product split over k
 };
@@ -546,15 +546,21 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
   float* pow2 = a.take<float>((size_t)bt);
   float* rest = a.take<float>((size_t)bt);
   float* rest2 = a.take<float>((size_t)bt);
-  Buffers w;
+  Buffers w = {};
+  const bool small = m <= 64;
+  const int longest = stage_of(p);
+  auto square = [&]() { return a.take<_Float16>((size_t)(bt * m * ldm)); };
   for (int k = 0; k < 2; k++) {
     w.x[k] = a.take<_Float16>((size_t)(bt * m * ldn));
     w.xt[k] = a.take<_Float16>((size_t)(bt * n * ldm));
-    w.gram[k] = a.take<_Float16>((size_t)(bt * m * ldm));
-    w.q[k] = a.take<_Float16>((size_t)(bt * m * ldm));
-    w.p[k] = a.take<_Float16>((size_t)(bt * m * ldm));
   }
-  w.w = a.take<_Float16>((size_t)(bt * m * ldm));
+  w.gram[0] = square();
+  if (small) {
+    w.p[0] = square();
+  } else {
+    w.q[0] = square();
+    if (longest > 1) w.gram[1] = square(), w.q[1] = square(), w.p[0] = square(), w.p[1] = square(), w.w = square();
+  }
   w.part = a.take<float>(share_floats(p));
   if (!run) return a.used;
 
@@ -566,7 +572,6 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
   auto op = [](const Mat& q, int64_t rows) { return Operand{q.p, q.ld, q.batch, (int)rows}; };
   const Mat none = {nullptr, 0, 0, kNone, 0};
   const int out = p.dtype == SMQ_DTYPE_F32 ? kF32 : p.dtype == SMQ_DTYPE_F16 ? kF16 : kBF16;
-  const int longest = stage_of(p);
   Mat X = mat(w.x[0], n, m, p.dtype == SMQ_DTYPE_F32 ? kSplit : kF16);
   Mat XT = mat(w.xt[0], m, n, p.dtype == SMQ_DTYPE_F32 ? kSplit : kDup);
   if (p.dtype == SMQ_DTYPE_F32)
@@ -577,7 +582,6 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
     first_layout(p, (const __bf16*)g, ld, stride, eps, part, pow2, rest, rest2, X, XT, st);
 
   double top = 1.0;  // bound of X's singular values
-  const bool small = m <= 64;
   // One workgroup a matrix also for the products with X: where they are short, or the stack fills the chip.
   if (small && p.steps <= 8 && (n <= 256 || batch >= 128)) {
     SmallArgs sa = {};

@@ -194,3 +194,13 @@ def test_c_abi_refuses_bad_alignment():
     assert lib.smq_group_norm_act(*gn, p + 4, big, None) == -2
     c = (ctypes.c_double * 3)(3.4445, -4.7750, 2.0315)
     assert lib.smq_orthogonalize(p, 6, 24, 0, p, 1, 4, 6, 5, c, 1e-7, p + 8, big, None) == -2
+
+
+def test_orthogonalize_workspace_is_what_a_call_uses():
+    """X and its transpose twice over as two 16-bit planes (16 bytes an element), squares of 4 bytes an element: two
+    where steps are taken one by one (float32), seven in stages; and up to eight float32 shares of a product."""
+    lib = N.lib()
+    for code, m, n, squares in ((0, 4096, 4096, 2), (2, 4096, 4096, 7), (0, 1024, 4096, 2), (0, 64, 4096, 2)):
+        shares = 0 if m == n else 8  # (a square of this size fills the chip)
+        room = 16 * m * n + 4 * m * m * (squares + shares) + 64 * 16 * (m + n)  # (and the rows' padding)
+        assert lib.smq_orthogonalize_workspace_bytes(code, 1, m, n) <= room
