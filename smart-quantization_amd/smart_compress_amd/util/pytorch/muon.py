@@ -18,6 +18,18 @@ from ... import _native as N
 __all__ = ["Muon", "orthogonalize"]
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+STACK_BYTES = 1 << 30  # workspace of one of Muon's calls: a few matrices of 4096 x 4096 fill the chip
+STACK_LIMIT = 65535  # matrices of one call
+
+
+def _stack_of(dtype: torch.dtype, rows: int, cols: int) -> int:
+    """How many matrices of this shape go into one call."""
+    if rows == 0 or cols == 0:
+        return STACK_LIMIT
+    each = N.lib().smq_orthogonalize_workspace_bytes(N.DTYPE_CODES[dtype], 1, rows, cols)
+    if each == 0:
+        N.check(-1, "Muon")
+    return max(1, min(STACK_LIMIT, STACK_BYTES // each))
 
 
 def orthogonalize(update: torch.Tensor, steps: int = 5,
@@ -68,7 +80,7 @@ class Muon(Optimizer):
     ``nesterov``, ``momentum m + (1 - momentum) g``, and ``p <- (1 - lr weight_decay) p
     - lr sqrt(max(1, rows / cols)) orthogonalize(update)``. A parameter of more than two dimensions (a
     convolution's weight) counts as the matrix [first, rest]. Parameters of one shape are
-    orthogonalised in one call."""
+    orthogonalised in one call, as many as 1 GiB of workspace (or one matrix) allows."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, steps: int = 5,
@@ -103,8 +115,11 @@ class Muon(Optimizer):
                 if p.grad.is_sparse:
                     raise RuntimeError("Muon: sparse gradients are not supported")
                 stacks.setdefault((p.shape, p.dtype, p.device), []).append(p)
-            for ps in stacks.values():
-                self._step_stack(group, ps)
+            for (shape, dtype, _), ps in stacks.items():
+                rows = shape[0]
+                most = _stack_of(dtype, rows, shape.numel() // max(rows, 1))
+                for k in range(0, len(ps), most):
+                    self._step_stack(group, ps[k:k + most])
         return loss
 
     def _step_stack(self, group, ps: List[torch.Tensor]):

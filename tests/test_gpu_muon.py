@@ -304,3 +304,35 @@ def test_16_bit_results_round_once(dtype):
             over = ((got - want).abs() - half).clamp(min=0).norm() / want.norm()
             print(name, k, over.item(), flush=True)
             assert over <= 4 * tight(max(x.shape[-2:])), (name, over)
+
+
+def test_muon_in_several_calls(monkeypatch):
+    """A stack over the workspace's budget steps as its parts do alone."""
+    from smart_compress_amd.util.pytorch import muon
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    start = [torch.randn(96, 160, generator=g, device="cuda") for _ in range(7)]
+    grads = [torch.randn(96, 160, generator=g, device="cuda") for _ in range(7)]
+    got, real = [], orthogonalize
+    for budget, whole in ((muon.STACK_BYTES, True), (3 << 20, False)):
+        monkeypatch.setattr(muon, "STACK_BYTES", budget)
+        ps = [torch.nn.Parameter(x.clone()) for x in start]
+        opt = Muon(ps, lr=0.1, weight_decay=0.1)
+        for p, x in zip(ps, grads):
+            p.grad = x.clone()
+        calls = []
+        monkeypatch.setattr(muon, "orthogonalize", lambda x, *a: (calls.append(len(x)), real(x, *a))[1])
+        opt.step()
+        assert sum(calls) == 7 and (len(calls) > 1) != whole
+        got.append([p.detach() for p in ps])
+        if not whole:  # the same bits as the parts stepped by optimizers of their own
+            at = 0
+            for n in list(calls):
+                qs = [torch.nn.Parameter(x.clone()) for x in start[at:at + n]]
+                for q, x in zip(qs, grads[at:at + n]):
+                    q.grad = x.clone()
+                Muon(qs, lr=0.1, weight_decay=0.1).step()
+                assert all(torch.equal(a, q.detach()) for a, q in zip(got[1][at:at + n], qs))
+                at += n
+    for a, c in zip(*got):
+        assert (a - c).norm() <= 0.1 * 2 * tight(160) * 96 ** 0.5 + 2.0 ** -23 * c.norm()

@@ -204,3 +204,25 @@ def test_orthogonalize_workspace_is_what_a_call_uses():
         shares = 0 if m == n else 8  # (a square of this size fills the chip)
         room = 16 * m * n + 4 * m * m * (squares + shares) + 64 * 16 * (m + n)  # (and the rows' padding)
         assert lib.smq_orthogonalize_workspace_bytes(code, 1, m, n) <= room
+
+
+def test_muon_bounds_its_stacks(monkeypatch):
+    """Parameters of one shape go in as many calls as 1 GiB of workspace each takes."""
+    from smart_compress_amd.util.pytorch import muon
+
+    calls = []
+    monkeypatch.setattr(muon, "orthogonalize", lambda x, *a: (calls.append(tuple(x.shape)), x)[1])
+    ps = [torch.nn.Parameter(torch.zeros(1024, 2048)) for _ in range(45)]
+    ps += [torch.nn.Parameter(torch.zeros(3, 0, 5)), torch.nn.Parameter(torch.zeros(3, 4))]
+    for k, p in enumerate(ps):
+        p.grad = torch.full_like(p, k + 1.0)
+    Muon(ps, lr=1.0, momentum=0.0).step()
+    assert [c[1:] for c in calls] == [(1024, 2048)] * (len(calls) - 2) + [(3, 0), (3, 4)]
+    assert sum(c[0] for c in calls[:-2]) == 45
+    for batch, rows, cols in calls[:-2]:
+        assert N.lib().smq_orthogonalize_workspace_bytes(0, batch, rows, cols) <= 1 << 30
+    assert len(calls) - 2 <= 2
+    for k, p in enumerate(ps[:45]):
+        assert (p == -(k + 1.0)).all()
+    big = muon._stack_of(torch.float32, 16384, 16384)
+    assert big == 1
