@@ -15,6 +15,8 @@
 //              deviations from them (no cancellation against a large mean), joined in fp64.
 // A thread owns V adjacent channels (16 bytes where the channel count allows) and walks rows, so its
 // parameters stay in registers. No atomics: the sums have a fixed order.
+#include <limits.h>
+
 #include "smq_common.h"
 
 namespace smq {
@@ -721,8 +723,26 @@ size_t align_up(size_t b) { return (b + 255) & ~size_t(255); }
 #define SMQ_GN_STREAM(T, V, KERNEL, UNUSED) \
   hipLaunchKernelGGL((KERNEL<T, V>), grid, dim3(256), 0, st, A)
 
+// f(part of the samples): a launch takes at most kSamples of them (its grid's limit).
+constexpr int kSamples = 65535;
+template <typename T, typename F>
+void by_samples(const Args& all, F f) {
+  for (int n0 = 0; n0 < all.n; n0 += kSamples) {
+    Args A = all;
+    const int64_t at = (int64_t)n0 * A.s * A.c, g = (int64_t)n0 * A.groups;
+    A.n = all.n - n0 < kSamples ? all.n - n0 : kSamples;
+    A.x = reinterpret_cast<const T*>(A.x) + at;
+    if (A.dy) A.dy = reinterpret_cast<const T*>(A.dy) + at;
+    A.y = reinterpret_cast<T*>(A.y) + at;
+    A.mean += g, A.rstd += g;
+    A.part += (int64_t)n0 * A.chunks * A.c, A.coef += g, A.chan += (int64_t)n0 * A.c;
+    f(A);
+    if (all.n - n0 <= kSamples) return;
+  }
+}
+
 template <typename T>
-void forward(Args& A, const Plan& p, hipStream_t st) {
+void forward(const Args& A, const Plan& p, hipStream_t st) {
   if (p.r) {
     const size_t lds = (size_t)(p.threads * p.v + 2 * (p.block / A.cg)) * 4;
     SMQ_GN_V(T, SMQ_GN_RES, resident_forward, lds);
@@ -735,7 +755,7 @@ void forward(Args& A, const Plan& p, hipStream_t st) {
 }
 
 template <typename T>
-void backward(Args& A, const Plan& p, float* dweight, float* dbias, hipStream_t st) {
+void backward(const Args& A, const Plan& p, hipStream_t st) {
   if (p.r) {
     const size_t lds = (size_t)(p.threads * p.v + 2 * (p.block / A.cg)) * 4;
     SMQ_GN_V(T, SMQ_GN_RES, resident_backward, lds);
@@ -745,8 +765,6 @@ void backward(Args& A, const Plan& p, float* dweight, float* dbias, hipStream_t 
     hipLaunchKernelGGL(join_sums, dim3(A.groups, (unsigned)A.n), dim3(256), 0, st, A);
     SMQ_GN_V(T, SMQ_GN_STREAM, stream_backward, 0);
   }
-  if (dweight || dbias)
-    hipLaunchKernelGGL(param_sums, dim3((A.c + 63) / 64), dim3(1024), 0, st, A.chan, A.n, A.c, dweight, dbias);
 }
 
 int validate(const char* who, int dtype, int64_t n, int64_t s, int64_t c, int64_t groups, int act) {
@@ -754,8 +772,8 @@ int validate(const char* who, int dtype, int64_t n, int64_t s, int64_t c, int64_
     set_error("%s: dtype %d is not one of SMQ_DTYPE_F32/F16/BF16", who, dtype);
     return SMQ_ERR_INVALID;
   }
-  if (n < 1 || s < 1 || c < 1 || n > 65535 || c > (1 << 20) || s > ((int64_t)1 << 40) / c) {
-    set_error("%s: needs 1 <= n <= 65535, 1 <= channels <= 2^20, 1 <= positions * channels <= 2^40, got "
+  if (n < 1 || s < 1 || c < 1 || n > INT_MAX || c > (1 << 20) || s > ((int64_t)1 << 40) / c) {
+    set_error("%s: needs 1 <= n < 2^31, 1 <= channels <= 2^20, 1 <= positions * channels <= 2^40, got "
               "%lld, %lld, %lld", who, (long long)n, (long long)c, (long long)s);
     return SMQ_ERR_INVALID;
   }
@@ -829,9 +847,12 @@ int smq_group_norm_act(const void* x, int dtype, void* y, int64_t n, int64_t pos
   A.s = positions, A.n = (int)n, A.c = c, A.groups = (int)groups, A.cg = cg;
   A.block = p.block, A.chunks = p.chunks, A.act = activation, A.eps = (float)eps;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == SMQ_DTYPE_F32) gn::forward<float>(A, p, st);
-  else if (dtype == SMQ_DTYPE_F16) gn::forward<_Float16>(A, p, st);
-  else gn::forward<__bf16>(A, p, st);
+  auto go = [&](auto t) {
+    by_samples<decltype(t)>(A, [&](const Args& part) { gn::forward<decltype(t)>(part, p, st); });
+  };
+  if (dtype == SMQ_DTYPE_F32) go(0.0f);
+  else if (dtype == SMQ_DTYPE_F16) go((_Float16)0);
+  else go((__bf16)0.0f);
   return check_launch("group_norm_act");
 }
 
@@ -861,9 +882,14 @@ int smq_group_norm_act_backward(const void* x, const void* dy, int dtype, void* 
   A.s = positions, A.n = (int)n, A.c = c, A.groups = (int)groups, A.cg = cg;
   A.block = p.block, A.chunks = p.chunks, A.act = activation;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == SMQ_DTYPE_F32) gn::backward<float>(A, p, dweight, dbias, st);
-  else if (dtype == SMQ_DTYPE_F16) gn::backward<_Float16>(A, p, dweight, dbias, st);
-  else gn::backward<__bf16>(A, p, dweight, dbias, st);
+  auto go = [&](auto t) {
+    by_samples<decltype(t)>(A, [&](const Args& part) { gn::backward<decltype(t)>(part, p, st); });
+  };
+  if (dtype == SMQ_DTYPE_F32) go(0.0f);
+  else if (dtype == SMQ_DTYPE_F16) go((_Float16)0);
+  else go((__bf16)0.0f);
+  if (dweight || dbias)
+    hipLaunchKernelGGL(param_sums, dim3((c + 63) / 64), dim3(1024), 0, st, A.chan, A.n, c, dweight, dbias);
   return check_launch("group_norm_act_backward");
 }
 

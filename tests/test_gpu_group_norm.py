@@ -297,3 +297,19 @@ def test_result_can_be_changed_in_place(shape, binding, monkeypatch):
             y = torch.relu((y + x) * 2.0)
         got.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
     assert all(torch.equal(a, c) for a, c in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups", [((65535, 8), 2), ((65536, 8), 4), ((100001, 24), 6), ((66000, 3, 5), 1),
+                                          ((70000, 4, 120), 2), ((65600, 1031), 1)])
+def test_more_samples_than_a_grid_has(shape, groups, dtype):
+    x, dy, w, b = make(shape, dtype, seed=51)
+    want, bound, _, grads, bounds = reference(x, groups, w, b, 1e-5, "silu", dy)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = group_norm_act(leaves[0], groups, leaves[1], leaves[2], 1e-5, "silu")
+    got = torch.autograd.grad(y, leaves, dy)
+    close(y, want, bound, dtype)
+    for g, e, t, d in zip(got, grads, bounds, (dtype, torch.float32, torch.float32)):
+        close(g, e, t, d)
+    half = group_norm_act(x[-7:], groups, w, b, 1e-5, "silu")
+    assert torch.equal(half, y[-7:])
