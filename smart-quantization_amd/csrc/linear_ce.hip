@@ -1208,6 +1208,12 @@ size_t smq_linear_ce_workspace_bytes(const void* hidden, int64_t hidden_ld, cons
   if (validate("linear_ce_workspace_bytes", hidden, hidden_ld, weight, weight_ld, dtype, &none, tokens,
                dim, vocab, SMQ_REDUCE_SUM) != SMQ_OK)
     return 0;
+  const int all = SMQ_CE_GRAD_HIDDEN | SMQ_CE_GRAD_WEIGHT | SMQ_CE_GRAD_BIAS;
+  if (piece < 0 || piece > (1 << 20) || (grad_flags & ~all)) {
+    set_error("linear_ce_workspace_bytes: needs 0 <= piece <= 2^20 and flags of SMQ_CE_GRAD_*, got %lld, %d",
+              (long long)piece, grad_flags);
+    return 0;
+  }
   const Shape s = {tokens, dim, vocab, piece, dtype};
   Head* head = nullptr;
   if (!grad_flags)

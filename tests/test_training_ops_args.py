@@ -226,3 +226,13 @@ def test_muon_bounds_its_stacks(monkeypatch):
         assert (p == -(k + 1.0)).all()
     big = muon._stack_of(torch.float32, 16384, 16384)
     assert big == 1
+
+
+def test_cross_entropy_workspace_query_refuses_what_the_backward_does():
+    lib = N.lib()
+    one = ctypes.c_int(0)
+    p = ctypes.addressof(one)
+    for piece, flags, ok in ((0, 0, True), (0, 7, True), (1 << 20, 1, True), (-1, 1, False),
+                             ((1 << 20) + 1, 1, False), (0, 8, False), (0, -1, False)):
+        assert (lib.smq_linear_ce_workspace_bytes(p, 64, p, 64, 0, 4, 64, 9, piece, flags) > 0) == ok
+    assert "piece" in err()
