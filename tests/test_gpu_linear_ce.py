@@ -649,3 +649,21 @@ def test_bad_targets_under_a_zero_gradient(tokens, dim, vocab, ignored, dtype):
     assert torch.equal(torch.isnan(loss), bad)
     assert torch.isnan(dh[bad]).all() and torch.isfinite(dh[~bad]).all()
     assert torch.isnan(dw).all() and torch.isnan(db).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,dim,vocab", [(9, 64, 400), (70, 36, 400), (70, 64, 400), (200, 64, 400), GATHERED])
+def test_ignored_rows_change_no_bit(tokens, dim, vocab, dtype):
+    """NaN, infinities and zeros in ignored rows: the loss and all gradients are those of the clean call."""
+    h, w, b, t = make(tokens, dim, vocab, dtype, True, 0.4, seed=36)
+    rows = torch.nonzero(t == -100).view(-1)
+    assert len(rows) > 2
+    dirty = h.clone()
+    dirty[rows[0]], dirty[rows[1]], dirty[rows[2:]] = float("nan"), float("inf"), 0.0
+    got = []
+    for x in (h, dirty):
+        leaves = [y.detach().requires_grad_() for y in (x, w, b)]
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+        got.append((loss, *torch.autograd.grad(loss, leaves, torch.tensor(-1.7, device="cuda"))))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    assert (got[1][1][rows] == 0).all() and torch.isfinite(got[1][0])
