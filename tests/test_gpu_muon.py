@@ -336,3 +336,26 @@ def test_muon_in_several_calls(monkeypatch):
                 at += n
     for a, c in zip(*got):
         assert (a - c).norm() <= 0.1 * 2 * tight(160) * 96 ** 0.5 + 2.0 ** -23 * c.norm()
+
+
+def test_float32_is_float32_class():
+    """Within tight(), twice that where singular values spread over 1000 (their small ones grow by more). One
+    plane of 2^-11 in place of two would be 1e-3 to 6e-3 off, a lost cross term 1e-3 to 2e-3."""
+    for name, x in shapes():
+        y = orthogonalize(x.float().cuda())
+        for k in (0, len(x) - 1):
+            want = reference(x[k].float())
+            off = ((y[k].double().cpu() - want).norm() / want.norm()).item()
+            print(name, k, off, flush=True)
+            assert off <= (2 if name == "ratio1000" else 1) * tight(max(x.shape[-2:])), (name, off)
+
+
+def test_float32_of_a_convolution_and_an_odd_matrix():
+    g = torch.Generator().manual_seed(6)
+    for m, n in ((512, 4608), (97, 161)):
+        low = torch.randn(m, m // 16, generator=g) @ torch.randn(m // 16, n, generator=g)
+        x = (low * (m // 16) ** -0.5 + 0.5 * torch.randn(m, n, generator=g)) * 1e-3
+        want = reference(x)
+        off = ((orthogonalize(x.cuda()).double().cpu() - want).norm() / want.norm()).item()
+        print(m, n, off, flush=True)
+        assert off <= tight(n)
