@@ -359,3 +359,19 @@ def test_float32_of_a_convolution_and_an_odd_matrix():
         off = ((orthogonalize(x.cuda()).double().cpu() - want).norm() / want.norm()).item()
         print(m, n, off, flush=True)
         assert off <= tight(n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 8, 9, 13])
+def test_every_number_of_steps(steps, dtype):
+    """Stages of three steps end on each remainder, in the one-workgroup kernel (up to 8 steps) and in launches;
+    each step past the fifth lets an error grow by 1.5 at most."""
+    bits, lowest = {torch.float32: (24, -126), torch.float16: (11, -14), torch.bfloat16: (8, -126)}[dtype]
+    for m, n in ((32, 64), (64, 48), (97, 161), (300, 320)):
+        x = matrix(2, m, n, 4.0, seed=steps).to(dtype)
+        y = orthogonalize(x.cuda(), steps=steps).double().cpu()
+        want = reference(x, steps=steps)
+        half = torch.ldexp(torch.ones_like(y), torch.frexp(y)[1].clamp(min=lowest + 1) - bits - 1)
+        over = ((y - want).abs() - half).clamp(min=0).norm() / want.norm()
+        print(m, n, over.item(), flush=True)
+        assert over <= (1 if dtype == torch.float32 else 4) * tight(max(m, n)) * 1.5 ** max(0, steps - 5)
