@@ -21,6 +21,7 @@
 // inputs are exact in one plane, so the first stage reads one plane of them. (One plane of each operand in the
 // last P X of bf16 results would save 80 us of 1156 at 6 x 1024 x 4096 and be 0.03 - 0.3 % off, against
 // the 0.17 % of the result's own rounding.)
+#include <limits.h>
 #include <math.h>
 
 #include "gemm_nt.h"
@@ -676,6 +677,16 @@ size_t enqueue(const Plan& p, const void* g, int64_t ld, int64_t stride, void* y
 }
 
 constexpr double kMostGrowth = 256.0;
+constexpr int64_t kStack = 65535;  // matrices of one walk through the launches (a grid's limit)
+// f(plan of a part of the stack, its first matrix): deeper stacks go part by part through one workspace.
+template <typename F>
+void by_stacks(const Plan& all, F f) {
+  for (int64_t b = 0; b < all.batch; b += kStack) {
+    Plan p = all;
+    p.batch = all.batch - b < kStack ? all.batch - b : kStack;
+    f(p, b);
+  }
+}
 
 int plan(const char* who, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps,
          const double* coefficients, Plan* p) {
@@ -683,8 +694,8 @@ int plan(const char* who, int dtype, int64_t batch, int64_t rows, int64_t cols, 
     set_error("%s: dtype %d is not one of SMQ_DTYPE_F32/F16/BF16", who, dtype);
     return SMQ_ERR_INVALID;
   }
-  if (batch < 1 || batch > 65535 || rows < 1 || cols < 1 || rows > (1 << 20) || cols > (1 << 20)) {
-    set_error("%s: needs 1 <= batch <= 65535 and 1 <= rows, cols <= 2^20, got %lld, %lld, %lld", who,
+  if (batch < 1 || batch > INT_MAX || rows < 1 || cols < 1 || rows > (1 << 20) || cols > (1 << 20)) {
+    set_error("%s: needs 1 <= batch < 2^31 and 1 <= rows, cols <= 2^20, got %lld, %lld, %lld", who,
               (long long)batch, (long long)rows, (long long)cols);
     return SMQ_ERR_INVALID;
   }
@@ -717,7 +728,14 @@ size_t smq_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t rows,
   const double c[3] = {1.0, 0.0, 0.0};
   Plan p;
   if (plan("orthogonalize_workspace_bytes", dtype, batch, rows, cols, 1, c, &p) != SMQ_OK) return 0;
-  return enqueue(p, nullptr, 0, 0, nullptr, 0.0, nullptr, false, nullptr) + 256;
+  size_t most = 0;
+  by_stacks(p, [&](const Plan& part, int64_t) {
+    if (part.batch < kStack || most == 0) {  // (full parts are alike)
+      const size_t need = enqueue(part, nullptr, 0, 0, nullptr, 0.0, nullptr, false, nullptr);
+      most = need > most ? need : most;
+    }
+  });
+  return most + 256;
 }
 
 int smq_orthogonalize(const void* x, int64_t ld, int64_t batch_stride, int dtype, void* y,
@@ -736,7 +754,12 @@ int smq_orthogonalize(const void* x, int64_t ld, int64_t batch_stride, int dtype
     set_error("orthogonalize: workspace: need %zu bytes on a 16-byte boundary, got %zu", need, workspace_bytes);
     return SMQ_ERR_WORKSPACE;
   }
-  enqueue(p, x, ld, batch_stride, y, eps, workspace, true, reinterpret_cast<hipStream_t>(stream));
+  const int64_t size = dtype == SMQ_DTYPE_F32 ? 4 : 2;
+  by_stacks(p, [&](const Plan& part, int64_t b) {
+    enqueue(part, reinterpret_cast<const char*>(x) + b * batch_stride * size, ld, batch_stride,
+            reinterpret_cast<char*>(y) + b * rows * cols * size, eps, workspace, true,
+            reinterpret_cast<hipStream_t>(stream));
+  });
   return check_launch("orthogonalize");
 }
 

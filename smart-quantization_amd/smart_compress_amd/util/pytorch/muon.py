@@ -19,17 +19,16 @@ __all__ = ["Muon", "orthogonalize"]
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 STACK_BYTES = 1 << 30  # workspace of one of Muon's calls: a few matrices of 4096 x 4096 fill the chip
-STACK_LIMIT = 65535  # matrices of one call
 
 
 def _stack_of(dtype: torch.dtype, rows: int, cols: int) -> int:
     """How many matrices of this shape go into one call."""
     if rows == 0 or cols == 0:
-        return STACK_LIMIT
+        return 1 << 30
     each = N.lib().smq_orthogonalize_workspace_bytes(N.DTYPE_CODES[dtype], 1, rows, cols)
     if each == 0:
         N.check(-1, "Muon")
-    return max(1, min(STACK_LIMIT, STACK_BYTES // each))
+    return max(1, STACK_BYTES // each)
 
 
 def orthogonalize(update: torch.Tensor, steps: int = 5,

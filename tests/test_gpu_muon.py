@@ -375,3 +375,18 @@ def test_every_number_of_steps(steps, dtype):
         over = ((y - want).abs() - half).clamp(min=0).norm() / want.norm()
         print(m, n, over.item(), flush=True)
         assert over <= (1 if dtype == torch.float32 else 4) * tight(max(m, n)) * 1.5 ** max(0, steps - 5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch,m,n", [(65535, 3, 5), (65536, 8, 6), (131075, 4, 4), (65600, 70, 66)])
+def test_stacks_beyond_a_grid(batch, m, n, dtype):
+    """More matrices than a grid's third dimension holds: each end of each part is what it is in a stack of its
+    own part's kind."""
+    g = torch.Generator(device="cuda").manual_seed(batch)
+    x = torch.randn(batch, m, n, generator=g, device="cuda", dtype=torch.float32).to(dtype)
+    y = orthogonalize(x)
+    assert torch.isfinite(y.float()).all()
+    for k in (0, 1, 65533, 65534, 65535, batch - 2, batch - 1):
+        if k < batch:
+            want, got = reference(x[k]), y[k].double().cpu()
+            assert (got - want).norm() / want.norm() <= 8 * tight(n) + torch.finfo(dtype).eps / 2, k
