@@ -698,7 +698,10 @@ int smq_cpu_smaq_decompress_f64(const void* packed, double* y, int64_t n, int n_
  * ignore_index have loss and gradient 0, whatever they hold; any other target outside [0, vocab) makes
  * its loss and gradient NaN. loss: one fp32 (mean over the rows taking part, NaN if there are none;
  * sum) or [tokens] (none); grad_loss the same shape. Gradients are written whole, in the inputs' dtype
- * (grad_bias fp32), rows packed; a NULL gradient is not computed. */
+ * (grad_bias fp32), rows packed; a NULL gradient is not computed. A row's loss and grad_hidden are as
+ * exact as if it were alone. float32 holds an element to 2^-38 of its row's largest, and in the sums of
+ * the gradients a term 2^-k of the largest row's to 2^(k / 2 - 38) of its own; for 16-bit types the
+ * gradient of the logits rounds to fp16 before those sums (beyond 16 tokens). */
 #define SMQ_REDUCE_NONE 0
 #define SMQ_REDUCE_MEAN 1
 #define SMQ_REDUCE_SUM 2
@@ -746,7 +749,8 @@ int smq_group_norm_act_backward(const void* x, const void* dy, int dtype, void* 
  *   X = x / (|x|_F + eps); steps times: A = X X^T, B = b A + c A A, X = a X + B X   (rows <= cols; else x^T)
  * into y [batch, rows, cols], packed, same dtype. x has unit column stride, row pitch ld and
  * batch_stride between matrices (elements); it may not overlap y. coefficients = {a, b, c} must keep
- * the singular values (at most 1 at the start) below 256 through all steps. */
+ * the singular values (at most 1 at the start) below 256 through all steps. float32-class in every
+ * type before the result's own rounding. */
 size_t smq_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);
 int smq_orthogonalize(const void* x, int64_t ld, int64_t batch_stride, int dtype, void* y,
                       int64_t batch, int64_t rows, int64_t cols, int steps,

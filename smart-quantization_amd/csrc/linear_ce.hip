@@ -13,10 +13,10 @@
 //   up to 16 tokens        no matrix cores: the weight is read as it is, once in the forward and twice in the
 //                          backward (1 x 768 x 30000 float32 forward: 23 us, 18 at the rate of a copy)
 //   float32, to 128        the logits on the fp32 matrix instructions from the inputs in place, where their rows
-//                          allow (64 x 1024 x 30000: forward 47 us, both directions 267)
+//                          allow (64 x 1024 x 30000: forward 47 us, both directions 275)
 //   the rest               16-bit matrix products; long ones over the rows that take part only (Kept).
 // Measured, forward and backward: 8192 x 4096 x 131072 bf16 33.5 ms (8 N V D operations with the logits'
-// second computation: 1050 TFLOP/s), 2048 x 768 x 30000 float32 1.29 ms, 777 x 1001 x 50001 fp16 with a third
+// second computation: 1050 TFLOP/s), 2048 x 768 x 30000 float32 1.32 ms, 777 x 1001 x 50001 fp16 with a third
 // of the rows ignored 0.63 ms. What bounds the large ones is the product itself, then dl's two copies.
 //
 // float32 inputs run as two fp16 planes (gemm_nt.h), in the logits each row scaled by a power of two of its
@@ -29,7 +29,8 @@
 // copy for dh, whose epilogue takes it: a row of dh is as exact as if it were alone. The sum over the rows in dw
 // has one scale, that of the largest |g| |h| of a row; a row 2^-k of it (float32, bf16) has half of k taken off
 // dl's transposed copy and half off h's, so that both stay in fp16's range (Row); dh's sum over float32 entries the
-// same of the largest |w|.
+// same of the largest |w|. A term 2^-k of the largest is off by 2^(k / 2 - 38) of its own two factors' largest
+// elements (float32); the row exponents cost one read more of the weight in each direction than one for all.
 #include <limits.h>
 
 #include <type_traits>
@@ -889,8 +890,9 @@ int validate(const char* who, const void* h, int64_t ldh, const void* w, int64_t
 
 // float32 logits of up to 128 tokens, where both tensors are operands as they are: on the fp32 matrix
 // instructions straight from them. Making planes of the weight moves it three times more; with more tokens
-// the planes' fivefold rate pays for that (64 x 1024 x 30000: 272 us a step against 330 with planes, 256
-// tokens about even, 130 x 484 x 48351, whose rows would have to be copied, 573 against 411).
+// the planes' fivefold rate pays for that (64 x 1024 x 30000: 275 us a step against 370 with planes, 128 tokens 363
+// against 417, 256 tokens 520 against 488; 130 x 484 x 48351, whose rows would have to be copied, was 573 with
+// the copies, 404 with planes).
 bool in_place32(const void* p, int64_t ld, int64_t cols) {
   return cols % 32 == 0 && ld % 4 == 0 && ld <= (1 << 20) && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
@@ -899,9 +901,9 @@ bool raw32(const void* h, int64_t ldh, const void* w, int64_t ldw, const Shape& 
 }
 // Whether the rows that take part are gathered: where a product is long against the copy of h (which float32
 // makes anyway) and the launch that finds them. Training, none / 15 % / 40 % ignored, gathered against not:
-// float32 512 x 768 x 30000 499 / 471 / 441 us against 491 / 488 / 484 (256 tokens 382 / 357 / 341, 375 /
-// 365 / 366), fp16 1024 x 1024 x 32000 478 / 447 / 392 against 466 / 464 / 461 (768 x 30000 383 / 360 / 328,
-// 365 / 362 / 361), fp16 2048 x 1024 x 50000 1300 / 1122 / 893 against 1282 / 1278 / 1271.
+// float32 512 x 768 x 30000 526 / 507 / 466 us against 518 / 513 / 504 (256 tokens 396 / 386 / 366, 387 /
+// 390 / 388), fp16 1024 x 1024 x 32000 492 / 455 / 403 against 476 / 474 / 472 (768 x 30000 390 / 366 / 327,
+// 376 / 373 / 372), fp16 2048 x 1024 x 50000 1323 / 1156 / 907 against 1310 / 1306 / 1298.
 bool gathered(const Shape& s) {
   return s.tokens > 128 && s.tokens * s.vocab >= ((int64_t)1 << (s.split() ? 33 : 35)) / s.dim;
 }

@@ -15,12 +15,13 @@
 // Rounding. Between products a matrix is held as two fp16 planes (23 bits) at a power-of-two scale that
 // keeps it in range (the host bounds the singular values step by step). One plane would be off by 0.15 %
 // on Gaussian matrices and by 1-4 % where a few strong directions hide the rest. A stage squares the
-// ratio of the singular values once more for each step behind its first: five steps measured 0.9 - 2.5e-6
-// off as single steps, 1.1 - 5.6e-6 as 2 + 2 + 1, 2 - 5e-6 as 3 + 2 (plain float32 products 0.6 - 3.4e-6).
-// float32 takes single steps; the 16-bit types, whose results round to 2^-11 and 2^-8, stages of 3. 16-bit
-// inputs are exact in one plane, so the first stage reads one plane of them. (One plane of each operand in the
-// last P X of bf16 results would save 80 us of 1156 at 6 x 1024 x 4096 and be 0.03 - 0.3 % off, against
-// the 0.17 % of the result's own rounding.)
+// ratio of the singular values once more for each step behind its first: five steps of nine float32 matrices
+// (48 x 80 to 1024 x 1536, ratios 4 to 1000) measured 0.7 - 1.4e-6 off as single steps, 3.2e-6 at ratio 1000;
+// 1.3 - 2.7e-6 as 2 + 2 + 1, 1.7 - 3.8e-6 as 3 + 2; plain float32 products 1.0 - 3.3e-6. float32 takes single
+// steps; the 16-bit types, whose results round to 2^-11 and 2^-8, stages of 3. 16-bit inputs are exact in one
+// plane, so the first stage reads one plane of them. (One plane of each operand in the last P X of bf16 results
+// would save 80 us of 1150 at 6 x 1024 x 4096 and be 0.03 - 0.3 % off, against the 0.17 % of the result's own
+// rounding.)
 #include <limits.h>
 #include <math.h>
 

@@ -36,9 +36,9 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     """``steps`` times ``A = X X^T; X = a X + (b A + c A A) X`` from ``X = update / (norm + eps)``,
     for a matrix [rows, cols] or a stack [batch, rows, cols] of them (float32, float16 or bfloat16,
     any strides, on a ROCm device); the result has the update's shape and dtype, contiguous. A matrix
-    with more rows than columns is worked on transposed. Accuracy: float32-class for float32 and
-    float16; for bfloat16 about the result's own rounding. ``coefficients`` have to keep singular
-    values that start at or below 1 bounded (below 256). Not differentiable."""
+    with more rows than columns is worked on transposed. Accuracy: float32-class in every type, then
+    rounded to it. ``coefficients`` have to keep singular values that start at or below 1 bounded
+    (below 256). Not differentiable."""
     who = "orthogonalize"
     N.require_device(update, who)
     if update.dtype not in N.DTYPE_CODES:

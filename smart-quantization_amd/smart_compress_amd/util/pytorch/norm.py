@@ -113,8 +113,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     ROCm device), with ``weight`` / ``bias`` [channels] in any of these dtypes and ``activation`` one
     of "none", "relu", "silu", "gelu" (the exact one). Channels-last memory is used as it is, other
     layouts are copied into it first; the result, of ``x``'s dtype, and ``x``'s gradient are channels
-    last. Statistics and the parameters' gradients are computed in float32 or wider; a group's single value normalises to 0.
-    No second derivative."""
+    last. Statistics and the parameters' gradients are computed in float32 or wider; a group's single
+    value normalises to 0. No second derivative."""
     who = "group_norm_act"
     params = [t for t in (weight, bias) if t is not None]
     device = x.device
