@@ -699,8 +699,9 @@ int smq_cpu_smaq_decompress_f64(const void* packed, double* y, int64_t n, int n_
  * its loss and gradient NaN. loss: one fp32 (mean over the rows taking part, NaN if there are none;
  * sum) or [tokens] (none); grad_loss the same shape. Gradients are written whole, in the inputs' dtype
  * (grad_bias fp32), rows packed; a NULL gradient is not computed. A row's loss and grad_hidden are as
- * exact as if it were alone. float32 holds an element to 2^-38 of its row's largest, and in the sums of
- * the gradients a term 2^-k of the largest row's to 2^(k / 2 - 38) of its own; for 16-bit types the
+ * exact as if it were alone. float32 holds an element to 2^-38 of its row's largest in the logits; in the
+ * sums of the gradients one of a row 2^-k of the largest to 2^-24 of its row's largest and its
+ * probability to 2^-38 (2^(k - 53) past k = 15), past k = 30 both to 2^(k / 2 - 38); for 16-bit types the
  * gradient of the logits rounds to fp16 before those sums (beyond 16 tokens). */
 #define SMQ_REDUCE_NONE 0
 #define SMQ_REDUCE_MEAN 1

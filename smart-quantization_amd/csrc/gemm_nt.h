@@ -767,12 +767,16 @@ static inline void launch(int tile, const Operand& A, const Operand& B, int kt, 
   }
 }
 
-// In a sum whose largest terms have scale 2^0 a term of 2^-k has this part of k taken off one of its factors and
-// the rest off the other, so that both stay in fp16's range. (Past 100 both are 0 there; the other factor's part
-// stays a normal float.)
-__device__ __forceinline__ int half_of(int k) { return k > 100 ? k - 50 : k >> 1; }
+// In a sum whose largest terms have scale 2^0 a term of 2^-k is the product of a factor (of the tensor's row, whose
+// largest element is at 2^14) and a probability (at 2^14 and far below): this part of k comes off the factor's
+// fp16 planes, the rest off the probability's, so that both stay in fp16's range. The factor keeps 2^-24 of its
+// row's largest for the first 15, and only then the probability loses from its end, 2^-39; past 30 they share.
+// (Past 100 both are 0 in fp16; the probability's part stays a normal float.)
+__device__ __forceinline__ int share_of(int k) {
+  return k > 100 ? k - 50 : k > 30 ? k >> 1 : k > 15 ? 15 : k;
+}
 // Power-of-two exponents of a matrix' rows: e[step * r] (step 0: *e for all of them); e NULL: 0. With `least`, the
-// smallest of them, half of the difference comes off.
+// smallest of them, their share of the difference comes off.
 struct Exponents {
   const int* e = nullptr;
   int step = 0;
@@ -781,7 +785,7 @@ struct Exponents {
   __device__ __forceinline__ int at(int r) const {
     if (!step) return all();
     const int v = e[step * r];
-    return least ? v - half_of(v - *least) : v;
+    return least ? v - share_of(v - *least) : v;
   }
 };
 // Layout pass: src [rows, cols] of type T, row pitch ld, times *factor (NULL: 1), to `d` row by row, times

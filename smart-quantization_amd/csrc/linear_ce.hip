@@ -27,10 +27,10 @@
 // that these products need anyway. dl is kept times 2^14, so that fp16 holds probabilities from 4e-9 up in
 // full precision, and the powers of two come off in the fp32 epilogues. A row's gradient g stays out of dl's
 // copy for dh, whose epilogue takes it: a row of dh is as exact as if it were alone. The sum over the rows in dw
-// has one scale, that of the largest |g| |h| of a row; a row 2^-k of it (float32, bf16) has half of k taken off
-// dl's transposed copy and half off h's, so that both stay in fp16's range (Row); dh's sum over float32 entries the
-// same of the largest |w|. A term 2^-k of the largest is off by 2^(k / 2 - 38) of its own two factors' largest
-// elements (float32); the row exponents cost one read more of the weight in each direction than one for all.
+// has one scale, that of the largest |g| |h| of a row; a row 2^-k of it (float32, bf16) has k taken off h's
+// transposed copy and dl's, shared so that both stay in fp16's range (share_of, Row); dh's sum over float32 entries
+// the same of the largest |w|. float32: h and w to 2^-24 of their row's largest and p to 2^-38 up to k = 15, p to
+// 2^(k - 53) up to k = 30, both to 2^(k / 2 - 38) beyond; the row exponents cost one read more of the weight in each direction than one for all.
 #include <limits.h>
 
 #include <type_traits>
@@ -53,12 +53,12 @@ struct Head {
   float scale_dh, scale_dw;  // the factors of the gradients
 };
 // What the backward keeps of a row. Where its |g| |h| is 2^-k of the largest row's, h's transposed copy has
-// 2^-half of it, dl's the rest: t is below 2^(half - k) in magnitude.
+// share_of(k) of k taken off, dl's the rest: t is below 2^(share - k) in magnitude.
 struct Row {
   float g;     // its gradient (ignored: 0, a bad target: NaN)
   float t;     // the factor of dl's transposed copy, g 2^(-exp_dw - turned)
   int exp;     // exponent of its h, whose largest magnitude it brings to [2^13, 2^14) (fp16: 0)
-  int turned;  // exponent of h's transposed copy, exp - half
+  int turned;  // exponent of h's transposed copy, exp - share
 };
 
 
@@ -675,7 +675,7 @@ __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const i
     int turned = e;
     if (!counts(g)) return Row{g, g, e, turned};
     const int k = most - size(m, g);
-    if (eh) turned -= half_of(k);
+    if (eh) turned -= share_of(k);
     return Row{g, ldexpf(g, -most - turned), e, turned};
   };
   if (kept.map) {
@@ -714,7 +714,7 @@ struct DlEpi {
       for (int k = 0; k < 4; k++) {
         en[k] = ew[n0 + lane % (TN * 8) * 4 + k];  // (past N: its padding)
         const int d = en[k] - least;
-        part[k] = ldexpf(1.0f, half_of(d) - d);
+        part[k] = ldexpf(1.0f, share_of(d) - d);
       }
     }
     Mat ot = this->ot;  // padded to whole k tiles of the rows there are

@@ -13,9 +13,10 @@ depend on timing.
 
 Precision beyond 16 tokens (up to 16 all of it is float32). A row's loss and its gradient of ``hidden``
 do not depend on how large other rows, or other rows' gradients, are. float32: an element of a row of
-``hidden`` or ``weight`` is held to 2^-38 of the row's largest; in the gradients' sums (over the
-entries for ``hidden``, over the rows for ``weight``) a term whose factor is 2^-k of the largest row's
-is held to 2^(k / 2 - 38) of its own, which is float32-class to k = 28. fp16 and bf16: the logits'
+``hidden`` or ``weight`` is held to 2^-38 of the row's largest in the logits; in the gradients' sums
+(over the entries for ``hidden``, over the rows for ``weight``) one whose row is 2^-k of the largest,
+by |weight| or by |incoming gradient| |hidden|, to 2^-24 of its row's largest up to k = 30 and the
+probability in front of it to 2^-38 (2^(k - 53) past k = 15); past k = 30 both to 2^(k / 2 - 38). fp16 and bf16: the logits'
 gradients round to fp16 (2^-11 at most) before those sums, which are float32; bits are lost, for
 ``weight``, by rows of fp16 ``hidden`` whose incoming gradient is 2^-28 and less of the largest, and,
 for ``hidden``, by entries of a bf16 ``weight`` 2^-30 and less of its largest element.

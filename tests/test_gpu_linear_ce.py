@@ -589,8 +589,8 @@ def test_a_large_gradient_leaves_the_others(tokens, dim, vocab, ignored, dtype):
 @pytest.mark.parametrize("tokens,dim,vocab,ignored", SPREAD)
 def test_the_weights_gradient_beside_large_rows(tokens, dim, vocab, ignored, power, dtype):
     """Rows of hidden 2^k above the others, each sure of one entry: the weight's and the bias' gradients of
-    the other entries are those of the small rows alone. Both operands of such a sum have half of k taken off,
-    which leaves them 2^(k / 2 - 38) of a row's largest product."""
+    the other entries are those of the small rows alone. The operands of such a sum share k, which leaves them
+    2^(k / 2 - 38) of a row's largest product and more."""
     h, w, b, t = make(tokens, dim, vocab, dtype, True, ignored, seed=33)
     t[::50] = 5
     large = torch.zeros(tokens, dtype=torch.bool, device="cuda")
@@ -614,8 +614,8 @@ def test_the_weights_gradient_beside_large_rows(tokens, dim, vocab, ignored, pow
 @pytest.mark.parametrize("tokens,dim,vocab,ignored", SPREAD)
 def test_hiddens_gradient_beside_a_large_entry(tokens, dim, vocab, ignored, power):
     """An entry of the weight 2^k above the others, masked by its bias: float32 gradients of hidden are those of
-    the other entries alone, whose factors in the sum have half of k taken off each: every term is off by
-    2^(k / 2 - 38) of its largest, and they add up as a random walk."""
+    the other entries alone, whose factors in the sum share k: every term is off by 2^(k / 2 - 38) of its largest
+    at most, and they add up as a random walk."""
     h, w, b, t = make(tokens, dim, vocab, torch.float32, True, ignored, seed=34)
     t = torch.where(t == -100, t, t % (vocab - 1))
     b[-1] = float("-inf")
@@ -667,3 +667,26 @@ def test_ignored_rows_change_no_bit(tokens, dim, vocab, dtype):
         got.append((loss, *torch.autograd.grad(loss, leaves, torch.tensor(-1.7, device="cuda"))))
     assert all(torch.equal(x, y) for x, y in zip(*got))
     assert (got[1][1][rows] == 0).all() and torch.isfinite(got[1][0])
+
+
+@pytest.mark.parametrize("tokens,dim,vocab", [(100, 64, 500), (60, 36, 500), (200, 100, 900)])
+def test_small_probabilities_of_small_rows(tokens, dim, vocab):
+    """Rows of hidden some 2^-13 of a few large ones, which are sure of one entry, under a bias that makes most
+    entries improbable (to 2^-23): the weight's gradient keeps 2^-38 of a probability in float32, as where all
+    rows are of one size."""
+    h, w, b, t = make(tokens, dim, vocab, torch.float32, True, 0, seed=37)
+    b[:] = torch.linspace(0, -16, vocab, device="cuda")
+    t %= 20
+    t[::50] = 5
+    large = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    large[::50] = True
+    h[~large] *= 2.0 ** -6
+    h[large] = 400.0 * w[5] / w[5].norm() ** 2
+    g = torch.randn(tokens, device="cuda")
+    leaf = w.detach().requires_grad_()
+    dw = torch.autograd.grad(linear_cross_entropy(h, leaf, t, b, reduction="none"), leaf, g)[0]
+    _, _, want, bounds = reference(h[~large], w, b, t[~large], "none", g[~large])
+    p = torch.softmax(h[large].double() @ w.double().t() + b.double(), 1)
+    others = torch.arange(20, vocab, device="cuda")
+    assert (p[:, others] < 2.0 ** -100).all()
+    close(dw[others], want[1][others], bounds[1][others], torch.float32)
