@@ -631,7 +631,8 @@ __global__ __launch_bounds__(1024) void join_loss_kernel(const float2* part, int
 // ---- backward -----------------------------------------------------------------------------------
 // One workgroup: the transposed weight's exponent (part: gw partial maxima, NULL: none), the rows' factors, and
 // what comes off again in the epilogues. Ignored rows get 0 or are left out (Kept), rows whose gradient is not
-// finite that gradient itself, rows whose target is no entry NaN. eh: the exponents of all rows of h (NULL: as they are).
+// finite that gradient itself, rows whose target is no entry NaN. eh: the exponents of all rows of h (NULL: as
+// they are).
 __global__ __launch_bounds__(1024) void factor_kernel(const float* grad, const int64_t* target,
                                                       int64_t ignore, int rows, int64_t vocab, int reduction,
                                                       const Head* head, const float* part, int gw,
@@ -1117,7 +1118,8 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   if (scaled) {
     top = a.take<float>(2 * kMaxParts);
     if (run && sp) maxima((const float*)h, ldh, (const float*)w, ldw, s, target, ignore, top, eh, ew, st);
-    else if (run) maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, eh, nullptr, st);
+    else if (run)
+      maxima((const __bf16*)h, ldh, (const __bf16*)w, ldw, s, target, ignore, top, eh, nullptr, st);
   }
   const Exponents turned_eh = scaled ? Exponents{&row->turned, 4} : Exponents();
   if (run)
@@ -1130,7 +1132,8 @@ size_t backward(const void* h, int64_t ldh, const void* w, int64_t ldw, Shape s,
   const int padt = operand_pad(s.tokens, sp);
   _Float16* ht = dw ? a.take<_Float16>((size_t)(s.dim * ldt)) : nullptr;
   const Mat turned_h = dw ? Mat{ht, ldt, 0, fmt, padt} : kNoMat;
-  if (run && raw && dw) layout(h, s.dtype, ldh, s.tokens, s.dim, {}, turned_eh, target, ignore, kNoMat, turned_h, st);  // (not gathered)
+  if (run && raw && dw)  // (not gathered)
+    layout(h, s.dtype, ldh, s.tokens, s.dim, {}, turned_eh, target, ignore, kNoMat, turned_h, st);
   const Operand A =
       raw ? Operand{h, 2 * ldh, 0, (int)s.tokens}
           : operand(a, h, ldh, s.tokens, s.dim, s, sp ? Exponents{&row->exp, 4} : Exponents(), turned_eh, pick,
