@@ -30,7 +30,8 @@
 // has one scale, that of the largest |g| |h| of a row; a row 2^-k of it (float32, bf16) has k taken off h's
 // transposed copy and dl's, shared so that both stay in fp16's range (share_of, Row); dh's sum over float32 entries
 // the same of the largest |w|. float32: h and w to 2^-24 of their row's largest and p to 2^-38 up to k = 15, p to
-// 2^(k - 53) up to k = 30, both to 2^(k / 2 - 38) beyond; the row exponents cost one read more of the weight in each direction than one for all.
+// 2^(k - 53) up to k = 30, both to 2^(k / 2 - 38) beyond. The row exponents cost one read more of the weight in
+// each direction than one for all.
 #include <limits.h>
 
 #include <type_traits>
